@@ -15,9 +15,9 @@
  *  - Pointers named d_* are DEVICE pointers; the caller owns every buffer.
  *  - stream is a hipStream_t passed as void* (NULL = default stream); every
  *    device entry point is asynchronous on it.  None allocates, except that
- *    swamp_qgemv_batched and swamp_qgemm take scratch memory for split
- *    reductions from a buffer the library keeps per (device, stream): see
- *    "Scratch" below.
+ *    swamp_qgemv_batched, swamp_qgemm and swamp_attn_paged take scratch memory
+ *    for split reductions from a buffer the library keeps per (device, stream):
+ *    see "Scratch" below.
  *  - Return 0 on success, a negative SWAMP_E* code on error; on error no
  *    output is written and nothing is launched.
  */
@@ -317,6 +317,131 @@ SWAMP_API int swamp_swiglu(const float *d_gate, const float *d_up, void *d_out,
  * quantizer swamp_quantize (swamp_quant.h). */
 SWAMP_API int swamp_quantize_q8_0(const void *d_x, uint32_t x_type, void *d_q, size_t n,
                         void *stream);
+
+/* ---- attention between the QKV and the O product ----
+ *
+ * Rotary positions, a paged cache of keys and values, and the causal attention
+ * that reads it.  Replaces, on the device, the engine's CPU steps between
+ * executor.rs:433-445 and the O projection: the rotation (swamp-engine/src/
+ * ops.rs:20-54), the paged cache's append (cache.rs) and the attention over it.
+ * The reference's gpu_attention_* entry points have other arguments and are not
+ * replaced.  Structures are read during the call and not kept; strides are in
+ * elements, and 0 stands for the dense one. */
+
+/* Pairs that turn together: (2i, 2i + 1), or (i, i + n_rot / 2). */
+enum { SWAMP_ROPE_PAIRS = 0, SWAMP_ROPE_HALVES = 1 };
+
+/* A rotation: pair i of the first n_rot dims of a head turns by
+ * p * d_freqs[i] radians at position p, and its length is multiplied by mscale
+ * (1: none); the dims from n_rot on pass unchanged.  n_rot even, 2 to head_dim.
+ * d_freqs: n_rot / 2 doubles on the device, 8-byte aligned. */
+typedef struct swamp_rope_spec {
+  const double *d_freqs;
+  int32_t n_rot;
+  uint32_t layout; /* SWAMP_ROPE_* */
+  float mscale;
+} swamp_rope_spec;
+
+/* A paged cache of one layer: position P of a sequence is slot P % page_size of
+ * the page that its page table names at P / page_size.  Element (page, head,
+ * slot, dim) of d_k and d_v lies at page * page_stride + head * head_stride +
+ * slot * slot_stride + dim; all strides 0: [page][head][slot][dim].
+ * dtype SWAMP_F16 or SWAMP_BF16; page_size a power of two up to 65536;
+ * head_dim a multiple of 8 up to 256; strides multiples of 8; d_k and d_v
+ * 16-byte aligned. */
+typedef struct swamp_kv_pages {
+  void *d_k, *d_v;
+  uint32_t dtype;
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+  int64_t page_stride, head_stride, slot_stride;
+} swamp_kv_pages;
+
+/* The new tokens of a batch of sequences.  All arrays are int32 on the device,
+ * so that a captured graph can be replayed with other lengths.
+ *   d_first[n_seq + 1]: sequence s has the new tokens (rows of q, k, v)
+ *     d_first[s] .. d_first[s + 1] - 1, none if the two are equal; ascending,
+ *     from 0 to at most n_tok.  Rows of no sequence are padding.
+ *   d_len[n_seq]: its tokens in the cache, the new ones among them: its i-th of
+ *     n new tokens is at position d_len[s] - n + i.
+ *   d_pages[n_seq][pages_stride]: its page table (pages_stride in entries, and
+ *     at least its pages).
+ *   max_new: at least the most new tokens that a sequence has.  max_len: about
+ *     the longest d_len; the work is split by it, results do not depend on its
+ *     being right.
+ *   d_bad (may be NULL): set to 1 where a position of a sequence that the call
+ *     has to read or write has no page (a table entry outside 0 .. n_pages - 1,
+ *     a position past the table or before 0).  No memory outside the pages is
+ *     touched then. */
+typedef struct swamp_seq_batch {
+  int32_t n_seq, n_tok, max_new, max_len;
+  const int32_t *d_first, *d_len, *d_pages;
+  int64_t pages_stride;
+  int32_t *d_bad;
+} swamp_seq_batch;
+
+/* Frequencies of a rotation, on the host: f_i = base^(-2i / n_rot), i < n_rot /
+ * 2, divided by divisors[i] where divisors is not NULL (a GGUF file's
+ * rope_freqs tensor).  factor > 1 stretches the context: orig_ctx = 0 divides
+ * every f_i by it; orig_ctx > 0 (the context the model was trained on) divides
+ * the pairs that turn less than beta_slow times in it, leaves those that turn
+ * more than beta_fast times, and blends linearly over the pairs between (the
+ * ramp of YaRN, Peng et al. 2023; usual values 32 and 1; its mscale,
+ * 0.1 ln(factor) + 1, is the caller's).  SWAMP_ESHAPE: n_rot odd or below 2;
+ * SWAMP_EINVAL: a value that makes no rotation. */
+SWAMP_API int swamp_rope_freqs(double *freqs, int n_rot, double base, double factor,
+                               int orig_ctx, double beta_fast, double beta_slow,
+                               const float *divisors);
+
+/* out[t][h] = x[t][h] turned by d_pos[t]: n_tok rows of n_heads heads of
+ * head_dim (even, up to 512), rows x_stride and out_stride apart.  x_type and
+ * out_type SWAMP_F32, SWAMP_F16 or SWAMP_BF16; computed in fp32 (the angle in
+ * 64 bits: positions of any size), rounded once.  d_out may be d_x with the
+ * same type and stride; otherwise they must not overlap.  Buffers aligned to
+ * their element. */
+SWAMP_API int swamp_rope(const swamp_rope_spec *rope, const int32_t *d_pos, const void *d_x,
+                         uint32_t x_type, int64_t x_stride, void *d_out, uint32_t out_type,
+                         int64_t out_stride, int n_tok, int n_heads, int head_dim, void *stream);
+
+/* The new tokens' k, turned by their positions, and v into the cache's pages,
+ * and q, turned, to d_q_out in the cache's type: what swamp_attn_paged reads,
+ * in one launch.  d_q [n_tok][n_heads][head_dim], d_k and d_v
+ * [n_tok][n_kv_heads][head_dim] of x_type (F32, F16, BF16), rows q_stride,
+ * k_stride, v_stride apart (the fused QKV product: three places of one row);
+ * d_q_out rows q_out_stride apart.  rope NULL: nothing is turned.  n_heads 0
+ * (d_q and d_q_out NULL): k and v only.  fp32 values are rounded once, to
+ * nearest even (fp16: beyond 65504 to infinity).  A token whose position has no
+ * page is left out of the cache (d_bad); rows of no sequence are not touched.
+ * Two sequences must not share the pages of their new tokens. */
+SWAMP_API int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
+                              const swamp_rope_spec *rope, const void *d_q, const void *d_k,
+                              const void *d_v, uint32_t x_type, int64_t q_stride,
+                              int64_t k_stride, int64_t v_stride, void *d_q_out,
+                              int64_t q_out_stride, int n_heads, void *stream);
+
+/* Attention of the new tokens over the cache: out[t][h] = sum_j p_j v_j / sum_j
+ * p_j with p_j = exp(scale q.k_j), over the positions j <= t's own and, with
+ * window > 0, j > t's own - window; head h reads cache head h / (n_heads /
+ * n_kv_heads).  d_q [n_tok][n_heads][head_dim] of the cache's type, 16-byte
+ * aligned rows q_stride (a multiple of 8) apart; d_out rows out_stride apart,
+ * of out_type F32, F16 or BF16, 16-byte aligned (out_stride a multiple of 8).
+ * Scores, softmax and sums are fp32.  With 16-bit output the weights p_j are
+ * rounded to the cache's type before they meet v, which costs about as much as
+ * the output's own rounding; with F32 output they keep 22 bits or more.
+ * Keys that a row does not see, and slots past d_len, do not reach its result,
+ * whatever they hold.  A row that sees no key gives 0; rows of no sequence are
+ * not touched; a row block that has to read a position without a page gives NaN
+ * (d_bad).
+ * A long cache is split over workgroups that leave partial sums in the stream's
+ * scratch ("Scratch" above; swamp_attn_paged_workspace reports it), joined in a
+ * fixed order: repeated calls give the same bits.  Without it (under capture,
+ * nothing reserved) the cache is not split. */
+SWAMP_API int swamp_attn_paged(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
+                               const void *d_q, int64_t q_stride, int n_heads, float scale,
+                               int window, void *d_out, uint32_t out_type, int64_t out_stride,
+                               void *stream);
+SWAMP_API size_t swamp_attn_paged_workspace(const swamp_kv_pages *cache,
+                                            const swamp_seq_batch *batch, int n_heads,
+                                            int window);
 
 /* ---- the reference's two existing C exports, host-pointer semantics ---- */
 

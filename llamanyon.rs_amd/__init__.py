@@ -33,6 +33,7 @@ TYPE_SIZE = {Q4_0: 18, Q8_0: 34, Q4_K: 144, Q6_K: 210}
 OK, EINVAL, EDTYPE, ESHAPE, ELAUNCH, ENODEVICE, EWORKSPACE = 0, -1, -2, -3, -4, -5, -6
 EIO, EMAGIC, EVERSION, ENOTFOUND, ETENSOR = -7, -8, -9, -10, -11
 MULTI_MAX = 8
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 
 # Every symbol include/swamp_qmm.h declares.
 GPU_SYMBOLS = (
@@ -43,6 +44,8 @@ GPU_SYMBOLS = (
     "swamp_quantize_q8_0", "swamp_fused_gemv_q4k", "swamp_gemv_q8_vnni",
     "swamp_qgemv_batched_workspace", "swamp_qgemm_workspace", "swamp_workspace_reserve",
     "swamp_qgemv_batched_noalloc", "swamp_qgemv_many",
+    "swamp_rope_freqs", "swamp_rope", "swamp_kv_append", "swamp_attn_paged",
+    "swamp_attn_paged_workspace",
 )
 # Every symbol include/swamp_gguf.h declares (also in libswamp_gpu.so).
 GGUF_SYMBOLS = (
@@ -82,6 +85,47 @@ c_size = ctypes.c_size_t
 c_vp = ctypes.c_void_p
 
 
+class Rope(ctypes.Structure):
+    """swamp_rope_spec: d_freqs holds n_rot / 2 doubles (rope_freqs) on the device."""
+
+    _fields_ = [("d_freqs", c_vp), ("n_rot", ctypes.c_int32), ("layout", ctypes.c_uint32),
+                ("mscale", ctypes.c_float)]
+
+    def __init__(self, d_freqs: int, n_rot: int, layout: int, mscale: float = 1.0):
+        super().__init__(d_freqs, n_rot, layout, mscale)
+
+
+class KvPages(ctypes.Structure):
+    """swamp_kv_pages: one layer's paged cache (strides in elements; all 0:
+    [page][head][slot][dim])."""
+
+    _fields_ = [("d_k", c_vp), ("d_v", c_vp), ("dtype", ctypes.c_uint32),
+                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64)]
+
+    def __init__(self, d_k: int, d_v: int, dtype: int, n_pages: int, page_size: int,
+                 n_kv_heads: int, head_dim: int, page_stride: int = 0, head_stride: int = 0,
+                 slot_stride: int = 0):
+        super().__init__(d_k, d_v, dtype, n_pages, page_size, n_kv_heads, head_dim, page_stride,
+                         head_stride, slot_stride)
+
+
+class SeqBatch(ctypes.Structure):
+    """swamp_seq_batch: the new tokens of n_seq sequences, and their pages."""
+
+    _fields_ = [("n_seq", ctypes.c_int32), ("n_tok", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("max_len", ctypes.c_int32), ("d_first", c_vp),
+                ("d_len", c_vp), ("d_pages", c_vp), ("pages_stride", ctypes.c_int64),
+                ("d_bad", c_vp)]
+
+    def __init__(self, n_seq: int, n_tok: int, max_new: int, max_len: int, d_first: int,
+                 d_len: int, d_pages: int, pages_stride: int, d_bad: int = 0):
+        super().__init__(n_seq, n_tok, max_new, max_len, d_first, d_len, d_pages, pages_stride,
+                         d_bad)
+
+
 def build(force: bool = False) -> None:
     """Compile both libraries in-tree with the package Makefile."""
     cmd = ["make", "-C", PKG_DIR, "-j8"]
@@ -98,7 +142,7 @@ def gpu_lib() -> ctypes.CDLL:
     if not os.path.exists(GPU_LIB_PATH):
         raise GpuError(ENODEVICE, f"{GPU_LIB_PATH} not built (run build())")
     lib = ctypes.CDLL(GPU_LIB_PATH)
-    u32, i32 = ctypes.c_uint32, ctypes.c_int
+    u32, i32, i64 = ctypes.c_uint32, ctypes.c_int, ctypes.c_int64
     sig = {
         "swamp_gpu_init": (i32, []),
         "swamp_strerror": (ctypes.c_char_p, [i32]),
@@ -131,6 +175,17 @@ def gpu_lib() -> ctypes.CDLL:
         "swamp_workspace_reserve": (i32, [c_vp, c_size]),
         "swamp_qgemv_batched_noalloc": (i32, [u32, c_vp, c_size, c_vp, c_vp, i32, i32, i32, i32,
                                               c_vp]),
+        "swamp_rope_freqs": (i32, [c_vp, i32, ctypes.c_double, ctypes.c_double, i32,
+                                   ctypes.c_double, ctypes.c_double, c_vp]),
+        "swamp_rope": (i32, [ctypes.POINTER(Rope), c_vp, c_vp, u32, i64, c_vp, u32, i64, i32, i32,
+                             i32, c_vp]),
+        "swamp_kv_append": (i32, [ctypes.POINTER(KvPages), ctypes.POINTER(SeqBatch),
+                                  ctypes.POINTER(Rope), c_vp, c_vp, c_vp, u32, i64, i64, i64, c_vp,
+                                  i64, i32, c_vp]),
+        "swamp_attn_paged": (i32, [ctypes.POINTER(KvPages), ctypes.POINTER(SeqBatch), c_vp, i64,
+                                   i32, ctypes.c_float, i32, c_vp, u32, i64, c_vp]),
+        "swamp_attn_paged_workspace": (c_size, [ctypes.POINTER(KvPages), ctypes.POINTER(SeqBatch),
+                                                i32, i32]),
         "swamp_gemv_q8_vnni": (ctypes.c_float, [c_vp, c_vp, i32, ctypes.c_float]),
         # GGUF reader (include/swamp_gguf.h)
         "swamp_gguf_open": (i32, [ctypes.c_char_p, ctypes.POINTER(c_vp)]),
@@ -337,6 +392,31 @@ def quantize_q8_0(d_x: int, x_type: int, d_q: int, n: int, stream: int = 0) -> N
     _check(gpu_lib().swamp_quantize_q8_0(d_x, x_type, d_q, n, stream), "swamp_quantize_q8_0")
 
 
+def rope(spec: Rope, d_pos: int, d_x: int, x_type: int, d_out: int, out_type: int, n_tok: int,
+         n_heads: int, head_dim: int, x_stride: int = 0, out_stride: int = 0,
+         stream: int = 0) -> None:
+    """n_tok rows of heads turned by their positions (ops.rs:20-54)."""
+    _check(gpu_lib().swamp_rope(spec, d_pos, d_x, x_type, x_stride, d_out, out_type, out_stride,
+                                n_tok, n_heads, head_dim, stream), "swamp_rope")
+
+
+def kv_append(cache: KvPages, batch: SeqBatch, spec: Optional[Rope], d_q: int, d_k: int, d_v: int,
+              x_type: int, d_q_out: int, n_heads: int, q_stride: int = 0, k_stride: int = 0,
+              v_stride: int = 0, q_out_stride: int = 0, stream: int = 0) -> None:
+    """New k (turned) and v into the cache's pages, q (turned) to d_q_out in its type."""
+    _check(gpu_lib().swamp_kv_append(cache, batch, spec, d_q, d_k, d_v, x_type, q_stride, k_stride,
+                                     v_stride, d_q_out, q_out_stride, n_heads, stream),
+           "swamp_kv_append")
+
+
+def attn_paged(cache: KvPages, batch: SeqBatch, d_q: int, n_heads: int, scale: float, d_out: int,
+               out_type: int, window: int = 0, q_stride: int = 0, out_stride: int = 0,
+               stream: int = 0) -> None:
+    """Causal attention of the batch's new tokens over the paged cache."""
+    _check(gpu_lib().swamp_attn_paged(cache, batch, d_q, q_stride, n_heads, scale, window, d_out,
+                                      out_type, out_stride, stream), "swamp_attn_paged")
+
+
 # ---------------------------------------------------------- host preparation
 
 def _np():
@@ -378,6 +458,21 @@ def to_bf16_bits(src):
     src = np.ascontiguousarray(src, dtype=np.float32)
     out = np.empty(src.shape, dtype=np.uint16)
     quant_lib().swamp_f32_to_bf16_array(src.ctypes.data, out.ctypes.data, src.size)
+    return out
+
+
+def rope_freqs(n_rot: int, base: float = 10000.0, factor: float = 1.0, orig_ctx: int = 0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0, divisors=None):
+    """Radians per position of each pair of a rotation (numpy float64, n_rot / 2)."""
+    np = _np()
+    if divisors is not None:
+        divisors = np.ascontiguousarray(divisors, dtype=np.float32)
+        if divisors.size != n_rot // 2:
+            raise ValueError("one divisor a pair")
+    out = np.empty(max(n_rot // 2, 1), dtype=np.float64)
+    _check(gpu_lib().swamp_rope_freqs(out.ctypes.data, n_rot, base, factor, orig_ctx, beta_fast,
+                                      beta_slow, None if divisors is None else divisors.ctypes.data),
+           "swamp_rope_freqs")
     return out
 
 

@@ -1,13 +1,14 @@
 // api.hip -- the C ABI of libswamp_gpu.so (declared in include/swamp_qmm.h).
 //
 // Validation and dispatch only; kernels live in dequant.hip, gemv.hip,
-// gemv_fused.hip, gemv_batched.hip, gemm.hip and gemm_i8.hip, and the rules
+// gemv_fused.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, rope.hip and attn.hip, and the rules
 // that choose between them by size in dispatch.hpp.  The error behaviour mirrors the
 // reference: shape asserts of fused_gemv_q4k (fused_gemv_q4k.rs:66-70) and
 // the bail! of forward_linear (linear.rs:23-25) become negative return
 // codes, checked before anything is launched; the two legacy host-pointer
 // exports keep their silent-return behaviour.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <thread>
 #include <vector>
@@ -112,6 +113,89 @@ int check_gemv_args(uint32_t dtype, const void *d_w, size_t w_len, int n_rows, i
 bool fused_cols_ok(uint32_t dt, int n_cols) {
   if (n_cols <= 0 || n_cols > 32768) return false;
   return n_cols % (dt == SWAMP_Q6_K ? 512 : dt == SWAMP_Q4_K ? 256 : 64) == 0;
+}
+
+bool is_float(uint32_t t) { return t == SWAMP_F32 || t == SWAMP_F16 || t == SWAMP_BF16; }
+
+// Longest sequences and rows of the paged entry points: grids and the row
+// arithmetic of the kernels stay within 32 bits.
+constexpr int kMaxSeqs = 65535, kMaxHeads = 4096, kMaxWindow = 1 << 30;
+
+int check_rope(const swamp_rope_spec *r, int head_dim) {
+  if (!r || !r->d_freqs || !aligned(r->d_freqs, 8)) return SWAMP_EINVAL;
+  if (r->layout != SWAMP_ROPE_PAIRS && r->layout != SWAMP_ROPE_HALVES) return SWAMP_EINVAL;
+  if (r->n_rot < 2 || r->n_rot % 2 != 0 || r->n_rot > head_dim) return SWAMP_ESHAPE;
+  return SWAMP_OK;
+}
+
+// The cache with its strides filled in; d_k and d_v are checked by the callers
+// that read or write it.
+int check_cache(const swamp_kv_pages *c, PagedCache &out) {
+  if (!c) return SWAMP_EINVAL;
+  if (c->dtype != SWAMP_F16 && c->dtype != SWAMP_BF16) return SWAMP_EDTYPE;
+  if (c->n_pages < 0 || c->n_kv_heads < 1 || c->n_kv_heads > kMaxHeads) return SWAMP_EINVAL;
+  if (c->page_size < 1 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0)
+    return SWAMP_ESHAPE;
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0) return SWAMP_ESHAPE;
+  const int64_t most = int64_t(1) << 40;  // page id * stride stays within 64 bits
+  for (int64_t v : {c->page_stride, c->head_stride, c->slot_stride}) {
+    if (v < 0 || v > most) return SWAMP_EINVAL;
+    if (v % 8 != 0) return SWAMP_ESHAPE;
+  }
+  out.slot_stride = c->slot_stride ? c->slot_stride : c->head_dim;
+  out.head_stride = c->head_stride ? c->head_stride : int64_t(c->page_size) * c->head_dim;
+  out.page_stride =
+      c->page_stride ? c->page_stride : int64_t(c->n_kv_heads) * c->page_size * c->head_dim;
+  if (out.slot_stride < c->head_dim) return SWAMP_ESHAPE;
+  out.k = static_cast<uint16_t *>(c->d_k);
+  out.v = static_cast<uint16_t *>(c->d_v);
+  out.n_pages = c->n_pages;
+  out.page_shift = __builtin_ctz(unsigned(c->page_size));
+  out.n_kv = c->n_kv_heads;
+  out.dim = c->head_dim;
+  return SWAMP_OK;
+}
+
+int check_batch(const swamp_seq_batch *b, SeqBatch &out) {
+  if (!b) return SWAMP_EINVAL;
+  if (b->n_seq < 0 || b->n_seq > kMaxSeqs || b->n_tok < 0 || b->max_new < 0 || b->max_len < 0 ||
+      b->pages_stride < 0)
+    return SWAMP_EINVAL;
+  out.first = b->d_first;
+  out.len = b->d_len;
+  out.pages = b->d_pages;
+  out.pages_stride = b->pages_stride;
+  out.bad = b->d_bad;
+  out.n_seq = b->n_seq;
+  out.n_tok = b->n_tok;
+  return SWAMP_OK;
+}
+bool batch_ok(const SeqBatch &b) {
+  return b.first && b.len && b.pages && aligned(b.first, 4) && aligned(b.len, 4) &&
+         aligned(b.pages, 4) && aligned(b.bad, 4);
+}
+bool cache_ok(const PagedCache &c) { return c.k && c.v && aligned(c.k, 16) && aligned(c.v, 16); }
+
+// Rows of n heads of dim elements, `stride` apart (0: dense).
+int check_rows(int64_t &stride, int n, int dim) {
+  if (stride < 0 || stride > (int64_t(1) << 40)) return SWAMP_EINVAL;
+  if (stride == 0) stride = int64_t(n) * dim;
+  return stride < int64_t(n) * dim ? SWAMP_ESHAPE : SWAMP_OK;
+}
+
+// The plan of an attention call; q and out are checked by the caller.
+int check_attn(const swamp_kv_pages *cache, const swamp_seq_batch *batch, int n_heads, int window,
+               AttnCall &c) {
+  if (int rc = check_cache(cache, c.cache)) return rc;
+  if (int rc = check_batch(batch, c.batch)) return rc;
+  if (n_heads < 1 || n_heads > kMaxHeads || window < 0) return SWAMP_EINVAL;
+  if (n_heads % cache->n_kv_heads != 0) return SWAMP_ESHAPE;
+  c.dtype = cache->dtype;
+  c.n_heads = n_heads;
+  c.window = window >= kMaxWindow ? 0 : window;  // no row is that far from its first key
+  c.max_new = std::min(batch->max_new, batch->n_tok);
+  c.max_len = batch->max_len;
+  return SWAMP_OK;
 }
 
 }  // namespace
@@ -496,6 +580,126 @@ int swamp_quantize_q8_0(const void *d_x, uint32_t x_type, void *d_q, size_t n, v
   if (!d_x || !d_q || !aligned(d_x, 4)) return SWAMP_EINVAL;
   if (int rc = ensure_device(nullptr)) return rc;
   return swamp_launch_quantize_q8_0(d_x, x_type, d_q, n, static_cast<hipStream_t>(stream));
+}
+
+int swamp_rope_freqs(double *freqs, int n_rot, double base, double factor, int orig_ctx,
+                     double beta_fast, double beta_slow, const float *divisors) {
+  if (n_rot < 2 || n_rot % 2 != 0) return SWAMP_ESHAPE;
+  if (!freqs || !(base > 1.0) || !std::isfinite(base) || !(factor > 0.0) || !std::isfinite(factor) ||
+      orig_ctx < 0)
+    return SWAMP_EINVAL;
+  const bool ramp = factor != 1.0 && orig_ctx > 0;
+  if (ramp && (!(beta_slow > 0.0) || !(beta_fast > beta_slow) || !std::isfinite(beta_fast)))
+    return SWAMP_EINVAL;
+  const int n = n_rot / 2;
+  if (divisors)
+    for (int i = 0; i < n; i++)
+      if (!(divisors[i] > 0.0f) || !std::isfinite(divisors[i])) return SWAMP_EINVAL;
+  // pair index whose frequency turns `beta` times in orig_ctx positions:
+  // orig_ctx base^(-2i / n_rot) = 2 pi beta
+  const double two_pi = 6.283185307179586476925;
+  auto pair_at = [&](double beta) {
+    return n_rot * std::log(orig_ctx / (beta * two_pi)) / (2.0 * std::log(base));
+  };
+  double lo = 0.0, hi = 0.0;
+  if (ramp) {
+    lo = std::max(0.0, std::floor(pair_at(beta_fast)));
+    hi = std::min(double(n_rot - 1), std::ceil(pair_at(beta_slow)));
+  }
+  for (int i = 0; i < n; i++) {
+    double f = std::pow(base, -2.0 * i / n_rot);
+    if (divisors) f /= double(divisors[i]);
+    if (ramp) {
+      const double slow = std::min(1.0, std::max(0.0, (i - lo) / std::max(0.001, hi - lo)));
+      f = f * (1.0 - slow) + f / factor * slow;
+    } else {
+      f /= factor;
+    }
+    freqs[i] = f;
+  }
+  return SWAMP_OK;
+}
+
+int swamp_rope(const swamp_rope_spec *rope, const int32_t *d_pos, const void *d_x, uint32_t x_type,
+               int64_t x_stride, void *d_out, uint32_t out_type, int64_t out_stride, int n_tok,
+               int n_heads, int head_dim, void *stream) {
+  if (!is_float(x_type) || !is_float(out_type)) return SWAMP_EDTYPE;
+  if (n_tok < 0 || n_heads < 0 || n_heads > kMaxHeads || head_dim < 2) return SWAMP_EINVAL;
+  if (head_dim % 2 != 0 || head_dim > 512) return SWAMP_ESHAPE;
+  if (int rc = check_rope(rope, head_dim)) return rc;
+  if (int rc = check_rows(x_stride, n_heads, head_dim)) return rc;
+  if (int rc = check_rows(out_stride, n_heads, head_dim)) return rc;
+  if (n_tok == 0 || n_heads == 0) return SWAMP_OK;
+  if (!d_pos || !d_x || !d_out || !aligned(d_pos, 4) || !aligned(d_x, type_size(x_type)) ||
+      !aligned(d_out, type_size(out_type)))
+    return SWAMP_EINVAL;
+  if (d_x == d_out && (x_type != out_type || x_stride != out_stride)) return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_rope(rope, d_pos, d_x, x_type, x_stride, d_out, out_type, out_stride, n_tok,
+                           n_heads, head_dim, static_cast<hipStream_t>(stream));
+}
+
+int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
+                    const swamp_rope_spec *rope, const void *d_q, const void *d_k, const void *d_v,
+                    uint32_t x_type, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                    void *d_q_out, int64_t q_out_stride, int n_heads, void *stream) {
+  PagedCache c;
+  SeqBatch b;
+  if (int rc = check_cache(cache, c)) return rc;
+  if (int rc = check_batch(batch, b)) return rc;
+  if (!is_float(x_type)) return SWAMP_EDTYPE;
+  if (n_heads < 0 || n_heads > kMaxHeads) return SWAMP_EINVAL;
+  if (rope)
+    if (int rc = check_rope(rope, c.dim)) return rc;
+  if (int rc = check_rows(q_stride, n_heads, c.dim)) return rc;
+  if (int rc = check_rows(k_stride, c.n_kv, c.dim)) return rc;
+  if (int rc = check_rows(v_stride, c.n_kv, c.dim)) return rc;
+  if (int rc = check_rows(q_out_stride, n_heads, c.dim)) return rc;
+  if (b.n_tok == 0 || b.n_seq == 0) return SWAMP_OK;
+  const uintptr_t al = type_size(x_type);
+  if (!cache_ok(c) || !batch_ok(b) || !d_k || !d_v || !aligned(d_k, al) || !aligned(d_v, al))
+    return SWAMP_EINVAL;
+  if (n_heads > 0 && (!d_q || !d_q_out || !aligned(d_q, al) || !aligned(d_q_out, 2)))
+    return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_kv_append(c, b, cache->dtype, rope, d_q, d_k, d_v, x_type, q_stride, k_stride,
+                                v_stride, d_q_out, q_out_stride, n_heads,
+                                static_cast<hipStream_t>(stream));
+}
+
+int swamp_attn_paged(const swamp_kv_pages *cache, const swamp_seq_batch *batch, const void *d_q,
+                     int64_t q_stride, int n_heads, float scale, int window, void *d_out,
+                     uint32_t out_type, int64_t out_stride, void *stream) {
+  AttnCall c;
+  if (int rc = check_attn(cache, batch, n_heads, window, c)) return rc;
+  if (!is_float(out_type)) return SWAMP_EDTYPE;
+  if (!std::isfinite(scale)) return SWAMP_EINVAL;
+  if (int rc = check_rows(q_stride, n_heads, c.cache.dim)) return rc;
+  if (int rc = check_rows(out_stride, n_heads, c.cache.dim)) return rc;
+  if (q_stride % 8 != 0 || out_stride % 8 != 0) return SWAMP_ESHAPE;
+  if (c.max_new == 0 || c.batch.n_seq == 0) return SWAMP_OK;
+  if (!cache_ok(c.cache) || !batch_ok(c.batch) || !d_q || !d_out || !aligned(d_q, 16) ||
+      !aligned(d_out, 16))
+    return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  c.out_type = out_type;
+  c.scale = scale;
+  c.q = d_q;
+  c.out = d_out;
+  c.q_stride = q_stride;
+  c.out_stride = out_stride;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Scratch sc = stream_scratch(s, swamp_attn_scratch_bytes(c));
+  return swamp_launch_attn_paged(c, sc, s);
+}
+
+size_t swamp_attn_paged_workspace(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
+                                  int n_heads, int window) {
+  AttnCall c;
+  if (check_attn(cache, batch, n_heads, window, c) != SWAMP_OK) return 0;
+  if (c.max_new == 0 || c.batch.n_seq == 0) return 0;
+  if (ensure_device(nullptr) != SWAMP_OK) return 0;
+  return swamp_attn_scratch_bytes(c);
 }
 
 void swamp_fused_gemv_q4k(const uint8_t *w_raw, const float *x, float *out, int n_rows,

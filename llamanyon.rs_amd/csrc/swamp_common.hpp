@@ -5,6 +5,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "paging.hpp"
 #include "swamp_qmm.h"
 
 namespace swamp {
@@ -145,8 +146,8 @@ inline Scratch stream_scratch(hipStream_t s, size_t bytes) {
 }  // namespace swamp
 
 // Internal launchers (defined in dequant.hip, gemv.hip, gemv_fused.hip,
-// gemv_tokens.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, producers.hip).  They
-// assume the arguments have been validated by api.cpp.
+// gemv_tokens.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, producers.hip,
+// rope.hip, attn.hip).  They assume the arguments have been validated by api.cpp.
 int swamp_launch_dequant(uint32_t dtype, const void *d_raw, float *d_dst,
                          size_t n, hipStream_t s);
 int swamp_launch_dequant_bf16(uint32_t dtype, const void *d_raw, void *d_dst, size_t n,
@@ -216,3 +217,13 @@ int swamp_launch_quantize_q8_0(const void *d_x, uint32_t x_type, void *d_q,
                                size_t n, hipStream_t s);
 int swamp_launch_i8dot(const int8_t *d_w, const int8_t *d_a, int k,
                        int *d_out, hipStream_t s);
+int swamp_launch_rope(const swamp_rope_spec *r, const int32_t *d_pos, const void *d_x,
+                      uint32_t x_type, int64_t x_stride, void *d_out, uint32_t out_type,
+                      int64_t out_stride, int n_tok, int n_heads, int head_dim, hipStream_t s);
+int swamp_launch_kv_append(const swamp::PagedCache &cache, const swamp::SeqBatch &b, uint32_t dtype,
+                           const swamp_rope_spec *r, const void *d_q, const void *d_k,
+                           const void *d_v, uint32_t x_type, int64_t q_stride, int64_t k_stride,
+                           int64_t v_stride, void *d_q_out, int64_t q_out_stride, int n_heads,
+                           hipStream_t s);
+size_t swamp_attn_scratch_bytes(const swamp::AttnCall &c);
+int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStream_t s);
