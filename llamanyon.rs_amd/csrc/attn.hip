@@ -1,92 +1,120 @@
-// attn.hip -- causal attention of a batch's new tokens over the paged cache
-// (swamp_attn_paged): o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j).
-//
-// One wave takes one row and one query head and walks the keys that the row
-// sees, in order: four dims a lane, the score summed across the wave, the
-// softmax's running maximum m and sum l beside the running output, which is
-// scaled by exp(m_old - m_new) where m grows (one pass over K and V).
-#include "paging.hpp"
-#include "swamp_common.hpp"
+// attn.hip -- swamp_attn_paged: how a call's keys are split over workgroups, and
+// the join of the pieces.  The attention itself is in attn_core.hpp, built per
+// cache type in attn_f16.hip and attn_bf16.hip.
+#include "attn_core.hpp"
+
+#include <algorithm>
+
+int swamp_attn_f16(const swamp_attn::Work &w, bool precise, hipStream_t s);
+int swamp_attn_bf16(const swamp_attn::Work &w, bool precise, hipStream_t s);
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f;
+using namespace swamp_attn;
 
-template <typename CT, typename OT>
-__global__ void __launch_bounds__(256)
-    attn_rows_kernel(swamp::PagedCache cache, swamp::SeqBatch b, const CT *__restrict__ q,
-                     int64_t q_stride, int n_heads, float scale, int window, OT *__restrict__ out,
-                     int64_t out_stride) {
-  const int lane = int(threadIdx.x & 63);
-  const int s = int(blockIdx.y);
-  const int64_t unit = int64_t(blockIdx.x) * 4 + int(threadIdx.x >> 6);
-  const int row = int(unit / n_heads), head = int(unit % n_heads);
-  const swamp::Seq sq = swamp::seq_of(b.first[s], b.first[s + 1], b.len[s], b.n_tok);
-  if (row >= sq.n) return;
-  const int64_t t = sq.t0 + row;
-  const int pos = sq.len - sq.n + row;
-  const swamp::Span keys = swamp::seen_by(pos, window);
-  const int d0 = 4 * lane, kv_head = head / (n_heads / cache.n_kv);
-  float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < 4; j++)
-    qv[j] = d0 < cache.dim ? float(q[t * q_stride + head * cache.dim + d0 + j]) : 0.f;
-  float m = -INFINITY, l = 0.f;
-  bool bad = false;
-  for (int p = keys.lo; p < keys.hi; p++) {
-    const int64_t col = swamp::page_col(p, cache.page_shift);
-    int32_t id = -1;
-    if (swamp::page_col_ok(p, col, b.pages_stride)) id = b.pages[s * b.pages_stride + col];
-    if (!swamp::page_ok(id, cache.n_pages)) {
-      bad = true;
-      break;
-    }
-    const int64_t at = swamp::slot_offset(id, p, kv_head, cache.page_shift, cache.page_stride,
-                                          cache.head_stride, cache.slot_stride);
-    float dot = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (d0 < cache.dim) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        dot += qv[j] * float(reinterpret_cast<const CT *>(cache.k)[at + d0 + j]);
-        v[j] = float(reinterpret_cast<const CT *>(cache.v)[at + d0 + j]);
-      }
-    }
-    const float x = swamp::wave_sum(dot) * scale * kLog2e;
-    const float grown = fmaxf(m, x), base = grown == -INFINITY ? 0.f : grown;
-    const float keep = __builtin_amdgcn_exp2f(m - base), w = __builtin_amdgcn_exp2f(x - base);
-    m = grown;
-    l = l * keep + w;
-#pragma unroll
-    for (int j = 0; j < 4; j++) o[j] = o[j] * keep + w * v[j];
+// out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over a row's pieces, in
+// their order.  A thread takes four dims of a row.
+__global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
+  const int per = w.cache.dim >> 2;
+  const int64_t n = int64_t(w.b.n_tok) * w.n_heads;  // rows of a piece
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t row = i / per;
+  const int d = int(i - row * per) * 4;
+  const int64_t t = row / w.n_heads;
+  if (row >= n || t < w.b.first[0] || t >= w.b.first[w.b.n_seq]) return;  // padding
+  float top = -INFINITY;
+#pragma unroll 8
+  for (int x = 0; x < w.splits; x++) top = fmaxf(top, w.stat[x * n + row][0]);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  bool sees = true;
+#pragma unroll 4
+  for (int x = 0; x < w.splits; x++) {
+    const f32x2 st = w.stat[x * n + row];
+    const float k = __builtin_amdgcn_exp2f(st[0] - base);
+    sees = sees && st[1] != -1.f;
+    sum += k * st[1];
+    if (st[0] != -INFINITY)
+      acc += k * *reinterpret_cast<const f32x4 *>(w.part + (x * n + row) * w.cache.dim + d);
   }
-  if (bad && b.bad && lane == 0) *b.bad = 1;
-  if (d0 < cache.dim) {
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      out[t * out_stride + head * cache.dim + d0 + j] =
-          OT(bad ? __builtin_nanf("") : keys.hi > keys.lo ? o[j] / l : 0.f);
-  }
+  put4(w, t, int(row - t * w.n_heads), w.cache.dim, d,
+       sees ? acc * (1.f / sum) : f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+struct Plan {
+  int blocks, one_block, splits, chunk;
+};
+
+// blocks: at most this many, of all sequences, whatever the rows' distribution.
+Plan plan_of(const swamp::AttnCall &c) {
+  const int group = c.n_heads / c.cache.n_kv;
+  const int64_t rows = int64_t(c.batch.n_tok) * group;
+  const int64_t most = (int64_t(c.max_new) * group + kRows - 1) / kRows;  // of a sequence
+  Plan p;
+  p.one_block = most <= 1;
+  p.blocks = int(p.one_block ? c.batch.n_seq
+                             : std::min((rows + int64_t(kRows - 1) * c.batch.n_seq) / kRows,
+                                        most * c.batch.n_seq));
+  const int slots = swamp::device_info().num_cus * (c.cache.dim <= 128 ? 2 : 1);
+  const int64_t base = int64_t(p.blocks) * c.cache.n_kv;
+  const int64_t keys =
+      c.window ? std::min<int64_t>(c.max_len, int64_t(c.window) + c.max_new) : c.max_len;
+  const bool few = int64_t(c.max_new) * group <= kFew;
+  const int64_t least = few ? 2 * kTile : 4 * kTile;
+  int64_t want = std::max<int64_t>(1, (few ? 2 : 1) * slots / std::max<int64_t>(base, 1));
+  want = std::max<int64_t>(1, std::min<int64_t>(want, keys / least));
+  p.chunk = int((((keys + want - 1) / want + 2 * kTile - 1) / (2 * kTile)) * 2 * kTile);
+  p.chunk = std::max(p.chunk, 2 * kTile);
+  p.splits = int(std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk));
+  return p;
+}
+
+size_t part_bytes(const swamp::AttnCall &c, int splits) {
+  return size_t(splits) * c.batch.n_tok * c.n_heads * c.cache.dim * 4;
+}
+size_t stat_bytes(const swamp::AttnCall &c, int splits) {
+  return size_t(splits) * c.batch.n_tok * c.n_heads * 8;
 }
 
 }  // namespace
 
-size_t swamp_attn_scratch_bytes(const swamp::AttnCall &) { return 0; }
+size_t swamp_attn_scratch_bytes(const swamp::AttnCall &c) {
+  const Plan p = plan_of(c);
+  if (p.splits <= 1) return 0;
+  return swamp::scratch_round(part_bytes(c, p.splits)) +
+         swamp::scratch_round(stat_bytes(c, p.splits));
+}
 
-int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &, hipStream_t s) {
-  const dim3 grid(unsigned((int64_t(c.max_new) * c.n_heads + 3) / 4), unsigned(c.batch.n_seq));
-  auto go = [&](auto ct, auto ot) {
-    typedef decltype(ct) C;
-    typedef decltype(ot) O;
-    attn_rows_kernel<C, O><<<grid, 256, 0, s>>>(c.cache, c.batch, static_cast<const C *>(c.q),
-                                                c.q_stride, c.n_heads, c.scale, c.window,
-                                                static_cast<O *>(c.out), c.out_stride);
-  };
-  auto with_out = [&](auto ct) {
-    if (c.out_type == SWAMP_F32) go(ct, float{});
-    else if (c.out_type == SWAMP_F16) go(ct, _Float16{});
-    else go(ct, __bf16{});
-  };
-  if (c.dtype == SWAMP_F16) with_out(_Float16{});
-  else with_out(__bf16{});
+int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStream_t s) {
+  const Plan p = plan_of(c);
+  Work w;
+  w.cache = c.cache;
+  w.b = c.batch;
+  w.q = static_cast<const uint16_t *>(c.q);
+  w.q_stride = c.q_stride;
+  w.out = c.out;
+  w.out_stride = c.out_stride;
+  w.out_type = c.out_type;
+  w.n_heads = c.n_heads;
+  w.group = c.n_heads / c.cache.n_kv;
+  w.window = c.window;
+  w.scale = c.scale;
+  w.blocks = p.blocks;
+  w.one_block = p.one_block;
+  w.splits = p.splits;
+  w.chunk = p.chunk;
+  w.part = nullptr;
+  w.stat = nullptr;
+  if (p.splits > 1) {
+    w.part = static_cast<float *>(sc.get(part_bytes(c, p.splits)));
+    w.stat = static_cast<f32x2 *>(sc.get(stat_bytes(c, p.splits)));
+    if (!w.part || !w.stat) w.splits = 1;
+  }
+  const bool precise = c.out_type == SWAMP_F32;
+  const int rc = c.dtype == SWAMP_F16 ? swamp_attn_f16(w, precise, s) : swamp_attn_bf16(w, precise, s);
+  if (rc != SWAMP_OK || w.splits == 1) return rc;
+  const int64_t n = int64_t(c.batch.n_tok) * c.n_heads * (c.cache.dim / 4);
+  join_kernel<<<dim3(unsigned((n + kThreads - 1) / kThreads)), kThreads, 0, s>>>(w);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }

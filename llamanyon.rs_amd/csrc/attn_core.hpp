@@ -1,0 +1,858 @@
+// attn_core.hpp -- causal attention of a batch's new tokens over the paged cache
+// (swamp_attn_paged): o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j).
+//
+// Mathematics.  One pass over the keys with the softmax's running maximum m and
+// sum l: a tile's scores s, m' = max(m, c max s) with c = scale log2 e, p =
+// 2^(c s - m'), l and o scaled by 2^(m - m') where m grows by more than kSlack
+// (p then reaches 2^kSlack at most; sums and the last division do not care).
+//
+// Tiles.  The rows of one cache head -- new tokens times the query heads that
+// share it -- are cut into blocks of 128, and a block takes its keys in tiles.
+// Scores are taken as S^T = K Q^T with 32 x 32 x 16 matrix instructions: a lane
+// then holds 16 of 32 keys of ONE row (lane % 32), so that maximum and sum stay
+// within the lane but for one exchange with lane ^ 32, and P^T is already the B
+// operand of O^T = V^T P^T (keys are summed in the order that S^T left them in,
+// V is read in the same order by the transposing LDS read).  Neither P nor the
+// statistics pass through LDS.
+//
+// Feeding.  Keys and values reach LDS by direct-to-LDS DMA, 16 bytes a lane in
+// groups of 16 keys.  A row of dim elements lies at a stride of S 16-byte
+// chunks: dims of 64, 128 and 256 XOR the chunk with the row (K: all rows of a
+// fragment read in different banks; V: the four rows of a transposing read),
+// other dims take an odd stride instead.
+//
+// Rows outside a block's keys are loaded from its nearest key: their weights
+// are 0 and what they hold is finite wherever the keys are.  A weight of 0 times
+// an infinity or NaN that only OTHER rows see would still spoil a row.  So a
+// result that is not finite is computed once more with such values taken out of
+// the tiles and added, row by row, to the rows that see them.
+#pragma once
+#include "paging.hpp"
+#include "swamp_common.hpp"
+
+namespace swamp_attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRows = 128;     // rows of a block
+constexpr int kFew = 32;       // rows up to which a block's waves share the keys instead
+constexpr int kTile = 64;      // keys of a workgroup's tile
+constexpr float kLog2e = 1.44269504088896341f;
+
+struct Work {
+  swamp::PagedCache cache;
+  swamp::SeqBatch b;
+  const uint16_t *q;
+  int64_t q_stride;
+  void *out;
+  int64_t out_stride;
+  uint32_t out_type;
+  int n_heads, group, window;
+  float scale;
+  int blocks;      // blocks of the grid (per head and split)
+  int one_block;   // no sequence has more than one
+  int splits;      // pieces of a sequence's keys
+  int chunk;       // keys of a piece (a multiple of kTile); the last takes the rest
+  float *part;     // [split][row][dim]: sums of a piece, splits > 1
+  f32x2 *stat;     // [split][row]: (m, l); l = -1: the row sees no key at all
+};
+
+// ---- LDS and DMA ----------------------------------------------------------
+// LDS is addressed by byte offset.  Not templates: the host pass rejects the
+// address-space cast inside a template instantiation.
+__device__ __forceinline__ uint32_t lds_base(uint8_t *smem) {
+  return uint32_t(uintptr_t((__attribute__((address_space(3))) uint8_t *)smem));
+}
+__device__ __forceinline__ s16x8 lds16(uint32_t at) {
+  return *(__attribute__((address_space(3))) s16x8 *)(uintptr_t)at;
+}
+__device__ __forceinline__ void lds16_put(uint32_t at, s16x8 v) {
+  *(__attribute__((address_space(3))) s16x8 *)(uintptr_t)at = v;
+}
+__device__ __forceinline__ f32x4 ldsf4(uint32_t at) {
+  return *(__attribute__((address_space(3))) f32x4 *)(uintptr_t)at;
+}
+__device__ __forceinline__ void ldsf4_put(uint32_t at, f32x4 v) {
+  *(__attribute__((address_space(3))) f32x4 *)(uintptr_t)at = v;
+}
+__device__ __forceinline__ float ldsf(uint32_t at) {
+  return *(__attribute__((address_space(3))) float *)(uintptr_t)at;
+}
+__device__ __forceinline__ void ldsf_put(uint32_t at, float v) {
+  *(__attribute__((address_space(3))) float *)(uintptr_t)at = v;
+}
+// Four rows' elements of one column: lane i of 16 names 8 bytes of row i / 4 and
+// gets column i of the 4 x 16 block.
+__device__ __forceinline__ s16x4 lds_tr(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)at);
+}
+
+// 16 bytes a lane into LDS (lane L writes at + 16 L).  Written as assembly
+// because the compiler waits for every DMA in flight before it lets a
+// transposing read pass; these have no output register, and every read of what
+// they bring stands behind a wait of wait_dma or wait_all.  (m0 has no other
+// user in these kernels.)
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const void *uni(const void *p) {
+  const uint64_t x = uint64_t(uintptr_t(p));
+  const uint32_t lo = uint32_t(uni(int(uint32_t(x)))), hi = uint32_t(uni(int(x >> 32)));
+  return reinterpret_cast<const void *>(uintptr_t(uint64_t(hi) << 32 | lo));
+}
+__device__ __forceinline__ void dma_uniform(const void *base, uint32_t off, uint32_t at) {
+#ifdef __HIP_DEVICE_COMPILE__
+  base = uni(base);
+  at = uint32_t(uni(int(at)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(at), "v"(off), "s"(base));
+#endif
+}
+__device__ __forceinline__ void dma_lane(const void *p, uint32_t at) {
+#ifdef __HIP_DEVICE_COMPILE__
+  at = uint32_t(uni(int(at)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(at), "v"(p));
+#endif
+}
+// At most N DMAs (and loads) of this wave in flight; its LDS reads are done.
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+// The same for all waves of the workgroup, and nothing in flight.
+__device__ __forceinline__ void wait_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// ---- element types --------------------------------------------------------
+template <typename CT>
+struct Op;
+template <>
+struct Op<_Float16> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr uint16_t kExp = 0x7C00;
+  static constexpr int kParts = 2;  // 11 bits each
+  // weights as fp16: 2^14 at most, so that what is left of a small weight after
+  // its first 11 bits is no subnormal
+  static constexpr float kLift = 14.f;
+  static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a),
+                                                  __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Op<__bf16> {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr uint16_t kExp = 0x7F80;
+  static constexpr int kParts = 3;  // 8 bits each
+  static constexpr float kLift = 0.f;
+  static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a),
+                                                   __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+
+// Eight weights as kParts operands of the cache's type: the nearest, and, where
+// the output is fp32 (NP > 1), what is left of them, again and again.
+template <typename CT, int NP>
+__device__ __forceinline__ void split_weights(const float *x, s16x8 *f) {
+  typedef typename Op<CT>::v2 v2;
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+  for (int n = 0; n < NP; n++) {
+    u32x4 bits;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const f32x2 two = {r[2 * i], r[2 * i + 1]};
+      const v2 h = __builtin_convertvector(two, v2);
+      bits[i] = __builtin_bit_cast(uint32_t, h);
+      if (n + 1 < NP) {
+        r[2 * i] -= float(h[0]);
+        r[2 * i + 1] -= float(h[1]);
+      }
+    }
+    f[n] = __builtin_bit_cast(s16x8, bits);
+  }
+}
+
+// ---- how the keys lie -----------------------------------------------------
+// D: most dims; exact: dim == D, a power of two.
+template <int D, bool kExact>
+struct Geo {
+  static constexpr int KS = D / 16;  // score steps of 16 dims
+  static constexpr int DB = D / 32;  // output blocks of 32 dims
+  static constexpr int NI = D / 32;  // DMAs of a group of 16 keys (1 KB each)
+  static constexpr uint32_t kGroup = NI * 1024;     // bytes of a group
+  static constexpr uint32_t kBuf = 8 * kGroup;      // K and V of a tile
+  static constexpr uint32_t kSmem = 2 * kBuf;       // and the next tile's
+  static constexpr uint32_t kExtra = 4 * 32 * 2 * 4;  // statistics of the waves
+  int nch, stride;  // 16-byte chunks of a row, and from row to row
+  __device__ __forceinline__ Geo(int dim) {
+    nch = kExact ? D / 8 : dim / 8;
+    stride = kExact ? nch : (nch | 1);
+  }
+  static __device__ __forceinline__ int k_chunk(int r, int c) {
+    return !kExact ? c : D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+  }
+  static __device__ __forceinline__ int v_chunk(int r, int c) {
+    return !kExact ? c : D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2);
+  }
+};
+
+// The keys lo .. hi - 1 of one sequence and cache head, on their way into LDS.
+template <int D, bool kExact>
+struct Feed {
+  typedef Geo<D, kExact> G;
+  const uint8_t *k, *v;     // slot 0 of page 0 of this head
+  const int32_t *table;
+  const void *stand_in;     // read in place of a page that is none
+  int64_t page_bytes, slot_bytes, cols;
+  int n_pages, shift, lo, hi;
+  bool whole;               // groups lie within a page, and offsets in 32 bits
+  bool bad;                 // this lane met a position without a page
+  uint32_t rows;            // row of the group (0..15) of DMA j at bits 4 j
+  uint32_t koff[G::NI], voff[G::NI];
+
+  __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane) {
+    k = reinterpret_cast<const uint8_t *>(w.cache.k + int64_t(head) * w.cache.head_stride);
+    v = reinterpret_cast<const uint8_t *>(w.cache.v + int64_t(head) * w.cache.head_stride);
+    table = w.b.pages + int64_t(s) * w.b.pages_stride;
+    stand_in = w.q;
+    page_bytes = w.cache.page_stride * 2;
+    slot_bytes = w.cache.slot_stride * 2;
+    cols = w.b.pages_stride;
+    n_pages = w.cache.n_pages;
+    shift = w.cache.page_shift;
+    whole = shift >= 4 && slot_bytes < (1 << 26);
+    bad = false;
+    rows = 0;
+#pragma unroll
+    for (int j = 0; j < G::NI; j++) {
+      const int i = 64 * j + lane, r = min(i / g.stride, 15), c = min(i - r * g.stride, g.nch - 1);
+      const uint32_t row = whole ? uint32_t(r) * uint32_t(slot_bytes) : 0;
+      rows |= uint32_t(r) << (4 * j);
+      koff[j] = row + 16 * G::k_chunk(r, c);
+      voff[j] = row + 16 * G::v_chunk(r, c);
+    }
+  }
+  // Page of the group at p0, for issue(): uniform.
+  __device__ __forceinline__ int page_of(int p0) const {
+    if (!whole) return 0;
+    const int p = min(max(p0, lo), hi - 1);
+    const int64_t col = swamp::page_col(p, shift);
+    if (!swamp::page_col_ok(p, col, cols)) return -1;
+    return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + uni(int(col)));
+  }
+  // DMAs of the 16 keys from p0 (a multiple of 16) to LDS: kK, kV say what.
+  template <bool kK, bool kV>
+  __device__ __forceinline__ void issue(int p0, int id, uint32_t at_k, uint32_t at_v) {
+    if (whole) {
+      const int first = min(max(p0, lo), hi - 1) & ~15;
+      const bool ok = swamp::page_ok(id, n_pages);
+      const int64_t at = int64_t(id) * page_bytes + (first & ((1 << shift) - 1)) * slot_bytes;
+      const void *kb = ok ? k + at : stand_in, *vb = ok ? v + at : stand_in;
+      bad |= !ok;
+      if (!ok || p0 < lo || p0 + 15 >= hi) {
+#pragma unroll
+        for (int j = 0; j < G::NI; j++) {
+          const int r = (rows >> (4 * j)) & 15, to = min(max(p0 + r, lo), hi - 1) - first;
+          const uint32_t move = ok ? uint32_t(to - r) * uint32_t(slot_bytes)
+                                   : uint32_t(-r) * uint32_t(slot_bytes);
+          if (kK) dma_uniform(kb, koff[j] + move, at_k + 1024 * j);
+          if (kV) dma_uniform(vb, voff[j] + move, at_v + 1024 * j);
+        }
+        return;
+      }
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) {
+        if (kK) dma_uniform(kb, koff[j], at_k + 1024 * j);
+        if (kV) dma_uniform(vb, voff[j], at_v + 1024 * j);
+      }
+      return;
+    }
+    int32_t ids[G::NI];
+#pragma unroll
+    for (int j = 0; j < G::NI; j++) {
+      const int p = min(max(p0 + int((rows >> (4 * j)) & 15), lo), hi - 1);
+      const int64_t col = swamp::page_col(p, shift);
+      ids[j] = swamp::page_col_ok(p, col, cols) ? table[col] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < G::NI; j++) {
+      const int p = min(max(p0 + int((rows >> (4 * j)) & 15), lo), hi - 1);
+      const bool ok = swamp::page_ok(ids[j], n_pages);
+      const int64_t at = int64_t(ids[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
+      const uint8_t *none = static_cast<const uint8_t *>(stand_in);
+      bad |= !ok;
+      if (kK) dma_lane((ok ? k + at : none) + koff[j], at_k + 1024 * j);
+      if (kV) dma_lane((ok ? v + at : none) + voff[j], at_v + 1024 * j);
+    }
+  }
+};
+
+// ---- one wave's 32 rows ---------------------------------------------------
+template <typename CT, int D, bool kExact, int NP>
+struct Rows {
+  typedef Geo<D, kExact> G;
+  typedef Op<CT> O;
+  static constexpr float kLift = NP > 1 ? O::kLift : 0.f;
+  // growth of the maximum that is left to the weights (fp16 parts have no room
+  // above kLift)
+  static constexpr float kSlack = NP > 1 && O::kLift > 0.f ? 0.f : 8.f;
+
+  s16x8 q[G::KS];
+  f32x16 o[G::DB];
+  float m, l, c;
+  int lo, hi;  // keys that this lane's row sees
+  uint32_t k_at[kExact ? G::KS : 1], v_at[kExact ? G::DB : 1];
+
+  __device__ __forceinline__ void addresses(const G &g, int lane) {
+    const int r = lane & 15, half = lane >> 5;
+    const uint32_t group = ((lane >> 4) & 1) * G::kGroup;
+    const int vr = 4 * half + ((lane & 15) >> 2);
+    const int vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vb = (lane & 1) * 8;
+    if constexpr (kExact) {
+#pragma unroll
+      for (int ks = 0; ks < G::KS; ks++)
+        k_at[ks] = group + 16 * (r * g.stride + G::k_chunk(r, 2 * ks + half));
+#pragma unroll
+      for (int db = 0; db < G::DB; db++)
+        v_at[db] = 16 * (vr * g.stride + G::v_chunk(vr, 4 * db + vc)) + vb;
+    } else {
+      k_at[0] = group + 16 * (r * g.stride + half);
+      v_at[0] = 16 * (vr * g.stride + vc) + vb;
+    }
+  }
+  __device__ __forceinline__ uint32_t k_addr(int ks) const {
+    return kExact ? k_at[ks] : k_at[0] + 32 * ks;
+  }
+  // rows vr and vr + 8 of a group share their swizzle
+  __device__ __forceinline__ uint32_t v_addr(int db) const {
+    return kExact ? v_at[db] : v_at[0] + 64 * db;
+  }
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[db][i] = 0.f;
+  }
+
+  // q's row as B operand; a negative scale goes into its signs.
+  __device__ __forceinline__ void load_q(const G &g, const uint16_t *row, float scale, int lane) {
+    c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);  // 0 would make NaN of a hidden key's -inf
+    const short sign = scale < 0.f ? short(0x8000) : short(0);
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ks++) {
+      const int ch = 2 * ks + (lane >> 5);
+      s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (ch < g.nch) {
+        x = *reinterpret_cast<const s16x8 *>(row + 8 * ch);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] ^= sign;
+      }
+      q[ks] = x;
+    }
+  }
+
+  // Scores of KB x 32 keys in LDS at k.
+  template <int KB>
+  __device__ __forceinline__ void scores(const G &g, uint32_t k, f32x16 *s, int lane) const {
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[kb][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ks++) {
+      if (!kExact && 2 * ks >= g.nch) break;
+#pragma unroll
+      for (int kb = 0; kb < KB; kb++) {
+        s16x8 a = lds16(k + k_addr(ks) + kb * 2 * G::kGroup);
+        // past an odd number of chunks lies the next row, which may hold NaN
+        if (!kExact && 2 * ks + 1 >= g.nch && lane >= 32) a = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        s[kb] = O::mma(a, q[ks], s[kb]);
+      }
+    }
+  }
+
+  // The weights of KB x 32 keys from position p on, in place; m, l and o follow.
+  template <int KB>
+  __device__ __forceinline__ void weights(f32x16 *s, int p, bool masked, int lane) {
+    if (masked) {
+      const int p0 = p + 4 * (lane >> 5);
+#pragma unroll
+      for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int key = p0 + 32 * kb + 8 * (i >> 2) + (i & 3);
+          if (key < lo || key >= hi) s[kb][i] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
+                                                       false, false);
+    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
+    if (__any(top > m + kSlack)) {
+      const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown;
+      const float keep = __builtin_amdgcn_exp2f(m - base);
+      m = grown;
+      l *= keep;
+#pragma unroll
+      for (int db = 0; db < G::DB; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[db][i] *= keep;
+    }
+    const float base = (m == -INFINITY ? 0.f : m) - kLift;
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
+        l += s[kb][i];
+      }
+  }
+
+  // o += V^T P^T over KB x 32 keys in LDS at v.
+  template <int KB>
+  __device__ __forceinline__ void gather(const G &g, uint32_t v, const f32x16 *s) {
+#pragma unroll
+    for (int kg = 0; kg < 2 * KB; kg++) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = s[kg >> 1][8 * (kg & 1) + i];
+      s16x8 p[NP];
+      split_weights<CT, NP>(x, p);
+      const uint32_t at = v + kg * G::kGroup;
+#pragma unroll
+      for (int db = 0; db < G::DB; db++) {
+        if (!kExact && 4 * db >= g.nch) break;
+        const s16x4 a = lds_tr(at + v_addr(db)), b = lds_tr(at + v_addr(db) + 128 * g.stride);
+        const s16x8 vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int n = 0; n < NP; n++) o[db] = O::mma(vf, p[n], o[db]);
+      }
+    }
+  }
+
+  // The values that are not finite among the 16 keys of the group in LDS at v:
+  // whether there are any (uniform).
+  __device__ __forceinline__ bool odd_values(const G &g, uint32_t v, int lane) const {
+    bool odd = false;
+    for (int i = lane; i < 16 * g.stride; i += 64) {
+      if (!kExact && i % g.stride >= g.nch) continue;
+      const s16x8 x = lds16(v + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 8; j++) odd |= (uint16_t(x[j]) & O::kExp) == O::kExp;
+    }
+    return __any(odd);
+  }
+  // Adds them to the rows that see them; p: position of the group's first key.
+  __device__ __forceinline__ void add_odd_values(const G &g, uint32_t v, int p, int lane) {
+    for (int r = 0; r < 16; r++) {
+      if (p + r < lo || p + r >= hi) continue;
+#pragma unroll
+      for (int db = 0; db < G::DB; db++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int d = 32 * db + 8 * i + 4 * (lane >> 5);
+          if (d >= 8 * g.nch) continue;
+          const uint32_t at = v + 16 * (r * g.stride + G::v_chunk(r, d >> 3)) + 2 * (d & 7);
+          const s16x4 x = *(__attribute__((address_space(3))) s16x4 *)(uintptr_t)at;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const short e = x[j];  // (a bit cast of x[j] itself takes element 0)
+            if ((uint16_t(e) & O::kExp) == O::kExp)
+              o[db][4 * i + j] += float(__builtin_bit_cast(CT, e));
+          }
+        }
+      }
+    }
+  }
+  // ... and puts 0 in their place.
+  __device__ __forceinline__ void clear_odd_values(const G &g, uint32_t v, int lane) const {
+    for (int i = lane; i < 16 * g.stride; i += 64) {
+      s16x8 x = lds16(v + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if ((uint16_t(x[j]) & O::kExp) == O::kExp) x[j] = 0;
+      lds16_put(v + 16 * i, x);
+    }
+  }
+
+  // An infinity or NaN among the sums of a row (dims below dim).
+  __device__ __forceinline__ bool not_finite(const G &g, int lane) const {
+    float z = 0.f;
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int d = 32 * db + 8 * (i >> 2) + 4 * (lane >> 5);
+        if (kExact || d < 8 * g.nch) z = __builtin_fmaf(o[db][i], 0.f, z);
+      }
+    return z != 0.f;
+  }
+  // l of both halves.
+  __device__ __forceinline__ float sum() const {
+    const auto both =
+        __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  }
+};
+
+__device__ __forceinline__ void put4(const Work &w, int64_t row, int head, int dim, int d, f32x4 x) {
+  const int64_t at = row * w.out_stride + int64_t(head) * dim + d;
+  if (w.out_type == SWAMP_F32) {
+    *reinterpret_cast<f32x4 *>(static_cast<float *>(w.out) + at) = x;
+  } else if (w.out_type == SWAMP_F16) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<h4 *>(static_cast<_Float16 *>(w.out) + at) = __builtin_convertvector(x, h4);
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<b4 *>(static_cast<__bf16 *>(w.out) + at) = __builtin_convertvector(x, b4);
+  }
+}
+
+// Sequence and block of the unit `at`: sequences 64 at a time, a lane each.
+__device__ __forceinline__ bool find_block(const Work &w, int at, int &s, int &blk, int lane) {
+  if (w.one_block) {
+    s = at;
+    blk = 0;
+    return s < w.b.n_seq;
+  }
+  for (int s0 = 0; s0 < w.b.n_seq; s0 += 64) {
+    int n = 0;
+    if (s0 + lane < w.b.n_seq) {
+      const swamp::Seq q = swamp::seq_of(w.b.first[s0 + lane], w.b.first[s0 + lane + 1], 0, w.b.n_tok);
+      n = int((int64_t(q.n) * w.group + kRows - 1) / kRows);
+    }
+    int upto = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += x;
+    }
+    const uint64_t past = __ballot(upto > at);
+    if (past) {
+      const int who = __builtin_ctzll(past);
+      s = s0 + who;
+      blk = at - (__shfl(upto, who, 64) - __shfl(n, who, 64));
+      return true;
+    }
+    at -= __shfl(upto, 63, 64);
+  }
+  return false;
+}
+
+// ---- the kernel -----------------------------------------------------------
+template <typename CT, int D, bool kExact, int NP>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_kernel(Work w) {
+  typedef Geo<D, kExact> G;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = uni(tid >> 6);
+  const uint32_t lds = lds_base(smem), extra = lds + G::kSmem;
+  const G g(w.cache.dim);
+  const int dim = kExact ? D : w.cache.dim;
+
+  // heads first: eight heads' workgroups keep to one XCD each, whose L2 then
+  // holds one head's keys; late blocks, which see the most keys, go first
+  const int n_kv = w.cache.n_kv;
+  const int head = int(blockIdx.x) % n_kv, unit = int(blockIdx.x) / n_kv;
+  const int split = unit % w.splits;
+  int s, blk;
+  if (!find_block(w, w.blocks - 1 - unit / w.splits, s, blk, lane)) return;
+  s = uni(s);
+  blk = uni(blk);
+  const swamp::Seq sq = swamp::seq_of(w.b.first[s], w.b.first[s + 1], w.b.len[s], w.b.n_tok);
+  const int64_t n_rows = int64_t(sq.n) * w.group;
+  const int64_t r0 = int64_t(blk) * kRows;
+  if (r0 >= n_rows) return;
+  const int rows = int(min(n_rows - r0, int64_t(kRows)));
+  const bool few = n_rows <= kFew;
+
+  // keys of the block, and of this piece of them
+  const int before = sq.len - sq.n;  // position of the first new token
+  const swamp::Span ka = swamp::seen_by(before + int(r0 / w.group), w.window);
+  const swamp::Span kz = swamp::seen_by(before + int((r0 + rows - 1) / w.group), w.window);
+  // (positions that the page table cannot hold are not walked; nor are the last
+  // below 2^31, so that a tile's end fits)
+  const int64_t room = min(w.b.pages_stride << w.cache.page_shift, (int64_t(1) << 31) - 512);
+  const int last = int(min(int64_t(kz.hi), room));
+  const int64_t from = (ka.lo & ~(kTile - 1)) + int64_t(split) * w.chunk;
+  const int begin = int(min(max(int64_t(ka.lo), from), int64_t(last)));
+  const int end = split == w.splits - 1 ? last : int(min(from + w.chunk, int64_t(last)));
+  const int tile0 = begin & ~(kTile - 1);
+  const int stop = end > begin ? end : tile0;  // of the tiles
+  if (w.splits > 1 && stop == tile0 && kz.hi <= room) {  // a piece without keys
+    for (int i = tid; i < rows; i += kThreads) {
+      const int64_t r = r0 + i, t = sq.t0 + r / w.group;
+      const swamp::Span seen = swamp::seen_by(before + int(r / w.group), w.window);
+      w.stat[(int64_t(split) * w.b.n_tok + t) * w.n_heads + head * w.group + int(r % w.group)] =
+          f32x2{-INFINITY, seen.hi > seen.lo ? 0.f : -1.f};
+    }
+    return;
+  }
+
+  // this lane's row
+  const int n = few ? (lane & 31) : 32 * wave + (lane & 31);
+  const int64_t rr = r0 + min(n, rows - 1);
+  const int tok = int(rr / w.group), hq = head * w.group + int(rr % w.group);
+  const int64_t t = int64_t(sq.t0) + tok;
+  const swamp::Span mine = swamp::seen_by(before + tok, w.window);
+  const bool store = n < rows;
+
+  Rows<CT, D, kExact, NP> a;
+  a.addresses(g, lane);
+  a.load_q(g, w.q + t * w.q_stride + int64_t(hq) * dim, w.scale, lane);
+  a.lo = mine.lo;
+  a.hi = mine.hi;
+  Feed<D, kExact> f;
+  f.init(w, g, s, head, lane);
+  f.bad = kz.hi > room;
+  f.lo = begin;
+  f.hi = end;
+  const int n_tiles = (stop - tile0 + kTile - 1) / kTile;
+  // which keys all rows of the wave see, and any
+  const int w0 = few ? 0 : min(32 * wave, rows - 1), w1 = few ? rows - 1 : min(32 * wave + 31, rows - 1);
+  const swamp::Span wa = swamp::seen_by(before + int((r0 + w0) / w.group), w.window);
+  const swamp::Span wz = swamp::seen_by(before + int((r0 + w1) / w.group), w.window);
+  const int any_lo = max(wa.lo, begin), any_hi = min(wz.hi, end);
+  const int all_lo = max(wz.lo, begin), all_hi = min(wa.hi, end);
+  // the row's own keys within this piece
+  a.lo = max(a.lo, begin);
+  a.hi = min(a.hi, end);
+
+  a.clear();
+  bool bad = false;
+  if (few) {
+    // Four waves, each with its own 32-key tiles and its own quarter of LDS:
+    // K (2 groups), then V.  No barrier: a wave waits for its own DMAs only.
+    const uint32_t at_k = lds + wave * (G::kSmem / kWaves), at_v = at_k + 2 * G::kGroup;
+    for (int safe = 0; safe < 2; safe++) {
+      int p = tile0 + 32 * wave;
+      int id0 = 0, id1 = 0;
+      if (p < stop) {
+        id0 = f.page_of(p);
+        id1 = f.page_of(p + 16);
+        f.template issue<true, false>(p, id0, at_k, 0);
+        f.template issue<true, false>(p + 16, id1, at_k + G::kGroup, 0);
+        f.template issue<false, true>(p, id0, 0, at_v);
+        f.template issue<false, true>(p + 16, id1, 0, at_v + G::kGroup);
+      }
+      while (p < stop) {
+        const int next = p + 32 * kWaves;
+        if (next < stop) {
+          id0 = f.page_of(next);
+          id1 = f.page_of(next + 16);
+        }
+        f32x16 sc[1];
+        wait_dma<2 * G::NI>();
+        a.template scores<1>(g, at_k, sc, lane);
+        lds_done();
+        if (next < stop) {
+          f.template issue<true, false>(next, id0, at_k, 0);
+          f.template issue<true, false>(next + 16, id1, at_k + G::kGroup, 0);
+        }
+        a.template weights<1>(sc, p, p < all_lo || p + 32 > all_hi, lane);
+        if (next < stop) wait_dma<2 * G::NI>();
+        else wait_dma<0>();
+        if (safe) {
+          for (int i = 0; i < 2; i++)
+            if (a.odd_values(g, at_v + i * G::kGroup, lane)) {
+              a.add_odd_values(g, at_v + i * G::kGroup, p + 16 * i, lane);
+              lds_done();
+              a.clear_odd_values(g, at_v + i * G::kGroup, lane);
+              lds_done();
+            }
+        }
+        a.template gather<1>(g, at_v, sc);
+        lds_done();
+        if (next < stop) {
+          f.template issue<false, true>(next, id0, 0, at_v);
+          f.template issue<false, true>(next + 16, id1, 0, at_v + G::kGroup);
+        }
+        p = next;
+      }
+      bad = __any(f.bad);
+      if (bad || safe || !__any(a.not_finite(g, lane))) break;
+      a.clear();
+    }
+
+    // the waves' sums meet in LDS, rows of dim floats (16-byte chunks swizzled
+    // by the row where there are enough of them)
+    const float l = bad ? __builtin_nanf("") : a.sum();
+    const uint32_t flip = dim % 32 == 0 ? 7 : 0;
+    wait_all();
+    {
+      const uint32_t mine_at = lds + wave * (G::kSmem / kWaves);
+      const int r = lane & 31;
+      if (lane < 32) {
+        ldsf_put(extra + 8 * (32 * wave + r), a.m);
+        ldsf_put(extra + 8 * (32 * wave + r) + 4, l);
+      }
+      if (r < rows) {
+#pragma unroll
+        for (int db = 0; db < G::DB; db++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int d = 32 * db + 8 * i + 4 * (lane >> 5);
+            if (d < dim)
+              ldsf4_put(mine_at + 4 * r * dim + 16 * ((d >> 2) ^ (r & flip)),
+                        f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2],
+                              a.o[db][4 * i + 3]});
+          }
+      }
+    }
+    __syncthreads();
+    const int per = dim >> 2;
+    for (int i = tid; i < rows * per; i += kThreads) {
+      const int r = i / per, d = 4 * (i - r * per);
+      float mw[kWaves], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWaves; x++) {
+        mw[x] = ldsf(extra + 8 * (32 * x + r));
+        top = fmaxf(top, mw[x]);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < kWaves; x++) {
+        const float k = __builtin_amdgcn_exp2f(mw[x] - base);
+        sum += k * ldsf(extra + 8 * (32 * x + r) + 4);
+        // a wave without keys of this row may have summed others' infinities
+        if (mw[x] != -INFINITY)
+          acc += k * ldsf4(lds + x * (G::kSmem / kWaves) + 4 * r * dim +
+                           16 * ((d >> 2) ^ (r & flip)));
+      }
+      const int64_t row = sq.t0 + r / w.group;
+      const int h = head * w.group + r % w.group;
+      const swamp::Span seen = swamp::seen_by(before + r / w.group, w.window);
+      const bool sees = seen.hi > seen.lo;
+      if (w.splits == 1) {
+        const float inv = 1.f / sum;
+        put4(w, row, h, dim, d, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+      } else {
+        const int64_t pr = (int64_t(split) * w.b.n_tok + row) * w.n_heads + h;
+        *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) = acc;
+        if (d == 0) w.stat[pr] = f32x2{top, sees ? sum : -1.f};
+      }
+    }
+    if (bad && w.b.bad && lane == 0) *w.b.bad = 1;
+    return;
+  }
+
+  // Rows of their own for every wave; the tile of 64 keys is shared, a wave
+  // brings in one group of 16 of it.  Two buffers (K: 4 groups, V: 4 groups).
+  for (int safe = 0; safe < 2; safe++) {
+    const int mine_at = 16 * wave;
+    int id = 0;
+    if (n_tiles > 0) {
+      id = f.page_of(tile0 + mine_at);
+      f.template issue<true, true>(tile0 + mine_at, id, lds + wave * G::kGroup,
+                                   lds + (4 + wave) * G::kGroup);
+      id = f.page_of(tile0 + kTile + mine_at);
+    }
+    for (int i = 0; i < n_tiles; i++) {
+      const uint32_t buf = lds + (i & 1) * G::kBuf, other = lds + (~i & 1) * G::kBuf;
+      const int p = tile0 + kTile * i;
+      wait_all();
+      if (i + 1 < n_tiles) {
+        f.template issue<true, true>(p + kTile + mine_at, id, other + wave * G::kGroup,
+                                     other + (4 + wave) * G::kGroup);
+        id = f.page_of(p + 2 * kTile + mine_at);
+      }
+      const bool work = p < any_hi && p + kTile > any_lo;
+      f32x16 sc[2];
+      if (work) {
+        a.template scores<2>(g, buf, sc, lane);
+        a.template weights<2>(sc, p, p < all_lo || p + kTile > all_hi, lane);
+      }
+      if (safe) {
+        const uint32_t v = buf + (4 + wave) * G::kGroup;
+        if (__syncthreads_or(a.odd_values(g, v, lane))) {
+          for (int j = 0; j < 4; j++)
+            a.add_odd_values(g, buf + (4 + j) * G::kGroup, p + 16 * j, lane);
+          __syncthreads();
+          a.clear_odd_values(g, v, lane);
+          __syncthreads();
+        }
+      }
+      if (work) a.template gather<2>(g, buf + 4 * G::kGroup, sc);
+    }
+    bad = __syncthreads_or(f.bad);
+    if (bad || safe || !__syncthreads_or(store && a.not_finite(g, lane))) break;
+    a.clear();
+  }
+  const float l = bad ? __builtin_nanf("") : a.sum();
+  if (bad && w.b.bad && tid == 0) *w.b.bad = 1;
+  if (!store) return;
+  const bool sees = mine.hi > mine.lo;
+  if (w.splits == 1) {
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = 32 * db + 8 * i + 4 * (lane >> 5);
+        if (kExact || d < dim)
+          put4(w, t, hq, dim, d,
+               sees ? f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2],
+                            a.o[db][4 * i + 3]} *
+                          inv
+                    : f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+    return;
+  }
+  const int64_t pr = (int64_t(split) * w.b.n_tok + t) * w.n_heads + hq;
+  if (lane < 32) w.stat[pr] = f32x2{a.m, sees ? l : -1.f};
+#pragma unroll
+  for (int db = 0; db < G::DB; db++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int d = 32 * db + 8 * i + 4 * (lane >> 5);
+      if (kExact || d < dim)
+        *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) =
+            f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2], a.o[db][4 * i + 3]};
+    }
+}
+
+template <typename CT, int D, bool kExact>
+int launch(const Work &w, bool precise, hipStream_t s) {
+  typedef Geo<D, kExact> G;
+  const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));
+  const uint32_t smem = G::kSmem + G::kExtra;
+  if (precise) attn_kernel<CT, D, kExact, Op<CT>::kParts><<<grid, kThreads, smem, s>>>(w);
+  else attn_kernel<CT, D, kExact, 1><<<grid, kThreads, smem, s>>>(w);
+  return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
+}
+
+template <typename CT>
+int launch_dim(const Work &w, bool precise, hipStream_t s) {
+  switch (w.cache.dim) {
+    case 64: return launch<CT, 64, true>(w, precise, s);
+    case 128: return launch<CT, 128, true>(w, precise, s);
+    case 256: return launch<CT, 256, true>(w, precise, s);
+  }
+  return w.cache.dim < 128 ? launch<CT, 128, false>(w, precise, s)
+                           : launch<CT, 256, false>(w, precise, s);
+}
+
+}  // namespace swamp_attn
