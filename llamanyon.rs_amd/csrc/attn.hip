@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
 }
 
 struct Plan {
-  int blocks, one_block, splits, chunk;
+  int blocks, one_block, few, splits, chunk;
 };
 
 // blocks: at most this many, of all sequences, whatever the rows' distribution.
@@ -56,13 +56,13 @@ Plan plan_of(const swamp::AttnCall &c) {
   p.blocks = int(p.one_block ? c.batch.n_seq
                              : std::min((rows + int64_t(kRows - 1) * c.batch.n_seq) / kRows,
                                         most * c.batch.n_seq));
+  p.few = int64_t(c.max_new) * group <= kFew;
   const int slots = swamp::device_info().num_cus * (c.cache.dim <= 128 ? 2 : 1);
   const int64_t base = int64_t(p.blocks) * c.cache.n_kv;
   const int64_t keys =
       c.window ? std::min<int64_t>(c.max_len, int64_t(c.window) + c.max_new) : c.max_len;
-  const bool few = int64_t(c.max_new) * group <= kFew;
-  const int64_t least = few ? 2 * kTile : 4 * kTile;
-  int64_t want = std::max<int64_t>(1, (few ? 2 : 1) * slots / std::max<int64_t>(base, 1));
+  const int64_t least = p.few ? 2 * kTile : 4 * kTile;
+  int64_t want = std::max<int64_t>(1, (p.few ? 2 : 1) * slots / std::max<int64_t>(base, 1));
   want = std::max<int64_t>(1, std::min<int64_t>(want, keys / least));
   p.chunk = int((((keys + want - 1) / want + 2 * kTile - 1) / (2 * kTile)) * 2 * kTile);
   p.chunk = std::max(p.chunk, 2 * kTile);
@@ -102,6 +102,7 @@ int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStr
   w.scale = c.scale;
   w.blocks = p.blocks;
   w.one_block = p.one_block;
+  w.few = p.few;
   w.splits = p.splits;
   w.chunk = p.chunk;
   w.part = nullptr;

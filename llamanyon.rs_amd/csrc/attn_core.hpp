@@ -19,7 +19,7 @@
 // groups of 16 keys.  A row of dim elements lies at a stride of S 16-byte
 // chunks: dims of 64, 128 and 256 XOR the chunk with the row (K: all rows of a
 // fragment read in different banks; V: the four rows of a transposing read),
-// other dims take an odd stride instead.
+// other dims take an odd stride of chunks instead.
 //
 // Rows outside a block's keys are loaded from its nearest key: their weights
 // are 0 and what they hold is finite wherever the keys are.  A weight of 0 times
@@ -42,7 +42,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRows = 128;     // rows of a block
-constexpr int kFew = 32;       // rows up to which a block's waves share the keys instead
+constexpr int kFew = 32;       // rows up to which a block's waves share the rows instead
 constexpr int kTile = 64;      // keys of a workgroup's tile
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -58,6 +58,7 @@ struct Work {
   float scale;
   int blocks;      // blocks of the grid (per head and split)
   int one_block;   // no sequence has more than one
+  int few;         // no sequence has more than kFew rows
   int splits;      // pieces of a sequence's keys
   int chunk;       // keys of a piece (a multiple of kTile); the last takes the rest
   float *part;     // [split][row][dim]: sums of a piece, splits > 1
@@ -70,8 +71,12 @@ struct Work {
 __device__ __forceinline__ uint32_t lds_base(uint8_t *smem) {
   return uint32_t(uintptr_t((__attribute__((address_space(3))) uint8_t *)smem));
 }
-__device__ __forceinline__ s16x8 lds16(uint32_t at) {
-  return *(__attribute__((address_space(3))) s16x8 *)(uintptr_t)at;
+// at + off, off a constant: the sum stays in the instruction's offset.
+#define SWAMP_LDS(T, at, off)                                          \
+  ((__attribute__((address_space(3))) T *)((__attribute__((            \
+       address_space(3))) uint8_t *)(uintptr_t)(at) + (off)))
+__device__ __forceinline__ s16x8 lds16(uint32_t at, uint32_t off = 0) {
+  return *SWAMP_LDS(s16x8, at, off);
 }
 __device__ __forceinline__ void lds16_put(uint32_t at, s16x8 v) {
   *(__attribute__((address_space(3))) s16x8 *)(uintptr_t)at = v;
@@ -90,8 +95,8 @@ __device__ __forceinline__ void ldsf_put(uint32_t at, float v) {
 }
 // Four rows' elements of one column: lane i of 16 names 8 bytes of row i / 4 and
 // gets column i of the 4 x 16 block.
-__device__ __forceinline__ s16x4 lds_tr(uint32_t at) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)at);
+__device__ __forceinline__ s16x4 lds_tr(uint32_t at, uint32_t off) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(SWAMP_LDS(s16x4, at, off));
 }
 
 // 16 bytes a lane into LDS (lane L writes at + 16 L).  Written as assembly
@@ -133,6 +138,28 @@ __device__ __forceinline__ void wait_all() {
 }
 __device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// x, which the compiler no longer knows: what rare paths compute from it is not
+// computed ahead of the loop and kept in registers meanwhile.
+template <typename T>
+__device__ __forceinline__ T fresh(T x) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
+
+// Whether x holds anywhere in the workgroup; 4 bytes a wave of LDS at `at`.
+__device__ __forceinline__ bool anywhere(bool x, uint32_t at) {
+  const uint32_t mine = __any(x) ? 1u : 0u;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) ldsf_put(at + (threadIdx.x >> 6) * 4, __uint_as_float(mine));
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) all |= __float_as_uint(ldsf(at + 4 * i));
+  return uni(int(all)) != 0;
+}
+
 // ---- element types --------------------------------------------------------
 template <typename CT>
 struct Op;
@@ -141,6 +168,7 @@ struct Op<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint16_t kExp = 0x7C00;
+  static constexpr float kMax = 65504.f;
   static constexpr int kParts = 2;  // 11 bits each
   // weights as fp16: 2^14 at most, so that what is left of a small weight after
   // its first 11 bits is no subnormal
@@ -155,6 +183,7 @@ struct Op<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint16_t kExp = 0x7F80;
+  static constexpr float kMax = 3.38953139e38f;
   static constexpr int kParts = 3;  // 8 bits each
   static constexpr float kLift = 0.f;
   static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
@@ -163,38 +192,15 @@ struct Op<__bf16> {
   }
 };
 
-// Eight weights as kParts operands of the cache's type: the nearest, and, where
-// the output is fp32 (NP > 1), what is left of them, again and again.
-template <typename CT, int NP>
-__device__ __forceinline__ void split_weights(const float *x, s16x8 *f) {
-  typedef typename Op<CT>::v2 v2;
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = x[i];
-#pragma unroll
-  for (int n = 0; n < NP; n++) {
-    u32x4 bits;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const f32x2 two = {r[2 * i], r[2 * i + 1]};
-      const v2 h = __builtin_convertvector(two, v2);
-      bits[i] = __builtin_bit_cast(uint32_t, h);
-      if (n + 1 < NP) {
-        r[2 * i] -= float(h[0]);
-        r[2 * i + 1] -= float(h[1]);
-      }
-    }
-    f[n] = __builtin_bit_cast(s16x8, bits);
-  }
-}
-
 // ---- how the keys lie -----------------------------------------------------
-// D: most dims; exact: dim == D, a power of two.
+// D: the head's dims, or (not exact) the most of them.
 template <int D, bool kExact>
 struct Geo {
-  static constexpr int KS = D / 16;  // score steps of 16 dims
-  static constexpr int DB = D / 32;  // output blocks of 32 dims
-  static constexpr int NI = D / 32;  // DMAs of a group of 16 keys (1 KB each)
+  static constexpr bool kPow2 = kExact && (D & (D - 1)) == 0;
+  static constexpr int KS = (D + 15) / 16;  // score steps of 16 dims
+  static constexpr int DB = (D + 31) / 32;  // output blocks of 32 dims
+  static constexpr int kStride = kPow2 ? D / 8 : kExact ? (D / 8) | 1 : D / 8 - 1;
+  static constexpr int NI = (kStride + 3) / 4;      // DMAs of a group of 16 keys (1 KB each)
   static constexpr uint32_t kGroup = NI * 1024;     // bytes of a group
   static constexpr uint32_t kBuf = 8 * kGroup;      // K and V of a tile
   static constexpr uint32_t kSmem = 2 * kBuf;       // and the next tile's
@@ -202,13 +208,14 @@ struct Geo {
   int nch, stride;  // 16-byte chunks of a row, and from row to row
   __device__ __forceinline__ Geo(int dim) {
     nch = kExact ? D / 8 : dim / 8;
-    stride = kExact ? nch : (nch | 1);
+    stride = kExact ? kStride : (nch | 1);
   }
+  __device__ __forceinline__ bool within(int d) const { return kPow2 || d < 8 * nch; }
   static __device__ __forceinline__ int k_chunk(int r, int c) {
-    return !kExact ? c : D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+    return !kPow2 ? c : D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
   }
   static __device__ __forceinline__ int v_chunk(int r, int c) {
-    return !kExact ? c : D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2);
+    return !kPow2 ? c : D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2);
   }
 };
 
@@ -266,6 +273,7 @@ struct Feed {
       const void *kb = ok ? k + at : stand_in, *vb = ok ? v + at : stand_in;
       bad |= !ok;
       if (!ok || p0 < lo || p0 + 15 >= hi) {
+        const uint32_t rows = fresh(this->rows);
 #pragma unroll
         for (int j = 0; j < G::NI; j++) {
           const int r = (rows >> (4 * j)) & 15, to = min(max(p0 + r, lo), hi - 1) - first;
@@ -283,6 +291,7 @@ struct Feed {
       }
       return;
     }
+    const uint32_t rows = fresh(this->rows);
     int32_t ids[G::NI];
 #pragma unroll
     for (int j = 0; j < G::NI; j++) {
@@ -317,31 +326,27 @@ struct Rows {
   f32x16 o[G::DB];
   float m, l, c;
   int lo, hi;  // keys that this lane's row sees
-  uint32_t k_at[kExact ? G::KS : 1], v_at[kExact ? G::DB : 1];
+  uint32_t k_at, v_at;  // LDS offsets of this lane's part of a fragment
 
   __device__ __forceinline__ void addresses(const G &g, int lane) {
     const int r = lane & 15, half = lane >> 5;
-    const uint32_t group = ((lane >> 4) & 1) * G::kGroup;
-    const int vr = 4 * half + ((lane & 15) >> 2);
-    const int vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vb = (lane & 1) * 8;
-    if constexpr (kExact) {
-#pragma unroll
-      for (int ks = 0; ks < G::KS; ks++)
-        k_at[ks] = group + 16 * (r * g.stride + G::k_chunk(r, 2 * ks + half));
-#pragma unroll
-      for (int db = 0; db < G::DB; db++)
-        v_at[db] = 16 * (vr * g.stride + G::v_chunk(vr, 4 * db + vc)) + vb;
-    } else {
-      k_at[0] = group + 16 * (r * g.stride + half);
-      v_at[0] = 16 * (vr * g.stride + vc) + vb;
-    }
+    k_at = ((lane >> 4) & 1) * G::kGroup + 16 * (r * g.stride + G::k_chunk(r, half));
+    const int vr = 4 * half + ((lane & 15) >> 2);  // and vr + 8, with the same swizzle
+    v_at = 16 * (vr * g.stride + G::v_chunk(vr, ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1))) +
+           (lane & 1) * 8;
   }
-  __device__ __forceinline__ uint32_t k_addr(int ks) const {
-    return kExact ? k_at[ks] : k_at[0] + 32 * ks;
+  // Step ks of the scores, block db of the values.  The swizzles leave their
+  // bits to an exclusive or (buffers begin at multiples of 1 KB).
+  static __device__ __forceinline__ s16x8 k_frag(uint32_t at, int ks, int kb) {
+    return G::kPow2 ? lds16(at ^ (32 * ks), kb * 2 * G::kGroup)
+                    : lds16(at, 32 * ks + kb * 2 * G::kGroup);
   }
-  // rows vr and vr + 8 of a group share their swizzle
-  __device__ __forceinline__ uint32_t v_addr(int db) const {
-    return kExact ? v_at[db] : v_at[0] + 64 * db;
+  static __device__ __forceinline__ s16x8 v_frag(const G &g, uint32_t at, int db, int kg) {
+    const uint32_t x = G::kPow2 ? at ^ (64 * db) : at;
+    const uint32_t off = kg * G::kGroup + (G::kPow2 ? 0 : 64 * db);
+    const s16x4 a = lds_tr(x, off);
+    const s16x4 b = kExact ? lds_tr(x, off + 128 * G::kStride) : lds_tr(x + 128 * g.stride, off);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
   __device__ __forceinline__ void clear() {
@@ -377,31 +382,38 @@ struct Rows {
     for (int kb = 0; kb < KB; kb++)
 #pragma unroll
       for (int i = 0; i < 16; i++) s[kb][i] = 0.f;
+    const uint32_t at = k + k_at;
 #pragma unroll
     for (int ks = 0; ks < G::KS; ks++) {
-      if (!kExact && 2 * ks >= g.nch) break;
 #pragma unroll
       for (int kb = 0; kb < KB; kb++) {
-        s16x8 a = lds16(k + k_addr(ks) + kb * 2 * G::kGroup);
-        // past an odd number of chunks lies the next row, which may hold NaN
-        if (!kExact && 2 * ks + 1 >= g.nch && lane >= 32) a = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        s16x8 a = k_frag(at, ks, kb);
+        // past the row's chunks lies the next row, which may hold NaN
+        if (!kExact && 2 * ks + (lane >> 5) >= g.nch) a = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
         s[kb] = O::mma(a, q[ks], s[kb]);
       }
     }
+    // fragments are read kAhead products before their own
+    constexpr int kAhead = 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);  // LDS reads
+#pragma unroll
+    for (int i = 0; i < KB * G::KS - kAhead; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix product
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
   }
 
-  // The weights of KB x 32 keys from position p on, in place; m, l and o follow.
+  // The maximum over KB x 32 keys from position p on; m, l and o follow.
   template <int KB>
-  __device__ __forceinline__ void weights(f32x16 *s, int p, bool masked, int lane) {
+  __device__ __forceinline__ void grow(f32x16 *s, int p, bool masked, int lane) {
     if (masked) {
-      const int p0 = p + 4 * (lane >> 5);
+      const uint32_t first = uint32_t(p + 4 * (fresh(lane) >> 5) - lo), n = uint32_t(max(hi - lo, 0));
 #pragma unroll
       for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int key = p0 + 32 * kb + 8 * (i >> 2) + (i & 3);
-          if (key < lo || key >= hi) s[kb][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; i++)
+          if (first + uint32_t(32 * kb + 8 * (i >> 2) + (i & 3)) >= n) s[kb][i] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
@@ -421,52 +433,83 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 16; i++) o[db][i] *= keep;
     }
-    const float base = (m == -INFINITY ? 0.f : m) - kLift;
-#pragma unroll
-    for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -base));
-        l += s[kb][i];
-      }
   }
 
-  // o += V^T P^T over KB x 32 keys in LDS at v.
+  // Weights 2 j and 2 j + 1 of the group kg, as parts of its operands p.
+  __device__ __forceinline__ void weigh(const f32x16 *s, int kg, int j, float base, u32x4 *p) {
+    typedef typename O::v2 v2;
+    f32x2 r;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      r[i] = __builtin_amdgcn_exp2f(
+          __builtin_fmaf(s[kg >> 1][8 * (kg & 1) + 2 * j + i], c, -base));
+      l += r[i];
+    }
+    // the nearest of the cache's type and, where the output is fp32, what is
+    // left of the weight, again and again
+#pragma unroll
+    for (int n = 0; n < NP; n++) {
+      const v2 h = __builtin_convertvector(r, v2);
+      p[n][j] = __builtin_bit_cast(uint32_t, h);
+      if (n + 1 < NP) r -= f32x2{float(h[0]), float(h[1])};
+    }
+  }
+  // o = o + V^T P^T over KB x 32 keys in LDS at v, scores s; l follows.  A step
+  // is one block of dims of one group of 16 keys: its product, the read of the
+  // values four steps on, and a share of the next group's weights, which the
+  // matrix pipe's time hides.
   template <int KB>
   __device__ __forceinline__ void gather(const G &g, uint32_t v, const f32x16 *s) {
+    constexpr int kSteps = 2 * KB * G::DB, kRing = 4;
+    const float base = (m == -INFINITY ? 0.f : m) - kLift;
+    const uint32_t at = v + v_at;
+    s16x8 ring[kRing];
+    u32x4 p[2][NP];
 #pragma unroll
-    for (int kg = 0; kg < 2 * KB; kg++) {
-      float x[8];
+    for (int f = 0; f < kRing; f++)
+      if (f < kSteps) ring[f] = v_frag(g, at, f % G::DB, f / G::DB);
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = s[kg >> 1][8 * (kg & 1) + i];
-      s16x8 p[NP];
-      split_weights<CT, NP>(x, p);
-      const uint32_t at = v + kg * G::kGroup;
+    for (int j = 0; j < 4; j++) weigh(s, 0, j, base, p[0]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int db = 0; db < G::DB; db++) {
-        if (!kExact && 4 * db >= g.nch) break;
-        const s16x4 a = lds_tr(at + v_addr(db)), b = lds_tr(at + v_addr(db) + 128 * g.stride);
-        const s16x8 vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int f = 0; f < kSteps; f++) {
+      const int kg = f / G::DB, db = f % G::DB;
 #pragma unroll
-        for (int n = 0; n < NP; n++) o[db] = O::mma(vf, p[n], o[db]);
+      for (int n = 0; n < NP; n++)
+        o[db] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg & 1][n]), o[db]);
+      if (f + kRing < kSteps)
+        ring[f % kRing] = v_frag(g, at, (f + kRing) % G::DB, (f + kRing) / G::DB);
+      if (kg + 1 < 2 * KB) {
+#pragma unroll
+        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++)
+          weigh(s, kg + 1, j, base, p[(kg + 1) & 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
+  // Bit 15 of every 16-bit half whose exponent is all ones.
+  static __device__ __forceinline__ uint32_t odd_halves(uint32_t x) {
+    constexpr uint32_t e = uint32_t(O::kExp) * 0x10001u, one = e & ~(e << 1);
+    return ((x & e) + one) & 0x80008000u;
+  }
   // The values that are not finite among the 16 keys of the group in LDS at v:
   // whether there are any (uniform).
   __device__ __forceinline__ bool odd_values(const G &g, uint32_t v, int lane) const {
-    bool odd = false;
+    uint32_t odd = 0;
+    lane = fresh(lane);
     for (int i = lane; i < 16 * g.stride; i += 64) {
-      if (!kExact && i % g.stride >= g.nch) continue;
-      const s16x8 x = lds16(v + 16 * i);
+      if (!G::kPow2 && i % g.stride >= g.nch) continue;
+      const u32x4 x = __builtin_bit_cast(u32x4, lds16(v + 16 * i));
 #pragma unroll
-      for (int j = 0; j < 8; j++) odd |= (uint16_t(x[j]) & O::kExp) == O::kExp;
+      for (int j = 0; j < 4; j++) odd |= odd_halves(x[j]);
     }
-    return __any(odd);
+    return __any(odd != 0);
   }
-  // Adds them to the rows that see them; p: position of the group's first key.
+  // Adds them to the rows that see them (y less its nearest finite value: 0 for
+  // all others); p: position of the group's first key.
   __device__ __forceinline__ void add_odd_values(const G &g, uint32_t v, int p, int lane) {
+    lane = fresh(lane);
     for (int r = 0; r < 16; r++) {
       if (p + r < lo || p + r >= hi) continue;
 #pragma unroll
@@ -474,14 +517,14 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int d = 32 * db + 8 * i + 4 * (lane >> 5);
-          if (d >= 8 * g.nch) continue;
+          if (!g.within(d)) continue;
           const uint32_t at = v + 16 * (r * g.stride + G::v_chunk(r, d >> 3)) + 2 * (d & 7);
           const s16x4 x = *(__attribute__((address_space(3))) s16x4 *)(uintptr_t)at;
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const short e = x[j];  // (a bit cast of x[j] itself takes element 0)
-            if ((uint16_t(e) & O::kExp) == O::kExp)
-              o[db][4 * i + j] += float(__builtin_bit_cast(CT, e));
+            const float y = float(__builtin_bit_cast(CT, e));
+            o[db][4 * i + j] += y - __builtin_amdgcn_fmed3f(y, -O::kMax, O::kMax);
           }
         }
       }
@@ -489,12 +532,12 @@ struct Rows {
   }
   // ... and puts 0 in their place.
   __device__ __forceinline__ void clear_odd_values(const G &g, uint32_t v, int lane) const {
+    lane = fresh(lane);
     for (int i = lane; i < 16 * g.stride; i += 64) {
-      s16x8 x = lds16(v + 16 * i);
+      u32x4 x = __builtin_bit_cast(u32x4, lds16(v + 16 * i));
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if ((uint16_t(x[j]) & O::kExp) == O::kExp) x[j] = 0;
-      lds16_put(v + 16 * i, x);
+      for (int j = 0; j < 4; j++) x[j] &= ~((odd_halves(x[j]) >> 15) * 0xFFFFu);
+      lds16_put(v + 16 * i, __builtin_bit_cast(s16x8, x));
     }
   }
 
@@ -506,7 +549,7 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int d = 32 * db + 8 * (i >> 2) + 4 * (lane >> 5);
-        if (kExact || d < 8 * g.nch) z = __builtin_fmaf(o[db][i], 0.f, z);
+        if (g.within(d)) z = __builtin_fmaf(o[db][i], 0.f, z);
       }
     return z != 0.f;
   }
@@ -562,217 +605,258 @@ __device__ __forceinline__ bool find_block(const Work &w, int at, int &s, int &b
   return false;
 }
 
-// ---- the kernel -----------------------------------------------------------
+// ---- a workgroup's share ---------------------------------------------------
+// Rows r0 .. r0 + rows - 1 of a sequence and cache head (row r: new token r /
+// group, head r % group), and a piece of the keys that they see.
+struct Piece {
+  swamp::Seq sq;
+  int64_t r0;
+  int rows;
+  int before;       // position of the first new token
+  int begin, end;   // keys of the piece
+  int tile0, stop;  // where its tiles begin; no tile begins at or past stop
+  bool over;        // the rows see positions that the page table cannot hold
+
+  __device__ __forceinline__ int64_t token(int64_t r, int group) const { return sq.t0 + r / group; }
+  __device__ __forceinline__ swamp::Span seen(int64_t r, const Work &w) const {
+    return swamp::seen_by(before + int(r / w.group), w.window);
+  }
+};
+
+// False: no rows.  A piece without keys says so in its statistics here.
+__device__ __forceinline__ bool find_piece(const Work &w, int s, int64_t r0, int max_rows,
+                                           int split, int head, Piece &p) {
+  p.sq = swamp::seq_of(w.b.first[s], w.b.first[s + 1], w.b.len[s], w.b.n_tok);
+  const int64_t n_rows = int64_t(p.sq.n) * w.group;
+  p.r0 = r0;
+  if (r0 >= n_rows) return false;
+  p.rows = int(min(n_rows - r0, int64_t(max_rows)));
+  p.before = p.sq.len - p.sq.n;
+  const swamp::Span ka = p.seen(r0, w), kz = p.seen(r0 + p.rows - 1, w);
+  // positions that the page table cannot hold are not walked; nor are the last
+  // below 2^31, so that a tile's end fits
+  const int64_t room = min(w.b.pages_stride << w.cache.page_shift, (int64_t(1) << 31) - 512);
+  const int last = int(min(int64_t(kz.hi), room));
+  const int64_t from = (ka.lo & ~(kTile - 1)) + int64_t(split) * w.chunk;
+  p.over = kz.hi > room;
+  p.begin = int(min(max(int64_t(ka.lo), from), int64_t(last)));
+  p.end = split == w.splits - 1 ? last : int(min(from + w.chunk, int64_t(last)));
+  p.tile0 = p.begin & ~(kTile - 1);
+  p.stop = p.end > p.begin ? p.end : p.tile0;
+  if (w.splits > 1 && p.stop == p.tile0 && !p.over) {
+    for (int i = int(threadIdx.x); i < p.rows; i += kThreads) {
+      const int64_t r = r0 + i, t = p.token(r, w.group);
+      const swamp::Span seen = p.seen(r, w);
+      w.stat[(int64_t(split) * w.b.n_tok + t) * w.n_heads + head * w.group + int(r % w.group)] =
+          f32x2{-INFINITY, seen.hi > seen.lo ? 0.f : -1.f};
+    }
+    return false;
+  }
+  return true;
+}
+
+// Blocks of up to kFew rows: the four waves share the rows, and each takes its
+// own 32-key tiles through its own quarter of LDS (K: 2 groups, V: 2 groups).
+// No barrier: a wave waits for its own DMAs only; K of the next tile is on its
+// way from the end of the scores, V from the end of the sums.
 template <typename CT, int D, bool kExact, int NP>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_kernel(Work w) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Work w) {
   typedef Geo<D, kExact> G;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = uni(tid >> 6);
   const uint32_t lds = lds_base(smem), extra = lds + G::kSmem;
   const G g(w.cache.dim);
   const int dim = kExact ? D : w.cache.dim;
+  const int head = int(blockIdx.x) % w.cache.n_kv, unit = int(blockIdx.x) / w.cache.n_kv;
+  const int split = unit % w.splits, s = unit / w.splits;
+  Piece pc;
+  if (!find_piece(w, s, 0, kFew, split, head, pc)) return;
 
+  const int64_t rr = min(lane & 31, pc.rows - 1);
+  const int hq = head * w.group + int(rr % w.group);
+  const int64_t t = pc.token(rr, w.group);
+  Rows<CT, D, kExact, NP> a;
+  a.addresses(g, lane);
+  a.load_q(g, w.q + t * w.q_stride + int64_t(hq) * dim, w.scale, lane);
+  const swamp::Span mine = pc.seen(rr, w);
+  a.lo = max(mine.lo, pc.begin);
+  a.hi = min(mine.hi, pc.end);
+  const int all_lo = max(pc.seen(pc.rows - 1, w).lo, pc.begin);
+  const int all_hi = min(pc.seen(0, w).hi, pc.end);
+  Feed<D, kExact> f;
+  f.init(w, g, s, head, lane);
+  f.bad = pc.over;
+  f.lo = pc.begin;
+  f.hi = pc.end;
+
+  const uint32_t at_k = lds + wave * (G::kSmem / kWaves), at_v = at_k + 2 * G::kGroup;
+  bool bad = false;
+  for (int safe = 0; safe < 2; safe++) {
+    a.clear();
+    int p = pc.tile0 + 32 * wave;
+    int id0 = 0, id1 = 0;
+    if (p < pc.stop) {
+      id0 = f.page_of(p);
+      id1 = f.page_of(p + 16);
+      f.template issue<true, false>(p, id0, at_k, 0);
+      f.template issue<true, false>(p + 16, id1, at_k + G::kGroup, 0);
+      f.template issue<false, true>(p, id0, 0, at_v);
+      f.template issue<false, true>(p + 16, id1, 0, at_v + G::kGroup);
+    }
+    while (p < pc.stop) {
+      const int next = p + 32 * kWaves;
+      if (next < pc.stop) {
+        id0 = f.page_of(next);
+        id1 = f.page_of(next + 16);
+      }
+      f32x16 sc[1];
+      wait_dma<2 * G::NI>();
+      a.template scores<1>(g, at_k, sc, lane);
+      lds_done();
+      if (next < pc.stop) {
+        f.template issue<true, false>(next, id0, at_k, 0);
+        f.template issue<true, false>(next + 16, id1, at_k + G::kGroup, 0);
+      }
+      a.template grow<1>(sc, p, p < all_lo || p + 32 > all_hi, lane);
+      if (next < pc.stop) wait_dma<2 * G::NI>();
+      else wait_dma<0>();
+      if (safe) {
+        for (int i = 0; i < 2; i++)
+          if (a.odd_values(g, at_v + i * G::kGroup, lane)) {
+            a.add_odd_values(g, at_v + i * G::kGroup, p + 16 * i, lane);
+            lds_done();
+            a.clear_odd_values(g, at_v + i * G::kGroup, lane);
+            lds_done();
+          }
+      }
+      a.template gather<1>(g, at_v, sc);
+      lds_done();
+      if (next < pc.stop) {
+        f.template issue<false, true>(next, id0, 0, at_v);
+        f.template issue<false, true>(next + 16, id1, 0, at_v + G::kGroup);
+      }
+      p = next;
+    }
+    bad = __any(f.bad);
+    if (bad || !__any(a.not_finite(g, lane))) break;
+  }
+
+  // the waves' sums meet in LDS, rows of dim floats (16-byte chunks swizzled by
+  // the row where there are enough of them)
+  const float l = bad ? __builtin_nanf("") : a.sum();
+  const uint32_t flip = dim % 32 == 0 ? 7 : 0;
+  const uint32_t mine_at = lds + wave * (G::kSmem / kWaves);
+  const int r = lane & 31;
+  if (lane < 32) {
+    ldsf_put(extra + 8 * (32 * wave + r), a.m);
+    ldsf_put(extra + 8 * (32 * wave + r) + 4, l);
+  }
+  if (r < pc.rows) {
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = 32 * db + 8 * i + 4 * (lane >> 5);
+        if (d < dim)
+          ldsf4_put(mine_at + 4 * r * dim + 16 * ((d >> 2) ^ (r & flip)),
+                    f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2],
+                          a.o[db][4 * i + 3]});
+      }
+  }
+  if (bad && w.b.bad && lane == 0) *w.b.bad = 1;
+  __syncthreads();
+  const int per = dim >> 2;
+  for (int i = tid; i < pc.rows * per; i += kThreads) {
+    const int row = i / per, d = 4 * (i - row * per);
+    float mw[kWaves], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWaves; x++) {
+      mw[x] = ldsf(extra + 8 * (32 * x + row));
+      top = fmaxf(top, mw[x]);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < kWaves; x++) {
+      const float k = __builtin_amdgcn_exp2f(mw[x] - base);
+      sum += k * ldsf(extra + 8 * (32 * x + row) + 4);
+      if (mw[x] != -INFINITY)
+        acc += k * ldsf4(lds + x * (G::kSmem / kWaves) + 4 * row * dim +
+                         16 * ((d >> 2) ^ (row & flip)));
+    }
+    const int64_t to = pc.token(row, w.group);
+    const int h = head * w.group + row % w.group;
+    const swamp::Span seen = pc.seen(row, w);
+    const bool sees = seen.hi > seen.lo;
+    if (w.splits == 1) {
+      put4(w, to, h, dim, d, sees ? acc * (1.f / sum) : f32x4{0.f, 0.f, 0.f, 0.f});
+    } else {
+      const int64_t pr = (int64_t(split) * w.b.n_tok + to) * w.n_heads + h;
+      *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) = acc;
+      if (d == 0) w.stat[pr] = f32x2{top, sees ? sum : -1.f};
+    }
+  }
+}
+
+// Blocks of up to kRows rows, 32 a wave.  The tile of 64 keys is shared: a wave
+// brings in one group of 16 of it.  Two buffers (K: 4 groups, V: 4 groups), one
+// barrier a tile.
+template <typename CT, int D, bool kExact, int NP>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(Work w) {
+  typedef Geo<D, kExact> G;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = uni(tid >> 6);
+  const uint32_t lds = lds_base(smem), extra = lds + G::kSmem;
+  const G g(w.cache.dim);
+  const int dim = kExact ? D : w.cache.dim;
   // heads first: eight heads' workgroups keep to one XCD each, whose L2 then
   // holds one head's keys; late blocks, which see the most keys, go first
-  const int n_kv = w.cache.n_kv;
-  const int head = int(blockIdx.x) % n_kv, unit = int(blockIdx.x) / n_kv;
+  const int head = int(blockIdx.x) % w.cache.n_kv, unit = int(blockIdx.x) / w.cache.n_kv;
   const int split = unit % w.splits;
   int s, blk;
   if (!find_block(w, w.blocks - 1 - unit / w.splits, s, blk, lane)) return;
   s = uni(s);
   blk = uni(blk);
-  const swamp::Seq sq = swamp::seq_of(w.b.first[s], w.b.first[s + 1], w.b.len[s], w.b.n_tok);
-  const int64_t n_rows = int64_t(sq.n) * w.group;
-  const int64_t r0 = int64_t(blk) * kRows;
-  if (r0 >= n_rows) return;
-  const int rows = int(min(n_rows - r0, int64_t(kRows)));
-  const bool few = n_rows <= kFew;
-
-  // keys of the block, and of this piece of them
-  const int before = sq.len - sq.n;  // position of the first new token
-  const swamp::Span ka = swamp::seen_by(before + int(r0 / w.group), w.window);
-  const swamp::Span kz = swamp::seen_by(before + int((r0 + rows - 1) / w.group), w.window);
-  // (positions that the page table cannot hold are not walked; nor are the last
-  // below 2^31, so that a tile's end fits)
-  const int64_t room = min(w.b.pages_stride << w.cache.page_shift, (int64_t(1) << 31) - 512);
-  const int last = int(min(int64_t(kz.hi), room));
-  const int64_t from = (ka.lo & ~(kTile - 1)) + int64_t(split) * w.chunk;
-  const int begin = int(min(max(int64_t(ka.lo), from), int64_t(last)));
-  const int end = split == w.splits - 1 ? last : int(min(from + w.chunk, int64_t(last)));
-  const int tile0 = begin & ~(kTile - 1);
-  const int stop = end > begin ? end : tile0;  // of the tiles
-  if (w.splits > 1 && stop == tile0 && kz.hi <= room) {  // a piece without keys
-    for (int i = tid; i < rows; i += kThreads) {
-      const int64_t r = r0 + i, t = sq.t0 + r / w.group;
-      const swamp::Span seen = swamp::seen_by(before + int(r / w.group), w.window);
-      w.stat[(int64_t(split) * w.b.n_tok + t) * w.n_heads + head * w.group + int(r % w.group)] =
-          f32x2{-INFINITY, seen.hi > seen.lo ? 0.f : -1.f};
-    }
-    return;
-  }
+  Piece pc;
+  if (!find_piece(w, s, int64_t(blk) * kRows, kRows, split, head, pc)) return;
 
   // this lane's row
-  const int n = few ? (lane & 31) : 32 * wave + (lane & 31);
-  const int64_t rr = r0 + min(n, rows - 1);
-  const int tok = int(rr / w.group), hq = head * w.group + int(rr % w.group);
-  const int64_t t = int64_t(sq.t0) + tok;
-  const swamp::Span mine = swamp::seen_by(before + tok, w.window);
-  const bool store = n < rows;
-
+  const bool store = 32 * wave + (lane & 31) < pc.rows;
+  const int64_t rr = pc.r0 + min(32 * wave + (lane & 31), pc.rows - 1);
+  const int hq = head * w.group + int(rr % w.group);
+  const int64_t t = pc.token(rr, w.group);
   Rows<CT, D, kExact, NP> a;
   a.addresses(g, lane);
   a.load_q(g, w.q + t * w.q_stride + int64_t(hq) * dim, w.scale, lane);
-  a.lo = mine.lo;
-  a.hi = mine.hi;
+  const swamp::Span mine = pc.seen(rr, w);
+  a.lo = max(mine.lo, pc.begin);
+  a.hi = min(mine.hi, pc.end);
+  // keys that any row of the wave sees, and that all do
+  const swamp::Span wa = pc.seen(pc.r0 + min(32 * wave, pc.rows - 1), w);
+  const swamp::Span wz = pc.seen(pc.r0 + min(32 * wave + 31, pc.rows - 1), w);
+  const int any_lo = max(wa.lo, pc.begin), any_hi = min(wz.hi, pc.end);
+  const int all_lo = max(wz.lo, pc.begin), all_hi = min(wa.hi, pc.end);
   Feed<D, kExact> f;
   f.init(w, g, s, head, lane);
-  f.bad = kz.hi > room;
-  f.lo = begin;
-  f.hi = end;
-  const int n_tiles = (stop - tile0 + kTile - 1) / kTile;
-  // which keys all rows of the wave see, and any
-  const int w0 = few ? 0 : min(32 * wave, rows - 1), w1 = few ? rows - 1 : min(32 * wave + 31, rows - 1);
-  const swamp::Span wa = swamp::seen_by(before + int((r0 + w0) / w.group), w.window);
-  const swamp::Span wz = swamp::seen_by(before + int((r0 + w1) / w.group), w.window);
-  const int any_lo = max(wa.lo, begin), any_hi = min(wz.hi, end);
-  const int all_lo = max(wz.lo, begin), all_hi = min(wa.hi, end);
-  // the row's own keys within this piece
-  a.lo = max(a.lo, begin);
-  a.hi = min(a.hi, end);
+  f.bad = pc.over;
+  f.lo = pc.begin;
+  f.hi = pc.end;
+  const int n_tiles = (pc.stop - pc.tile0 + kTile - 1) / kTile;
 
-  a.clear();
   bool bad = false;
-  if (few) {
-    // Four waves, each with its own 32-key tiles and its own quarter of LDS:
-    // K (2 groups), then V.  No barrier: a wave waits for its own DMAs only.
-    const uint32_t at_k = lds + wave * (G::kSmem / kWaves), at_v = at_k + 2 * G::kGroup;
-    for (int safe = 0; safe < 2; safe++) {
-      int p = tile0 + 32 * wave;
-      int id0 = 0, id1 = 0;
-      if (p < stop) {
-        id0 = f.page_of(p);
-        id1 = f.page_of(p + 16);
-        f.template issue<true, false>(p, id0, at_k, 0);
-        f.template issue<true, false>(p + 16, id1, at_k + G::kGroup, 0);
-        f.template issue<false, true>(p, id0, 0, at_v);
-        f.template issue<false, true>(p + 16, id1, 0, at_v + G::kGroup);
-      }
-      while (p < stop) {
-        const int next = p + 32 * kWaves;
-        if (next < stop) {
-          id0 = f.page_of(next);
-          id1 = f.page_of(next + 16);
-        }
-        f32x16 sc[1];
-        wait_dma<2 * G::NI>();
-        a.template scores<1>(g, at_k, sc, lane);
-        lds_done();
-        if (next < stop) {
-          f.template issue<true, false>(next, id0, at_k, 0);
-          f.template issue<true, false>(next + 16, id1, at_k + G::kGroup, 0);
-        }
-        a.template weights<1>(sc, p, p < all_lo || p + 32 > all_hi, lane);
-        if (next < stop) wait_dma<2 * G::NI>();
-        else wait_dma<0>();
-        if (safe) {
-          for (int i = 0; i < 2; i++)
-            if (a.odd_values(g, at_v + i * G::kGroup, lane)) {
-              a.add_odd_values(g, at_v + i * G::kGroup, p + 16 * i, lane);
-              lds_done();
-              a.clear_odd_values(g, at_v + i * G::kGroup, lane);
-              lds_done();
-            }
-        }
-        a.template gather<1>(g, at_v, sc);
-        lds_done();
-        if (next < stop) {
-          f.template issue<false, true>(next, id0, 0, at_v);
-          f.template issue<false, true>(next + 16, id1, 0, at_v + G::kGroup);
-        }
-        p = next;
-      }
-      bad = __any(f.bad);
-      if (bad || safe || !__any(a.not_finite(g, lane))) break;
-      a.clear();
-    }
-
-    // the waves' sums meet in LDS, rows of dim floats (16-byte chunks swizzled
-    // by the row where there are enough of them)
-    const float l = bad ? __builtin_nanf("") : a.sum();
-    const uint32_t flip = dim % 32 == 0 ? 7 : 0;
-    wait_all();
-    {
-      const uint32_t mine_at = lds + wave * (G::kSmem / kWaves);
-      const int r = lane & 31;
-      if (lane < 32) {
-        ldsf_put(extra + 8 * (32 * wave + r), a.m);
-        ldsf_put(extra + 8 * (32 * wave + r) + 4, l);
-      }
-      if (r < rows) {
-#pragma unroll
-        for (int db = 0; db < G::DB; db++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int d = 32 * db + 8 * i + 4 * (lane >> 5);
-            if (d < dim)
-              ldsf4_put(mine_at + 4 * r * dim + 16 * ((d >> 2) ^ (r & flip)),
-                        f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2],
-                              a.o[db][4 * i + 3]});
-          }
-      }
-    }
-    __syncthreads();
-    const int per = dim >> 2;
-    for (int i = tid; i < rows * per; i += kThreads) {
-      const int r = i / per, d = 4 * (i - r * per);
-      float mw[kWaves], top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWaves; x++) {
-        mw[x] = ldsf(extra + 8 * (32 * x + r));
-        top = fmaxf(top, mw[x]);
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int x = 0; x < kWaves; x++) {
-        const float k = __builtin_amdgcn_exp2f(mw[x] - base);
-        sum += k * ldsf(extra + 8 * (32 * x + r) + 4);
-        // a wave without keys of this row may have summed others' infinities
-        if (mw[x] != -INFINITY)
-          acc += k * ldsf4(lds + x * (G::kSmem / kWaves) + 4 * r * dim +
-                           16 * ((d >> 2) ^ (r & flip)));
-      }
-      const int64_t row = sq.t0 + r / w.group;
-      const int h = head * w.group + r % w.group;
-      const swamp::Span seen = swamp::seen_by(before + r / w.group, w.window);
-      const bool sees = seen.hi > seen.lo;
-      if (w.splits == 1) {
-        const float inv = 1.f / sum;
-        put4(w, row, h, dim, d, sees ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f});
-      } else {
-        const int64_t pr = (int64_t(split) * w.b.n_tok + row) * w.n_heads + h;
-        *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) = acc;
-        if (d == 0) w.stat[pr] = f32x2{top, sees ? sum : -1.f};
-      }
-    }
-    if (bad && w.b.bad && lane == 0) *w.b.bad = 1;
-    return;
-  }
-
-  // Rows of their own for every wave; the tile of 64 keys is shared, a wave
-  // brings in one group of 16 of it.  Two buffers (K: 4 groups, V: 4 groups).
   for (int safe = 0; safe < 2; safe++) {
+    a.clear();
     const int mine_at = 16 * wave;
     int id = 0;
     if (n_tiles > 0) {
-      id = f.page_of(tile0 + mine_at);
-      f.template issue<true, true>(tile0 + mine_at, id, lds + wave * G::kGroup,
+      id = f.page_of(pc.tile0 + mine_at);
+      f.template issue<true, true>(pc.tile0 + mine_at, id, lds + wave * G::kGroup,
                                    lds + (4 + wave) * G::kGroup);
-      id = f.page_of(tile0 + kTile + mine_at);
+      id = f.page_of(pc.tile0 + kTile + mine_at);
     }
     for (int i = 0; i < n_tiles; i++) {
       const uint32_t buf = lds + (i & 1) * G::kBuf, other = lds + (~i & 1) * G::kBuf;
-      const int p = tile0 + kTile * i;
+      const int p = pc.tile0 + kTile * i;
       wait_all();
       if (i + 1 < n_tiles) {
         f.template issue<true, true>(p + kTile + mine_at, id, other + wave * G::kGroup,
@@ -783,11 +867,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_kernel(Work w
       f32x16 sc[2];
       if (work) {
         a.template scores<2>(g, buf, sc, lane);
-        a.template weights<2>(sc, p, p < all_lo || p + kTile > all_hi, lane);
+        a.template grow<2>(sc, p, p < all_lo || p + kTile > all_hi, lane);
       }
       if (safe) {
         const uint32_t v = buf + (4 + wave) * G::kGroup;
-        if (__syncthreads_or(a.odd_values(g, v, lane))) {
+        if (anywhere(a.odd_values(g, v, lane), extra)) {
           for (int j = 0; j < 4; j++)
             a.add_odd_values(g, buf + (4 + j) * G::kGroup, p + 16 * j, lane);
           __syncthreads();
@@ -797,50 +881,40 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_kernel(Work w
       }
       if (work) a.template gather<2>(g, buf + 4 * G::kGroup, sc);
     }
-    bad = __syncthreads_or(f.bad);
-    if (bad || safe || !__syncthreads_or(store && a.not_finite(g, lane))) break;
-    a.clear();
+    bad = anywhere(f.bad, extra);
+    if (bad || !anywhere(store && a.not_finite(g, lane), extra)) break;
   }
   const float l = bad ? __builtin_nanf("") : a.sum();
   if (bad && w.b.bad && tid == 0) *w.b.bad = 1;
   if (!store) return;
   const bool sees = mine.hi > mine.lo;
-  if (w.splits == 1) {
-    const float inv = 1.f / l;
-#pragma unroll
-    for (int db = 0; db < G::DB; db++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int d = 32 * db + 8 * i + 4 * (lane >> 5);
-        if (kExact || d < dim)
-          put4(w, t, hq, dim, d,
-               sees ? f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2],
-                            a.o[db][4 * i + 3]} *
-                          inv
-                    : f32x4{0.f, 0.f, 0.f, 0.f});
-      }
-    return;
-  }
   const int64_t pr = (int64_t(split) * w.b.n_tok + t) * w.n_heads + hq;
-  if (lane < 32) w.stat[pr] = f32x2{a.m, sees ? l : -1.f};
+  const float inv = 1.f / l;
+  if (w.splits > 1 && lane < 32) w.stat[pr] = f32x2{a.m, sees ? l : -1.f};
 #pragma unroll
   for (int db = 0; db < G::DB; db++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int d = 32 * db + 8 * i + 4 * (lane >> 5);
-      if (kExact || d < dim)
-        *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) =
-            f32x4{a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2], a.o[db][4 * i + 3]};
+      if (!g.within(d)) continue;
+      const f32x4 x = {a.o[db][4 * i], a.o[db][4 * i + 1], a.o[db][4 * i + 2], a.o[db][4 * i + 3]};
+      if (w.splits == 1) put4(w, t, hq, dim, d, sees ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+      else *reinterpret_cast<f32x4 *>(w.part + pr * dim + d) = x;
     }
+}
+
+template <typename CT, int D, bool kExact, int NP>
+void launch_kind(const Work &w, hipStream_t s) {
+  typedef Geo<D, kExact> G;
+  const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));
+  if (w.few) attn_few_kernel<CT, D, kExact, NP><<<grid, kThreads, G::kSmem + G::kExtra, s>>>(w);
+  else attn_many_kernel<CT, D, kExact, NP><<<grid, kThreads, G::kSmem + G::kExtra, s>>>(w);
 }
 
 template <typename CT, int D, bool kExact>
 int launch(const Work &w, bool precise, hipStream_t s) {
-  typedef Geo<D, kExact> G;
-  const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));
-  const uint32_t smem = G::kSmem + G::kExtra;
-  if (precise) attn_kernel<CT, D, kExact, Op<CT>::kParts><<<grid, kThreads, smem, s>>>(w);
-  else attn_kernel<CT, D, kExact, 1><<<grid, kThreads, smem, s>>>(w);
+  if (precise) launch_kind<CT, D, kExact, Op<CT>::kParts>(w, s);
+  else launch_kind<CT, D, kExact, 1>(w, s);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
 
@@ -848,6 +922,8 @@ template <typename CT>
 int launch_dim(const Work &w, bool precise, hipStream_t s) {
   switch (w.cache.dim) {
     case 64: return launch<CT, 64, true>(w, precise, s);
+    case 80: return launch<CT, 80, true>(w, precise, s);
+    case 96: return launch<CT, 96, true>(w, precise, s);
     case 128: return launch<CT, 128, true>(w, precise, s);
     case 256: return launch<CT, 256, true>(w, precise, s);
   }
