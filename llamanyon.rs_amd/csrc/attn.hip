@@ -12,8 +12,12 @@ namespace {
 
 using namespace swamp_attn;
 
-// out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over a row's pieces, in
-// their order.  A thread takes four dims of a row.
+constexpr int kJoinWide = 4;  // pieces up to which a thread joins them all
+
+// out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over a row's pieces, in a
+// fixed order.
+
+// A thread takes four dims of a row and all pieces.
 __global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
   const int per = w.cache.dim >> 2;
   const int64_t n = int64_t(w.b.n_tok) * w.n_heads;  // rows of a piece
@@ -40,6 +44,50 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
   }
   put4(w, t, int(row - t * w.n_heads), w.cache.dim, d,
        sees ? acc * (1.f / sum) : f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+// A workgroup takes a row: `per` threads (dim / 4 rounded up to a power of two)
+// for the dims, 256 / per shares of the pieces.  For few rows in many pieces,
+// whose loads would otherwise wait for one another.
+__global__ void __launch_bounds__(kThreads) join_wide_kernel(Work w, int per) {
+  __shared__ f32x4 accs[kThreads];
+  __shared__ float sums[kThreads], tops[kWaves];
+  __shared__ int blind;
+  const int64_t n = int64_t(w.b.n_tok) * w.n_heads, row = blockIdx.x, t = row / w.n_heads;
+  if (t < w.b.first[0] || t >= w.b.first[w.b.n_seq]) return;  // padding
+  const int tid = int(threadIdx.x), share = tid / per, shares = kThreads / per;
+  const int d = 4 * (tid - share * per);
+  float top = -INFINITY;
+  for (int x = tid; x < w.splits; x += kThreads) top = fmaxf(top, w.stat[x * n + row][0]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  if (tid == 0) blind = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) top = fmaxf(top, tops[i]);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int x = share; x < w.splits; x += shares) {
+    const f32x2 st = w.stat[x * n + row];
+    const float k = __builtin_amdgcn_exp2f(st[0] - base);
+    if (st[1] == -1.f) blind = 1;
+    sum += k * st[1];
+    if (st[0] != -INFINITY && d < w.cache.dim)
+      acc += k * *reinterpret_cast<const f32x4 *>(w.part + (x * n + row) * w.cache.dim + d);
+  }
+  accs[tid] = acc;
+  sums[tid] = sum;
+  __syncthreads();
+  if (share != 0 || d >= w.cache.dim) return;
+  for (int i = 1; i < shares; i++) {
+    acc += accs[i * per + tid];
+    sum += sums[i * per + tid];
+  }
+  put4(w, t, int(row - t * w.n_heads), w.cache.dim, d,
+       blind ? f32x4{0.f, 0.f, 0.f, 0.f} : acc * (1.f / sum));
 }
 
 struct Plan {
@@ -115,7 +163,14 @@ int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStr
   const bool precise = c.out_type == SWAMP_F32;
   const int rc = c.dtype == SWAMP_F16 ? swamp_attn_f16(w, precise, s) : swamp_attn_bf16(w, precise, s);
   if (rc != SWAMP_OK || w.splits == 1) return rc;
-  const int64_t n = int64_t(c.batch.n_tok) * c.n_heads * (c.cache.dim / 4);
-  join_kernel<<<dim3(unsigned((n + kThreads - 1) / kThreads)), kThreads, 0, s>>>(w);
+  const int64_t rows = int64_t(c.batch.n_tok) * c.n_heads;
+  if (w.splits > kJoinWide) {
+    int per = 2;
+    while (4 * per < c.cache.dim) per *= 2;
+    join_wide_kernel<<<dim3(unsigned(rows)), kThreads, 0, s>>>(w, per);
+  } else {
+    const int64_t n = rows * (c.cache.dim / 4);
+    join_kernel<<<dim3(unsigned((n + kThreads - 1) / kThreads)), kThreads, 0, s>>>(w);
+  }
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }

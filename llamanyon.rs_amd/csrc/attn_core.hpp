@@ -30,6 +30,8 @@
 #include "paging.hpp"
 #include "swamp_common.hpp"
 
+#include <type_traits>
+
 namespace swamp_attn {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -220,7 +222,10 @@ struct Geo {
 };
 
 // The keys lo .. hi - 1 of one sequence and cache head, on their way into LDS.
-template <int D, bool kExact>
+// kWhole: a group of 16 keys lies within a page and its offsets in 32 bits, so
+// that a group's page and address are the scalar unit's; else every lane has its
+// own.
+template <int D, bool kExact, bool kWhole>
 struct Feed {
   typedef Geo<D, kExact> G;
   const uint8_t *k, *v;     // slot 0 of page 0 of this head
@@ -228,10 +233,13 @@ struct Feed {
   const void *stand_in;     // read in place of a page that is none
   int64_t page_bytes, slot_bytes, cols;
   int n_pages, shift, lo, hi;
-  bool whole;               // groups lie within a page, and offsets in 32 bits
   bool bad;                 // this lane met a position without a page
   uint32_t rows;            // row of the group (0..15) of DMA j at bits 4 j
   uint32_t koff[G::NI], voff[G::NI];
+
+  struct Page {  // of a group: one id, or each lane's for its DMAs
+    int32_t id[kWhole ? 1 : G::NI];
+  };
 
   __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane) {
     k = reinterpret_cast<const uint8_t *>(w.cache.k + int64_t(head) * w.cache.head_stride);
@@ -243,71 +251,83 @@ struct Feed {
     cols = w.b.pages_stride;
     n_pages = w.cache.n_pages;
     shift = w.cache.page_shift;
-    whole = shift >= 4 && slot_bytes < (1 << 26);
     bad = false;
     rows = 0;
 #pragma unroll
     for (int j = 0; j < G::NI; j++) {
       const int i = 64 * j + lane, r = min(i / g.stride, 15), c = min(i - r * g.stride, g.nch - 1);
-      const uint32_t row = whole ? uint32_t(r) * uint32_t(slot_bytes) : 0;
+      const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) : 0;
       rows |= uint32_t(r) << (4 * j);
       koff[j] = row + 16 * G::k_chunk(r, c);
       voff[j] = row + 16 * G::v_chunk(r, c);
     }
   }
-  // Page of the group at p0, for issue(): uniform.
-  __device__ __forceinline__ int page_of(int p0) const {
-    if (!whole) return 0;
-    const int p = min(max(p0, lo), hi - 1);
-    const int64_t col = swamp::page_col(p, shift);
-    if (!swamp::page_col_ok(p, col, cols)) return -1;
-    return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + uni(int(col)));
+  __device__ __forceinline__ int within(int p) const { return min(max(p, lo), hi - 1); }
+  // Entry `col` of the page table, by the scalar unit; -1 past its end.
+  __device__ __forceinline__ int entry(int64_t col) const {
+    return col < cols ? *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(
+                            table + uni(int(col)))
+                      : -1;
   }
-  // DMAs of the 16 keys from p0 (a multiple of 16) to LDS: kK, kV say what.
-  template <bool kK, bool kV>
-  __device__ __forceinline__ void issue(int p0, int id, uint32_t at_k, uint32_t at_v) {
-    if (whole) {
-      const int first = min(max(p0, lo), hi - 1) & ~15;
-      const bool ok = swamp::page_ok(id, n_pages);
-      const int64_t at = int64_t(id) * page_bytes + (first & ((1 << shift) - 1)) * slot_bytes;
-      const void *kb = ok ? k + at : stand_in, *vb = ok ? v + at : stand_in;
+  // Pages of the group at p0 (a multiple of 16), for issue().  kNow: the ids are
+  // needed before other loads of this wave have come in, whose wait they would
+  // share as vector loads; the scalar unit then brings them page by page.
+  template <bool kNow>
+  __device__ __forceinline__ Page pages_of(int p0) const {
+    Page pg;
+    if constexpr (kWhole) {
+      pg.id[0] = entry(swamp::page_col(within(p0), shift));
+    } else if constexpr (kNow) {
+      const int first = within(p0) >> shift, last = within(p0 + 15) >> shift;
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) pg.id[j] = -1;
+      for (int c = first; c <= last; c++) {
+        const int id = entry(c);
+#pragma unroll
+        for (int j = 0; j < G::NI; j++)
+          if (within(p0 + int((rows >> (4 * j)) & 15)) >> shift == c) pg.id[j] = id;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) {
+        const int p = within(p0 + int((rows >> (4 * j)) & 15));
+        const int64_t col = swamp::page_col(p, shift);
+        pg.id[j] = swamp::page_col_ok(p, col, cols) ? table[col] : -1;
+      }
+    }
+    return pg;
+  }
+  // DMAs of the group at p0 to LDS: its keys (kK) or values.
+  template <bool kK>
+  __device__ __forceinline__ void issue(int p0, const Page &pg, uint32_t at) {
+    const uint8_t *base = kK ? k : v;
+    const uint32_t *off = kK ? koff : voff;
+    if constexpr (kWhole) {
+      const int first = within(p0) & ~15;
+      const bool ok = swamp::page_ok(pg.id[0], n_pages);
+      const int64_t to = int64_t(pg.id[0]) * page_bytes + (first & ((1 << shift) - 1)) * slot_bytes;
+      const void *from = ok ? base + to : stand_in;
       bad |= !ok;
       if (!ok || p0 < lo || p0 + 15 >= hi) {
         const uint32_t rows = fresh(this->rows);
 #pragma unroll
         for (int j = 0; j < G::NI; j++) {
-          const int r = (rows >> (4 * j)) & 15, to = min(max(p0 + r, lo), hi - 1) - first;
-          const uint32_t move = ok ? uint32_t(to - r) * uint32_t(slot_bytes)
-                                   : uint32_t(-r) * uint32_t(slot_bytes);
-          if (kK) dma_uniform(kb, koff[j] + move, at_k + 1024 * j);
-          if (kV) dma_uniform(vb, voff[j] + move, at_v + 1024 * j);
+          const int r = (rows >> (4 * j)) & 15, row = ok ? within(p0 + r) - first : 0;
+          dma_uniform(from, off[j] + uint32_t(row - r) * uint32_t(slot_bytes), at + 1024 * j);
         }
         return;
       }
 #pragma unroll
+      for (int j = 0; j < G::NI; j++) dma_uniform(from, off[j], at + 1024 * j);
+    } else {
+#pragma unroll
       for (int j = 0; j < G::NI; j++) {
-        if (kK) dma_uniform(kb, koff[j], at_k + 1024 * j);
-        if (kV) dma_uniform(vb, voff[j], at_v + 1024 * j);
+        const int p = within(p0 + int((rows >> (4 * j)) & 15));
+        const bool ok = swamp::page_ok(pg.id[j], n_pages);
+        const int64_t to = int64_t(pg.id[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
+        bad |= !ok;
+        dma_lane((ok ? base + to : static_cast<const uint8_t *>(stand_in)) + off[j], at + 1024 * j);
       }
-      return;
-    }
-    const uint32_t rows = fresh(this->rows);
-    int32_t ids[G::NI];
-#pragma unroll
-    for (int j = 0; j < G::NI; j++) {
-      const int p = min(max(p0 + int((rows >> (4 * j)) & 15), lo), hi - 1);
-      const int64_t col = swamp::page_col(p, shift);
-      ids[j] = swamp::page_col_ok(p, col, cols) ? table[col] : -1;
-    }
-#pragma unroll
-    for (int j = 0; j < G::NI; j++) {
-      const int p = min(max(p0 + int((rows >> (4 * j)) & 15), lo), hi - 1);
-      const bool ok = swamp::page_ok(ids[j], n_pages);
-      const int64_t at = int64_t(ids[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
-      const uint8_t *none = static_cast<const uint8_t *>(stand_in);
-      bad |= !ok;
-      if (kK) dma_lane((ok ? k + at : none) + koff[j], at_k + 1024 * j);
-      if (kV) dma_lane((ok ? v + at : none) + voff[j], at_v + 1024 * j);
     }
   }
 };
@@ -404,26 +424,27 @@ struct Rows {
     __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
   }
 
-  // The maximum over KB x 32 keys from position p on; m, l and o follow.
+  // Keys from position p on that this row does not see: score -infinity.
   template <int KB>
-  __device__ __forceinline__ void grow(f32x16 *s, int p, bool masked, int lane) {
-    if (masked) {
-      const uint32_t first = uint32_t(p + 4 * (fresh(lane) >> 5) - lo), n = uint32_t(max(hi - lo, 0));
-#pragma unroll
-      for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (first + uint32_t(32 * kb + 8 * (i >> 2) + (i & 3)) >= n) s[kb][i] = -INFINITY;
-    }
-    float top = s[0][0];
+  __device__ __forceinline__ void hide(f32x16 *s, int p, int lane) const {
+    const uint32_t first = uint32_t(p + 4 * (fresh(lane) >> 5) - lo), n = uint32_t(max(hi - lo, 0));
 #pragma unroll
     for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
+      for (int i = 0; i < 16; i++)
+        if (first + uint32_t(32 * kb + 8 * (i >> 2) + (i & 3)) >= n) s[kb][i] = -INFINITY;
+  }
+  // c times the row's largest score, from the two halves' largest.
+  __device__ __forceinline__ float join_halves(float top) const {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
                                                        false, false);
-    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
-    if (__any(top > m + kSlack)) {
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
+  }
+  // Some row's maximum has to follow a tile with the largest scores top.
+  __device__ __forceinline__ bool grows(float top) const { return __any(top > m + kSlack); }
+  // m follows; l and o with it.
+  __device__ __forceinline__ void grow(float top) {
+    if (grows(top)) {
       const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown;
       const float keep = __builtin_amdgcn_exp2f(m - base);
       m = grown;
@@ -434,6 +455,14 @@ struct Rows {
         for (int i = 0; i < 16; i++) o[db][i] *= keep;
     }
   }
+  template <int KB>
+  __device__ __forceinline__ float largest(const f32x16 *s) const {
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 16 * KB; e++) top = fmaxf(top, s[e >> 4][e & 15]);
+    return join_halves(top);
+  }
+  __device__ __forceinline__ float base_of() const { return (m == -INFINITY ? 0.f : m) - kLift; }
 
   // Weights 2 j and 2 j + 1 of the group kg, as parts of its operands p.
   __device__ __forceinline__ void weigh(const f32x16 *s, int kg, int j, float base, u32x4 *p) {
@@ -453,15 +482,18 @@ struct Rows {
       p[n][j] = __builtin_bit_cast(uint32_t, h);
       if (n + 1 < NP) r -= f32x2{float(h[0]), float(h[1])};
     }
+    // (not moved to where they are used, past the products that hide this)
+#pragma unroll
+    for (int n = 0; n < NP; n++) p[n][j] = fresh(p[n][j]);
+    l = fresh(l);
   }
-  // o = o + V^T P^T over KB x 32 keys in LDS at v, scores s; l follows.  A step
-  // is one block of dims of one group of 16 keys: its product, the read of the
-  // values four steps on, and a share of the next group's weights, which the
-  // matrix pipe's time hides.
-  template <int KB>
-  __device__ __forceinline__ void gather(const G &g, uint32_t v, const f32x16 *s) {
-    constexpr int kSteps = 2 * KB * G::DB, kRing = 4;
-    const float base = (m == -INFINITY ? 0.f : m) - kLift;
+  // A tile of 32 keys after its scores and grow(): weights, and o = o + V^T P^T
+  // over the values in LDS at v.  A step is one block of dims of one group of 16
+  // keys: its product, the read of the values four steps on, and a share of the
+  // next group's weights, which the matrix pipe's time hides.
+  __device__ __forceinline__ void rest(const G &g, uint32_t v, const f32x16 *s) {
+    constexpr int kSteps = 2 * G::DB, kRing = 4;
+    const float base = base_of();
     const uint32_t at = v + v_at;
     s16x8 ring[kRing];
     u32x4 p[2][NP];
@@ -476,15 +508,123 @@ struct Rows {
       const int kg = f / G::DB, db = f % G::DB;
 #pragma unroll
       for (int n = 0; n < NP; n++)
-        o[db] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg & 1][n]), o[db]);
+        o[db] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg][n]), o[db]);
       if (f + kRing < kSteps)
         ring[f % kRing] = v_frag(g, at, (f + kRing) % G::DB, (f + kRing) / G::DB);
-      if (kg + 1 < 2 * KB) {
+      if (kg == 0) {
 #pragma unroll
-        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++)
-          weigh(s, kg + 1, j, base, p[(kg + 1) & 1]);
+        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++) weigh(s, 1, j, base, p[1]);
       }
       __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // ---- scores a tile ahead of the sums (attn_many_kernel) ----
+  // p holds a tile's weights; those of its last group are made with the next
+  // tile's scores (KB 2: from the half of s that the first products leave alone).
+
+  // Scores of the tile whose keys are in LDS at k; kPending: and the last group
+  // of the tile before.
+  template <int KB, bool kPending>
+  __device__ __forceinline__ void scores_ahead(const G &g, uint32_t k, f32x16 *s, u32x4 (&p)[2 * KB][NP],
+                                               float base, int lane) {
+    constexpr int kSteps = KB * G::KS, kRing = 4;
+    const uint32_t at = k + k_at;
+    s16x8 ring[kRing];
+#pragma unroll
+    for (int f = 0; f < kRing; f++) ring[f] = k_frag(at, f % G::KS, f / G::KS);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < kSteps; f++) {
+      const int kb = f / G::KS, ks = f % G::KS;
+      s16x8 a = ring[f % kRing];
+      if (!kExact && 2 * ks + (lane >> 5) >= g.nch) a = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (ks == 0) s[kb] = O::mma(a, q[ks], f32x16{});
+      else s[kb] = O::mma(a, q[ks], s[kb]);
+      if (f + kRing < kSteps)
+        ring[f % kRing] = k_frag(at, (f + kRing) % G::KS, (f + kRing) / G::KS);
+      if (KB == 2 && kPending && kb == 0) {
+#pragma unroll
+        for (int j = 4 * ks / G::KS; j < 4 * (ks + 1) / G::KS; j++) weigh(s, 3, j, base, p[3]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // The maximum over the scores s, then the weights of all groups but a pending
+  // one; kSums: while o = o + V^T P^T runs with the weights in p, which the new
+  // ones replace group by group.
+  template <int KB, bool kSums>
+  __device__ __forceinline__ void weigh_ahead(const G &g, uint32_t v, const f32x16 *s,
+                                              u32x4 (&p)[2 * KB][NP], float &base) {
+    constexpr int kSteps = 2 * KB * G::DB, kRing = 4;
+    const uint32_t at = v + v_at;
+    s16x8 ring[kRing];
+    if (kSums) {
+#pragma unroll
+      for (int f = 0; f < kRing; f++)
+        if (f < kSteps) ring[f] = v_frag(g, at, f % G::DB, f / G::DB);
+    }
+    float top = s[0][0], keep = 1.f;
+    bool grew = false;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < kSteps; f++) {
+      const int kg = f / G::DB, db = f % G::DB;
+      if (kSums) {
+#pragma unroll
+        for (int n = 0; n < NP; n++)
+          o[db] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg][n]), o[db]);
+        if (f + kRing < kSteps)
+          ring[f % kRing] = v_frag(g, at, (f + kRing) % G::DB, (f + kRing) / G::DB);
+      }
+      if (kg == 0) {
+#pragma unroll
+        for (int e = 16 * KB * db / G::DB; e < 16 * KB * (db + 1) / G::DB; e++)
+          top = fmaxf(top, s[e >> 4][e & 15]);
+        if (db + 1 == G::DB) {
+          top = join_halves(top);
+          grew = grows(top);
+          const float grown = grew ? fmaxf(m, top) : m;
+          const float zero = grown == -INFINITY ? 0.f : grown;
+          keep = __builtin_amdgcn_exp2f(m - zero);
+          m = grown;
+          base = zero - kLift;
+          l *= keep;
+        }
+      } else {
+#pragma unroll
+        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++)
+          weigh(s, kg - 1, j, base, p[kg - 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (KB == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) weigh(s, 1, j, base, p[1]);
+    }
+    if (kSums && grew) {
+#pragma unroll
+      for (int db = 0; db < G::DB; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[db][i] *= keep;
+    }
+  }
+  // The last tile's sums.
+  template <int KB>
+  __device__ __forceinline__ void sums(const G &g, uint32_t v, const f32x16 *s,
+                                       u32x4 (&p)[2 * KB][NP], float base) {
+    const uint32_t at = v + v_at;
+    if (KB == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) weigh(s, 3, j, base, p[3]);
+    }
+#pragma unroll
+    for (int f = 0; f < 2 * KB * G::DB; f++) {
+      const int kg = f / G::DB, db = f % G::DB;
+      const s16x8 vf = v_frag(g, at, db, kg);
+#pragma unroll
+      for (int n = 0; n < NP; n++)
+        o[db] = O::mma(vf, __builtin_bit_cast(s16x8, p[kg][n]), o[db]);
     }
   }
 
@@ -659,7 +799,7 @@ __device__ __forceinline__ bool find_piece(const Work &w, int s, int64_t r0, int
 // own 32-key tiles through its own quarter of LDS (K: 2 groups, V: 2 groups).
 // No barrier: a wave waits for its own DMAs only; K of the next tile is on its
 // way from the end of the scores, V from the end of the sums.
-template <typename CT, int D, bool kExact, int NP>
+template <typename CT, int D, bool kExact, bool kWhole, int NP>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Work w) {
   typedef Geo<D, kExact> G;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -683,7 +823,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   a.hi = min(mine.hi, pc.end);
   const int all_lo = max(pc.seen(pc.rows - 1, w).lo, pc.begin);
   const int all_hi = min(pc.seen(0, w).hi, pc.end);
-  Feed<D, kExact> f;
+  typedef Feed<D, kExact, kWhole> F;
+  F f;
   f.init(w, g, s, head, lane);
   f.bad = pc.over;
   f.lo = pc.begin;
@@ -694,31 +835,35 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   for (int safe = 0; safe < 2; safe++) {
     a.clear();
     int p = pc.tile0 + 32 * wave;
-    int id0 = 0, id1 = 0;
+    typename F::Page pg[2];
     if (p < pc.stop) {
-      id0 = f.page_of(p);
-      id1 = f.page_of(p + 16);
-      f.template issue<true, false>(p, id0, at_k, 0);
-      f.template issue<true, false>(p + 16, id1, at_k + G::kGroup, 0);
-      f.template issue<false, true>(p, id0, 0, at_v);
-      f.template issue<false, true>(p + 16, id1, 0, at_v + G::kGroup);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        pg[i] = f.template pages_of<true>(p + 16 * i);
+        f.template issue<true>(p + 16 * i, pg[i], at_k + i * G::kGroup);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) f.template issue<false>(p + 16 * i, pg[i], at_v + i * G::kGroup);
     }
     while (p < pc.stop) {
       const int next = p + 32 * kWaves;
-      if (next < pc.stop) {
-        id0 = f.page_of(next);
-        id1 = f.page_of(next + 16);
+      const bool more = next < pc.stop;
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) pg[i] = f.template pages_of<true>(next + 16 * i);
       }
       f32x16 sc[1];
       wait_dma<2 * G::NI>();
       a.template scores<1>(g, at_k, sc, lane);
       lds_done();
-      if (next < pc.stop) {
-        f.template issue<true, false>(next, id0, at_k, 0);
-        f.template issue<true, false>(next + 16, id1, at_k + G::kGroup, 0);
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          f.template issue<true>(next + 16 * i, pg[i], at_k + i * G::kGroup);
       }
-      a.template grow<1>(sc, p, p < all_lo || p + 32 > all_hi, lane);
-      if (next < pc.stop) wait_dma<2 * G::NI>();
+      if (p < all_lo || p + 32 > all_hi) a.template hide<1>(sc, p, lane);
+      a.grow(a.template largest<1>(sc));
+      if (more) wait_dma<2 * G::NI>();
       else wait_dma<0>();
       if (safe) {
         for (int i = 0; i < 2; i++)
@@ -729,11 +874,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
             lds_done();
           }
       }
-      a.template gather<1>(g, at_v, sc);
+      a.rest(g, at_v, sc);
       lds_done();
-      if (next < pc.stop) {
-        f.template issue<false, true>(next, id0, 0, at_v);
-        f.template issue<false, true>(next + 16, id1, 0, at_v + G::kGroup);
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          f.template issue<false>(next + 16 * i, pg[i], at_v + i * G::kGroup);
       }
       p = next;
     }
@@ -798,12 +944,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   }
 }
 
-// Blocks of up to kRows rows, 32 a wave.  The tile of 64 keys is shared: a wave
-// brings in one group of 16 of it.  Two buffers (K: 4 groups, V: 4 groups), one
-// barrier a tile.
-template <typename CT, int D, bool kExact, int NP>
+// Blocks of up to kRows rows, 32 a wave.  A tile of 32 KB keys is shared, each wave
+// brings in a part of it.  Scores run a tile ahead of the sums: while tile i is
+// summed and tile i + 1 scored, K of i + 2 and V of i + 1 are on their way, and
+// one barrier a tile orders all of it.  K and V have two buffers each.
+template <typename CT, int D, bool kExact, bool kWhole, int NP>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(Work w) {
   typedef Geo<D, kExact> G;
+  // heads of 256 dims: the sums alone are 128 registers
+  constexpr int KB = D <= 128 ? 2 : 1, kKeys = 32 * KB;
+  constexpr uint32_t kPart = 2 * KB * G::kGroup;  // K or V of a tile
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = uni(tid >> 6);
   const uint32_t lds = lds_base(smem), extra = lds + G::kSmem;
@@ -836,54 +986,92 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
   const swamp::Span wz = pc.seen(pc.r0 + min(32 * wave + 31, pc.rows - 1), w);
   const int any_lo = max(wa.lo, pc.begin), any_hi = min(wz.hi, pc.end);
   const int all_lo = max(wz.lo, pc.begin), all_hi = min(wa.hi, pc.end);
-  Feed<D, kExact> f;
+  typedef Feed<D, kExact, kWhole> F;
+  F f;
   f.init(w, g, s, head, lane);
   f.bad = pc.over;
   f.lo = pc.begin;
   f.hi = pc.end;
-  const int n_tiles = (pc.stop - pc.tile0 + kTile - 1) / kTile;
+  const int n_tiles = (pc.stop - pc.tile0 + kKeys - 1) / kKeys;
 
-  bool bad = false;
-  for (int safe = 0; safe < 2; safe++) {
-    a.clear();
-    const int mine_at = 16 * wave;
-    int id = 0;
-    if (n_tiles > 0) {
-      id = f.page_of(pc.tile0 + mine_at);
-      f.template issue<true, true>(pc.tile0 + mine_at, id, lds + wave * G::kGroup,
-                                   lds + (4 + wave) * G::kGroup);
-      id = f.page_of(pc.tile0 + kTile + mine_at);
-    }
-    for (int i = 0; i < n_tiles; i++) {
-      const uint32_t buf = lds + (i & 1) * G::kBuf, other = lds + (~i & 1) * G::kBuf;
-      const int p = pc.tile0 + kTile * i;
+  // K and V of tile i.  Tiles of 64 keys: each wave a group of either; of 32: two
+  // waves K, two waves V.
+  const int part = 16 * (KB == 2 ? wave : wave & 1);
+  typename F::Page ahead, behind;  // pages of the tiles whose K and V are next
+  auto bring_k = [&](int i) {
+    if (KB == 2 || wave < 2)
+      f.template issue<true>(pc.tile0 + i * kKeys + part, ahead,
+                             lds + (i & 1) * kPart + (part >> 4) * G::kGroup);
+  };
+  auto bring_v = [&](int i) {
+    if (KB == 2 || wave >= 2)
+      f.template issue<false>(pc.tile0 + i * kKeys + part, behind,
+                              lds + (2 + (i & 1)) * kPart + (part >> 4) * G::kGroup);
+  };
+  auto pages = [&](int i) {
+    behind = ahead;
+    ahead = f.template pages_of<false>(pc.tile0 + i * kKeys + part);
+  };
+  auto k_of = [&](int i) { return lds + (i & 1) * kPart; };
+  auto v_of = [&](int i) { return lds + (2 + (i & 1)) * kPart; };
+  // tiles with keys that rows of this wave see, and of which they see every key
+  const int first = any_hi > any_lo ? (any_lo - pc.tile0) / kKeys : n_tiles;
+  const int last = any_hi > any_lo ? (any_hi - pc.tile0 + kKeys - 1) / kKeys : n_tiles;
+  auto plain = [&](int i) {
+    const int p = pc.tile0 + i * kKeys;
+    return p >= all_lo && p + kKeys <= all_hi;
+  };
+  auto run = [&](auto safe) {
+    // Turn i = -1 .. n_tiles - 1: K of tile i + 1 and V of tile i are there, and
+    // nobody reads what K of i + 2 and V of i + 1 go over.  ahead = pages of tile
+    // i + 2, behind = of i + 1.
+    auto turn = [&](int i) {
       wait_all();
-      if (i + 1 < n_tiles) {
-        f.template issue<true, true>(p + kTile + mine_at, id, other + wave * G::kGroup,
-                                     other + (4 + wave) * G::kGroup);
-        id = f.page_of(p + 2 * kTile + mine_at);
-      }
-      const bool work = p < any_hi && p + kTile > any_lo;
-      f32x16 sc[2];
-      if (work) {
-        a.template scores<2>(g, buf, sc, lane);
-        a.template grow<2>(sc, p, p < all_lo || p + kTile > all_hi, lane);
-      }
-      if (safe) {
-        const uint32_t v = buf + (4 + wave) * G::kGroup;
-        if (anywhere(a.odd_values(g, v, lane), extra)) {
-          for (int j = 0; j < 4; j++)
-            a.add_odd_values(g, buf + (4 + j) * G::kGroup, p + 16 * j, lane);
+      if (i + 2 < n_tiles) bring_k(i + 2);
+      if (i + 1 < n_tiles) bring_v(i + 1);
+      pages(min(i + 3, n_tiles));
+      if constexpr (decltype(safe)::value) {
+        if (i < 0) return;
+        const uint32_t v = v_of(i), mine_v = v + (part >> 4) * G::kGroup;
+        if (anywhere(a.odd_values(g, mine_v, lane), extra)) {
+          for (int j = 0; j < 2 * KB; j++)
+            a.add_odd_values(g, v + j * G::kGroup, pc.tile0 + i * kKeys + 16 * j, lane);
           __syncthreads();
-          a.clear_odd_values(g, v, lane);
+          a.clear_odd_values(g, mine_v, lane);
           __syncthreads();
         }
       }
-      if (work) a.template gather<2>(g, buf + 4 * G::kGroup, sc);
+    };
+    a.clear();
+    if (n_tiles == 0) return;
+    ahead = f.template pages_of<false>(pc.tile0 + part);
+    bring_k(0);
+    pages(1);
+    int i = -1;
+    for (; i + 1 < first; i++) turn(i);
+    if (first < last) {
+      f32x16 sc[KB];
+      u32x4 wt[2 * KB][NP];
+      float base = 0.f;
+      turn(i);
+      a.template scores_ahead<KB, false>(g, k_of(i + 1), sc, wt, base, lane);
+      if (!plain(i + 1)) a.template hide<KB>(sc, pc.tile0 + (i + 1) * kKeys, lane);
+      a.template weigh_ahead<KB, false>(g, 0, sc, wt, base);
+      for (i++; i + 1 < last; i++) {
+        turn(i);
+        a.template scores_ahead<KB, true>(g, k_of(i + 1), sc, wt, base, lane);
+        if (!plain(i + 1)) a.template hide<KB>(sc, pc.tile0 + (i + 1) * kKeys, lane);
+        a.template weigh_ahead<KB, true>(g, v_of(i), sc, wt, base);
+      }
+      turn(i);
+      a.template sums<KB>(g, v_of(i), sc, wt, base);
+      i++;
     }
-    bad = anywhere(f.bad, extra);
-    if (bad || !anywhere(store && a.not_finite(g, lane), extra)) break;
-  }
+    for (; i < n_tiles; i++) turn(i);
+  };
+  run(std::false_type{});
+  const bool bad = anywhere(f.bad, extra);
+  if (!bad && anywhere(store && a.not_finite(g, lane), extra)) run(std::true_type{});
   const float l = bad ? __builtin_nanf("") : a.sum();
   if (bad && w.b.bad && tid == 0) *w.b.bad = 1;
   if (!store) return;
@@ -903,18 +1091,24 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
     }
 }
 
-template <typename CT, int D, bool kExact, int NP>
+template <typename CT, int D, bool kExact, bool kWhole, int NP>
 void launch_kind(const Work &w, hipStream_t s) {
   typedef Geo<D, kExact> G;
   const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));
-  if (w.few) attn_few_kernel<CT, D, kExact, NP><<<grid, kThreads, G::kSmem + G::kExtra, s>>>(w);
-  else attn_many_kernel<CT, D, kExact, NP><<<grid, kThreads, G::kSmem + G::kExtra, s>>>(w);
+  const uint32_t smem = G::kSmem + G::kExtra;
+  if (w.few) attn_few_kernel<CT, D, kExact, kWhole, NP><<<grid, kThreads, smem, s>>>(w);
+  else attn_many_kernel<CT, D, kExact, kWhole, NP><<<grid, kThreads, smem, s>>>(w);
 }
 
 template <typename CT, int D, bool kExact>
 int launch(const Work &w, bool precise, hipStream_t s) {
-  if (precise) launch_kind<CT, D, kExact, Op<CT>::kParts>(w, s);
-  else launch_kind<CT, D, kExact, 1>(w, s);
+  constexpr int kParts = Op<CT>::kParts;
+  // (heads of other sizes take every lane's own pages: the general form)
+  const bool whole = kExact && w.cache.page_shift >= 4 && w.cache.slot_stride < (1 << 25);
+  if (whole && precise) launch_kind<CT, D, kExact, kExact, kParts>(w, s);
+  else if (whole) launch_kind<CT, D, kExact, kExact, 1>(w, s);
+  else if (precise) launch_kind<CT, D, kExact, false, kParts>(w, s);
+  else launch_kind<CT, D, kExact, false, 1>(w, s);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
 
