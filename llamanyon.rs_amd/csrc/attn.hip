@@ -10,8 +10,6 @@ int swamp_attn_bf16(const swamp_attn::Work &w, bool precise, hipStream_t s);
 
 namespace {
 
-using namespace swamp_attn;
-
 constexpr int kJoinWide = 4;  // pieces up to which a thread joins them all
 
 // out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over a row's pieces, in a

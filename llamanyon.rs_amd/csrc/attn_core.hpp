@@ -67,6 +67,12 @@ struct Work {
   f32x2 *stat;     // [split][row]: (m, l); l = -1: the row sees no key at all
 };
 
+}  // namespace swamp_attn
+
+namespace {
+
+using namespace swamp_attn;
+
 // ---- LDS and DMA ----------------------------------------------------------
 // LDS is addressed by byte offset.  Not templates: the host pass rejects the
 // address-space cast inside a template instantiation.
@@ -1125,4 +1131,4 @@ int launch_dim(const Work &w, bool precise, hipStream_t s) {
                            : launch<CT, 256, false>(w, precise, s);
 }
 
-}  // namespace swamp_attn
+}  // namespace

@@ -2,5 +2,5 @@
 #include "attn_core.hpp"
 
 int swamp_attn_f16(const swamp_attn::Work &w, bool precise, hipStream_t s) {
-  return swamp_attn::launch_dim<_Float16>(w, precise, s);
+  return launch_dim<_Float16>(w, precise, s);
 }
