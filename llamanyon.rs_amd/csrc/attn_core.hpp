@@ -118,13 +118,40 @@ __device__ __forceinline__ const void *uni(const void *p) {
   const uint32_t lo = uint32_t(uni(int(uint32_t(x)))), hi = uint32_t(uni(int(x >> 32)));
   return reinterpret_cast<const void *>(uintptr_t(uint64_t(hi) << 32 | lo));
 }
-__device__ __forceinline__ void dma_uniform(const void *base, uint32_t off, uint32_t at) {
+// N of them, from base + off[j] to at + 1024 j.  The instruction's offset counts
+// for both addresses, so that one m0 serves four; off[j] holds dma_lift(j) to
+// make up for it.
+constexpr uint32_t dma_lift(int j) { return 1024u * (3 - j % 4); }
+template <int N>
+__device__ __forceinline__ void dma_uniform(const uint8_t *base, const uint32_t *off, uint32_t at) {
 #ifdef __HIP_DEVICE_COMPILE__
-  base = uni(base);
-  at = uint32_t(uni(int(at)));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(at), "v"(off), "s"(base));
+  const void *from = uni(base - dma_lift(0));
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const uint32_t to = uint32_t(uni(int(at + 1024 * j)));
+    if (N - j >= 4)
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+          "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+          "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+          "global_load_lds_dwordx4 %4, %5 offset:3072"
+          :
+          : "s"(to), "v"(off[j]), "v"(off[j + 1]), "v"(off[j + 2]), "v"(off[j + 3]), "s"(from));
+    else if (N - j == 3)
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %4\n\t"
+          "global_load_lds_dwordx4 %2, %4 offset:1024\n\t"
+          "global_load_lds_dwordx4 %3, %4 offset:2048"
+          :
+          : "s"(to), "v"(off[j]), "v"(off[j + 1]), "v"(off[j + 2]), "s"(from));
+    else
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+          "global_load_lds_dwordx4 %2, %3 offset:1024"
+          :
+          : "s"(to), "v"(off[j]), "v"(off[j + 1]), "s"(from));
+  }
+  static_assert(N % 4 != 1, "no form of one");
 #endif
 }
 __device__ __forceinline__ void dma_lane(const void *p, uint32_t at) {
@@ -228,23 +255,28 @@ struct Geo {
 };
 
 // The keys lo .. hi - 1 of one sequence and cache head, on their way into LDS.
-// kWhole: a group of 16 keys lies within a page and its offsets in 32 bits, so
-// that a group's page and address are the scalar unit's; else every lane has its
-// own.
+// kWhole: a group of 16 keys lies within a page, pages and the way from page to
+// page are below 4 GB; a group's address is then the scalar unit's.  Else every
+// lane has its own.
 template <int D, bool kExact, bool kWhole>
 struct Feed {
   typedef Geo<D, kExact> G;
   const uint8_t *k, *v;     // slot 0 of page 0 of this head
   const int32_t *table;
-  const void *stand_in;     // read in place of a page that is none
+  const void *stand_in;     // read in place of a page that is none (not kWhole)
   int64_t page_bytes, slot_bytes, cols;
   int n_pages, shift, lo, hi;
-  bool bad;                 // this lane met a position without a page
+  int bad;                  // this lane met a position without a page
   uint32_t rows;            // row of the group (0..15) of DMA j at bits 4 j
   uint32_t koff[G::NI], voff[G::NI];
 
-  struct Page {  // of a group: one id, or each lane's for its DMAs
+  // Where a group of 16 keys lies: page ids (kWhole: one, the scalar unit's; else
+  // a lane's own for each DMA), and, once they are there, the group's offset.
+  struct Place {
     int32_t id[kWhole ? 1 : G::NI];
+    int64_t at;
+    int p0;
+    bool edge;  // not all its keys are among lo .. hi - 1
   };
 
   __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane) {
@@ -257,12 +289,12 @@ struct Feed {
     cols = w.b.pages_stride;
     n_pages = w.cache.n_pages;
     shift = w.cache.page_shift;
-    bad = false;
+    bad = 0;
     rows = 0;
 #pragma unroll
     for (int j = 0; j < G::NI; j++) {
       const int i = 64 * j + lane, r = min(i / g.stride, 15), c = min(i - r * g.stride, g.nch - 1);
-      const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) : 0;
+      const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) + dma_lift(j) : 0;
       rows |= uint32_t(r) << (4 * j);
       koff[j] = row + 16 * G::k_chunk(r, c);
       voff[j] = row + 16 * G::v_chunk(r, c);
@@ -275,64 +307,74 @@ struct Feed {
                             table + uni(int(col)))
                       : -1;
   }
-  // Pages of the group at p0 (a multiple of 16), for issue().  kNow: the ids are
+  // Page ids of the group at p0 (a multiple of 16), on their way.  kNow: they are
   // needed before other loads of this wave have come in, whose wait they would
   // share as vector loads; the scalar unit then brings them page by page.
   template <bool kNow>
-  __device__ __forceinline__ Page pages_of(int p0) const {
-    Page pg;
+  __device__ __forceinline__ Place find(int p0) const {
+    Place g;
+    g.p0 = p0;
     if constexpr (kWhole) {
-      pg.id[0] = entry(swamp::page_col(within(p0), shift));
+      g.id[0] = entry(swamp::page_col(within(p0), shift));
     } else if constexpr (kNow) {
       const int first = within(p0) >> shift, last = within(p0 + 15) >> shift;
 #pragma unroll
-      for (int j = 0; j < G::NI; j++) pg.id[j] = -1;
+      for (int j = 0; j < G::NI; j++) g.id[j] = -1;
       for (int c = first; c <= last; c++) {
         const int id = entry(c);
 #pragma unroll
         for (int j = 0; j < G::NI; j++)
-          if (within(p0 + int((rows >> (4 * j)) & 15)) >> shift == c) pg.id[j] = id;
+          if (within(p0 + int((rows >> (4 * j)) & 15)) >> shift == c) g.id[j] = id;
       }
     } else {
 #pragma unroll
       for (int j = 0; j < G::NI; j++) {
         const int p = within(p0 + int((rows >> (4 * j)) & 15));
         const int64_t col = swamp::page_col(p, shift);
-        pg.id[j] = swamp::page_col_ok(p, col, cols) ? table[col] : -1;
+        g.id[j] = swamp::page_col_ok(p, col, cols) ? table[col] : -1;
       }
     }
-    return pg;
+    return g;
   }
-  // DMAs of the group at p0 to LDS: its keys (kK) or values.
+  // The ids are there.
+  __device__ __forceinline__ void arrive(Place &g) {
+    if constexpr (kWhole) {
+      const uint32_t slot = uint32_t(within(g.p0)) & ((1u << shift) - 16);
+      g.at = int64_t(uint64_t(uint32_t(g.id[0])) * uint32_t(page_bytes) +
+                     uint64_t(slot) * uint32_t(slot_bytes));
+      g.edge = g.p0 < lo || g.p0 + 15 >= hi;
+      bad |= swamp::page_ok(g.id[0], n_pages) ? 0 : 1;
+    }
+  }
+  // DMAs of the group's keys (kK) or values to LDS; kWhole: none without a page
+  // (the result is NaN then).
   template <bool kK>
-  __device__ __forceinline__ void issue(int p0, const Page &pg, uint32_t at) {
+  __device__ __forceinline__ void issue(const Place &g, uint32_t to) {
     const uint8_t *base = kK ? k : v;
     const uint32_t *off = kK ? koff : voff;
     if constexpr (kWhole) {
-      const int first = within(p0) & ~15;
-      const bool ok = swamp::page_ok(pg.id[0], n_pages);
-      const int64_t to = int64_t(pg.id[0]) * page_bytes + (first & ((1 << shift) - 1)) * slot_bytes;
-      const void *from = ok ? base + to : stand_in;
-      bad |= !ok;
-      if (!ok || p0 < lo || p0 + 15 >= hi) {
-        const uint32_t rows = fresh(this->rows);
-#pragma unroll
-        for (int j = 0; j < G::NI; j++) {
-          const int r = (rows >> (4 * j)) & 15, row = ok ? within(p0 + r) - first : 0;
-          dma_uniform(from, off[j] + uint32_t(row - r) * uint32_t(slot_bytes), at + 1024 * j);
-        }
+      if (!swamp::page_ok(g.id[0], n_pages)) return;
+      if (!g.edge) {
+        dma_uniform<G::NI>(base + g.at, off, to);
         return;
       }
+      const uint32_t rows = fresh(this->rows);
+      const int first = within(g.p0) & ~15;
+      uint32_t moved[G::NI];
 #pragma unroll
-      for (int j = 0; j < G::NI; j++) dma_uniform(from, off[j], at + 1024 * j);
+      for (int j = 0; j < G::NI; j++) {
+        const int r = (rows >> (4 * j)) & 15;
+        moved[j] = off[j] + uint32_t(within(g.p0 + r) - first - r) * uint32_t(slot_bytes);
+      }
+      dma_uniform<G::NI>(base + g.at, moved, to);
     } else {
 #pragma unroll
       for (int j = 0; j < G::NI; j++) {
-        const int p = within(p0 + int((rows >> (4 * j)) & 15));
-        const bool ok = swamp::page_ok(pg.id[j], n_pages);
-        const int64_t to = int64_t(pg.id[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
-        bad |= !ok;
-        dma_lane((ok ? base + to : static_cast<const uint8_t *>(stand_in)) + off[j], at + 1024 * j);
+        const int p = within(g.p0 + int((rows >> (4 * j)) & 15));
+        const bool ok = swamp::page_ok(g.id[j], n_pages);
+        const int64_t at = int64_t(g.id[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
+        bad |= ok ? 0 : 1;
+        dma_lane((ok ? base + at : static_cast<const uint8_t *>(stand_in)) + off[j], to + 1024 * j);
       }
     }
   }
@@ -841,22 +883,24 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   for (int safe = 0; safe < 2; safe++) {
     a.clear();
     int p = pc.tile0 + 32 * wave;
-    typename F::Page pg[2];
+    typename F::Place at[2];
     if (p < pc.stop) {
 #pragma unroll
+      for (int i = 0; i < 2; i++) at[i] = f.template find<true>(p + 16 * i);
+#pragma unroll
       for (int i = 0; i < 2; i++) {
-        pg[i] = f.template pages_of<true>(p + 16 * i);
-        f.template issue<true>(p + 16 * i, pg[i], at_k + i * G::kGroup);
+        f.arrive(at[i]);
+        f.template issue<true>(at[i], at_k + i * G::kGroup);
       }
 #pragma unroll
-      for (int i = 0; i < 2; i++) f.template issue<false>(p + 16 * i, pg[i], at_v + i * G::kGroup);
+      for (int i = 0; i < 2; i++) f.template issue<false>(at[i], at_v + i * G::kGroup);
     }
     while (p < pc.stop) {
       const int next = p + 32 * kWaves;
       const bool more = next < pc.stop;
       if (more) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) pg[i] = f.template pages_of<true>(next + 16 * i);
+        for (int i = 0; i < 2; i++) at[i] = f.template find<true>(next + 16 * i);
       }
       f32x16 sc[1];
       wait_dma<2 * G::NI>();
@@ -864,8 +908,10 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
       lds_done();
       if (more) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-          f.template issue<true>(next + 16 * i, pg[i], at_k + i * G::kGroup);
+        for (int i = 0; i < 2; i++) {
+          f.arrive(at[i]);
+          f.template issue<true>(at[i], at_k + i * G::kGroup);
+        }
       }
       if (p < all_lo || p + 32 > all_hi) a.template hide<1>(sc, p, lane);
       a.grow(a.template largest<1>(sc));
@@ -884,8 +930,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
       lds_done();
       if (more) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-          f.template issue<false>(next + 16 * i, pg[i], at_v + i * G::kGroup);
+        for (int i = 0; i < 2; i++) f.template issue<false>(at[i], at_v + i * G::kGroup);
       }
       p = next;
     }
@@ -1003,21 +1048,15 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
   // K and V of tile i.  Tiles of 64 keys: each wave a group of either; of 32: two
   // waves K, two waves V.
   const int part = 16 * (KB == 2 ? wave : wave & 1);
-  typename F::Page ahead, behind;  // pages of the tiles whose K and V are next
+  typename F::Place ahead, behind;  // of the tiles whose K and V are next
+  const uint32_t part_at = lds + (part >> 4) * G::kGroup;
   auto bring_k = [&](int i) {
-    if (KB == 2 || wave < 2)
-      f.template issue<true>(pc.tile0 + i * kKeys + part, ahead,
-                             lds + (i & 1) * kPart + (part >> 4) * G::kGroup);
+    if (KB == 2 || wave < 2) f.template issue<true>(ahead, part_at + (i & 1) * kPart);
   };
   auto bring_v = [&](int i) {
-    if (KB == 2 || wave >= 2)
-      f.template issue<false>(pc.tile0 + i * kKeys + part, behind,
-                              lds + (2 + (i & 1)) * kPart + (part >> 4) * G::kGroup);
+    if (KB == 2 || wave >= 2) f.template issue<false>(behind, part_at + (2 + (i & 1)) * kPart);
   };
-  auto pages = [&](int i) {
-    behind = ahead;
-    ahead = f.template pages_of<false>(pc.tile0 + i * kKeys + part);
-  };
+  auto find = [&](int i) { return f.template find<false>(pc.tile0 + i * kKeys + part); };
   auto k_of = [&](int i) { return lds + (i & 1) * kPart; };
   auto v_of = [&](int i) { return lds + (2 + (i & 1)) * kPart; };
   // tiles with keys that rows of this wave see, and of which they see every key
@@ -1029,13 +1068,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
   };
   auto run = [&](auto safe) {
     // Turn i = -1 .. n_tiles - 1: K of tile i + 1 and V of tile i are there, and
-    // nobody reads what K of i + 2 and V of i + 1 go over.  ahead = pages of tile
-    // i + 2, behind = of i + 1.
+    // nobody reads what K of i + 2 and V of i + 1 go over.  ahead = the place of
+    // tile i + 2, behind = of i + 1.
     auto turn = [&](int i) {
       wait_all();
+      if (i + 2 < n_tiles) f.arrive(ahead);
+      const typename F::Place then = find(min(i + 3, n_tiles));
       if (i + 2 < n_tiles) bring_k(i + 2);
       if (i + 1 < n_tiles) bring_v(i + 1);
-      pages(min(i + 3, n_tiles));
+      behind = ahead;
+      ahead = then;
       if constexpr (decltype(safe)::value) {
         if (i < 0) return;
         const uint32_t v = v_of(i), mine_v = v + (part >> 4) * G::kGroup;
@@ -1050,9 +1092,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
     };
     a.clear();
     if (n_tiles == 0) return;
-    ahead = f.template pages_of<false>(pc.tile0 + part);
+    ahead = find(0);
+    f.arrive(ahead);
     bring_k(0);
-    pages(1);
+    behind = ahead;
+    ahead = find(1);
     int i = -1;
     for (; i + 1 < first; i++) turn(i);
     if (first < last) {
@@ -1110,7 +1154,9 @@ template <typename CT, int D, bool kExact>
 int launch(const Work &w, bool precise, hipStream_t s) {
   constexpr int kParts = Op<CT>::kParts;
   // (heads of other sizes take every lane's own pages: the general form)
-  const bool whole = kExact && w.cache.page_shift >= 4 && w.cache.slot_stride < (1 << 25);
+  const bool whole = kExact && w.cache.page_shift >= 4 &&
+                     w.cache.page_stride < (int64_t(1) << 31) &&
+                     (w.cache.slot_stride << w.cache.page_shift) < (int64_t(1) << 30);
   if (whole && precise) launch_kind<CT, D, kExact, kExact, kParts>(w, s);
   else if (whole) launch_kind<CT, D, kExact, kExact, 1>(w, s);
   else if (precise) launch_kind<CT, D, kExact, false, kParts>(w, s);
