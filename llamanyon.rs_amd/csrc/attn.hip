@@ -10,108 +10,129 @@ int swamp_attn_bf16(const swamp_attn::Work &w, bool precise, hipStream_t s);
 
 namespace {
 
-constexpr int kJoinWide = 4;  // pieces up to which a thread joins them all
-
-// out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over a row's pieces, in a
-// fixed order.
-
-// A thread takes four dims of a row and all pieces.
-__global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
-  const int per = w.cache.dim >> 2;
-  const int64_t n = int64_t(w.b.n_tok) * w.n_heads;  // rows of a piece
-  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t row = i / per;
-  const int d = int(i - row * per) * 4;
-  const int64_t t = row / w.n_heads;
-  if (row >= n || t < w.b.first[0] || t >= w.b.first[w.b.n_seq]) return;  // padding
-  float top = -INFINITY;
-#pragma unroll 8
-  for (int x = 0; x < w.splits; x++) top = fmaxf(top, w.stat[x * n + row][0]);
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  bool sees = true;
-#pragma unroll 4
-  for (int x = 0; x < w.splits; x++) {
-    const f32x2 st = w.stat[x * n + row];
-    const float k = __builtin_amdgcn_exp2f(st[0] - base);
-    sees = sees && st[1] != -1.f;
-    sum += k * st[1];
-    if (st[0] != -INFINITY)
-      acc += k * *reinterpret_cast<const f32x4 *>(w.part + (x * n + row) * w.cache.dim + d);
-  }
-  put4(w, t, int(row - t * w.n_heads), w.cache.dim, d,
-       sees ? acc * (1.f / sum) : f32x4{0.f, 0.f, 0.f, 0.f});
-}
-
-// A workgroup takes a row: `per` threads (dim / 4 rounded up to a power of two)
-// for the dims, 256 / per shares of the pieces.  For few rows in many pieces,
-// whose loads would otherwise wait for one another.
-__global__ void __launch_bounds__(kThreads) join_wide_kernel(Work w, int per) {
+// out = sum_x 2^(m_x - m) o_x / sum_x 2^(m_x - m) l_x over the pieces x of a row, in
+// a fixed order.  `per` threads (dim / 4 rounded up to a power of two) times
+// `shares` take a row: four dims and one run of the pieces each, kBatch pieces'
+// loads at a time, and the runs meet in LDS.
+//
+// A kernel of its own.  Joined by the last workgroup of each row instead (a
+// counter, and sums that bypass the L2 of an XCD, which others do not see), 64
+// sequences of up to 8192 tokens in 4 pieces took 279 us against 231, one of
+// 131072 in 32 pieces 117 against 100, and 700 tokens 12 as now.
+template <int kBatch>
+__global__ void __launch_bounds__(kThreads) join_kernel(Work w, int per, int shares) {
   __shared__ f32x4 accs[kThreads];
-  __shared__ float sums[kThreads], tops[kWaves];
-  __shared__ int blind;
-  const int64_t n = int64_t(w.b.n_tok) * w.n_heads, row = blockIdx.x, t = row / w.n_heads;
-  if (t < w.b.first[0] || t >= w.b.first[w.b.n_seq]) return;  // padding
-  const int tid = int(threadIdx.x), share = tid / per, shares = kThreads / per;
-  const int d = 4 * (tid - share * per);
-  float top = -INFINITY;
-  for (int x = tid; x < w.splits; x += kThreads) top = fmaxf(top, w.stat[x * n + row][0]);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if ((tid & 63) == 0) tops[tid >> 6] = top;
-  if (tid == 0) blind = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWaves; i++) top = fmaxf(top, tops[i]);
-  const float base = top == -INFINITY ? 0.f : top;
+  __shared__ f32x2 stats[kThreads];
+  const int tid = int(threadIdx.x), team = per * shares;
+  const int64_t n = int64_t(w.b.n_tok) * w.n_heads;
+  const int64_t row = int64_t(blockIdx.x) * (kThreads / team) + tid / team, t = row / w.n_heads;
+  const int share = tid % team / per, d = 4 * (tid % per), dim = w.cache.dim;
+  // (rows of no sequence are not touched)
+  const bool mine = row < n && d < dim && t >= w.b.first[0] && t < w.b.first[w.b.n_seq];
+  const int run = (w.splits + shares - 1) / shares;
+  const int x1 = min((share + 1) * run, w.splits);
+  float m = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-#pragma unroll 4
-  for (int x = share; x < w.splits; x += shares) {
-    const f32x2 st = w.stat[x * n + row];
-    const float k = __builtin_amdgcn_exp2f(st[0] - base);
-    if (st[1] == -1.f) blind = 1;
-    sum += k * st[1];
-    if (st[0] != -INFINITY && d < w.cache.dim)
-      acc += k * *reinterpret_cast<const f32x4 *>(w.part + (x * n + row) * w.cache.dim + d);
+  bool sees = true;
+  for (int x0 = share * run; mine && x0 < x1; x0 += kBatch) {
+    f32x2 st[kBatch];
+    f32x4 o[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      const int64_t at = min(x0 + i, x1 - 1) * n + row;
+      st[i] = w.stat[at];
+      o[i] = *reinterpret_cast<const f32x4 *>(w.part + at * dim + d);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) top = fmaxf(top, st[i][0]);
+    const float base = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - base);
+    m = top;
+    acc *= keep;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      if (x0 + i >= x1) break;
+      const float k = __builtin_amdgcn_exp2f(st[i][0] - base);
+      sees = sees && st[i][1] != -1.f;
+      l += k * st[i][1];
+      if (st[i][0] != -INFINITY) acc += k * o[i];  // (else nothing was written)
+    }
   }
-  accs[tid] = acc;
-  sums[tid] = sum;
-  __syncthreads();
-  if (share != 0 || d >= w.cache.dim) return;
-  for (int i = 1; i < shares; i++) {
-    acc += accs[i * per + tid];
-    sum += sums[i * per + tid];
+  if (shares > 1) {
+    accs[tid] = acc;
+    stats[tid] = f32x2{m, l};
+    __syncthreads();
+    if (share == 0) {
+      float top = m;
+      for (int i = 1; i < shares; i++) top = fmaxf(top, stats[tid + i * per][0]);
+      const float base = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - base);
+      acc *= keep;
+      l *= keep;
+      for (int i = 1; i < shares; i++) {
+        const f32x2 st = stats[tid + i * per];
+        const float k = __builtin_amdgcn_exp2f(st[0] - base);
+        l += k * st[1];
+        if (st[0] != -INFINITY) acc += k * accs[tid + i * per];
+      }
+    }
   }
-  put4(w, t, int(row - t * w.n_heads), w.cache.dim, d,
-       blind ? f32x4{0.f, 0.f, 0.f, 0.f} : acc * (1.f / sum));
+  if (mine && share == 0)
+    put4(w, t, int(row - t * w.n_heads), dim, d,
+         sees ? acc * (1.f / l) : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
 struct Plan {
   int blocks, one_block, few, splits, chunk;
 };
 
+// Pieces of the keys that make attn_many_kernel shortest, by a model of its time
+// on this card, us: a tile takes 0.55 + 0.007 dim where a CU has one workgroup
+// and 0.6 more for each further one (heads of 128: 1.45 and 2.06 us measured), a
+// workgroup's start and end three tiles, and a join 4 us and its sums' way
+// through memory.
+int many_splits(int64_t base, int64_t rows, int64_t keys, int dim, int cus) {
+  const int most = dim <= 64 ? 3 : dim <= 128 ? 2 : 1;  // workgroups of a CU
+  const double tiles = double(keys) / kTile;
+  double best = 0;
+  int want = 1;
+  for (int n = 1; n <= 16 && n <= std::max<int64_t>(1, keys / (4 * kTile)); n++) {
+    const int64_t load = std::min<int64_t>(most, (base * n + cus - 1) / cus);
+    const double rounds = std::max(1.0, double(base) * n / (double(cus) * most));
+    double t = rounds * (tiles / n + 3) * (0.55 + 0.007 * dim + 0.6 * double(load - 1));
+    if (n > 1) t += 4 + n * double(rows) * dim * 8 / 6e6;
+    if (n == 1 || t < best) best = t, want = n;
+  }
+  return want;
+}
+
 // blocks: at most this many, of all sequences, whatever the rows' distribution.
 Plan plan_of(const swamp::AttnCall &c) {
-  const int group = c.n_heads / c.cache.n_kv;
-  const int64_t rows = int64_t(c.batch.n_tok) * group;
-  const int64_t most = (int64_t(c.max_new) * group + kRows - 1) / kRows;  // of a sequence
+  const int group = c.n_heads / c.cache.n_kv, cus = swamp::device_info().num_cus;
+  const int64_t rows = int64_t(c.batch.n_tok) * group;  // of a cache head
+  const int64_t most = (int64_t(c.max_new) * group + kRows - 1) / kRows;  // blocks of a sequence
   Plan p;
+  p.few = int64_t(c.max_new) * group <= kFew;
   p.one_block = most <= 1;
   p.blocks = int(p.one_block ? c.batch.n_seq
                              : std::min((rows + int64_t(kRows - 1) * c.batch.n_seq) / kRows,
                                         most * c.batch.n_seq));
-  p.few = int64_t(c.max_new) * group <= kFew;
-  const int slots = swamp::device_info().num_cus * (c.cache.dim <= 128 ? 2 : 1);
-  const int64_t base = int64_t(p.blocks) * c.cache.n_kv;
-  const int64_t keys =
-      c.window ? std::min<int64_t>(c.max_len, int64_t(c.window) + c.max_new) : c.max_len;
-  const int64_t least = p.few ? 2 * kTile : 4 * kTile;
-  int64_t want = std::max<int64_t>(1, (p.few ? 2 : 1) * slots / std::max<int64_t>(base, 1));
-  want = std::max<int64_t>(1, std::min<int64_t>(want, keys / least));
-  p.chunk = int((((keys + want - 1) / want + 2 * kTile - 1) / (2 * kTile)) * 2 * kTile);
-  p.chunk = std::max(p.chunk, 2 * kTile);
+  const int64_t base = std::max<int64_t>(1, int64_t(p.blocks) * c.cache.n_kv);
+  const int64_t seen = int64_t(c.window) + (p.few ? c.max_new : kRows / group) + kTile;
+  const int64_t keys = c.window ? std::min<int64_t>(c.max_len, seen) : c.max_len;
+  int64_t want;
+  if (p.few)
+    // one workgroup a CU (64 workgroups over 4001 keys: 256 in all 22.4 us, 512
+    // 25.2, 64 60), and pieces that even out sequences of unequal length (256 over
+    // up to 6000 keys: 2048 each 39.9 us, whole 47.0)
+    want = std::max(cus / base, keys / 2048);
+  else
+    want = many_splits(base, rows * c.cache.n_kv, keys, c.cache.dim, cus);
+  // a piece is whole tiles; of a few rows one for each wave at least
+  const int step = p.few ? 32 * kWaves : kTile;
+  want = std::max<int64_t>(1, want);
+  p.chunk = int(((keys + want - 1) / want + step - 1) / step * step);
+  p.chunk = std::max(p.chunk, step);
   p.splits = int(std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk));
   return p;
 }
@@ -161,14 +182,12 @@ int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStr
   const bool precise = c.out_type == SWAMP_F32;
   const int rc = c.dtype == SWAMP_F16 ? swamp_attn_f16(w, precise, s) : swamp_attn_bf16(w, precise, s);
   if (rc != SWAMP_OK || w.splits == 1) return rc;
-  const int64_t rows = int64_t(c.batch.n_tok) * c.n_heads;
-  if (w.splits > kJoinWide) {
-    int per = 2;
-    while (4 * per < c.cache.dim) per *= 2;
-    join_wide_kernel<<<dim3(unsigned(rows)), kThreads, 0, s>>>(w, per);
-  } else {
-    const int64_t n = rows * (c.cache.dim / 4);
-    join_kernel<<<dim3(unsigned((n + kThreads - 1) / kThreads)), kThreads, 0, s>>>(w);
-  }
+  int per = 2, shares = 1;
+  while (4 * per < c.cache.dim) per *= 2;
+  while (shares * 2 * per <= kThreads && shares * 8 < w.splits) shares *= 2;
+  const int64_t rows = int64_t(c.batch.n_tok) * c.n_heads, each = kThreads / (per * shares);
+  const dim3 grid(unsigned((rows + each - 1) / each));
+  if (w.splits <= 4) join_kernel<4><<<grid, kThreads, 0, s>>>(w, per, shares);
+  else join_kernel<8><<<grid, kThreads, 0, s>>>(w, per, shares);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
