@@ -579,6 +579,7 @@ struct Rows {
     constexpr int kSteps = KB * G::KS, kRing = 4;
     const uint32_t at = k + k_at;
     s16x8 ring[kRing];
+    f32x16 other = {};
 #pragma unroll
     for (int f = 0; f < kRing; f++) ring[f] = k_frag(at, f % G::KS, f / G::KS);
     __builtin_amdgcn_sched_barrier(0);
@@ -587,8 +588,10 @@ struct Rows {
       const int kb = f / G::KS, ks = f % G::KS;
       s16x8 a = ring[f % kRing];
       if (!kExact && 2 * ks + (lane >> 5) >= g.nch) a = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (ks == 0) s[kb] = O::mma(a, q[ks], f32x16{});
-      else s[kb] = O::mma(a, q[ks], s[kb]);
+      // (KB 1: one wave a SIMD, so that a chain of products each on the last's
+      // result would leave the pipe idle: two chains)
+      if (KB == 1 && ks % 2 == 1) other = O::mma(a, q[ks], ks == 1 ? f32x16{} : other);
+      else s[kb] = O::mma(a, q[ks], ks == 0 ? f32x16{} : s[kb]);
       if (f + kRing < kSteps)
         ring[f % kRing] = k_frag(at, (f + kRing) % G::KS, (f + kRing) / G::KS);
       if (KB == 2 && kPending && kb == 0) {
@@ -596,6 +599,10 @@ struct Rows {
         for (int j = 4 * ks / G::KS; j < 4 * (ks + 1) / G::KS; j++) weigh(s, 3, j, base, p[3]);
       }
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if (KB == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[0][i] += other[i];
     }
   }
   // The maximum over the scores s, then the weights of all groups but a pending
@@ -656,6 +663,17 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 16; i++) o[db][i] *= keep;
     }
+    if (kSums) stay();
+  }
+  // Sums of heads above 128 dims keep to the accumulator registers: with the rest
+  // they would not fit, and the compiler moves all of them forth and back.
+  __device__ __forceinline__ void stay() {
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (D > 128) {
+#pragma unroll
+      for (int db = 0; db < G::DB; db++) asm volatile("" : "+a"(o[db]));
+    }
+#endif
   }
   // The last tile's sums.
   template <int KB>
