@@ -257,15 +257,16 @@ struct Geo {
 // The keys lo .. hi - 1 of one sequence and cache head, on their way into LDS.
 // kWhole: a group of 16 keys lies within a page, pages and the way from page to
 // page are below 4 GB; a group's address is then the scalar unit's.  Else every
-// lane has its own.
+// lane has its own, and reads page 0 in place of one that is none (q's first row
+// where the cache has no pages).
 template <int D, bool kExact, bool kWhole>
 struct Feed {
   typedef Geo<D, kExact> G;
   const uint8_t *k, *v;     // slot 0 of page 0 of this head
   const int32_t *table;
-  const void *stand_in;     // read in place of a page that is none (not kWhole)
   int64_t page_bytes, slot_bytes, cols;
   int n_pages, shift, lo, hi;
+  bool near;                // page_bytes and a group's way in a page fit 32 bits
   int bad;                  // this lane met a position without a page
   uint32_t rows;            // row of the group (0..15) of DMA j at bits 4 j
   uint32_t koff[G::NI], voff[G::NI];
@@ -274,32 +275,41 @@ struct Feed {
   // a lane's own for each DMA), and, once they are there, the group's offset.
   struct Place {
     int32_t id[kWhole ? 1 : G::NI];
-    int64_t at;
+    int64_t at[kWhole ? 1 : G::NI];
     int p0;
-    bool edge;  // not all its keys are among lo .. hi - 1
   };
 
   __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane) {
     k = reinterpret_cast<const uint8_t *>(w.cache.k + int64_t(head) * w.cache.head_stride);
     v = reinterpret_cast<const uint8_t *>(w.cache.v + int64_t(head) * w.cache.head_stride);
     table = w.b.pages + int64_t(s) * w.b.pages_stride;
-    stand_in = w.q;
     page_bytes = w.cache.page_stride * 2;
     slot_bytes = w.cache.slot_stride * 2;
     cols = w.b.pages_stride;
     n_pages = w.cache.n_pages;
+    if (!kWhole && n_pages == 0) {
+      k = v = reinterpret_cast<const uint8_t *>(w.q);
+      page_bytes = slot_bytes = 0;
+    }
     shift = w.cache.page_shift;
+    near = (page_bytes >> 32) == 0 && slot_bytes < (1 << 26) && shift <= 4;
     bad = 0;
     rows = 0;
 #pragma unroll
     for (int j = 0; j < G::NI; j++) {
       const int i = 64 * j + lane, r = min(i / g.stride, 15), c = min(i - r * g.stride, g.nch - 1);
-      const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) + dma_lift(j) : 0;
+      // a row's way within its page (kWhole: within its group), where it fits
+      const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) + dma_lift(j)
+                           : near ? uint32_t(r & ((1 << shift) - 1)) * uint32_t(slot_bytes)
+                                  : 0;
       rows |= uint32_t(r) << (4 * j);
       koff[j] = row + 16 * G::k_chunk(r, c);
       voff[j] = row + 16 * G::v_chunk(r, c);
     }
   }
+  __device__ __forceinline__ int row_of(int j) const { return int((rows >> (4 * j)) & 15); }
+  // All 16 keys from p0 on are among lo .. hi - 1.
+  __device__ __forceinline__ bool inside(int p0) const { return p0 >= lo && p0 + 15 < hi; }
   __device__ __forceinline__ int within(int p) const { return min(max(p, lo), hi - 1); }
   // Entry `col` of the page table, by the scalar unit; -1 past its end.
   __device__ __forceinline__ int entry(int64_t col) const {
@@ -324,9 +334,14 @@ struct Feed {
         const int id = entry(c);
 #pragma unroll
         for (int j = 0; j < G::NI; j++)
-          if (within(p0 + int((rows >> (4 * j)) & 15)) >> shift == c) g.id[j] = id;
+          if (within(p0 + row_of(j)) >> shift == c) g.id[j] = id;
       }
+    } else if (inside(p0) && swamp::page_col_ok(p0, swamp::page_col(p0 + 15, shift), cols)) {
+      const int32_t *from = table + swamp::page_col(p0, shift);
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) g.id[j] = from[uint32_t(row_of(j)) >> shift];
     } else {
+      const uint32_t rows = fresh(this->rows);
 #pragma unroll
       for (int j = 0; j < G::NI; j++) {
         const int p = within(p0 + int((rows >> (4 * j)) & 15));
@@ -340,10 +355,29 @@ struct Feed {
   __device__ __forceinline__ void arrive(Place &g) {
     if constexpr (kWhole) {
       const uint32_t slot = uint32_t(within(g.p0)) & ((1u << shift) - 16);
-      g.at = int64_t(uint64_t(uint32_t(g.id[0])) * uint32_t(page_bytes) +
-                     uint64_t(slot) * uint32_t(slot_bytes));
-      g.edge = g.p0 < lo || g.p0 + 15 >= hi;
+      g.at[0] = int64_t(uint64_t(uint32_t(g.id[0])) * uint32_t(page_bytes) +
+                        uint64_t(slot) * uint32_t(slot_bytes));
       bad |= swamp::page_ok(g.id[0], n_pages) ? 0 : 1;
+    } else {
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) {
+        const bool ok = swamp::page_ok(g.id[j], n_pages);
+        bad |= ok ? 0 : 1;
+        if (!ok) g.id[j] = 0;
+      }
+      if (near && inside(g.p0)) {
+#pragma unroll
+        for (int j = 0; j < G::NI; j++)
+          g.at[j] = int64_t(uint64_t(uint32_t(g.id[j])) * uint32_t(page_bytes));
+      } else {
+        const uint32_t rows = fresh(this->rows);
+        const int in_page = (1 << shift) - 1;
+#pragma unroll
+        for (int j = 0; j < G::NI; j++) {
+          const int r = (rows >> (4 * j)) & 15, slot = within(g.p0 + r) & in_page;
+          g.at[j] = g.id[j] * page_bytes + (slot - (near ? r & in_page : 0)) * slot_bytes;
+        }
+      }
     }
   }
   // DMAs of the group's keys (kK) or values to LDS; kWhole: none without a page
@@ -354,8 +388,8 @@ struct Feed {
     const uint32_t *off = kK ? koff : voff;
     if constexpr (kWhole) {
       if (!swamp::page_ok(g.id[0], n_pages)) return;
-      if (!g.edge) {
-        dma_uniform<G::NI>(base + g.at, off, to);
+      if (inside(g.p0)) {
+        dma_uniform<G::NI>(base + g.at[0], off, to);
         return;
       }
       const uint32_t rows = fresh(this->rows);
@@ -366,16 +400,10 @@ struct Feed {
         const int r = (rows >> (4 * j)) & 15;
         moved[j] = off[j] + uint32_t(within(g.p0 + r) - first - r) * uint32_t(slot_bytes);
       }
-      dma_uniform<G::NI>(base + g.at, moved, to);
+      dma_uniform<G::NI>(base + g.at[0], moved, to);
     } else {
 #pragma unroll
-      for (int j = 0; j < G::NI; j++) {
-        const int p = within(g.p0 + int((rows >> (4 * j)) & 15));
-        const bool ok = swamp::page_ok(g.id[j], n_pages);
-        const int64_t at = int64_t(g.id[j]) * page_bytes + (p & ((1 << shift) - 1)) * slot_bytes;
-        bad |= ok ? 0 : 1;
-        dma_lane((ok ? base + at : static_cast<const uint8_t *>(stand_in)) + off[j], to + 1024 * j);
-      }
+      for (int j = 0; j < G::NI; j++) dma_lane(base + g.at[j] + off[j], to + 1024 * j);
     }
   }
 };
