@@ -370,8 +370,8 @@ typedef struct swamp_kv_pages {
  *     being right.
  *   d_bad (may be NULL): set to 1 where a position of a sequence that the call
  *     has to read or write has no page (a table entry outside 0 .. n_pages - 1,
- *     a position past the table or before 0).  No memory outside the pages is
- *     touched then. */
+ *     a position past the table or before 0; in attention also one of the last
+ *     512 below 2^31).  No memory outside the pages is touched then. */
 typedef struct swamp_seq_batch {
   int32_t n_seq, n_tok, max_new, max_len;
   const int32_t *d_first, *d_len, *d_pages;

@@ -21,6 +21,16 @@
 // fragment read in different banks; V: the four rows of a transposing read),
 // other dims take an odd stride of chunks instead.
 //
+// Bounds and measures.  Decoding is HBM's: all keys once, 5.2 to 5.4 TB/s of the
+// 6.0 that a long read reaches (one token over 131072 keys 100 us).  Prompts are
+// the matrix pipe's and its power's: 4096 tokens of 64 heads of 128 dims take 274
+// us, 1000 TFLOP/s, where a bf16 product of the library reaches 1130 to 1230; of
+// 296 us on a slower card the exponentials cost 19, the DMAs 33, and what is left
+// without them, products, maximum and conversion, runs at 1175 TFLOP/s.  Two waves a
+// SIMD (203 registers) fill each other's gaps; blocks of 256 rows in workgroups of
+// eight waves halve the DMAs and lost more to their common barrier (64 dims: 93 ->
+// 107 us).
+//
 // Rows outside a block's keys are loaded from its nearest key: their weights
 // are 0 and what they hold is finite wherever the keys are.  A weight of 0 times
 // an infinity or NaN that only OTHER rows see would still spoil a row.  So a
@@ -107,17 +117,18 @@ __device__ __forceinline__ s16x4 lds_tr(uint32_t at, uint32_t off) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(SWAMP_LDS(s16x4, at, off));
 }
 
-// 16 bytes a lane into LDS (lane L writes at + 16 L).  Written as assembly
-// because the compiler waits for every DMA in flight before it lets a
-// transposing read pass; these have no output register, and every read of what
-// they bring stands behind a wait of wait_dma or wait_all.  (m0 has no other
-// user in these kernels.)
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ const void *uni(const void *p) {
   const uint64_t x = uint64_t(uintptr_t(p));
   const uint32_t lo = uint32_t(uni(int(uint32_t(x)))), hi = uint32_t(uni(int(x >> 32)));
   return reinterpret_cast<const void *>(uintptr_t(uint64_t(hi) << 32 | lo));
 }
+
+// DMA, 16 bytes a lane into LDS (lane L writes at + 16 L).  Written as assembly
+// because the compiler waits for every DMA in flight before it lets a transposing
+// read pass.  They have no output register, every read of what they bring stands
+// behind a wait of wait_dma or wait_all, and m0 has no other user in these kernels.
+//
 // N of them, from base + off[j] to at + 1024 j.  The instruction's offset counts
 // for both addresses, so that one m0 serves four; off[j] holds dma_lift(j) to
 // make up for it.
@@ -154,6 +165,7 @@ __device__ __forceinline__ void dma_uniform(const uint8_t *base, const uint32_t 
   static_assert(N % 4 != 1, "no form of one");
 #endif
 }
+// One, with every lane's own address.
 __device__ __forceinline__ void dma_lane(const void *p, uint32_t at) {
 #ifdef __HIP_DEVICE_COMPILE__
   at = uint32_t(uni(int(at)));
@@ -292,15 +304,16 @@ struct Feed {
       page_bytes = slot_bytes = 0;
     }
     shift = w.cache.page_shift;
-    near = (page_bytes >> 32) == 0 && slot_bytes < (1 << 26) && shift <= 4;
+    near = (page_bytes >> 32) == 0 && slot_bytes < (1 << 26);
+    const int in_page = min((1 << shift) - 1, 15);
     bad = 0;
     rows = 0;
 #pragma unroll
     for (int j = 0; j < G::NI; j++) {
       const int i = 64 * j + lane, r = min(i / g.stride, 15), c = min(i - r * g.stride, g.nch - 1);
-      // a row's way within its page (kWhole: within its group), where it fits
+      // a row's way within its group's part of a page, where it fits
       const uint32_t row = kWhole ? uint32_t(r) * uint32_t(slot_bytes) + dma_lift(j)
-                           : near ? uint32_t(r & ((1 << shift) - 1)) * uint32_t(slot_bytes)
+                           : near ? uint32_t(r & in_page) * uint32_t(slot_bytes)
                                   : 0;
       rows |= uint32_t(r) << (4 * j);
       koff[j] = row + 16 * G::k_chunk(r, c);
@@ -365,17 +378,18 @@ struct Feed {
         bad |= ok ? 0 : 1;
         if (!ok) g.id[j] = 0;
       }
+      const int in_page = (1 << shift) - 1;
       if (near && inside(g.p0)) {
+        const int64_t first = (g.p0 & in_page) * slot_bytes;
 #pragma unroll
         for (int j = 0; j < G::NI; j++)
-          g.at[j] = int64_t(uint64_t(uint32_t(g.id[j])) * uint32_t(page_bytes));
+          g.at[j] = first + int64_t(uint64_t(uint32_t(g.id[j])) * uint32_t(page_bytes));
       } else {
         const uint32_t rows = fresh(this->rows);
-        const int in_page = (1 << shift) - 1;
 #pragma unroll
         for (int j = 0; j < G::NI; j++) {
           const int r = (rows >> (4 * j)) & 15, slot = within(g.p0 + r) & in_page;
-          g.at[j] = g.id[j] * page_bytes + (slot - (near ? r & in_page : 0)) * slot_bytes;
+          g.at[j] = g.id[j] * page_bytes + (slot - (near ? r & in_page & 15 : 0)) * slot_bytes;
         }
       }
     }
@@ -869,7 +883,8 @@ __device__ __forceinline__ bool find_piece(const Work &w, int s, int64_t r0, int
   const swamp::Span ka = p.seen(r0, w), kz = p.seen(r0 + p.rows - 1, w);
   // positions that the page table cannot hold are not walked; nor are the last
   // below 2^31, so that a tile's end fits
-  const int64_t room = min(w.b.pages_stride << w.cache.page_shift, (int64_t(1) << 31) - 512);
+  const int64_t room = min(min(w.b.pages_stride, int64_t(1) << 31) << w.cache.page_shift,
+                           (int64_t(1) << 31) - 512);
   const int last = int(min(int64_t(kz.hi), room));
   const int64_t from = (ka.lo & ~(kTile - 1)) + int64_t(split) * w.chunk;
   p.over = kz.hi > room;
