@@ -122,10 +122,12 @@ Plan plan_of(const swamp::AttnCall &c) {
   const int64_t keys = c.window ? std::min<int64_t>(c.max_len, seen) : c.max_len;
   int64_t want;
   if (p.few)
+    // none below the time of the join (8 workgroups, 128 dims, 512 keys: whole 9.6
+    // us, in pieces 11.1; 1024 keys: 14.2 and 10.8; 64 dims, 1024 keys: 10.6 and 11);
     // one workgroup a CU (64 workgroups over 4001 keys: 256 in all 22.4 us, 512
     // 25.2, 64 60), and pieces that even out sequences of unequal length (256 over
     // up to 6000 keys: 2048 each 39.9 us, whole 47.0)
-    want = std::max(cus / base, keys / 2048);
+    want = keys * c.cache.dim <= 65536 ? 1 : std::max(cus / base, keys / 2048);
   else
     want = many_splits(base, rows * c.cache.n_kv, keys, c.cache.dim, cus);
   // a piece is whole tiles; of a few rows one for each wave at least

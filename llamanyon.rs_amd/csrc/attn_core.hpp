@@ -283,11 +283,11 @@ struct Feed {
   uint32_t rows;            // row of the group (0..15) of DMA j at bits 4 j
   uint32_t koff[G::NI], voff[G::NI];
 
-  // Where a group of 16 keys lies: page ids (kWhole: one, the scalar unit's; else
-  // a lane's own for each DMA), and, once they are there, the group's offset.
+  // Where a group of 16 keys lies: page ids (kWhole: one, the scalar unit's, and,
+  // once it is there, the group's offset; else a lane's own for each DMA).
   struct Place {
     int32_t id[kWhole ? 1 : G::NI];
-    int64_t at[kWhole ? 1 : G::NI];
+    int64_t at;
     int p0;
   };
 
@@ -368,8 +368,8 @@ struct Feed {
   __device__ __forceinline__ void arrive(Place &g) {
     if constexpr (kWhole) {
       const uint32_t slot = uint32_t(within(g.p0)) & ((1u << shift) - 16);
-      g.at[0] = int64_t(uint64_t(uint32_t(g.id[0])) * uint32_t(page_bytes) +
-                        uint64_t(slot) * uint32_t(slot_bytes));
+      g.at = int64_t(uint64_t(uint32_t(g.id[0])) * uint32_t(page_bytes) +
+                     uint64_t(slot) * uint32_t(slot_bytes));
       bad |= swamp::page_ok(g.id[0], n_pages) ? 0 : 1;
     } else {
 #pragma unroll
@@ -377,20 +377,6 @@ struct Feed {
         const bool ok = swamp::page_ok(g.id[j], n_pages);
         bad |= ok ? 0 : 1;
         if (!ok) g.id[j] = 0;
-      }
-      const int in_page = (1 << shift) - 1;
-      if (near && inside(g.p0)) {
-        const int64_t first = (g.p0 & in_page) * slot_bytes;
-#pragma unroll
-        for (int j = 0; j < G::NI; j++)
-          g.at[j] = first + int64_t(uint64_t(uint32_t(g.id[j])) * uint32_t(page_bytes));
-      } else {
-        const uint32_t rows = fresh(this->rows);
-#pragma unroll
-        for (int j = 0; j < G::NI; j++) {
-          const int r = (rows >> (4 * j)) & 15, slot = within(g.p0 + r) & in_page;
-          g.at[j] = g.id[j] * page_bytes + (slot - (near ? r & in_page & 15 : 0)) * slot_bytes;
-        }
       }
     }
   }
@@ -403,7 +389,7 @@ struct Feed {
     if constexpr (kWhole) {
       if (!swamp::page_ok(g.id[0], n_pages)) return;
       if (inside(g.p0)) {
-        dma_uniform<G::NI>(base + g.at[0], off, to);
+        dma_uniform<G::NI>(base + g.at, off, to);
         return;
       }
       const uint32_t rows = fresh(this->rows);
@@ -414,10 +400,25 @@ struct Feed {
         const int r = (rows >> (4 * j)) & 15;
         moved[j] = off[j] + uint32_t(within(g.p0 + r) - first - r) * uint32_t(slot_bytes);
       }
-      dma_uniform<G::NI>(base + g.at[0], moved, to);
+      dma_uniform<G::NI>(base + g.at, moved, to);
     } else {
+      const int in_page = (1 << shift) - 1;
+      if (near && inside(g.p0)) {
+        const uint8_t *first = base + (g.p0 & in_page) * slot_bytes;
 #pragma unroll
-      for (int j = 0; j < G::NI; j++) dma_lane(base + g.at[j] + off[j], to + 1024 * j);
+        for (int j = 0; j < G::NI; j++)
+          dma_lane(first + uint64_t(uint32_t(g.id[j])) * uint32_t(page_bytes) + off[j],
+                   to + 1024 * j);
+        return;
+      }
+      const uint32_t rows = fresh(this->rows);
+#pragma unroll
+      for (int j = 0; j < G::NI; j++) {
+        const int r = (rows >> (4 * j)) & 15, slot = within(g.p0 + r) & in_page;
+        dma_lane(base + g.id[j] * page_bytes + (slot - (near ? r & in_page & 15 : 0)) * slot_bytes +
+                     off[j],
+                 to + 1024 * j);
+      }
     }
   }
 };
