@@ -555,35 +555,56 @@ struct Rows {
   }
   __device__ __forceinline__ float base_of() const { return (m == -INFINITY ? 0.f : m) - kLift; }
 
-  // Weights 2 j and 2 j + 1 of the group kg, as parts of its operands p.
-  __device__ __forceinline__ void weigh(const f32x16 *s, int kg, int j, float base, u32x4 *p) {
-    typedef typename O::v2 v2;
-    f32x2 r;
+  // Weights 2 j and 2 j + 1 of the group kg, in three stages, so that none waits for
+  // the one before it where steps take them in turn: x = c s - base, ...
+  __device__ __forceinline__ void weigh_in(const f32x16 *s, int kg, int j, float base,
+                                           float *x) const {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      r[i] = __builtin_amdgcn_exp2f(
-          __builtin_fmaf(s[kg >> 1][8 * (kg & 1) + 2 * j + i], c, -base));
-      l += r[i];
-    }
-    // the nearest of the cache's type and, where the output is fp32, what is
-    // left of the weight, again and again
+    for (int i = 0; i < 2; i++)
+      x[i] = fresh(__builtin_fmaf(s[kg >> 1][8 * (kg & 1) + 2 * j + i], c, -base));
+  }
+  // ... 2^x, ...
+  static __device__ __forceinline__ void weigh_up(float *x) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) x[i] = fresh(__builtin_amdgcn_exp2f(x[i]));
+  }
+  // ... and its parts in the group's operands p: the nearest of the cache's type and,
+  // where the output is fp32, what is left of the weight, again and again.  (fresh:
+  // not moved to where they are used, past the products that hide this.)
+  __device__ __forceinline__ void weigh_out(const float *x, int j, u32x4 *p) {
+    typedef typename O::v2 v2;
+    f32x2 r = {x[0], x[1]};
+    l += r[0];
+    l += r[1];
 #pragma unroll
     for (int n = 0; n < NP; n++) {
       const v2 h = __builtin_convertvector(r, v2);
       p[n][j] = __builtin_bit_cast(uint32_t, h);
       if (n + 1 < NP) r -= f32x2{float(h[0]), float(h[1])};
     }
-    // (not moved to where they are used, past the products that hide this)
 #pragma unroll
     for (int n = 0; n < NP; n++) p[n][j] = fresh(p[n][j]);
     l = fresh(l);
+  }
+  // Groups from kg0 on, their pairs of weights counted through: what step f of kSteps
+  // does for kPairs of them (steps up to kSteps + 1 finish the last).
+  template <int kPairs, int kSteps>
+  __device__ __forceinline__ void weigh_step(const f32x16 *s, int kg0, int f, float base,
+                                             float (*x)[2], u32x4 (*p)[NP]) {
+    auto first = [](int g) { return g < 0 ? 0 : g > kSteps ? kPairs : kPairs * g / kSteps; };
+#pragma unroll
+    for (int q = first(f - 2); q < first(f - 1); q++) weigh_out(x[q], q & 3, p[kg0 + (q >> 2)]);
+#pragma unroll
+    for (int q = first(f - 1); q < first(f); q++) weigh_up(x[q]);
+#pragma unroll
+    for (int q = first(f); q < first(f + 1); q++) weigh_in(s, kg0 + (q >> 2), q & 3, base, x[q]);
   }
   // A tile of 32 keys after its scores and grow(): weights, and o = o + V^T P^T
   // over the values in LDS at v.  A step is one block of dims of one group of 16
   // keys: its product, the read of the values four steps on, and a share of the
   // next group's weights, which the matrix pipe's time hides.
   __device__ __forceinline__ void rest(const G &g, uint32_t v, const f32x16 *s) {
-    constexpr int kSteps = 2 * G::DB, kRing = 4;
+    constexpr int kSteps = 2 * G::DB, kRing = 4, kIn = G::DB > 2 ? G::DB - 2 : 1;
     const float base = base_of();
     const uint32_t at = v + v_at;
     s16x8 ring[kRing];
@@ -591,20 +612,22 @@ struct Rows {
 #pragma unroll
     for (int f = 0; f < kRing; f++)
       if (f < kSteps) ring[f] = v_frag(g, at, f % G::DB, f / G::DB);
+    float x[4][2], y[4][2];
 #pragma unroll
-    for (int j = 0; j < 4; j++) weigh(s, 0, j, base, p[0]);
+    for (int f = 0; f < 3; f++) weigh_step<4, 1>(s, 0, f, base, x, p);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = 0; f < kSteps; f++) {
-      const int kg = f / G::DB, db = f % G::DB;
+      const int kg = f / G::DB;
 #pragma unroll
       for (int n = 0; n < NP; n++)
-        o[db] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg][n]), o[db]);
+        o[f % G::DB] = O::mma(ring[f % kRing], __builtin_bit_cast(s16x8, p[kg][n]), o[f % G::DB]);
       if (f + kRing < kSteps)
         ring[f % kRing] = v_frag(g, at, (f + kRing) % G::DB, (f + kRing) / G::DB);
-      if (kg == 0) {
+      if (kg == 0) weigh_step<4, kIn>(s, 1, f, base, y, p);
+      if (f + 1 == G::DB) {
 #pragma unroll
-        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++) weigh(s, 1, j, base, p[1]);
+        for (int h = G::DB; h < kIn + 2; h++) weigh_step<4, kIn>(s, 1, h, base, y, p);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -623,6 +646,7 @@ struct Rows {
     const uint32_t at = k + k_at;
     s16x8 ring[kRing];
     f32x16 other = {};
+    float w[4][2];
 #pragma unroll
     for (int f = 0; f < kRing; f++) ring[f] = k_frag(at, f % G::KS, f / G::KS);
     __builtin_amdgcn_sched_barrier(0);
@@ -637,10 +661,8 @@ struct Rows {
       else s[kb] = O::mma(a, q[ks], ks == 0 ? f32x16{} : s[kb]);
       if (f + kRing < kSteps)
         ring[f % kRing] = k_frag(at, (f + kRing) % G::KS, (f + kRing) / G::KS);
-      if (KB == 2 && kPending && kb == 0) {
-#pragma unroll
-        for (int j = 4 * ks / G::KS; j < 4 * (ks + 1) / G::KS; j++) weigh(s, 3, j, base, p[3]);
-      }
+      // (weigh_in reads s[1], whose own products begin at step KS)
+      if (KB == 2 && kPending && f < G::KS + 2) weigh_step<4, G::KS>(s, 3, f, base, w, p);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (KB == 1) {
@@ -662,7 +684,9 @@ struct Rows {
       for (int f = 0; f < kRing; f++)
         if (f < kSteps) ring[f] = v_frag(g, at, f % G::DB, f / G::DB);
     }
-    float top = s[0][0], keep = 1.f;
+    // of all groups but the last, each behind the sums that its old weights are for
+    constexpr int kPairs = KB == 2 ? 12 : 4;
+    float top = s[0][0], keep = 1.f, w[kPairs][2];
     bool grew = false;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -690,15 +714,16 @@ struct Rows {
           l *= keep;
         }
       } else {
-#pragma unroll
-        for (int j = 4 * db / G::DB; j < 4 * (db + 1) / G::DB; j++)
-          weigh(s, kg - 1, j, base, p[kg - 1]);
+        weigh_step<kPairs, kSteps - G::DB>(s, 0, f - G::DB, base, w, p);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int f = kSteps - G::DB; f < kSteps - G::DB + 2; f++)
+      weigh_step<kPairs, kSteps - G::DB>(s, 0, f, base, w, p);
     if (KB == 1) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) weigh(s, 1, j, base, p[1]);
+      for (int f = 0; f < 3; f++) weigh_step<4, 1>(s, 1, f, base, w, p);
     }
     if (kSums && grew) {
 #pragma unroll
@@ -723,9 +748,10 @@ struct Rows {
   __device__ __forceinline__ void sums(const G &g, uint32_t v, const f32x16 *s,
                                        u32x4 (&p)[2 * KB][NP], float base) {
     const uint32_t at = v + v_at;
+    float w[4][2];
     if (KB == 2) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) weigh(s, 3, j, base, p[3]);
+      for (int f = 0; f < 3; f++) weigh_step<4, 1>(s, 3, f, base, w, p);
     }
 #pragma unroll
     for (int f = 0; f < 2 * KB * G::DB; f++) {
