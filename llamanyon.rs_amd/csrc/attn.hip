@@ -4,6 +4,7 @@
 #include "attn_core.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 int swamp_attn_f16(const swamp_attn::Work &w, bool precise, hipStream_t s);
 int swamp_attn_bf16(const swamp_attn::Work &w, bool precise, hipStream_t s);
@@ -90,16 +91,20 @@ struct Plan {
 // on this card, us: a tile takes 0.55 + 0.007 dim where a CU has one workgroup
 // and 0.6 more for each further one (heads of 128: 1.45 and 2.06 us measured), a
 // workgroup's start and end three tiles, and a join 4 us and its sums' way
-// through memory.
+// through memory.  A last round that is not full costs its share, as most rows
+// see less than the longest sequence, and a little more: without it 45
+// workgroups of 256 dims go in 6 pieces instead of 5, 38.8 us and 30.8.  Down
+// to one tile a piece pays (7 workgroups, 256 dims, 554 keys: pieces of four
+// tiles 34.8 us, of one 23.7).
 int many_splits(int64_t base, int64_t rows, int64_t keys, int dim, int cus) {
   const int most = dim <= 64 ? 3 : dim <= 128 ? 2 : 1;  // workgroups of a CU
   const double tiles = double(keys) / kTile;
   double best = 0;
   int want = 1;
-  for (int n = 1; n <= 16 && n <= std::max<int64_t>(1, keys / (4 * kTile)); n++) {
+  for (int n = 1; n <= 16 && n <= std::max<int64_t>(1, keys / kTile); n++) {
     const int64_t load = std::min<int64_t>(most, (base * n + cus - 1) / cus);
     const double rounds = std::max(1.0, double(base) * n / (double(cus) * most));
-    double t = rounds * (tiles / n + 3) * (0.55 + 0.007 * dim + 0.6 * double(load - 1));
+    double t = (0.95 * rounds + 0.05 * std::ceil(rounds)) * (tiles / n + 3) * (0.55 + 0.007 * dim + 0.6 * double(load - 1));
     if (n > 1) t += 4 + n * double(rows) * dim * 8 / 6e6;
     if (n == 1 || t < best) best = t, want = n;
   }
