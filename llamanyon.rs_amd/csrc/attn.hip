@@ -126,15 +126,24 @@ Plan plan_of(const swamp::AttnCall &c) {
   const int64_t seen = int64_t(c.window) + (p.few ? c.max_new : kRows / group) + kTile;
   const int64_t keys = c.window ? std::min<int64_t>(c.max_len, seen) : c.max_len;
   int64_t want;
-  if (p.few)
+  if (p.few) {
+    // one workgroup a CU, of short heads two while a piece keeps two steps (64
+    // workgroups of 128 dims over 4001 keys: 256 in all 22.4 us, 512 25.2, 64 60;
+    // 22 of 64 dims over up to 22634 keys: 528 in all 27.5, 242 41.5; 2 over 20345:
+    // 160 in all 13.3, 318 14.8)
+    want = cus / base;
+    if (c.cache.dim <= 64) want = std::max(want, std::min(2 * cus / base, keys / (64 * kWaves)));
+    // sequences of unequal length in a piece or two each: pieces of 2048 keys even
+    // them out (256 workgroups over up to 6000 keys 39.9 us, whole 47.0; 115 over
+    // up to 14540: 68.5, in two 78.9); where there are more pieces these are too
+    // many (70 of 256 dims over up to 13260 keys: 124 us, in three 109)
+    if (want < 3) want = std::max(want, keys / 2048);
     // none below the time of the join (8 workgroups, 128 dims, 512 keys: whole 9.6
-    // us, in pieces 11.1; 1024 keys: 14.2 and 10.8; 64 dims, 1024 keys: 10.6 and 11);
-    // one workgroup a CU (64 workgroups over 4001 keys: 256 in all 22.4 us, 512
-    // 25.2, 64 60), and pieces that even out sequences of unequal length (256 over
-    // up to 6000 keys: 2048 each 39.9 us, whole 47.0)
-    want = keys * c.cache.dim <= 65536 ? 1 : std::max(cus / base, keys / 2048);
-  else
+    // us, in pieces 11.1; 1024 keys: 14.2 and 10.8; 64 dims, 1024 keys: 10.6 and 11)
+    if (keys * c.cache.dim <= 65536) want = 1;
+  } else {
     want = many_splits(base, rows * c.cache.n_kv, keys, c.cache.dim, cus);
+  }
   // a piece is whole tiles; of a few rows one for each wave at least
   const int step = p.few ? 32 * kWaves : kTile;
   want = std::max<int64_t>(1, want);
