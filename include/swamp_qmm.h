@@ -326,7 +326,8 @@ SWAMP_API int swamp_quantize_q8_0(const void *d_x, uint32_t x_type, void *d_q, s
  * ops.rs:20-54), the paged cache's append (cache.rs) and the attention over it.
  * The reference's gpu_attention_* entry points have other arguments and are not
  * replaced.  Structures are read during the call and not kept; strides are in
- * elements, and 0 stands for the dense one. */
+ * elements, 2^40 at most, and 0 stands for the dense one.  SWAMP_EINVAL where the
+ * rows, pages or page tables that a call names would reach past 2^58 elements. */
 
 /* Pairs that turn together: (2i, 2i + 1), or (i, i + n_rot / 2). */
 enum { SWAMP_ROPE_PAIRS = 0, SWAMP_ROPE_HALVES = 1 };

@@ -121,6 +121,14 @@ bool is_float(uint32_t t) { return t == SWAMP_F32 || t == SWAMP_F16 || t == SWAM
 // arithmetic of the kernels stay within 32 bits.
 constexpr int kMaxSeqs = 65535, kMaxHeads = 4096, kMaxWindow = 1 << 30;
 
+// Strides, and how far a call's buffers reach (in elements): what the kernels add
+// up in 64 bits, in bytes too, stays far from wrapping, so that an index that was
+// checked cannot name memory outside its buffer.
+constexpr int64_t kMaxStride = int64_t(1) << 40, kMaxExtent = int64_t(1) << 58;
+// The last of n rows, pages or tables `stride` apart begins within kMaxExtent
+// (neither negative).
+bool within(int64_t n, int64_t stride) { return n < 2 || stride <= kMaxExtent / (n - 1); }
+
 int check_rope(const swamp_rope_spec *r, int head_dim) {
   if (!r || !r->d_freqs || !aligned(r->d_freqs, 8)) return SWAMP_EINVAL;
   if (r->layout != SWAMP_ROPE_PAIRS && r->layout != SWAMP_ROPE_HALVES) return SWAMP_EINVAL;
@@ -137,9 +145,8 @@ int check_cache(const swamp_kv_pages *c, PagedCache &out) {
   if (c->page_size < 1 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0)
     return SWAMP_ESHAPE;
   if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0) return SWAMP_ESHAPE;
-  const int64_t most = int64_t(1) << 40;  // page id * stride stays within 64 bits
   for (int64_t v : {c->page_stride, c->head_stride, c->slot_stride}) {
-    if (v < 0 || v > most) return SWAMP_EINVAL;
+    if (v < 0 || v > kMaxStride) return SWAMP_EINVAL;
     if (v % 8 != 0) return SWAMP_ESHAPE;
   }
   out.slot_stride = c->slot_stride ? c->slot_stride : c->head_dim;
@@ -147,6 +154,9 @@ int check_cache(const swamp_kv_pages *c, PagedCache &out) {
   out.page_stride =
       c->page_stride ? c->page_stride : int64_t(c->n_kv_heads) * c->page_size * c->head_dim;
   if (out.slot_stride < c->head_dim) return SWAMP_ESHAPE;
+  if (!within(c->n_pages, out.page_stride) || !within(c->n_kv_heads, out.head_stride) ||
+      !within(c->page_size, out.slot_stride))
+    return SWAMP_EINVAL;
   out.k = static_cast<uint16_t *>(c->d_k);
   out.v = static_cast<uint16_t *>(c->d_v);
   out.n_pages = c->n_pages;
@@ -159,7 +169,7 @@ int check_cache(const swamp_kv_pages *c, PagedCache &out) {
 int check_batch(const swamp_seq_batch *b, SeqBatch &out) {
   if (!b) return SWAMP_EINVAL;
   if (b->n_seq < 0 || b->n_seq > kMaxSeqs || b->n_tok < 0 || b->max_new < 0 || b->max_len < 0 ||
-      b->pages_stride < 0)
+      b->pages_stride < 0 || !within(b->n_seq, b->pages_stride))
     return SWAMP_EINVAL;
   out.first = b->d_first;
   out.len = b->d_len;
@@ -176,10 +186,11 @@ bool batch_ok(const SeqBatch &b) {
 }
 bool cache_ok(const PagedCache &c) { return c.k && c.v && aligned(c.k, 16) && aligned(c.v, 16); }
 
-// Rows of n heads of dim elements, `stride` apart (0: dense).
-int check_rows(int64_t &stride, int n, int dim) {
-  if (stride < 0 || stride > (int64_t(1) << 40)) return SWAMP_EINVAL;
+// n_tok rows of n heads of dim elements, `stride` apart (0: dense).
+int check_rows(int64_t &stride, int n_tok, int n, int dim) {
+  if (stride < 0 || stride > kMaxStride) return SWAMP_EINVAL;
   if (stride == 0) stride = int64_t(n) * dim;
+  if (!within(n_tok, stride)) return SWAMP_EINVAL;
   return stride < int64_t(n) * dim ? SWAMP_ESHAPE : SWAMP_OK;
 }
 
@@ -627,8 +638,8 @@ int swamp_rope(const swamp_rope_spec *rope, const int32_t *d_pos, const void *d_
   if (n_tok < 0 || n_heads < 0 || n_heads > kMaxHeads || head_dim < 2) return SWAMP_EINVAL;
   if (head_dim % 2 != 0 || head_dim > 512) return SWAMP_ESHAPE;
   if (int rc = check_rope(rope, head_dim)) return rc;
-  if (int rc = check_rows(x_stride, n_heads, head_dim)) return rc;
-  if (int rc = check_rows(out_stride, n_heads, head_dim)) return rc;
+  if (int rc = check_rows(x_stride, n_tok, n_heads, head_dim)) return rc;
+  if (int rc = check_rows(out_stride, n_tok, n_heads, head_dim)) return rc;
   if (n_tok == 0 || n_heads == 0) return SWAMP_OK;
   if (!d_pos || !d_x || !d_out || !aligned(d_pos, 4) || !aligned(d_x, type_size(x_type)) ||
       !aligned(d_out, type_size(out_type)))
@@ -651,10 +662,10 @@ int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
   if (n_heads < 0 || n_heads > kMaxHeads) return SWAMP_EINVAL;
   if (rope)
     if (int rc = check_rope(rope, c.dim)) return rc;
-  if (int rc = check_rows(q_stride, n_heads, c.dim)) return rc;
-  if (int rc = check_rows(k_stride, c.n_kv, c.dim)) return rc;
-  if (int rc = check_rows(v_stride, c.n_kv, c.dim)) return rc;
-  if (int rc = check_rows(q_out_stride, n_heads, c.dim)) return rc;
+  if (int rc = check_rows(q_stride, b.n_tok, n_heads, c.dim)) return rc;
+  if (int rc = check_rows(k_stride, b.n_tok, c.n_kv, c.dim)) return rc;
+  if (int rc = check_rows(v_stride, b.n_tok, c.n_kv, c.dim)) return rc;
+  if (int rc = check_rows(q_out_stride, b.n_tok, n_heads, c.dim)) return rc;
   if (b.n_tok == 0 || b.n_seq == 0) return SWAMP_OK;
   const uintptr_t al = type_size(x_type);
   if (!cache_ok(c) || !batch_ok(b) || !d_k || !d_v || !aligned(d_k, al) || !aligned(d_v, al))
@@ -674,8 +685,8 @@ int swamp_attn_paged(const swamp_kv_pages *cache, const swamp_seq_batch *batch, 
   if (int rc = check_attn(cache, batch, n_heads, window, c)) return rc;
   if (!is_float(out_type)) return SWAMP_EDTYPE;
   if (!std::isfinite(scale)) return SWAMP_EINVAL;
-  if (int rc = check_rows(q_stride, n_heads, c.cache.dim)) return rc;
-  if (int rc = check_rows(out_stride, n_heads, c.cache.dim)) return rc;
+  if (int rc = check_rows(q_stride, c.batch.n_tok, n_heads, c.cache.dim)) return rc;
+  if (int rc = check_rows(out_stride, c.batch.n_tok, n_heads, c.cache.dim)) return rc;
   if (q_stride % 8 != 0 || out_stride % 8 != 0) return SWAMP_ESHAPE;
   if (c.max_new == 0 || c.batch.n_seq == 0) return SWAMP_OK;
   if (!cache_ok(c.cache) || !batch_ok(c.batch) || !d_q || !d_out || !aligned(d_q, 16) ||
