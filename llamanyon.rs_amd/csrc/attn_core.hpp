@@ -37,6 +37,7 @@
 // result that is not finite is computed once more with such values taken out of
 // the tiles and added, row by row, to the rows that see them.
 #pragma once
+#include "attn_plan.hpp"
 #include "paging.hpp"
 #include "swamp_common.hpp"
 
@@ -52,10 +53,6 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kRows = 128;     // rows of a block
-constexpr int kFew = 32;       // rows up to which a block's waves share the rows instead
-constexpr int kTile = 64;      // keys of a workgroup's tile
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct Work {
