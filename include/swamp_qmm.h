@@ -367,8 +367,8 @@ typedef struct swamp_kv_pages {
  *   d_pages[n_seq][pages_stride]: its page table (pages_stride in entries, and
  *     at least its pages).
  *   max_new: at least the most new tokens that a sequence has.  max_len: about
- *     the longest d_len; the work is split by it, results do not depend on its
- *     being right.
+ *     the longest d_len, any value from 0 on; the work is split by it, results do
+ *     not depend on its being right.
  *   d_bad (may be NULL): set to 1 where a position of a sequence that the call
  *     has to read or write has no page (a table entry outside 0 .. n_pages - 1,
  *     a position past the table or before 0; in attention also one of the last
@@ -435,7 +435,9 @@ SWAMP_API int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch
  * A long cache is split over workgroups that leave partial sums in the stream's
  * scratch ("Scratch" above; swamp_attn_paged_workspace reports it), joined in a
  * fixed order: repeated calls give the same bits.  Without it (under capture,
- * nothing reserved) the cache is not split. */
+ * nothing reserved) the cache is not split.  SWAMP_ESHAPE for more work than one
+ * launch holds: 2^24 blocks of 128 rows (token times query head of a cache head,
+ * at least one block a sequence) over all cache heads. */
 SWAMP_API int swamp_attn_paged(const swamp_kv_pages *cache, const swamp_seq_batch *batch,
                                const void *d_q, int64_t q_stride, int n_heads, float scale,
                                int window, void *d_out, uint32_t out_type, int64_t out_stride,

@@ -13,6 +13,7 @@
 #include <thread>
 #include <vector>
 
+#include "attn_plan.hpp"
 #include "swamp_common.hpp"
 #include "swamp_gguf.h"
 
@@ -206,7 +207,7 @@ int check_attn(const swamp_kv_pages *cache, const swamp_seq_batch *batch, int n_
   c.window = window >= kMaxWindow ? 0 : window;  // no row is that far from its first key
   c.max_new = std::min(batch->max_new, batch->n_tok);
   c.max_len = batch->max_len;
-  return SWAMP_OK;
+  return c.max_new == 0 || attn_fits(c) ? SWAMP_OK : SWAMP_ESHAPE;
 }
 
 }  // namespace

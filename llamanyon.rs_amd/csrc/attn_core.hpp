@@ -905,10 +905,7 @@ __device__ __forceinline__ bool find_piece(const Work &w, int s, int64_t r0, int
   p.rows = int(min(n_rows - r0, int64_t(max_rows)));
   p.before = p.sq.len - p.sq.n;
   const swamp::Span ka = p.seen(r0, w), kz = p.seen(r0 + p.rows - 1, w);
-  // positions that the page table cannot hold are not walked; nor are the last
-  // below 2^31, so that a tile's end fits
-  const int64_t room = min(min(w.b.pages_stride, int64_t(1) << 31) << w.cache.page_shift,
-                           (int64_t(1) << 31) - 512);
+  const int64_t room = swamp::walked(w.b.pages_stride, w.cache.page_shift);
   const int last = int(min(int64_t(kz.hi), room));
   const int64_t from = (ka.lo & ~(kTile - 1)) + int64_t(split) * w.chunk;
   p.over = kz.hi > room;
@@ -1235,7 +1232,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
 template <typename CT, int D, bool kExact, bool kWhole, int NP>
 void launch_kind(const Work &w, hipStream_t s) {
   typedef Geo<D, kExact> G;
-  const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));
+  const dim3 grid(unsigned(w.blocks) * unsigned(w.splits) * unsigned(w.cache.n_kv));  // (kMaxGroups)
   const uint32_t smem = G::kSmem + G::kExtra;
   if (w.few) attn_few_kernel<CT, D, kExact, kWhole, NP><<<grid, kThreads, smem, s>>>(w);
   else attn_many_kernel<CT, D, kExact, kWhole, NP><<<grid, kThreads, smem, s>>>(w);

@@ -24,6 +24,18 @@ using swamp_attn::kRows;
 using swamp_attn::kTile;
 using swamp_attn::kWaves;
 
+// Workgroups that one launch can have: its threads are counted in 32 bits.
+constexpr int64_t kMaxGroups = (int64_t(1) << 32) / swamp_attn::kThreads - 1;
+// Positions from here on are not walked, so that a tile's end is still an int.
+constexpr int64_t kLastPosition = (int64_t(1) << 31) - 512;
+
+// Positions that a page table holds and that are walked.
+SWAMP_HD int64_t walked(int64_t pages_stride, int page_shift) {
+  const int64_t cols = int64_t(1) << 31;
+  const int64_t room = (pages_stride < cols ? pages_stride : cols) << page_shift;
+  return room < kLastPosition ? room : kLastPosition;
+}
+
 struct AttnPlan {
   int blocks, one_block, few, splits, chunk;
 };
@@ -52,20 +64,36 @@ inline int many_splits(int64_t base, int64_t rows, int64_t keys, int dim, int cu
   return want;
 }
 
-// blocks: at most this many, of all sequences, whatever the rows' distribution.
+// Blocks of rows of a cache head, of a sequence at most `most`, of all sequences at
+// most this many, whatever the rows' distribution.
+inline int64_t attn_blocks(const AttnCall &c, int64_t &most) {
+  const int group = c.n_heads / c.cache.n_kv;
+  const int64_t rows = int64_t(c.batch.n_tok) * group;
+  most = (int64_t(c.max_new) * group + kRows - 1) / kRows;
+  return most <= 1 ? c.batch.n_seq
+                   : std::min((rows + int64_t(kRows - 1) * c.batch.n_seq) / kRows,
+                              most * c.batch.n_seq);
+}
+// One launch holds the call.
+inline bool attn_fits(const AttnCall &c) {
+  int64_t most;
+  return attn_blocks(c, most) * c.cache.n_kv <= kMaxGroups;
+}
+
+// Of a call that attn_fits.
 inline AttnPlan plan_attn(const AttnCall &c, int cus) {
   const int group = c.n_heads / c.cache.n_kv;
   const int64_t rows = int64_t(c.batch.n_tok) * group;  // of a cache head
-  const int64_t most = (int64_t(c.max_new) * group + kRows - 1) / kRows;  // blocks of a sequence
+  int64_t most;
   AttnPlan p;
+  p.blocks = int(attn_blocks(c, most));
   p.few = int64_t(c.max_new) * group <= kFew;
   p.one_block = most <= 1;
-  p.blocks = int(p.one_block ? c.batch.n_seq
-                             : std::min((rows + int64_t(kRows - 1) * c.batch.n_seq) / kRows,
-                                        most * c.batch.n_seq));
   const int64_t base = std::max<int64_t>(1, int64_t(p.blocks) * c.cache.n_kv);
   const int64_t seen = int64_t(c.window) + (p.few ? c.max_new : kRows / group) + kTile;
-  const int64_t keys = c.window ? std::min<int64_t>(c.max_len, seen) : c.max_len;
+  const int64_t held = std::min<int64_t>(
+      c.max_len, walked(c.batch.pages_stride, c.cache.page_shift));
+  const int64_t keys = c.window ? std::min(held, seen) : held;
   int64_t want;
   if (p.few) {
     // one workgroup a CU, of short heads two while a piece keeps two steps (64
@@ -85,12 +113,15 @@ inline AttnPlan plan_attn(const AttnCall &c, int cus) {
   } else {
     want = many_splits(base, rows * c.cache.n_kv, keys, c.cache.dim, cus);
   }
+  // what one launch holds, and the join's, which has a row a workgroup at worst
+  want = std::min(want, kMaxGroups / base);
+  if (int64_t(c.batch.n_tok) * c.n_heads > kMaxGroups) want = 1;
   // a piece is whole tiles; of a few rows one for each wave at least
-  const int step = p.few ? 32 * kWaves : kTile;
+  const int64_t step = p.few ? 32 * kWaves : kTile;
   want = std::max<int64_t>(1, want);
-  p.chunk = int(((keys + want - 1) / want + step - 1) / step * step);
-  p.chunk = std::max(p.chunk, step);
-  p.splits = int(std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk));
+  const int64_t chunk = std::max(((keys + want - 1) / want + step - 1) / step * step, step);
+  p.chunk = int(chunk);  // (kLastPosition is whole steps)
+  p.splits = int(std::max<int64_t>(1, (keys + chunk - 1) / chunk));
   return p;
 }
 
