@@ -37,9 +37,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Work w, int per, int sha
     f32x4 o[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; i++) {
-      const int64_t at = min(x0 + i, x1 - 1) * n + row;
-      st[i] = w.stat[at];
-      o[i] = *reinterpret_cast<const f32x4 *>(w.part + at * dim + d);
+      st[i] = w.stat[min(x0 + i, x1 - 1) * n + row];
+    }
+    // (a piece without keys of the row wrote no sums, and where max_len is far above
+    // the lengths most are such)
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (st[i][0] != -INFINITY)
+        o[i] = *reinterpret_cast<const f32x4 *>(
+            w.part + (min(x0 + i, x1 - 1) * n + row) * dim + d);
     }
     float top = m;
 #pragma unroll
@@ -54,7 +61,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Work w, int per, int sha
       const float k = __builtin_amdgcn_exp2f(st[i][0] - base);
       sees = sees && st[i][1] != -1.f;
       l += k * st[i][1];
-      if (st[i][0] != -INFINITY) acc += k * o[i];  // (else nothing was written)
+      acc += k * o[i];
     }
   }
   if (shares > 1) {

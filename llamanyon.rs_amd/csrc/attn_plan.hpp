@@ -29,6 +29,13 @@ constexpr int64_t kMaxGroups = (int64_t(1) << 32) / swamp_attn::kThreads - 1;
 // Positions from here on are not walked, so that a tile's end is still an int.
 constexpr int64_t kLastPosition = (int64_t(1) << 31) - 512;
 
+// Pieces of a call that is cut for evenness rather than to fill the card, and bytes
+// of partial sums that a call may ask the stream's scratch for.  Pieces are written
+// and read once each, 256 dim bytes a block of 32 rows against 4 dim bytes a key:
+// a few percent of the time wherever the lengths are near max_len.
+constexpr int kMostPieces = 16;
+constexpr size_t kPartBytes = size_t(256) << 20;
+
 // Positions that a page table holds and that are walked.
 SWAMP_HD int64_t walked(int64_t pages_stride, int page_shift) {
   const int64_t cols = int64_t(1) << 31;
@@ -54,7 +61,7 @@ inline int many_splits(int64_t base, int64_t rows, int64_t keys, int dim, int cu
   const double tiles = double(keys) / kTile;
   double best = 0;
   int want = 1;
-  for (int n = 1; n <= 16 && n <= std::max<int64_t>(1, keys / kTile); n++) {
+  for (int n = 1; n <= kMostPieces && n <= std::max<int64_t>(1, keys / kTile); n++) {
     const int64_t load = std::min<int64_t>(most, (base * n + cus - 1) / cus);
     const double rounds = std::max(1.0, double(base) * n / (double(cus) * most));
     double t = (0.95 * rounds + 0.05 * std::ceil(rounds)) * (tiles / n + 3) * (0.55 + 0.007 * dim + 0.6 * double(load - 1));
@@ -62,6 +69,18 @@ inline int many_splits(int64_t base, int64_t rows, int64_t keys, int dim, int cu
     if (n == 1 || t < best) best = t, want = n;
   }
   return want;
+}
+
+inline size_t attn_part_bytes(const AttnCall &c, int splits) {
+  return size_t(splits) * c.batch.n_tok * c.n_heads * c.cache.dim * 4;
+}
+inline size_t attn_stat_bytes(const AttnCall &c, int splits) {
+  return size_t(splits) * c.batch.n_tok * c.n_heads * 8;
+}
+
+// Sums and statistics of one piece.
+inline size_t attn_piece_bytes(const AttnCall &c) {
+  return attn_part_bytes(c, 1) + attn_stat_bytes(c, 1);
 }
 
 // Blocks of rows of a cache head, of a sequence at most `most`, of all sequences at
@@ -106,13 +125,17 @@ inline AttnPlan plan_attn(const AttnCall &c, int cus) {
     // them out (256 workgroups over up to 6000 keys 39.9 us, whole 47.0; 115 over
     // up to 14540: 68.5, in two 78.9); where there are more pieces these are too
     // many (70 of 256 dims over up to 13260 keys: 124 us, in three 109)
-    if (want < 3) want = std::max(want, keys / 2048);
+    // (kMostPieces at most, as max_len may be far above the lengths: 64 sequences of
+    // 1000 tokens, 512 workgroups, under a max_len of 131072: in 64 pieces 164 us, in
+    // 16 43, while 11 of up to 36000 keep their 105 and 186 at 64 and 128 dims)
+    if (want < 3) want = std::max(want, std::min<int64_t>(kMostPieces, keys / 2048));
     // none below the time of the join (8 workgroups, 128 dims, 512 keys: whole 9.6
     // us, in pieces 11.1; 1024 keys: 14.2 and 10.8; 64 dims, 1024 keys: 10.6 and 11)
     if (keys * c.cache.dim <= 65536) want = 1;
   } else {
     want = many_splits(base, rows * c.cache.n_kv, keys, c.cache.dim, cus);
   }
+  want = std::min(want, int64_t(kPartBytes / std::max<size_t>(1, attn_piece_bytes(c))));
   // what one launch holds, and the join's, which has a row a workgroup at worst
   want = std::min(want, kMaxGroups / base);
   if (int64_t(c.batch.n_tok) * c.n_heads > kMaxGroups) want = 1;
@@ -123,13 +146,6 @@ inline AttnPlan plan_attn(const AttnCall &c, int cus) {
   p.chunk = int(chunk);  // (kLastPosition is whole steps)
   p.splits = int(std::max<int64_t>(1, (keys + chunk - 1) / chunk));
   return p;
-}
-
-inline size_t attn_part_bytes(const AttnCall &c, int splits) {
-  return size_t(splits) * c.batch.n_tok * c.n_heads * c.cache.dim * 4;
-}
-inline size_t attn_stat_bytes(const AttnCall &c, int splits) {
-  return size_t(splits) * c.batch.n_tok * c.n_heads * 8;
 }
 
 }  // namespace swamp

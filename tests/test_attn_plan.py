@@ -109,3 +109,27 @@ def test_calls_past_one_launch_are_refused(pkg):
     assert call(dict(n_kv_heads=257), many, 257) == pkg.ESHAPE
     tokens = dict(n_seq=1, n_tok=2 ** 31 - 1, max_new=2 ** 31 - 1)
     assert call(dict(n_kv_heads=2), tokens, 4) == pkg.ESHAPE
+
+
+@pytest.mark.parametrize("length", [2 ** 17, 2 ** 20, 2 ** 24, 2 ** 31 - 1])
+def test_pieces_and_their_sums_stay_bounded(lib, length):
+    """A captured step's max_len is its context's limit, whatever the lengths are: at
+    most 16 pieces where the rows alone fill the card, and 256 MB of partial sums."""
+    for seqs in (11, 16, 64, 300, 5000):
+        for new in (1, 4, 32, 200):
+            a = dict(seqs=seqs, tok=seqs * new, new=new, len=length, heads=64, kv=8, dim=128)
+            p = Plan(lib, **a)
+            assert p.splits == 1 or p.bytes <= 2 ** 28, a
+            assert p.splits <= 16, a
+
+
+def test_piece_counts_of_ordinary_lengths(lib):
+    """Where neither bound is met the count is what the measured rules say."""
+    def pieces(**a):
+        return Plan(lib, **a).splits
+    one = dict(seqs=1, tok=1, new=1, heads=32, kv=8, dim=128)
+    assert pieces(len=131072, **one) == 32 and pieces(len=512, **one) == 1
+    assert pieces(seqs=64, tok=63, new=1, len=8192, heads=64, kv=8, dim=128) == 4
+    assert pieces(seqs=8, tok=40, new=5, len=4001, heads=32, kv=8, dim=128) == 4
+    assert pieces(seqs=1, tok=512, new=512, len=16384, heads=32, kv=8, dim=128) == 4
+    assert pieces(seqs=1, tok=4096, new=4096, len=4096, heads=64, kv=8, dim=128) == 1
