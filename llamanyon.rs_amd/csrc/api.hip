@@ -120,7 +120,7 @@ bool is_float(uint32_t t) { return t == SWAMP_F32 || t == SWAMP_F16 || t == SWAM
 
 // Longest sequences and rows of the paged entry points: grids and the row
 // arithmetic of the kernels stay within 32 bits.
-constexpr int kMaxSeqs = 65535, kMaxHeads = 4096, kMaxWindow = 1 << 30;
+constexpr int kMaxSeqs = 65535, kMaxHeads = 4096;
 
 // Strides, and how far a call's buffers reach (in elements): what the kernels add
 // up in 64 bits, in bytes too, stays far from wrapping, so that an index that was
@@ -204,7 +204,7 @@ int check_attn(const swamp_kv_pages *cache, const swamp_seq_batch *batch, int n_
   if (n_heads % cache->n_kv_heads != 0) return SWAMP_ESHAPE;
   c.dtype = cache->dtype;
   c.n_heads = n_heads;
-  c.window = window >= kMaxWindow ? 0 : window;  // no row is that far from its first key
+  c.window = window;
   c.max_new = std::min(batch->max_new, batch->n_tok);
   c.max_len = batch->max_len;
   return c.max_new == 0 || attn_fits(c) ? SWAMP_OK : SWAMP_ESHAPE;
