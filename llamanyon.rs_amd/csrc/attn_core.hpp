@@ -5,6 +5,7 @@
 // sum l: a tile's scores s, m' = max(m, c max s) with c = scale log2 e, p =
 // 2^(c s - m'), l and o scaled by 2^(m - m') where m grows by more than kSlack
 // (p then reaches 2^kSlack at most; sums and the last division do not care).
+// fp16 weights are lifted, and m follows the tiles down as well (Rows::kFall).
 //
 // Tiles.  The rows of one cache head -- new tokens times the query heads that
 // share it -- are cut into blocks of 128, and a block takes its keys in tiles.
@@ -214,9 +215,7 @@ struct Op<_Float16> {
   static constexpr uint16_t kExp = 0x7C00;
   static constexpr float kMax = 65504.f;
   static constexpr int kParts = 2;  // 11 bits each
-  // weights as fp16: 2^14 at most, so that what is left of a small weight after
-  // its first 11 bits is no subnormal
-  static constexpr float kLift = 14.f;
+  static constexpr bool kNarrow = true;  // a weight's range, see Rows::kFall
   static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a),
                                                   __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -229,7 +228,7 @@ struct Op<__bf16> {
   static constexpr uint16_t kExp = 0x7F80;
   static constexpr float kMax = 3.38953139e38f;
   static constexpr int kParts = 3;  // 8 bits each
-  static constexpr float kLift = 0.f;
+  static constexpr bool kNarrow = false;
   static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a),
                                                    __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -425,10 +424,21 @@ template <typename CT, int D, bool kExact, int NP>
 struct Rows {
   typedef Geo<D, kExact> G;
   typedef Op<CT> O;
-  static constexpr float kLift = NP > 1 ? O::kLift : 0.f;
-  // growth of the maximum that is left to the weights (fp16 parts have no room
-  // above kLift)
-  static constexpr float kSlack = NP > 1 && O::kLift > 0.f ? 0.f : 8.f;
+  // Weights are 2^(c s - m + kLift), and a tile's largest may pass m by kSlack.
+  //
+  // fp16 has no step below 2^-24, so that a weight loses bits below 2^-14, or with
+  // two parts, whose second begins 11 bits down, below 2^-3.  Weights are lifted to
+  // the top of its range, 2^15; and where a tile's largest score is more than kFall
+  // below m, m falls to it, or the many small weights of a row whose first key
+  // takes nearly all would lose them (a first key 20 nats above 5000 others and
+  // with a value near 0: the result off by 1% without).  What a weight loses is
+  // then 2^-25 against its own tile's largest, 2^(kLift - kFall) at least: 2^-24 of
+  // it, with two parts 2^-31.  l and o grow where m falls: it falls no further than
+  // takes l to 2^kTop, and o, 2^16 times that at most, stays within fp32.
+  static constexpr bool kNarrow = O::kNarrow;
+  static constexpr float kLift = !kNarrow ? 0.f : NP > 1 ? 14.f : 7.f;
+  static constexpr float kSlack = kNarrow && NP > 1 ? 0.f : 8.f;
+  static constexpr float kFall = 8.f, kTop = 80.f;
 
   s16x8 q[G::KS];
   f32x16 o[G::DB];
@@ -528,14 +538,23 @@ struct Rows {
                                                        false, false);
     return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
   }
-  // Some row's maximum has to follow a tile with the largest scores top.
-  __device__ __forceinline__ bool grows(float top) const { return __any(top > m + kSlack); }
+  // Some row's m has to follow a tile with the largest scores top.
+  __device__ __forceinline__ bool moves(float top) const {
+    return __any(top > m + kSlack || (kNarrow && top < m - kFall));
+  }
+  // Where it goes.
+  __device__ __forceinline__ float follow(float top) const {
+    float to = fmaxf(m, top);
+    if (kNarrow && top < m - kFall)
+      to = fmaxf(top, m - fmaxf(kTop - float(__builtin_amdgcn_frexp_expf(sum())), 0.f));
+    return to;
+  }
   // m follows; l and o with it.
-  __device__ __forceinline__ void grow(float top) {
-    if (grows(top)) {
-      const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown;
+  __device__ __forceinline__ void move(float top) {
+    if (moves(top)) {
+      const float to = follow(top), base = to == -INFINITY ? 0.f : to;
       const float keep = __builtin_amdgcn_exp2f(m - base);
-      m = grown;
+      m = to;
       l *= keep;
 #pragma unroll
       for (int db = 0; db < G::DB; db++)
@@ -596,7 +615,7 @@ struct Rows {
 #pragma unroll
     for (int q = first(f); q < first(f + 1); q++) weigh_in(s, kg0 + (q >> 2), q & 3, base, x[q]);
   }
-  // A tile of 32 keys after its scores and grow(): weights, and o = o + V^T P^T
+  // A tile of 32 keys after its scores and move(): weights, and o = o + V^T P^T
   // over the values in LDS at v.  A step is one block of dims of one group of 16
   // keys: its product, the read of the values four steps on, and a share of the
   // next group's weights, which the matrix pipe's time hides.
@@ -684,7 +703,7 @@ struct Rows {
     // of all groups but the last, each behind the sums that its old weights are for
     constexpr int kPairs = KB == 2 ? 12 : 4;
     float top = s[0][0], keep = 1.f, w[kPairs][2];
-    bool grew = false;
+    bool moved = false;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = 0; f < kSteps; f++) {
@@ -702,11 +721,11 @@ struct Rows {
           top = fmaxf(top, s[e >> 4][e & 15]);
         if (db + 1 == G::DB) {
           top = join_halves(top);
-          grew = grows(top);
-          const float grown = grew ? fmaxf(m, top) : m;
-          const float zero = grown == -INFINITY ? 0.f : grown;
+          moved = moves(top);
+          const float to = moved ? follow(top) : m;
+          const float zero = to == -INFINITY ? 0.f : to;
           keep = __builtin_amdgcn_exp2f(m - zero);
-          m = grown;
+          m = to;
           base = zero - kLift;
           l *= keep;
         }
@@ -722,7 +741,7 @@ struct Rows {
 #pragma unroll
       for (int f = 0; f < 3; f++) weigh_step<4, 1>(s, 1, f, base, w, p);
     }
-    if (kSums && grew) {
+    if (kSums && moved) {
 #pragma unroll
       for (int db = 0; db < G::DB; db++)
 #pragma unroll
@@ -998,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
         }
       }
       if (p < all_lo || p + 32 > all_hi) a.template hide<1>(sc, p, lane);
-      a.grow(a.template largest<1>(sc));
+      a.move(a.template largest<1>(sc));
       if (more) wait_dma<2 * G::NI>();
       else wait_dma<0>();
       if (safe) {
