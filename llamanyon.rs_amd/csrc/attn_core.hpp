@@ -430,9 +430,9 @@ struct Rows {
   // two parts, whose second begins 11 bits down, below 2^-3.  Weights are lifted to
   // the top of its range, 2^15; and where a tile's largest score is more than kFall
   // below m, m falls to it, or the many small weights of a row whose first key
-  // takes nearly all would lose them (a first key 20 nats above 5000 others and
-  // with a value near 0: the result off by 1% without).  What a weight loses is
-  // then 2^-25 against its own tile's largest, 2^(kLift - kFall) at least: 2^-24 of
+  // takes nearly all would lose them (one 16 nats above 3000 others, of a value
+  // of 0: the result off by 6% without either, at 18 all of it gone).  What a weight
+  // loses is then 2^-25 against its own tile's largest, 2^(kLift - kFall) at least: 2^-24 of
   // it, with two parts 2^-31.  l and o grow where m falls: it falls no further than
   // takes l to 2^kTop, and o, 2^16 times that at most, stays within fp32.
   static constexpr bool kNarrow = O::kNarrow;

@@ -83,6 +83,35 @@ def test_small_weights_of_an_fp16_cache(pkg, dev, new, n, dim, below, spread, ou
     assert torch.all(err <= bound), (err / bound).max()
 
 
+@pytest.mark.parametrize("new,n,dim", [(1, 700, 128), (1, 3000, 64), (60, 400, 128), (50, 300, 96),
+                                       (40, 300, 256)])
+def test_fp16_output_of_a_bf16_cache(pkg, dev, new, n, dim):
+    """An output of 11 bits: the weights carry at least as many, and not bf16's 8.
+    Two keys whose values differ by their sign: what a weight's rounding moves is not
+    averaged away."""
+    print("[gpu case] fp16 of bf16", new, n, dim, flush=True)
+    c = Paged([new], [n], 1, dim, 16, BF16)
+    k, v = (x.clone() for x in c.keys(0))
+    k[:, 0, 0] = -60.0
+    k[0, 0, 0], k[1, 0, 0] = 0.0, -0.4921875  # its weight lies between two bf16 numbers
+    v[0], v[1] = 1.0, -1.0
+    for p in range(n):
+        c.put(0, p, k=k[p], v=v[p])
+    q = torch.zeros((new, 2, dim), dtype=torch.bfloat16)
+    q[:, :, 0] = 1
+    want, _ = attention(c, q, 1.0)
+    # sum p |v| / sum p is 1: half an fp16 step of each weight, and of the output; the
+    # exponential's and the sums' 8 roundings of 2^-24
+    bound = 2.0 ** -11 + want.abs() * 2.0 ** -11 + 8 * 2.0 ** -24
+    err = (_run(pkg, c, q, 1.0, F16).double() - want).abs()
+    assert torch.all(err <= bound), (err / bound).max()
+    c2 = Paged([new], [n], 2, dim, 16, BF16)
+    q2 = (torch.randn((new, 4, dim), generator=c2.g) * 1.5).bfloat16()
+    want, bound = attention(c2, q2, 1 / math.sqrt(dim), 0, True, F16)
+    err = (_run(pkg, c2, q2, 1 / math.sqrt(dim), F16).double() - want).abs()
+    assert torch.all(err <= bound), (err / bound).max()
+
+
 @pytest.mark.parametrize("code,out_code", [(F16, F16), (F16, F32), (BF16, BF16)])
 @pytest.mark.parametrize("new,n,dim", [(1, 1500, 64), (80, 900, 128), (40, 600, 256)])
 def test_maximum_that_falls_and_rises(pkg, dev, code, out_code, new, n, dim):
