@@ -116,6 +116,9 @@ __device__ __forceinline__ s16x4 lds_tr(uint32_t at, uint32_t off) {
 }
 
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uni(float x) {
+  return __uint_as_float(uint32_t(uni(int(__float_as_uint(x)))));
+}
 __device__ __forceinline__ const void *uni(const void *p) {
   const uint64_t x = uint64_t(uintptr_t(p));
   const uint32_t lo = uint32_t(uni(int(uint32_t(x)))), hi = uint32_t(uni(int(x >> 32)));
@@ -266,8 +269,9 @@ struct Geo {
 // kWhole: a group of 16 keys lies within a page, pages and the way from page to
 // page are below 4 GB; a group's address is then the scalar unit's.  Else every
 // lane has its own, and reads page 0 in place of one that is none (q's first row
-// where the cache has no pages).
-template <int D, bool kExact, bool kWhole>
+// where the cache has no pages).  kOne: this wave brings keys only or values only,
+// whose pointer and offsets are k and koff then.
+template <int D, bool kExact, bool kWhole, bool kOne>
 struct Feed {
   typedef Geo<D, kExact> G;
   const uint8_t *k, *v;     // slot 0 of page 0 of this head
@@ -287,9 +291,11 @@ struct Feed {
     int p0;
   };
 
-  __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane) {
+  __device__ __forceinline__ void init(const Work &w, const G &g, int s, int head, int lane,
+                                       bool values = false) {
     k = reinterpret_cast<const uint8_t *>(w.cache.k + int64_t(head) * w.cache.head_stride);
     v = reinterpret_cast<const uint8_t *>(w.cache.v + int64_t(head) * w.cache.head_stride);
+    if (kOne && values) k = v;
     table = w.b.pages + int64_t(s) * w.b.pages_stride;
     page_bytes = w.cache.page_stride * 2;
     slot_bytes = w.cache.slot_stride * 2;
@@ -312,7 +318,7 @@ struct Feed {
                            : near ? uint32_t(r & in_page) * uint32_t(slot_bytes)
                                   : 0;
       rows |= uint32_t(r) << (4 * j);
-      koff[j] = row + 16 * G::k_chunk(r, c);
+      koff[j] = row + 16 * (kOne && values ? G::v_chunk(r, c) : G::k_chunk(r, c));
       voff[j] = row + 16 * G::v_chunk(r, c);
     }
   }
@@ -380,8 +386,8 @@ struct Feed {
   // (the result is NaN then).
   template <bool kK>
   __device__ __forceinline__ void issue(const Place &g, uint32_t to) {
-    const uint8_t *base = kK ? k : v;
-    const uint32_t *off = kK ? koff : voff;
+    const uint8_t *base = kK || kOne ? k : v;
+    const uint32_t *off = kK || kOne ? koff : voff;
     if constexpr (kWhole) {
       if (!swamp::page_ok(g.id[0], n_pages)) return;
       if (inside(g.p0)) {
@@ -479,6 +485,9 @@ struct Rows {
   // q's row as B operand; a negative scale goes into its signs.
   __device__ __forceinline__ void load_q(const G &g, const uint16_t *row, float scale, int lane) {
     c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);  // 0 would make NaN of a hidden key's -inf
+    // (the scalar unit's where vector registers are few; prompts of 64 dims lose by it,
+    // 85 us and 88)
+    if constexpr (D >= 128) c = uni(c);
     const short sign = scale < 0.f ? short(0x8000) : short(0);
 #pragma unroll
     for (int ks = 0; ks < G::KS; ks++) {
@@ -491,6 +500,14 @@ struct Rows {
       }
       q[ks] = x;
     }
+#ifdef __HIP_DEVICE_COMPILE__
+    // (above 128 dims in accumulator registers, where products read it as well: with
+    // the sums they are more than half of those)
+    if constexpr (D > 128) {
+#pragma unroll
+      for (int ks = 0; ks < G::KS; ks++) asm volatile("" : "+a"(q[ks]));
+    }
+#endif
   }
 
   // Scores of KB x 32 keys in LDS at k.
@@ -974,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   a.hi = min(mine.hi, pc.end);
   const int all_lo = max(pc.seen(pc.rows - 1, w).lo, pc.begin);
   const int all_hi = min(pc.seen(0, w).hi, pc.end);
-  typedef Feed<D, kExact, kWhole> F;
+  typedef Feed<D, kExact, kWhole, false> F;
   F f;
   f.init(w, g, s, head, lane);
   f.bad = pc.over;
@@ -985,7 +1002,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Wo
   bool bad = false;
   for (int safe = 0; safe < 2; safe++) {
     a.clear();
-    int p = pc.tile0 + 32 * wave;
+    // (fresh, or the first tile's addresses are kept for the second pass)
+    int p = uni(fresh(pc.tile0 + 32 * wave));
     typename F::Place at[2];
     if (p < pc.stop) {
 #pragma unroll
@@ -1128,7 +1146,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
   const bool store = 32 * wave + (lane & 31) < pc.rows;
   const int64_t rr = pc.r0 + min(32 * wave + (lane & 31), pc.rows - 1);
   const int hq = head * w.group + int(rr % w.group);
-  const int64_t t = pc.token(rr, w.group);
+  const int t = int(pc.token(rr, w.group));
   Rows<CT, D, kExact, NP> a;
   a.addresses(g, lane);
   a.load_q(g, w.q + t * w.q_stride + int64_t(hq) * dim, w.scale, lane);
@@ -1140,55 +1158,66 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
   const swamp::Span wz = pc.seen(pc.r0 + min(32 * wave + 31, pc.rows - 1), w);
   const int any_lo = max(wa.lo, pc.begin), any_hi = min(wz.hi, pc.end);
   const int all_lo = max(wz.lo, pc.begin), all_hi = min(wa.hi, pc.end);
-  typedef Feed<D, kExact, kWhole> F;
+  typedef Feed<D, kExact, kWhole, KB == 1> F;
   F f;
-  f.init(w, g, s, head, lane);
+  f.init(w, g, s, head, lane, wave >= 2);
   f.bad = pc.over;
   f.lo = pc.begin;
   f.hi = pc.end;
+  int tile0 = pc.tile0;
   const int n_tiles = (pc.stop - pc.tile0 + kKeys - 1) / kKeys;
 
   // K and V of tile i.  Tiles of 64 keys: each wave a group of either; of 32: two
   // waves K, two waves V.
   const int part = 16 * (KB == 2 ? wave : wave & 1);
-  typename F::Place ahead, behind;  // of the tiles whose K and V are next
+  // Places of the tiles whose K and V are next.  Tiles of 32: a wave brings one of
+  // the two and knows `ahead` only, `lead` tiles from the turn's.
+  typename F::Place ahead, behind;
+  const int lead = KB == 2 || wave < 2 ? 2 : 1;
   const uint32_t part_at = lds + (part >> 4) * G::kGroup;
   auto bring_k = [&](int i) {
     if (KB == 2 || wave < 2) f.template issue<true>(ahead, part_at + (i & 1) * kPart);
   };
   auto bring_v = [&](int i) {
-    if (KB == 2 || wave >= 2) f.template issue<false>(behind, part_at + (2 + (i & 1)) * kPart);
+    if (KB == 2) f.template issue<false>(behind, part_at + (2 + (i & 1)) * kPart);
+    else if (wave >= 2) f.template issue<false>(ahead, part_at + (2 + (i & 1)) * kPart);
   };
-  auto find = [&](int i) { return f.template find<false>(pc.tile0 + i * kKeys + part); };
+  auto find = [&](int i) { return f.template find<false>(tile0 + i * kKeys + part); };
   auto k_of = [&](int i) { return lds + (i & 1) * kPart; };
   auto v_of = [&](int i) { return lds + (2 + (i & 1)) * kPart; };
   // tiles with keys that rows of this wave see, and of which they see every key
   const int first = any_hi > any_lo ? (any_lo - pc.tile0) / kKeys : n_tiles;
   const int last = any_hi > any_lo ? (any_hi - pc.tile0 + kKeys - 1) / kKeys : n_tiles;
   auto plain = [&](int i) {
-    const int p = pc.tile0 + i * kKeys;
+    const int p = tile0 + i * kKeys;
     return p >= all_lo && p + kKeys <= all_hi;
   };
   auto run = [&](auto safe) {
+    // (nor are the first tile's addresses, or q, kept for the second pass where
+    // registers are few)
+    if constexpr (decltype(safe)::value && D > 128) {
+      tile0 = uni(fresh(tile0));
+      a.load_q(g, w.q + fresh(t * w.q_stride + int64_t(hq) * dim), w.scale, lane);
+    }
     // (A wave on its way through products goes before one that prepares a tile: 4096
     // tokens over themselves 274 -> 272 us, 512 over 16384 keys 146 -> 141.)
     // Turn i = -1 .. n_tiles - 1: K of tile i + 1 and V of tile i are there, and
     // nobody reads what K of i + 2 and V of i + 1 go over.  ahead = the place of
-    // tile i + 2, behind = of i + 1.
+    // tile i + lead, behind = of i + 1.
     auto turn = [&](int i) {
       wait_all();
-      if (i + 2 < n_tiles) f.arrive(ahead);
-      const typename F::Place then = find(min(i + 3, n_tiles));
+      if (i + lead < n_tiles) f.arrive(ahead);
+      const typename F::Place then = find(min(i + lead + 1, n_tiles));
       if (i + 2 < n_tiles) bring_k(i + 2);
       if (i + 1 < n_tiles) bring_v(i + 1);
-      behind = ahead;
+      if (KB == 2) behind = ahead;
       ahead = then;
       if constexpr (decltype(safe)::value) {
         if (i < 0) return;
         const uint32_t v = v_of(i), mine_v = v + (part >> 4) * G::kGroup;
         if (anywhere(a.odd_values(g, mine_v, lane), extra)) {
           for (int j = 0; j < 2 * KB; j++)
-            a.add_odd_values(g, v + j * G::kGroup, pc.tile0 + i * kKeys + 16 * j, lane);
+            a.add_odd_values(g, v + j * G::kGroup, tile0 + i * kKeys + 16 * j, lane);
           __syncthreads();
           a.clear_odd_values(g, mine_v, lane);
           __syncthreads();
@@ -1198,10 +1227,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
     a.clear();
     if (n_tiles == 0) return;
     ahead = find(0);
-    f.arrive(ahead);
-    bring_k(0);
-    behind = ahead;
-    ahead = find(1);
+    if (lead == 2) {
+      f.arrive(ahead);
+      bring_k(0);
+      if (KB == 2) behind = ahead;
+      ahead = find(1);
+    }
     int i = -1;
     for (; i + 1 < first; i++) turn(i);
     if (first < last) {
@@ -1210,13 +1241,13 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_many_kernel(W
       float base = 0.f;
       turn(i);
       a.template scores_ahead<KB, false>(g, k_of(i + 1), sc, wt, base, lane);
-      if (!plain(i + 1)) a.template hide<KB>(sc, pc.tile0 + (i + 1) * kKeys, lane);
+      if (!plain(i + 1)) a.template hide<KB>(sc, tile0 + (i + 1) * kKeys, lane);
       a.template weigh_ahead<KB, false>(g, 0, sc, wt, base);
       for (i++; i + 1 < last; i++) {
         turn(i);
         __builtin_amdgcn_s_setprio(1);
         a.template scores_ahead<KB, true>(g, k_of(i + 1), sc, wt, base, lane);
-        if (!plain(i + 1)) a.template hide<KB>(sc, pc.tile0 + (i + 1) * kKeys, lane);
+        if (!plain(i + 1)) a.template hide<KB>(sc, tile0 + (i + 1) * kKeys, lane);
         a.template weigh_ahead<KB, true>(g, v_of(i), sc, wt, base);
         __builtin_amdgcn_s_setprio(0);
       }
