@@ -75,6 +75,18 @@ class AttentionLayer:
             "y": torch.empty((n_tok, self.width), device="cuda"),
         }
 
+    def scratch(self, batch, prompt):
+        """Bytes that the calls of a step take from the stream's scratch: what to reserve
+        before a capture.  They run one after the other and share it, so the most of them."""
+        lib, n = self.pkg.gpu_lib(), batch.n_tok
+        shapes = ((self.qkv_rows, self.width, 0), (self.width, self.n_heads * self.dim, 1))
+        needs = [lib.swamp_attn_paged_workspace(self.cache, batch, self.n_heads, 0)]
+        for rows, cols, accumulate in shapes:
+            needs.append(lib.swamp_qgemm_workspace(self.dtype, self.pkg.BF16, n, rows, cols) if prompt
+                         else lib.swamp_qgemv_batched_workspace(self.dtype, n, rows, cols,
+                                                                accumulate))
+        return max(needs)
+
     def __call__(self, hidden, batch, buf):
         """hidden [tokens][width] fp32 += the layer's attention, on the current stream:
         the new tokens of `batch`, all of them (buffers(..., prompt=True)) or one a
@@ -149,8 +161,7 @@ def main():
     token = torch.randn((n, layer.width), device="cuda")
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     side.wait_stream(torch.cuda.current_stream())
-    need = layer.pkg.gpu_lib().swamp_attn_paged_workspace(layer.cache, batch1, layer.n_heads, 0)
-    layer.pkg.workspace_reserve(side.cuda_stream, need + (1 << 20))
+    layer.pkg.workspace_reserve(side.cuda_stream, layer.scratch(batch1, prompt=False))
     with torch.cuda.graph(graph, stream=side):
         lens += 1
         layer(token, batch1, buf1)
