@@ -622,7 +622,9 @@ int swamp_rope_freqs(double *freqs, int n_rot, double base, double factor, int o
     double f = std::pow(base, -2.0 * i / n_rot);
     if (divisors) f /= double(divisors[i]);
     if (ramp) {
-      const double slow = std::min(1.0, std::max(0.0, (i - lo) / std::max(0.001, hi - lo)));
+      // (from hi on all of it, also where hi lies before the first pair)
+      const double slow =
+          i >= hi ? 1.0 : std::min(1.0, std::max(0.0, (i - lo) / std::max(0.001, hi - lo)));
       f = f * (1.0 - slow) + f / factor * slow;
     } else {
       f /= factor;
