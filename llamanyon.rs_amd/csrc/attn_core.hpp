@@ -5,7 +5,8 @@
 // sum l: a tile's scores s, m' = max(m, c max s) with c = scale log2 e, p =
 // 2^(c s - m'), l and o scaled by 2^(m - m') where m grows by more than kSlack
 // (p then reaches 2^kSlack at most; sums and the last division do not care).
-// fp16 weights are lifted, and m follows the tiles down as well (Rows::kFall).
+// For fp16 weights m lies below the maximum, and follows the tiles down as well
+// (Rows::kFall).
 //
 // Tiles.  The rows of one cache head -- new tokens times the query heads that
 // share it -- are cut into blocks of 128, and a block takes its keys in tiles.
@@ -430,17 +431,21 @@ template <typename CT, int D, bool kExact, int NP>
 struct Rows {
   typedef Geo<D, kExact> G;
   typedef Op<CT> O;
-  // Weights are 2^(c s - m + kLift), and a tile's largest may pass m by kSlack.
+  // Weights are 2^(c s - m).  A tile that moves m puts it kLift below its largest
+  // score, and its largest may pass that by kSlack.
   //
   // fp16 has no step below 2^-24, so that a weight loses bits below 2^-14, or with
   // two parts, whose second begins 11 bits down, below 2^-3.  Weights are lifted to
-  // the top of its range, 2^15; and where a tile's largest score is more than kFall
-  // below m, m falls to it, or the many small weights of a row whose first key
-  // takes nearly all would lose them (one 16 nats above 3000 others, of a value
+  // the top of its range, 2^15; and where a tile's largest would be lifted by less
+  // than kLift - kFall, m falls to it, or the many small weights of a row whose first
+  // key takes nearly all would lose them (one 16 nats above 3000 others, of a value
   // of 0: the result off by 6% without either, at 18 all of it gone).  What a weight
-  // loses is then 2^-25 against its own tile's largest, 2^(kLift - kFall) at least: 2^-24 of
-  // it, with two parts 2^-31.  l and o grow where m falls: it falls no further than
-  // takes l to 2^kTop, and o, 2^16 times that at most, stays within fp32.
+  // loses is then 2^-25 against its own tile's largest, 2^(kLift - kFall) at least:
+  // 2^-24 of it, with two parts 2^-31.  l and o grow where m falls: it falls no
+  // further than takes l to 2^kTop, and o, 2^16 times that at most, stays within fp32.
+  // Scores have their own rounding, 2^-24 of them: m keeps clear of the range's end
+  // by that much (scores of 2^24 and more; from 2^25 on the range is too short to
+  // hold it and weights lose bits again).
   static constexpr bool kNarrow = O::kNarrow;
   static constexpr float kLift = !kNarrow ? 0.f : NP > 1 ? 14.f : 7.f;
   static constexpr float kSlack = kNarrow && NP > 1 ? 0.f : 8.f;
@@ -556,15 +561,19 @@ struct Rows {
     return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
   }
   // Some row's m has to follow a tile with the largest scores top.
+  __device__ __forceinline__ bool falls(float top) const {
+    return kNarrow && top < m + (kLift - kFall);
+  }
   __device__ __forceinline__ bool moves(float top) const {
-    return __any(top > m + kSlack || (kNarrow && top < m - kFall));
+    const float most = m + (kLift + kSlack);
+    return __any(top > (kNarrow ? __builtin_fmaf(fabsf(m), -0x1p-22f, most) : most) || falls(top));
   }
   // Where it goes.
   __device__ __forceinline__ float follow(float top) const {
-    float to = fmaxf(m, top);
-    if (kNarrow && top < m - kFall)
-      to = fmaxf(top, m - fmaxf(kTop - float(__builtin_amdgcn_frexp_expf(sum())), 0.f));
-    return to;
+    if (!kNarrow) return fmaxf(m, top);
+    const float at = top == -INFINITY ? top : __builtin_fmaf(fabsf(top), 0x1p-23f, top - kLift);
+    const float room = kTop - float(__builtin_amdgcn_frexp_expf(sum()));
+    return fmaxf(at, falls(top) ? m - fmaxf(room, 0.f) : m);
   }
   // m follows; l and o with it.
   __device__ __forceinline__ void move(float top) {
@@ -586,7 +595,7 @@ struct Rows {
     for (int e = 1; e < 16 * KB; e++) top = fmaxf(top, s[e >> 4][e & 15]);
     return join_halves(top);
   }
-  __device__ __forceinline__ float base_of() const { return (m == -INFINITY ? 0.f : m) - kLift; }
+  __device__ __forceinline__ float base_of() const { return m == -INFINITY ? 0.f : m; }
 
   // Weights 2 j and 2 j + 1 of the group kg, in three stages, so that none waits for
   // the one before it where steps take them in turn: x = c s - base, ...
@@ -740,10 +749,9 @@ struct Rows {
           top = join_halves(top);
           moved = moves(top);
           const float to = moved ? follow(top) : m;
-          const float zero = to == -INFINITY ? 0.f : to;
-          keep = __builtin_amdgcn_exp2f(m - zero);
+          base = to == -INFINITY ? 0.f : to;
+          keep = __builtin_amdgcn_exp2f(m - base);
           m = to;
-          base = zero - kLift;
           l *= keep;
         }
       } else {

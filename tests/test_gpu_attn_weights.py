@@ -1,6 +1,7 @@
 """The softmax weights of swamp_attn_paged on the GPU, against 64 bits on the CPU,
 where the keys that make a row's result weigh far less than its largest one: a
 first key that takes nearly all of the weight and whose own value is 0."""
+import copy
 import math
 
 import pytest
@@ -133,3 +134,41 @@ def test_maximum_that_falls_and_rises(pkg, dev, code, out_code, new, n, dim):
     want, bound = attention(c, q, 1.0, 0, out_code == F32, out_code)
     err = (_run(pkg, c, q, 1.0, out_code).double() - want).abs()
     assert torch.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("out_code", [F16, F32])
+@pytest.mark.parametrize("new,n,dim", [(1, 300, 64), (60, 300, 64), (50, 200, 128), (40, 200, 256)])
+def test_fp16_scores_far_from_0(pkg, dev, new, n, dim, out_code):
+    """Scores of 2^25, whose own step is 4, and a maximum that grows by one such step
+    where it may or may not be followed: the weights' ratios are what the scores'
+    differences say, and none leaves fp16's range."""
+    print("[gpu case] scores of 2^25", new, n, dim, NAME[out_code], flush=True)
+    c = Paged([new], [n], 1, dim, 16, F16)
+    k, v = (x.clone() for x in c.keys(0))
+    k[:, 0, 0], k[:, 0, 1] = 16384.0, 0.0
+    k[n // 2:, 0, 1] = 4.0
+    for p in range(n):
+        c.put(0, p, k=k[p])
+    q = torch.zeros((new, 2, dim), dtype=torch.float16)
+    q[:, :, 0], q[:, :, 1] = 2048.0, 1.0
+    for scale in (0.55, 0.9, 1.0, 1.3, 1.4, 1.44, 1.47, 1.5, 1.56, 1.6, 1.8, -1.0):
+        want, _ = attention(c, q, scale)
+        mean, _ = attention(_with_values(c, v.abs()), q, scale)
+        # scores are exact, and what their products with c are off by is common to all
+        # keys but for 2^-24 of their difference, 4; weights as stated, in numerator only
+        # (the sum has them whole), and 8 sqrt(n) 2^-24 for the additions of either
+        rel = (2.0 ** -22 if out_code == F32 else 2.0 ** -11) + 2.0 ** -24 * (40 + 16 * math.sqrt(n))
+        bound = mean * rel + want.abs() * half_step(out_code) + 2.0 ** -25
+        got = _run(pkg, c, q, scale, out_code)
+        assert got.isfinite().all(), scale
+        err = (got.double() - want).abs()
+        assert torch.all(err <= bound), (scale, (err / bound).max())
+
+
+def _with_values(c, v):
+    """The cache with other values, for the oracle."""
+    other = copy.copy(c)
+    other.v = c.v.clone()
+    for p in range(c.lens[0]):
+        other.put(0, p, v=v[p])
+    return other
