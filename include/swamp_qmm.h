@@ -427,9 +427,9 @@ SWAMP_API int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch
  * of out_type F32, F16 or BF16, 16-byte aligned (out_stride a multiple of 8).
  * Scores, softmax and sums are fp32.  The weights p_j are rounded before they
  * meet v: with 16-bit output to the cache's type, by 2^-8 of each (bf16) or 2^-11
- * (fp16) at most; with F32 output, and F16 output of a bf16 cache, to 22 bits or more.  fp16 weights far below the
- * largest of the 64 keys beside them are off by 2^-24 of that one's (F32 output:
- * 2^-31) instead.
+ * (fp16) at most; with F32 output to 22 bits or more, with F16 output of a bf16
+ * cache to 16.  fp16 weights far below the largest of the 64 keys beside them are
+ * off by 2^-24 of that one's (F32 output: 2^-31) instead.
  * Keys that a row does not see, and slots past d_len, do not reach its result,
  * whatever they hold.  A row that sees no key gives 0; rows of no sequence are
  * not touched; a row block that has to read a position without a page gives NaN

@@ -3,8 +3,8 @@
 // type in attn_f16.hip and attn_bf16.hip.
 #include "attn_core.hpp"
 
-int swamp_attn_f16(const swamp_attn::Work &w, bool precise, hipStream_t s);
-int swamp_attn_bf16(const swamp_attn::Work &w, bool precise, hipStream_t s);
+int swamp_attn_f16(const swamp_attn::Work &w, int parts, hipStream_t s);
+int swamp_attn_bf16(const swamp_attn::Work &w, int parts, hipStream_t s);
 
 namespace {
 
@@ -122,15 +122,16 @@ int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStr
     w.stat = static_cast<f32x2 *>(sc.get(swamp::attn_stat_bytes(c, p.splits)));
     if (!w.part || !w.stat) w.splits = 1;
   }
-  // Weights in several parts where the output has more bits than the cache's type.
-  // Elsewhere one rounding of theirs, 2^-8 or 2^-11, is as large as the output's own.
-  // (Two or three products for one of the sums cost blocks of many rows a third to a
-  // half, 4096 tokens of 32 heads of 128 dims 159 us and 215; few rows 1 to 2% in full
-  // batches and up to 15% in short calls, 16 drafts of 4 tokens over 2000 keys of 80
-  // dims 17.9 us and 20.2.)
-  const bool precise =
-      c.out_type == SWAMP_F32 || (c.out_type == SWAMP_F16 && c.dtype == SWAMP_BF16);
-  const int rc = c.dtype == SWAMP_F16 ? swamp_attn_f16(w, precise, s) : swamp_attn_bf16(w, precise, s);
+  // Weights in as many parts of the cache's type as the output has bits for: 11 a part
+  // in fp16, 8 in bf16.  With 16-bit output of the cache's own type, or less, one
+  // rounding of theirs is as large as the output's.  (A further product for one of the
+  // sums costs blocks of many rows about a third each: 4096 tokens of 32 heads of 128
+  // dims, fp16 160 us and 218, bf16 151, 199 and 241; few rows 1 to 2% in full batches
+  // and up to 15% in short calls, 16 drafts of 4 tokens over 2000 keys of 80 dims 17.9
+  // us and 20.2.)
+  const bool half_of_bf16 = c.dtype == SWAMP_BF16 && c.out_type == SWAMP_F16;
+  const int parts = c.out_type == SWAMP_F32 ? 3 : half_of_bf16 ? 2 : 1;
+  const int rc = c.dtype == SWAMP_F16 ? swamp_attn_f16(w, parts, s) : swamp_attn_bf16(w, parts, s);
   if (rc != SWAMP_OK || w.splits == 1) return rc;
   int per = 2, shares = 1;
   while (4 * per < c.cache.dim) per *= 2;

@@ -218,7 +218,7 @@ struct Op<_Float16> {
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint16_t kExp = 0x7C00;
   static constexpr float kMax = 65504.f;
-  static constexpr int kParts = 2;  // 11 bits each
+  static constexpr int kParts = 2;  // 11 bits each: 22
   static constexpr bool kNarrow = true;  // a weight's range, see Rows::kFall
   static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a),
@@ -231,7 +231,7 @@ struct Op<__bf16> {
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint16_t kExp = 0x7F80;
   static constexpr float kMax = 3.38953139e38f;
-  static constexpr int kParts = 3;  // 8 bits each
+  static constexpr int kParts = 3;  // 8 bits each: 24
   static constexpr bool kNarrow = false;
   static __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a),
@@ -1297,30 +1297,32 @@ void launch_kind(const Work &w, hipStream_t s) {
 }
 
 template <typename CT, int D, bool kExact>
-int launch(const Work &w, bool precise, hipStream_t s) {
-  constexpr int kParts = Op<CT>::kParts;
+int launch(const Work &w, int parts, hipStream_t s) {
   // (heads of other sizes take every lane's own pages: the general form)
   const bool whole = kExact && w.cache.page_shift >= 4 &&
                      w.cache.page_stride < (int64_t(1) << 31) &&
                      (w.cache.slot_stride << w.cache.page_shift) < (int64_t(1) << 30);
-  if (whole && precise) launch_kind<CT, D, kExact, kExact, kParts>(w, s);
-  else if (whole) launch_kind<CT, D, kExact, kExact, 1>(w, s);
-  else if (precise) launch_kind<CT, D, kExact, false, kParts>(w, s);
-  else launch_kind<CT, D, kExact, false, 1>(w, s);
+  auto go = [&](auto np) {
+    if (whole) launch_kind<CT, D, kExact, kExact, decltype(np)::value>(w, s);
+    else launch_kind<CT, D, kExact, false, decltype(np)::value>(w, s);
+  };
+  if (parts == 1) go(std::integral_constant<int, 1>{});
+  else if (parts == 2) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, Op<CT>::kParts>{});
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
 
 template <typename CT>
-int launch_dim(const Work &w, bool precise, hipStream_t s) {
+int launch_dim(const Work &w, int parts, hipStream_t s) {
   switch (w.cache.dim) {
-    case 64: return launch<CT, 64, true>(w, precise, s);
-    case 80: return launch<CT, 80, true>(w, precise, s);
-    case 96: return launch<CT, 96, true>(w, precise, s);
-    case 128: return launch<CT, 128, true>(w, precise, s);
-    case 256: return launch<CT, 256, true>(w, precise, s);
+    case 64: return launch<CT, 64, true>(w, parts, s);
+    case 80: return launch<CT, 80, true>(w, parts, s);
+    case 96: return launch<CT, 96, true>(w, parts, s);
+    case 128: return launch<CT, 128, true>(w, parts, s);
+    case 256: return launch<CT, 256, true>(w, parts, s);
   }
-  return w.cache.dim < 128 ? launch<CT, 128, false>(w, precise, s)
-                           : launch<CT, 256, false>(w, precise, s);
+  return w.cache.dim < 128 ? launch<CT, 128, false>(w, parts, s)
+                           : launch<CT, 256, false>(w, parts, s);
 }
 
 }  // namespace

@@ -11,8 +11,9 @@ import test_codegen as cg
 pytestmark = pytest.mark.skipif(not os.path.exists(cg.HIPCC), reason="hipcc not found")
 
 # kernels of each unit: rope and append by type pair, width and layout; the join by
-# batch; attention by head size (5, and two general ones), page form, rows and parts
-UNITS = {"rope.hip": 60, "attn.hip": 2, "attn_f16.hip": 48, "attn_bf16.hip": 48}
+# batch; attention by head size and page form (5 of two, and two general sizes), rows,
+# and parts of the weights (fp16 2, bf16 3)
+UNITS = {"rope.hip": 60, "attn.hip": 2, "attn_f16.hip": 48, "attn_bf16.hip": 72}
 
 
 def test_no_kernel_uses_scratch(tmp_path):
