@@ -396,7 +396,7 @@ SWAMP_API int swamp_rope_freqs(double *freqs, int n_rot, double base, double fac
 /* out[t][h] = x[t][h] turned by d_pos[t]: n_tok rows of n_heads heads of
  * head_dim (even, up to 512), rows x_stride and out_stride apart.  x_type and
  * out_type SWAMP_F32, SWAMP_F16 or SWAMP_BF16; computed in fp32 (the angle in
- * 64 bits: positions of any size), rounded once.  d_out may be d_x with the
+ * 64 bits: positions of any size), rounded once; fewer than 2^24 tokens a call.  d_out may be d_x with the
  * same type and stride; otherwise they must not overlap.  Buffers aligned to
  * their element. */
 SWAMP_API int swamp_rope(const swamp_rope_spec *rope, const int32_t *d_pos, const void *d_x,
@@ -435,8 +435,8 @@ SWAMP_API int swamp_kv_append(const swamp_kv_pages *cache, const swamp_seq_batch
  * not touched; a row block that has to read a position without a page gives NaN
  * (d_bad).
  * A long cache is split over workgroups that leave partial sums in the stream's
- * scratch ("Scratch" above; swamp_attn_paged_workspace reports it), joined in a
- * fixed order: repeated calls give the same bits.  Without it (under capture,
+ * scratch ("Scratch" above; swamp_attn_paged_workspace reports it, 256 MB at
+ * most), joined in a fixed order: repeated calls give the same bits.  Without it (under capture,
  * nothing reserved) the cache is not split.  SWAMP_ESHAPE for more work than one
  * launch holds: 2^24 blocks of 128 rows (token times query head of a cache head,
  * at least one block a sequence) over all cache heads. */

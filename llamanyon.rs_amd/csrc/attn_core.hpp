@@ -23,13 +23,13 @@
 // fragment read in different banks; V: the four rows of a transposing read),
 // other dims take an odd stride of chunks instead.
 //
-// Bounds and measures.  Decoding is HBM's: all keys once, 5.2 to 5.4 TB/s of the
-// 6.0 that a long read reaches (one token over 131072 keys 100 us).  Prompts are
+// Bounds and measures.  Decoding is HBM's: all keys once, 5.2 to 5.5 TB/s of the
+// 6.0 that a long read reaches (one token over 131072 keys 98 us).  Prompts are
 // the matrix pipe's and its power's: 4096 tokens of 64 heads of 128 dims take 274
 // us, 1000 TFLOP/s, where a bf16 product of the library reaches 1130 to 1230; of
 // 296 us on a slower card the exponentials cost 19, the DMAs 33, and what is left
 // without them, products, maximum and conversion, runs at 1175 TFLOP/s.  Two waves a
-// SIMD (203 registers) fill each other's gaps; blocks of 256 rows in workgroups of
+// SIMD (201 registers) fill each other's gaps; blocks of 256 rows in workgroups of
 // eight waves halve the DMAs and lost more to their common barrier (64 dims: 93 ->
 // 107 us).
 //
@@ -973,8 +973,9 @@ __device__ __forceinline__ bool find_piece(const Work &w, int s, int64_t r0, int
 // own 32-key tiles through its own quarter of LDS (K: 2 groups, V: 2 groups).
 // No barrier: a wave waits for its own DMAs only; K of the next tile is on its
 // way from the end of the scores, V from the end of the sums.
-// Eight waves a CU keep about 96 KB of loads in flight, what HBM's latency asks
-// for: one token over 131072 keys 100 us, 64 ragged sequences of up to 8192 226 us.
+// A wave has a tile of K and one of V on their way, 8 KB each of 128 dims, a CU's four
+// waves up to 64 KB: one token over 131072 keys, one workgroup a CU, 98 us; 64 ragged
+// sequences of up to 8192 in 2048 workgroups 225 us.
 template <typename CT, int D, bool kExact, bool kWhole, int NP>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attn_few_kernel(Work w) {
   typedef Geo<D, kExact> G;
