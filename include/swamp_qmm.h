@@ -15,8 +15,8 @@
  *  - Pointers named d_* are DEVICE pointers; the caller owns every buffer.
  *  - stream is a hipStream_t passed as void* (NULL = default stream); every
  *    device entry point is asynchronous on it.  None allocates, except that
- *    swamp_qgemv_batched, swamp_qgemm and swamp_attn_paged take scratch memory
- *    for split reductions from a buffer the library keeps per (device, stream):
+ *    swamp_qgemv_batched, swamp_qgemm, swamp_attn_paged, swamp_gemm_rows_i8 and
+ *    swamp_beam_select take scratch memory for split reductions from a buffer the library keeps per (device, stream):
  *    see "Scratch" below.
  *  - Return 0 on success, a negative SWAMP_E* code on error; on error no
  *    output is written and nothing is launched.
@@ -447,6 +447,143 @@ SWAMP_API int swamp_attn_paged(const swamp_kv_pages *cache, const swamp_seq_batc
 SWAMP_API size_t swamp_attn_paged_workspace(const swamp_kv_pages *cache,
                                             const swamp_seq_batch *batch, int n_heads,
                                             int window);
+
+/* ---- many rows at once: 8-bit products, beam selection, pages ----
+ *
+ * What a step of many sequences that share prompts takes besides the above:
+ * products of its rows in 8-bit integers, the selection among its logits, and
+ * the cache's pages that follow the selection.  No counterparts in the reference. */
+
+/* Rows to 8-bit codes with one scale a row: d_scale[i] = max_k |x[i][k]| / 127 in
+ * fp32, q[i][k] = x[i][k] / d_scale[i] in fp32, rounded to the nearest integer, even
+ * ones where two are as near (-127 .. 127).  Activations (a scale for each token) and
+ * weights (for each output row) alike.  A row whose scale would lie below 2^-126 is
+ * taken for zeros (scale 0); one that holds an infinity or NaN gets the scale NaN and
+ * codes 0, so that its products are NaN and no other's.
+ * x_type F32, F16 or BF16, rows x_stride elements apart; codes q_stride bytes apart
+ * (0: dense); buffers aligned to their element.  Bytes between the rows are left
+ * as they are.  n_cols == 0: scales 0. */
+SWAMP_API int swamp_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_stride,
+                                  int8_t *d_q, int64_t q_stride, float *d_scale, int n_rows,
+                                  int n_cols, void *stream);
+
+/* y[i][r] = d_x_scale[i] d_w_scale[r] sum_k x[i][k] w[r][k] over 8-bit codes, m rows
+ * of x and n_rows of w.  The sum is exact (int32, any codes); the product with both
+ * scales is taken in 64 bits and rounded to fp32, with accumulate != 0 added to y in
+ * fp32, and rounded to y_type (F32, F16 or BF16).  n_cols < 131072; code rows
+ * x_stride and w_stride bytes apart (0: dense), multiples of 16 below 2^23, d_x and
+ * d_w 16-byte aligned: of every row n_cols bytes are used; those between the rows, and
+ * behind the last one up to the next multiple of 16, may be read.  y_stride in elements
+ * (0: dense), d_y aligned to its element; m n_rows < 2^38.  n_cols == 0: a sum of
+ * nothing.
+ * Few rows split the sum over workgroups, whose parts meet in the stream's scratch
+ * (swamp_gemm_rows_i8_workspace reports it); without it the sum is not split.  The
+ * bits are the same either way. */
+SWAMP_API int swamp_gemm_rows_i8(const int8_t *d_x, int64_t x_stride, const float *d_x_scale,
+                                 const int8_t *d_w, int64_t w_stride, const float *d_w_scale,
+                                 void *d_y, uint32_t y_type, int64_t y_stride, int m, int n_rows,
+                                 int n_cols, int accumulate, void *stream);
+SWAMP_API size_t swamp_gemm_rows_i8_workspace(int m, int n_rows, int n_cols);
+
+/* n_seq sequences of n_beam beams each (1 to 64), rows sequence * n_beam + beam of
+ * all arrays; vocab tokens (1 to 2^20); the n_out (1 to 64) best continuations of
+ * each sequence are taken.  eos: the token that ends a beam, -1: none does. */
+typedef struct swamp_beam_spec {
+  int32_t n_seq, n_beam, vocab, n_out, eos;
+} swamp_beam_spec;
+
+/* The best continuations of every sequence over its beams and the vocabulary.
+ * Token v of beam b scores d_score[b] + x_v - log sum_u exp x_u, x the beam's row of
+ * d_logits (type F32, F16 or BF16, rows stride elements apart, 0: dense), in 64 bits.
+ * The n_out largest of a sequence are written in falling order, equal ones by beam,
+ * then token:
+ *   d_parent[n_seq][n_out]    the row (sequence * n_beam + beam) that is continued
+ *   d_token[n_seq][n_out]     by this token
+ *   d_out_score[n_seq][n_out] the score, rounded to fp32
+ *   d_out_done (may be NULL)  1 where the token is eos or the beam had ended, else 0
+ * Within a beam tokens rank by their logits.  A beam with d_done (int32; NULL: none)
+ * not 0 has ended: it has one continuation, eos at its own score, and its logits are
+ * not read.  A token of logit -infinity is none, and neither is any of a beam of score
+ * -infinity, or of one whose score or whose row's sum is NaN or +infinity (a row
+ * that holds NaN or +infinity).  Where fewer than n_out are left the rest has
+ * parent and token -1, score -infinity and done 0.
+ * With n_out == n_beam, d_out_score may be d_score and d_out_done may be d_done;
+ * otherwise outputs and inputs must not overlap.  d_logits aligned to its element.
+ * Takes scratch for the rows' parts (swamp_beam_select_workspace); SWAMP_EWORKSPACE
+ * without it. */
+SWAMP_API int swamp_beam_select(const swamp_beam_spec *spec, const void *d_logits, uint32_t type,
+                                int64_t stride, const float *d_score, const int32_t *d_done,
+                                int32_t *d_parent, int32_t *d_token, float *d_out_score,
+                                int32_t *d_out_done, void *stream);
+SWAMP_API size_t swamp_beam_select_workspace(const swamp_beam_spec *spec);
+
+/* Who holds the pages of a cache, on the device: d_refs[n_pages] counts the page
+ * tables that name a page (0: it is free), and bit p % 32 of d_used[p / 32] is set
+ * where d_refs[p] > 0; (n_pages + 31) / 32 words, bits past n_pages 0.  All zeros: an
+ * empty pool.  page_size as in swamp_kv_pages.  All layers of a model share a pool
+ * where they share page tables.  Calls on one pool must be ordered by the caller. */
+typedef struct swamp_page_pool {
+  int32_t n_pages, page_size;
+  int32_t *d_refs;
+  uint32_t *d_used;
+} swamp_page_pool;
+
+/* The page tables of n_seq sequences (2048 at most), on the device as in
+ * swamp_seq_batch: d_len tokens, of which a sequence holds the pages that its table
+ * names at 0 .. ceil(d_len / page_size) - 1 (pages_stride at most).  What the tables
+ * hold behind that is neither read nor written.  A table names a page once; entries
+ * outside 0 .. n_pages - 1 are no pages.  d_bad (may be NULL): set to 1 where a
+ * sequence does not get a page that it needs. */
+typedef struct swamp_page_tables {
+  int32_t n_seq;
+  int32_t *d_len, *d_pages;
+  int64_t pages_stride;
+  int32_t *d_bad;
+} swamp_page_tables;
+
+/* A list of pages to copy, on the device: d_src[i] to d_dst[i], i < *d_count <= cap.
+ * What the arrays hold behind the list is left as it is. */
+typedef struct swamp_page_moves {
+  int32_t cap;
+  int32_t *d_src, *d_dst, *d_count;
+} swamp_page_moves;
+
+/* Sequence s becomes a fork of sequence d_parent[s] as it was before the call, or
+ * empty (-1, or any other value that is no sequence): its pages and length; counts
+ * follow, and pages that no table names any more are free.  The pages are shared, the
+ * last one too: swamp_pages_extend parts who writes it. */
+SWAMP_API int swamp_pages_fork(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                               const int32_t *d_parent, void *stream);
+
+/* Pages for d_new[s] more tokens of every sequence (NULL: one each; below 1: none), and
+ * d_len grows by them: what swamp_kv_append takes next.  One sequence after the other:
+ * where its last page has room and other tables name it as well, the sequence gets a
+ * page of its own in its place, listed in `moves` to be copied (cap >= n_seq); then its
+ * new pages.  Every one is the lowest that is free.  Where none is left the entry
+ * becomes -1 (its tokens have no page), where the table is too short nothing is
+ * written; both set d_bad. */
+SWAMP_API int swamp_pages_extend(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                                 const int32_t *d_new, const swamp_page_moves *moves,
+                                 void *stream);
+
+/* Sequences keep their first d_keep[s] tokens (NULL: none) and give back the pages
+ * behind them; one that has fewer stays as it is.  Table entries stay. */
+SWAMP_API int swamp_pages_trim(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                               const int32_t *d_keep, void *stream);
+
+/* Moves pages to the lowest places: of the U pages in use the i-th lowest that lies at
+ * U or above moves to the i-th lowest free place below U, moves->cap of them at most.
+ * Counts and tables follow, `moves` gets the list.  `tables` must hold every sequence of
+ * the pool; the caches' pages must be copied (swamp_kv_copy) before they are read. */
+SWAMP_API int swamp_pages_compact(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                                  const swamp_page_moves *moves, void *stream);
+
+/* Copies the listed pages' keys and values in n_caches caches (a model's layers) of
+ * one type, shape and strides.  No page of the list's d_dst may be in it another time.
+ * Pairs with an id outside 0 .. n_pages - 1 are left out.  SWAMP_ESHAPE for caches that
+ * differ and for pages of 2^33 elements or more. */
+SWAMP_API int swamp_kv_copy(const swamp_kv_pages *caches, int n_caches,
+                            const swamp_page_moves *moves, void *stream);
 
 /* ---- the reference's two existing C exports, host-pointer semantics ---- */
 

@@ -45,7 +45,10 @@ GPU_SYMBOLS = (
     "swamp_qgemv_batched_workspace", "swamp_qgemm_workspace", "swamp_workspace_reserve",
     "swamp_qgemv_batched_noalloc", "swamp_qgemv_many",
     "swamp_rope_freqs", "swamp_rope", "swamp_kv_append", "swamp_attn_paged",
-    "swamp_attn_paged_workspace",
+    "swamp_attn_paged_workspace", "swamp_quantize_rows", "swamp_gemm_rows_i8",
+    "swamp_gemm_rows_i8_workspace", "swamp_beam_select", "swamp_beam_select_workspace",
+    "swamp_pages_fork", "swamp_pages_extend", "swamp_pages_trim", "swamp_pages_compact",
+    "swamp_kv_copy",
 )
 # Every symbol include/swamp_gguf.h declares (also in libswamp_gpu.so).
 GGUF_SYMBOLS = (
@@ -126,6 +129,50 @@ class SeqBatch(ctypes.Structure):
                          d_bad)
 
 
+class BeamSpec(ctypes.Structure):
+    """swamp_beam_spec: n_seq sequences of n_beam beams, the n_out best continuations."""
+
+    _fields_ = [("n_seq", ctypes.c_int32), ("n_beam", ctypes.c_int32), ("vocab", ctypes.c_int32),
+                ("n_out", ctypes.c_int32), ("eos", ctypes.c_int32)]
+
+    def __init__(self, n_seq: int, n_beam: int, vocab: int, n_out: int, eos: int = -1):
+        super().__init__(n_seq, n_beam, vocab, n_out, eos)
+
+
+class PagePool(ctypes.Structure):
+    """swamp_page_pool: counts (int32) and bits (uint32) of a cache's pages; zeros: empty."""
+
+    _fields_ = [("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("d_refs", c_vp),
+                ("d_used", c_vp)]
+
+    def __init__(self, n_pages: int, page_size: int, d_refs: int, d_used: int):
+        super().__init__(n_pages, page_size, d_refs, d_used)
+
+
+class PageTables(ctypes.Structure):
+    """swamp_page_tables: lengths and page tables of n_seq sequences (int32)."""
+
+    _fields_ = [("n_seq", ctypes.c_int32), ("d_len", c_vp), ("d_pages", c_vp),
+                ("pages_stride", ctypes.c_int64), ("d_bad", c_vp)]
+
+    def __init__(self, n_seq: int, d_len: int, d_pages: int, pages_stride: int, d_bad: int = 0):
+        super().__init__(n_seq, d_len, d_pages, pages_stride, d_bad)
+
+
+class PageMoves(ctypes.Structure):
+    """swamp_page_moves: a list of pages to copy, cap at most (int32)."""
+
+    _fields_ = [("cap", ctypes.c_int32), ("d_src", c_vp), ("d_dst", c_vp), ("d_count", c_vp)]
+
+    def __init__(self, cap: int, d_src: int, d_dst: int, d_count: int):
+        super().__init__(cap, d_src, d_dst, d_count)
+
+
+def kv_caches(caches: Sequence[KvPages]):
+    """The array that kv_copy takes: a model's layers."""
+    return (KvPages * len(caches))(*caches)
+
+
 def build(force: bool = False) -> None:
     """Compile both libraries in-tree with the package Makefile."""
     cmd = ["make", "-C", PKG_DIR, "-j8"]
@@ -186,6 +233,22 @@ def gpu_lib() -> ctypes.CDLL:
                                    i32, ctypes.c_float, i32, c_vp, u32, i64, c_vp]),
         "swamp_attn_paged_workspace": (c_size, [ctypes.POINTER(KvPages), ctypes.POINTER(SeqBatch),
                                                 i32, i32]),
+        "swamp_quantize_rows": (i32, [c_vp, u32, i64, c_vp, i64, c_vp, i32, i32, c_vp]),
+        "swamp_gemm_rows_i8": (i32, [c_vp, i64, c_vp, c_vp, i64, c_vp, c_vp, u32, i64, i32, i32,
+                                     i32, i32, c_vp]),
+        "swamp_gemm_rows_i8_workspace": (c_size, [i32, i32, i32]),
+        "swamp_beam_select": (i32, [ctypes.POINTER(BeamSpec), c_vp, u32, i64, c_vp, c_vp, c_vp,
+                                    c_vp, c_vp, c_vp, c_vp]),
+        "swamp_beam_select_workspace": (c_size, [ctypes.POINTER(BeamSpec)]),
+        "swamp_pages_fork": (i32, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTables), c_vp,
+                                   c_vp]),
+        "swamp_pages_extend": (i32, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTables), c_vp,
+                                     ctypes.POINTER(PageMoves), c_vp]),
+        "swamp_pages_trim": (i32, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTables), c_vp,
+                                   c_vp]),
+        "swamp_pages_compact": (i32, [ctypes.POINTER(PagePool), ctypes.POINTER(PageTables),
+                                      ctypes.POINTER(PageMoves), c_vp]),
+        "swamp_kv_copy": (i32, [ctypes.POINTER(KvPages), i32, ctypes.POINTER(PageMoves), c_vp]),
         "swamp_gemv_q8_vnni": (ctypes.c_float, [c_vp, c_vp, i32, ctypes.c_float]),
         # GGUF reader (include/swamp_gguf.h)
         "swamp_gguf_open": (i32, [ctypes.c_char_p, ctypes.POINTER(c_vp)]),
@@ -415,6 +478,58 @@ def attn_paged(cache: KvPages, batch: SeqBatch, d_q: int, n_heads: int, scale: f
     """Causal attention of the batch's new tokens over the paged cache."""
     _check(gpu_lib().swamp_attn_paged(cache, batch, d_q, q_stride, n_heads, scale, window, d_out,
                                       out_type, out_stride, stream), "swamp_attn_paged")
+
+
+def quantize_rows(d_x: int, x_type: int, d_q: int, d_scale: int, n_rows: int, n_cols: int,
+                  x_stride: int = 0, q_stride: int = 0, stream: int = 0) -> None:
+    """Rows to 8-bit codes with one fp32 scale each (activations, weights)."""
+    _check(gpu_lib().swamp_quantize_rows(d_x, x_type, x_stride, d_q, q_stride, d_scale, n_rows,
+                                         n_cols, stream), "swamp_quantize_rows")
+
+
+def gemm_rows_i8(d_x: int, d_x_scale: int, d_w: int, d_w_scale: int, d_y: int, y_type: int, m: int,
+                 n_rows: int, n_cols: int, x_stride: int = 0, w_stride: int = 0, y_stride: int = 0,
+                 accumulate: bool = False, stream: int = 0) -> None:
+    """Products of 8-bit rows with 8-bit weight rows, one scale a row on both sides."""
+    _check(gpu_lib().swamp_gemm_rows_i8(d_x, x_stride, d_x_scale, d_w, w_stride, d_w_scale, d_y,
+                                        y_type, y_stride, m, n_rows, n_cols,
+                                        1 if accumulate else 0, stream), "swamp_gemm_rows_i8")
+
+
+def beam_select(spec: BeamSpec, d_logits: int, logits_type: int, d_score: int, d_parent: int,
+                d_token: int, d_out_score: int, d_done: int = 0, d_out_done: int = 0,
+                logits_stride: int = 0, stream: int = 0) -> None:
+    """The best continuations of every sequence over its beams and the vocabulary."""
+    _check(gpu_lib().swamp_beam_select(spec, d_logits, logits_type, logits_stride, d_score, d_done,
+                                       d_parent, d_token, d_out_score, d_out_done, stream),
+           "swamp_beam_select")
+
+
+def pages_fork(pool: PagePool, tables: PageTables, d_parent: int, stream: int = 0) -> None:
+    """Every sequence becomes a fork of its parent: pages shared, counts kept."""
+    _check(gpu_lib().swamp_pages_fork(pool, tables, d_parent, stream), "swamp_pages_fork")
+
+
+def pages_extend(pool: PagePool, tables: PageTables, d_new: int, moves: PageMoves,
+                 stream: int = 0) -> None:
+    """Pages for d_new more tokens of each sequence (0: one token each); pages that it
+    would share while writing are listed in moves."""
+    _check(gpu_lib().swamp_pages_extend(pool, tables, d_new, moves, stream), "swamp_pages_extend")
+
+
+def pages_trim(pool: PagePool, tables: PageTables, d_keep: int = 0, stream: int = 0) -> None:
+    """Sequences keep their first d_keep tokens (0: none) and give back the other pages."""
+    _check(gpu_lib().swamp_pages_trim(pool, tables, d_keep, stream), "swamp_pages_trim")
+
+
+def pages_compact(pool: PagePool, tables: PageTables, moves: PageMoves, stream: int = 0) -> None:
+    """Pages in use move to the lowest places; moves lists what to copy."""
+    _check(gpu_lib().swamp_pages_compact(pool, tables, moves, stream), "swamp_pages_compact")
+
+
+def kv_copy(caches, moves: PageMoves, stream: int = 0) -> None:
+    """The listed pages of all caches (kv_caches) copied."""
+    _check(gpu_lib().swamp_kv_copy(caches, len(caches), moves, stream), "swamp_kv_copy")
 
 
 # ---------------------------------------------------------- host preparation

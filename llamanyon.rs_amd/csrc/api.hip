@@ -1,8 +1,8 @@
 // api.hip -- the C ABI of libswamp_gpu.so (declared in include/swamp_qmm.h).
 //
 // Validation and dispatch only; kernels live in dequant.hip, gemv.hip,
-// gemv_fused.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, rope.hip and attn.hip, and the rules
-// that choose between them by size in dispatch.hpp.  The error behaviour mirrors the
+// gemv_fused.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, rope.hip, attn.hip, rows_i8.hip,
+// beam.hip and pages.hip, and the rules that choose between them by size in dispatch.hpp.  The error behaviour mirrors the
 // reference: shape asserts of fused_gemv_q4k (fused_gemv_q4k.rs:66-70) and
 // the bail! of forward_linear (linear.rs:23-25) become negative return
 // codes, checked before anything is launched; the two legacy host-pointer
@@ -193,6 +193,65 @@ int check_rows(int64_t &stride, int n_tok, int n, int dim) {
   if (stride == 0) stride = int64_t(n) * dim;
   if (!within(n_tok, stride)) return SWAMP_EINVAL;
   return stride < int64_t(n) * dim ? SWAMP_ESHAPE : SWAMP_OK;
+}
+
+// A row stride in elements (0: dense), of n_rows rows of n.
+int check_stride(int64_t &stride, int n_rows, int n) { return check_rows(stride, n_rows, 1, n); }
+
+constexpr int kMaxBeams = 64, kMaxVocab = 1 << 20, kMaxCodeCols = 131071;
+constexpr int64_t kMaxCodeStride = int64_t(1) << 23, kMaxProducts = int64_t(1) << 38;
+
+int check_beams(const swamp_beam_spec *b, BeamCall &c) {
+  if (!b || b->n_seq < 0 || b->eos < -1) return SWAMP_EINVAL;
+  if (b->n_beam < 1 || b->n_beam > kMaxBeams || b->n_out < 1 || b->n_out > kMaxBeams ||
+      b->vocab < 1 || b->vocab > kMaxVocab || b->eos >= b->vocab || b->n_seq > kMaxSeqs)
+    return SWAMP_ESHAPE;
+  c.n_seq = b->n_seq;
+  c.n_beam = b->n_beam;
+  c.vocab = b->vocab;
+  c.n_out = b->n_out;
+  c.eos = b->eos;
+  return SWAMP_OK;
+}
+
+int check_pool(const swamp_page_pool *p, PagePool &out) {
+  if (!p || p->n_pages < 0) return SWAMP_EINVAL;
+  if (p->page_size < 1 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)) != 0)
+    return SWAMP_ESHAPE;
+  if (p->n_pages > 0 && (!p->d_refs || !p->d_used)) return SWAMP_EINVAL;
+  if (!aligned(p->d_refs, 4) || !aligned(p->d_used, 4)) return SWAMP_EINVAL;
+  out.n_pages = p->n_pages;
+  out.shift = __builtin_ctz(unsigned(p->page_size));
+  out.refs = p->d_refs;
+  out.used = p->d_used;
+  return SWAMP_OK;
+}
+
+int check_tables(const swamp_page_tables *t, PageTables &out) {
+  if (!t || t->n_seq < 0 || t->pages_stride < 0 || t->pages_stride > kMaxStride)
+    return SWAMP_EINVAL;
+  if (t->n_seq > kMaxPageSeqs) return SWAMP_ESHAPE;
+  if (t->n_seq > 0 && (!t->d_len || (t->pages_stride > 0 && !t->d_pages))) return SWAMP_EINVAL;
+  if (!aligned(t->d_len, 4) || !aligned(t->d_pages, 4) || !aligned(t->d_bad, 4))
+    return SWAMP_EINVAL;
+  out.n_seq = t->n_seq;
+  out.len = t->d_len;
+  out.pages = t->d_pages;
+  out.stride = t->pages_stride;
+  out.bad = t->d_bad;
+  return SWAMP_OK;
+}
+
+int check_moves(const swamp_page_moves *m, PageMoves &out) {
+  if (!m || m->cap < 0 || !m->d_count || (m->cap > 0 && (!m->d_src || !m->d_dst)))
+    return SWAMP_EINVAL;
+  if (!aligned(m->d_src, 4) || !aligned(m->d_dst, 4) || !aligned(m->d_count, 4))
+    return SWAMP_EINVAL;
+  out.cap = m->cap;
+  out.src = m->d_src;
+  out.dst = m->d_dst;
+  out.count = m->d_count;
+  return SWAMP_OK;
 }
 
 // The plan of an attention call; q and out are checked by the caller.
@@ -714,6 +773,164 @@ size_t swamp_attn_paged_workspace(const swamp_kv_pages *cache, const swamp_seq_b
   if (c.max_new == 0 || c.batch.n_seq == 0) return 0;
   if (ensure_device(nullptr) != SWAMP_OK) return 0;
   return swamp_attn_scratch_bytes(c);
+}
+
+int swamp_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_stride, int8_t *d_q,
+                        int64_t q_stride, float *d_scale, int n_rows, int n_cols, void *stream) {
+  if (!is_float(x_type)) return SWAMP_EDTYPE;
+  if (n_rows < 0 || n_cols < 0) return SWAMP_EINVAL;
+  if (int rc = check_stride(x_stride, n_rows, n_cols)) return rc;
+  if (int rc = check_stride(q_stride, n_rows, n_cols)) return rc;
+  if (n_rows == 0) return SWAMP_OK;
+  if (!d_scale || !aligned(d_scale, 4)) return SWAMP_EINVAL;
+  if (n_cols > 0 && (!d_x || !d_q || !aligned(d_x, type_size(x_type)))) return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_quantize_rows(d_x, x_type, x_stride, d_q, q_stride, d_scale, n_rows, n_cols,
+                                    static_cast<hipStream_t>(stream));
+}
+
+int swamp_gemm_rows_i8(const int8_t *d_x, int64_t x_stride, const float *d_x_scale,
+                       const int8_t *d_w, int64_t w_stride, const float *d_w_scale, void *d_y,
+                       uint32_t y_type, int64_t y_stride, int m, int n_rows, int n_cols,
+                       int accumulate, void *stream) {
+  if (!is_float(y_type)) return SWAMP_EDTYPE;
+  if (m < 0 || n_rows < 0 || n_cols < 0) return SWAMP_EINVAL;
+  if (n_cols > kMaxCodeCols) return SWAMP_ESHAPE;
+  if (int rc = check_stride(x_stride, m, n_cols)) return rc;
+  if (int rc = check_stride(w_stride, n_rows, n_cols)) return rc;
+  if (int rc = check_stride(y_stride, m, n_rows)) return rc;
+  if (x_stride % 16 != 0 || w_stride % 16 != 0 || x_stride >= kMaxCodeStride ||
+      w_stride >= kMaxCodeStride || int64_t(m) * n_rows >= kMaxProducts)
+    return SWAMP_ESHAPE;
+  if (m == 0 || n_rows == 0) return SWAMP_OK;
+  if (!d_x_scale || !d_w_scale || !d_y || !aligned(d_x_scale, 4) || !aligned(d_w_scale, 4) ||
+      !aligned(d_y, type_size(y_type)))
+    return SWAMP_EINVAL;
+  if (n_cols > 0 && (!d_x || !d_w)) return SWAMP_EINVAL;
+  if (!aligned(d_x, 16) || !aligned(d_w, 16)) return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  const GemmI8Call c{d_x,      d_w,      d_x_scale, d_w_scale, d_y,    y_type,
+                     x_stride, w_stride, y_stride,  m,         n_rows, n_cols, accumulate ? 1 : 0};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Scratch sc = stream_scratch(s, swamp_gemm_rows_i8_scratch_bytes(m, n_rows, n_cols));
+  return swamp_launch_gemm_rows_i8(c, sc, s);
+}
+
+size_t swamp_gemm_rows_i8_workspace(int m, int n_rows, int n_cols) {
+  if (m <= 0 || n_rows <= 0 || n_cols <= 0 || n_cols > kMaxCodeCols ||
+      int64_t(m) * n_rows >= kMaxProducts)
+    return 0;
+  if (ensure_device(nullptr) != SWAMP_OK) return 0;
+  return swamp_gemm_rows_i8_scratch_bytes(m, n_rows, n_cols);
+}
+
+int swamp_beam_select(const swamp_beam_spec *spec, const void *d_logits, uint32_t type,
+                      int64_t stride, const float *d_score, const int32_t *d_done,
+                      int32_t *d_parent, int32_t *d_token, float *d_out_score, int32_t *d_out_done,
+                      void *stream) {
+  BeamCall c;
+  if (!is_float(type)) return SWAMP_EDTYPE;
+  if (int rc = check_beams(spec, c)) return rc;
+  if (d_done && c.eos < 0) return SWAMP_EINVAL;
+  if (int rc = check_stride(stride, c.n_seq * c.n_beam, c.vocab)) return rc;
+  if (c.n_seq == 0) return SWAMP_OK;
+  if (!d_logits || !d_score || !d_parent || !d_token || !d_out_score) return SWAMP_EINVAL;
+  if (!aligned(d_logits, type_size(type)) || !aligned(d_score, 4) || !aligned(d_done, 4) ||
+      !aligned(d_parent, 4) || !aligned(d_token, 4) || !aligned(d_out_score, 4) ||
+      !aligned(d_out_done, 4))
+    return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  c.type = type;
+  c.logits = d_logits;
+  c.stride = stride;
+  c.score = d_score;
+  c.done = d_done;
+  c.parent = d_parent;
+  c.token = d_token;
+  c.out_score = d_out_score;
+  c.out_done = d_out_done;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Scratch sc = stream_scratch(s, swamp_beam_scratch_bytes(c));
+  return swamp_launch_beam_select(c, sc, s);
+}
+
+size_t swamp_beam_select_workspace(const swamp_beam_spec *spec) {
+  BeamCall c;
+  if (check_beams(spec, c) != SWAMP_OK || c.n_seq == 0) return 0;
+  if (ensure_device(nullptr) != SWAMP_OK) return 0;
+  return swamp_beam_scratch_bytes(c);
+}
+
+int swamp_pages_fork(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                     const int32_t *d_parent, void *stream) {
+  PagePool p;
+  PageTables t;
+  if (int rc = check_pool(pool, p)) return rc;
+  if (int rc = check_tables(tables, t)) return rc;
+  if (t.n_seq == 0) return SWAMP_OK;
+  if (!d_parent || !aligned(d_parent, 4)) return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_pages_fork(p, t, d_parent, static_cast<hipStream_t>(stream));
+}
+
+int swamp_pages_extend(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                       const int32_t *d_new, const swamp_page_moves *moves, void *stream) {
+  PagePool p;
+  PageTables t;
+  PageMoves m;
+  if (int rc = check_pool(pool, p)) return rc;
+  if (int rc = check_tables(tables, t)) return rc;
+  if (int rc = check_moves(moves, m)) return rc;
+  if (m.cap < t.n_seq) return SWAMP_ESHAPE;
+  if (!aligned(d_new, 4)) return SWAMP_EINVAL;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_pages_extend(p, t, d_new, m, static_cast<hipStream_t>(stream));
+}
+
+int swamp_pages_trim(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                     const int32_t *d_keep, void *stream) {
+  PagePool p;
+  PageTables t;
+  if (int rc = check_pool(pool, p)) return rc;
+  if (int rc = check_tables(tables, t)) return rc;
+  if (!aligned(d_keep, 4)) return SWAMP_EINVAL;
+  if (t.n_seq == 0) return SWAMP_OK;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_pages_trim(p, t, d_keep, static_cast<hipStream_t>(stream));
+}
+
+int swamp_pages_compact(const swamp_page_pool *pool, const swamp_page_tables *tables,
+                        const swamp_page_moves *moves, void *stream) {
+  PagePool p;
+  PageTables t;
+  PageMoves m;
+  if (int rc = check_pool(pool, p)) return rc;
+  if (int rc = check_tables(tables, t)) return rc;
+  if (int rc = check_moves(moves, m)) return rc;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_pages_compact(p, t, m, static_cast<hipStream_t>(stream));
+}
+
+int swamp_kv_copy(const swamp_kv_pages *caches, int n_caches, const swamp_page_moves *moves,
+                  void *stream) {
+  PageMoves m;
+  if (int rc = check_moves(moves, m)) return rc;
+  if (n_caches < 0 || (n_caches > 0 && !caches)) return SWAMP_EINVAL;
+  PagedCache first, c;
+  for (int i = 0; i < n_caches; i++) {
+    if (int rc = check_cache(&caches[i], c)) return rc;
+    if (c.n_pages > 0 && !cache_ok(c)) return SWAMP_EINVAL;
+    if (i == 0) first = c;
+    if (caches[i].dtype != caches[0].dtype || c.n_pages != first.n_pages ||
+        c.page_shift != first.page_shift || c.n_kv != first.n_kv || c.dim != first.dim ||
+        c.page_stride != first.page_stride || c.head_stride != first.head_stride ||
+        c.slot_stride != first.slot_stride)
+      return SWAMP_ESHAPE;
+  }
+  if (n_caches == 0 || m.cap == 0 || first.n_pages == 0) return SWAMP_OK;
+  if (((int64_t(first.n_kv) << first.page_shift) * first.dim) >> 33) return SWAMP_ESHAPE;
+  if (int rc = ensure_device(nullptr)) return rc;
+  return swamp_launch_kv_copy(first, caches, n_caches, m, static_cast<hipStream_t>(stream));
 }
 
 void swamp_fused_gemv_q4k(const uint8_t *w_raw, const float *x, float *out, int n_rows,

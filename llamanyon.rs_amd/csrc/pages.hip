@@ -1,0 +1,457 @@
+// pages.hip -- who holds the pages of a paged cache, and copies of pages: forking
+// (swamp_pages_fork), growing (swamp_pages_extend), cutting (swamp_pages_trim),
+// compacting (swamp_pages_compact) and swamp_kv_copy.
+//
+// A page's count is the number of page tables that name it, so a call's results are
+// sums and lowest places, which no order of atomics changes.
+#include "swamp_common.hpp"
+
+#include <algorithm>
+
+namespace {
+
+using swamp::held_cols;
+using swamp::page_ok;
+using swamp::PageMoves;
+using swamp::PagePool;
+using swamp::PageTables;
+
+constexpr int kSeqs = swamp::kMaxPageSeqs;
+constexpr int kTile = 16;     // table columns that a workgroup turns at a time
+constexpr int kBlock = 1024;  // threads of the one workgroup that ranks pages
+
+// ---- fork -----------------------------------------------------------------
+// T'[s] = T[parent s], in place: a workgroup takes 16 columns of all rows into LDS.
+// A page gains (children of its row) - 1 per row that names it.  Rows that share
+// pages lie together and name them in the same column: a thread runs down a column
+// and adds a run of equal pages' gains at once, and where a prompt's beams only
+// change places the sum is 0 and nothing is written.
+__global__ void __launch_bounds__(256) fork_tables_kernel(PagePool pool, PageTables t,
+                                                          const int32_t *__restrict__ d_parent) {
+  extern __shared__ int smem[];
+  const int n = t.n_seq, tid = int(threadIdx.x);
+  int *tile = smem, *gain = tile + n * kTile, *cols = gain + n, *parent = cols + n;
+  __shared__ int most;
+  if (tid == 0) most = 0;
+  for (int s = tid; s < n; s += 256) gain[s] = -1;
+  __syncthreads();
+  int top = 0;
+  for (int s = tid; s < n; s += 256) {
+    const int p = d_parent[s];
+    parent[s] = uint32_t(p) < uint32_t(n) ? p : -1;
+    cols[s] = int(held_cols(t.len[s], pool.shift, t.stride));
+    top = max(top, cols[s]);
+    if (uint32_t(p) < uint32_t(n)) atomicAdd(&gain[p], 1);
+  }
+  atomicMax(&most, top);
+  __syncthreads();
+  const int c = tid % kTile;
+  const int rows = (n + 15) / 16, r0 = min(tid / kTile * rows, n), r1 = min(r0 + rows, n);
+  for (int64_t c0 = int64_t(blockIdx.x) * kTile; c0 < most; c0 += int64_t(gridDim.x) * kTile) {
+    for (int i = tid; i < n * kTile; i += 256) {
+      const int s = i / kTile;
+      tile[i] = c0 + c < cols[s] ? t.pages[s * t.stride + c0 + c] : -1;
+    }
+    __syncthreads();
+    int id = -1, sum = 0;
+    for (int s = r0; s < r1; s++) {
+      const int e = tile[s * kTile + c];
+      if (e != id) {
+        if (sum != 0 && page_ok(id, pool.n_pages)) atomicAdd(&pool.refs[id], sum);
+        id = e;
+        sum = 0;
+      }
+      sum += gain[s];
+    }
+    if (sum != 0 && page_ok(id, pool.n_pages)) atomicAdd(&pool.refs[id], sum);
+    for (int i = tid; i < n * kTile; i += 256) {
+      const int s = i / kTile, p = parent[s];
+      if (p != s && p >= 0 && c0 + c < cols[p])
+        t.pages[s * t.stride + c0 + c] = tile[p * kTile + c];
+    }
+    __syncthreads();
+  }
+}
+
+// Every table and count is final: which pages are in use, and the lengths.
+__global__ void __launch_bounds__(256) fork_finish_kernel(PagePool pool, PageTables t,
+                                                          const int32_t *__restrict__ d_parent) {
+  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const uint64_t used = __ballot(id < pool.n_pages && pool.refs[id] > 0);
+  if (threadIdx.x % 32 == 0 && id < pool.n_pages)
+    pool.used[id / 32] = uint32_t(threadIdx.x % 64 ? used >> 32 : used);
+  if (blockIdx.x != 0) return;
+  __shared__ int lens[kSeqs];
+  for (int s = int(threadIdx.x); s < t.n_seq; s += 256) lens[s] = t.len[s];
+  __syncthreads();
+  for (int s = int(threadIdx.x); s < t.n_seq; s += 256) {
+    const int p = d_parent[s];
+    t.len[s] = uint32_t(p) < uint32_t(t.n_seq) ? lens[p] : 0;
+  }
+}
+
+// ---- one workgroup's sums -------------------------------------------------
+// The sum of x over the threads before this one, and over all; `part` holds a value
+// for each wave and is free again after the next barrier of the caller.
+template <typename T>
+__device__ __forceinline__ T scan(T x, T *part, T &total) {
+  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
+  T incl = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const T below = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += below;
+  }
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kBlock / 64; w++) {
+    const T p = part[w];
+    if (w < wave) before += p;
+    total += p;
+  }
+  __syncthreads();
+  return before + incl - x;
+}
+
+// Word w of the pages in use; pages past the last count as used where `fill`.
+__device__ __forceinline__ uint32_t used_word(const PagePool &pool, int64_t w, bool fill) {
+  const int64_t first = 32 * w;
+  if (first >= pool.n_pages) return fill ? ~0u : 0u;
+  const int64_t n = pool.n_pages - first;
+  const uint32_t there = n >= 32 ? ~0u : (1u << n) - 1, x = pool.used[w];
+  return fill ? x | ~there : x & there;
+}
+
+constexpr int kWords = 4;  // of a thread in a round: 131072 pages
+
+// ---- extend ---------------------------------------------------------------
+// One workgroup: what every sequence needs (two a thread), where its pages begin in
+// the row of all pages handed out, then one pass over the free pages in rising
+// order, each finding its owner by bisection.  Of the h sequences that would write
+// one shared page in turn, the j-th finds refs - j tables naming it.
+__global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTables t,
+                                                        const int32_t *__restrict__ d_new,
+                                                        PageMoves moves) {
+  __shared__ __attribute__((aligned(16))) int tail[kSeqs];  // the shared page it would write, or -1
+  __shared__ int copy[kSeqs];     // its place in the list, or -1
+  __shared__ int first[kSeqs];    // its first new column
+  __shared__ int64_t off[kSeqs + 1];
+  __shared__ int64_t part[kBlock / 64];
+  __shared__ int listed;
+  const int n = t.n_seq, tid = int(threadIdx.x);
+  const int mask = (1 << pool.shift) - 1;
+  bool bad = false;
+  int refs[2], grown[2], fresh[2];
+  if (tid == 0) listed = 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int s = 2 * tid + i;
+    tail[s] = -1;
+    refs[i] = grown[i] = fresh[i] = 0;
+    if (s >= n) continue;
+    const int len = max(t.len[s], 0);
+    const int want = d_new ? max(d_new[s], 0) : 1, more = min(want, INT32_MAX - len);
+    const int64_t last = len >> pool.shift;
+    const int64_t c0 = (int64_t(len) + mask) >> pool.shift;
+    const int64_t c1 = (int64_t(len) + more + mask) >> pool.shift;
+    grown[i] = len + more;
+    first[s] = int(min(c0, t.stride));
+    fresh[i] = int(min(c1, t.stride) - min(c0, t.stride));
+    bad |= more > 0 && c1 > t.stride;
+    bad |= want > more;
+    if (more > 0 && (len & mask) != 0 && last < t.stride) {
+      const int id = t.pages[s * t.stride + last];
+      if (page_ok(id, pool.n_pages)) {
+        refs[i] = pool.refs[id];
+        if (refs[i] > 1) tail[s] = id;
+      } else {
+        bad = true;
+      }
+    }
+  }
+  __syncthreads();
+  int copies[2];
+  int64_t need = 0, total;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int s = 2 * tid + i;
+    copies[i] = 0;
+    if (tail[s] >= 0) {
+      int before = 0;
+      for (int o = 0; o < s; o++) before += tail[o] == tail[s] ? 1 : 0;
+      copies[i] = before < refs[i] - 1 ? 1 : 0;
+    }
+    need += copies[i] + fresh[i];
+  }
+  const int64_t at = scan<int64_t>(need, part, total);
+  int64_t n_copies;
+  const int64_t place = scan<int64_t>(copies[0] + copies[1], part, n_copies);
+  off[2 * tid] = at;
+  off[2 * tid + 1] = at + copies[0] + fresh[0];
+  copy[2 * tid] = copies[0] ? int(place) : -1;
+  copy[2 * tid + 1] = copies[1] ? int(place) + copies[0] : -1;
+  if (tid == 0) off[kSeqs] = total;
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    if (copies[i]) atomicSub(&pool.refs[tail[2 * tid + i]], 1);
+  __syncthreads();
+
+  int64_t base = 0;  // free pages before this round's
+  const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
+  for (int64_t w0 = 0; base < total && w0 < words; w0 += kBlock * kWords) {
+    uint32_t free[kWords];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      free[i] = ~used_word(pool, w0 + tid * kWords + i, true);
+      mine += __builtin_popcount(free[i]);
+    }
+    int64_t found;
+    int64_t rank = base + scan<int64_t>(mine, part, found);
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      const int64_t w = w0 + tid * kWords + i;
+      uint32_t left = free[i];
+      while (left != 0 && rank < total) {
+        const int bit = __builtin_ctz(left), id = int(32 * w) + bit;
+        left &= left - 1;
+        int lo = 0, hi = kSeqs;  // off[lo] <= rank < off[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (off[mid] <= rank) lo = mid;
+          else hi = mid;
+        }
+        const int which = int(rank - off[lo]);
+        int32_t *row = t.pages + lo * t.stride;
+        const int c = copy[lo];
+        if (c >= 0 && which == 0) {
+          row[first[lo] - 1] = id;
+          moves.src[c] = tail[lo];
+          moves.dst[c] = id;
+          atomicAdd(&listed, 1);
+        } else {
+          row[first[lo] + which - (c >= 0 ? 1 : 0)] = id;
+        }
+        pool.refs[id] = 1;
+        rank++;
+      }
+      if (left != free[i]) pool.used[w] = used_word(pool, w, false) | (free[i] & ~left);
+    }
+    base += found;
+  }
+  // what no page was left for
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int s = 2 * tid + i;
+    if (s >= n) continue;
+    const int64_t all = copies[i] + fresh[i], got = min(max(base - off[s], int64_t(0)), all);
+    bad |= got < all;
+    for (int64_t k = got; k < all; k++)
+      t.pages[s * t.stride + first[s] + k - copies[i]] = -1;
+    t.len[s] = grown[i];
+  }
+  if (bad && t.bad) *t.bad = 1;
+  __syncthreads();
+  if (tid == 0) *moves.count = listed;
+}
+
+// ---- trim -----------------------------------------------------------------
+__global__ void __launch_bounds__(256) trim_kernel(PagePool pool, PageTables t,
+                                                   const int32_t *__restrict__ d_keep) {
+  const int s = int(blockIdx.x);
+  const int len = max(t.len[s], 0), keep = min(len, d_keep ? max(d_keep[s], 0) : 0);
+  const int64_t c1 = held_cols(len, pool.shift, t.stride);
+  for (int64_t c = held_cols(keep, pool.shift, t.stride) + threadIdx.x; c < c1; c += 256) {
+    const int id = t.pages[s * t.stride + c];
+    if (page_ok(id, pool.n_pages) && atomicSub(&pool.refs[id], 1) == 1)
+      atomicAnd(&pool.used[id / 32], ~(1u << (id % 32)));
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) t.len[s] = keep;
+}
+
+// ---- compact --------------------------------------------------------------
+__global__ void __launch_bounds__(kBlock) compact_list_kernel(PagePool pool, PageMoves moves) {
+  __shared__ int64_t part[kBlock / 64];
+  const int tid = int(threadIdx.x);
+  const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
+  int64_t n_used = 0, sum;
+  for (int64_t w = tid; w < words; w += kBlock) n_used += __builtin_popcount(used_word(pool, w, false));
+  scan<int64_t>(n_used, part, sum);
+  n_used = sum;
+  int64_t holes = 0, high = 0;  // before this round's words
+  for (int64_t w0 = 0; w0 < words; w0 += kBlock * kWords) {
+    uint32_t hole[kWords], up[kWords];
+    int64_t mine = 0;  // holes, and 2^32 times the pages above
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      const int64_t w = w0 + tid * kWords + i, below = n_used - 32 * w;
+      const uint32_t low = below >= 32 ? ~0u : below <= 0 ? 0u : (1u << below) - 1;
+      hole[i] = ~used_word(pool, w, true) & low;
+      up[i] = used_word(pool, w, false) & ~low;
+      mine += __builtin_popcount(hole[i]) + (int64_t(__builtin_popcount(up[i])) << 32);
+    }
+    const int64_t before = scan<int64_t>(mine, part, sum);
+    int64_t h = holes + (before & 0xFFFFFFFF), u = high + (before >> 32);
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      const int first = int(32 * (w0 + tid * kWords + i));
+      for (uint32_t x = hole[i]; x != 0 && h < moves.cap; x &= x - 1)
+        moves.dst[h++] = first + __builtin_ctz(x);
+      for (uint32_t x = up[i]; x != 0 && u < moves.cap; x &= x - 1)
+        moves.src[u++] = first + __builtin_ctz(x);
+    }
+    holes += sum & 0xFFFFFFFF;
+    high += sum >> 32;
+  }
+  if (tid == 0) *moves.count = int(min(high, int64_t(moves.cap)));
+}
+
+// Counts of the pages that move (block column 0), and a row's entries: where the
+// list, which rises, holds an entry as a source it becomes the place it moves to.
+__global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTables t,
+                                                           PageMoves moves) {
+  const int n = *moves.count;
+  if (n == 0) return;
+  const int from = moves.src[0], to = moves.src[n - 1];
+  const int64_t threads = int64_t(gridDim.x) * gridDim.y * 256;
+  const int64_t me = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+  for (int64_t i = me; i < n; i += threads) {
+    const int a = moves.src[i], b = moves.dst[i];
+    pool.refs[b] = pool.refs[a];
+    pool.refs[a] = 0;
+    atomicAnd(&pool.used[a / 32], ~(1u << (a % 32)));
+    atomicOr(&pool.used[b / 32], 1u << (b % 32));
+  }
+  const int s = int(blockIdx.x);
+  if (s >= t.n_seq) return;
+  const int64_t cols = held_cols(t.len[s], pool.shift, t.stride);
+  for (int64_t c = int64_t(blockIdx.y) * 256 + threadIdx.x; c < cols; c += int64_t(gridDim.y) * 256) {
+    const int id = t.pages[s * t.stride + c];
+    if (id < from || id > to) continue;
+    int lo = 0, hi = n;  // src[lo] <= id < src[hi]
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (moves.src[mid] <= id) lo = mid;
+      else hi = mid;
+    }
+    if (moves.src[lo] == id) t.pages[s * t.stride + c] = moves.dst[lo];
+  }
+}
+
+// ---- copy -----------------------------------------------------------------
+// HBM's: a page is read and written once, 4 KB a wave at a time.  The list's length
+// is on the device, so a fixed grid runs over (pair, segment of a page).
+constexpr int kCaches = 64;  // of a launch
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+
+struct CopyWork {
+  uint16_t *base[2 * kCaches];  // keys and values of each cache
+  PageMoves moves;
+  int64_t page_stride, head_stride, slot_stride;  // elements
+  int n_pages, shift, row_chunks, chunks, segs;   // 16-byte chunks of a row and of a page
+  int flat;                                       // a page's rows lie without gaps
+};
+
+__global__ void __launch_bounds__(256) copy_kernel(CopyWork w) {
+  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
+  uint16_t *base = w.base[blockIdx.y];
+  const int n = min(*w.moves.count, w.moves.cap);
+  const int64_t items = int64_t(n) * w.segs;
+  for (int64_t item = int64_t(blockIdx.x) * 4 + wave; item < items; item += int64_t(gridDim.x) * 4) {
+    const int pair = int(item / w.segs), seg = int(item - int64_t(pair) * w.segs);
+    const int a = w.moves.src[pair], b = w.moves.dst[pair];
+    if (!page_ok(a, w.n_pages) || !page_ok(b, w.n_pages)) continue;
+    const uint16_t *src = base + a * w.page_stride;
+    uint16_t *dst = base + b * w.page_stride;
+    int64_t at[4];
+    u32x4v v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int c = seg * 256 + 64 * i + lane;
+      at[i] = int64_t(c) * 8;
+      if (!w.flat) {
+        const int row = c / w.row_chunks;
+        at[i] = (row >> w.shift) * w.head_stride + (row & ((1 << w.shift) - 1)) * w.slot_stride +
+                (c - row * w.row_chunks) * 8;
+      }
+      if (c < w.chunks) v[i] = *reinterpret_cast<const u32x4v *>(src + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (seg * 256 + 64 * i + lane < w.chunks) *reinterpret_cast<u32x4v *>(dst + at[i]) = v[i];
+  }
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH; }
+
+}  // namespace
+
+int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int32_t *d_parent,
+                            hipStream_t s) {
+  const size_t lds = size_t(t.n_seq) * (kTile + 3) * 4;
+  if (lds > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void *>(&fork_tables_kernel),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)) != hipSuccess)
+    return SWAMP_ELAUNCH;
+  const int64_t tiles = std::max<int64_t>(1, (t.stride + kTile - 1) / kTile);
+  fork_tables_kernel<<<unsigned(std::min<int64_t>(tiles, 1024)), 256, lds, s>>>(pool, t, d_parent);
+  const unsigned blocks = unsigned(std::max<int64_t>(1, (int64_t(pool.n_pages) + 255) / 256));
+  fork_finish_kernel<<<blocks, 256, 0, s>>>(pool, t, d_parent);
+  return launched();
+}
+
+int swamp_launch_pages_extend(const PagePool &pool, const PageTables &t, const int32_t *d_new,
+                              const PageMoves &moves, hipStream_t s) {
+  extend_kernel<<<1, kBlock, 0, s>>>(pool, t, d_new, moves);
+  return launched();
+}
+
+int swamp_launch_pages_trim(const PagePool &pool, const PageTables &t, const int32_t *d_keep,
+                            hipStream_t s) {
+  trim_kernel<<<unsigned(t.n_seq), 256, 0, s>>>(pool, t, d_keep);
+  return launched();
+}
+
+int swamp_launch_pages_compact(const PagePool &pool, const PageTables &t, const PageMoves &moves,
+                               hipStream_t s) {
+  compact_list_kernel<<<1, kBlock, 0, s>>>(pool, moves);
+  const dim3 grid(unsigned(std::max(t.n_seq, 64)),
+                  unsigned(std::max<int64_t>(1, std::min<int64_t>(t.stride / 256, 16))));
+  compact_move_kernel<<<grid, 256, 0, s>>>(pool, t, moves);
+  return launched();
+}
+
+int swamp_launch_kv_copy(const swamp::PagedCache &c, const swamp_kv_pages *caches, int n_caches,
+                         const PageMoves &moves, hipStream_t s) {
+  CopyWork w;
+  w.moves = moves;
+  w.page_stride = c.page_stride;
+  w.head_stride = c.head_stride;
+  w.slot_stride = c.slot_stride;
+  w.n_pages = c.n_pages;
+  w.shift = c.page_shift;
+  w.row_chunks = c.dim / 8;
+  w.chunks = (c.n_kv << c.page_shift) * w.row_chunks;
+  w.segs = (w.chunks + 255) / 256;
+  const int64_t slots = int64_t(1) << c.page_shift;
+  w.flat = (c.slot_stride == c.dim && (c.n_kv == 1 || c.head_stride == slots * c.dim)) ||
+           ((c.n_kv == 1 || c.head_stride == c.dim) &&
+            (slots == 1 || c.slot_stride == int64_t(c.n_kv) * c.dim));
+  for (int i0 = 0; i0 < n_caches; i0 += kCaches) {
+    const int n = std::min(n_caches - i0, kCaches);
+    for (int i = 0; i < n; i++) {
+      w.base[2 * i] = static_cast<uint16_t *>(caches[i0 + i].d_k);
+      w.base[2 * i + 1] = static_cast<uint16_t *>(caches[i0 + i].d_v);
+    }
+    // (waves for every segment of the list's most, 16 workgroups a CU in all)
+    const int64_t most = (int64_t(moves.cap) * w.segs + 3) / 4;
+    const int64_t room = std::max(1, 16 * swamp::device_info().num_cus / (2 * n));
+    const dim3 grid(unsigned(std::max<int64_t>(1, std::min(most, room))), unsigned(2 * n));
+    copy_kernel<<<grid, 256, 0, s>>>(w);
+  }
+  return launched();
+}

@@ -38,6 +38,47 @@ struct SeqBatch {
   int n_seq, n_tok;
 };
 
+// swamp_page_pool, swamp_page_tables and swamp_page_moves, checked.
+constexpr int kMaxPageSeqs = 2048;
+struct PagePool {
+  int n_pages, shift;
+  int32_t *refs;
+  uint32_t *used;
+};
+struct PageTables {
+  int n_seq;
+  int32_t *len, *pages;
+  int64_t stride;
+  int32_t *bad;
+};
+struct PageMoves {
+  int cap;
+  int32_t *src, *dst, *count;
+};
+
+// One swamp_beam_select call, checked.
+struct BeamCall {
+  int n_seq, n_beam, vocab, n_out, eos;
+  uint32_t type;
+  const void *logits;
+  int64_t stride;
+  const float *score;
+  const int32_t *done;
+  int32_t *parent, *token;
+  float *out_score;
+  int32_t *out_done;
+};
+
+// One swamp_gemm_rows_i8 call, checked.
+struct GemmI8Call {
+  const int8_t *x, *w;
+  const float *x_scale, *w_scale;
+  void *y;
+  uint32_t y_type;
+  int64_t x_stride, w_stride, y_stride;
+  int m, n, k, accumulate;
+};
+
 // One swamp_attn_paged call, checked.
 struct AttnCall {
   PagedCache cache;
@@ -82,6 +123,11 @@ SWAMP_HD Span seen_by(int pos, int window) {
 SWAMP_HD int64_t page_col(int pos, int shift) { return int64_t(pos >> shift); }
 SWAMP_HD bool page_col_ok(int pos, int64_t col, int64_t pages_stride) {
   return pos >= 0 && col < pages_stride;
+}
+// Table entries that a sequence of len tokens holds.
+SWAMP_HD int64_t held_cols(int len, int shift, int64_t stride) {
+  const int64_t n = len <= 0 ? 0 : (int64_t(len) + (int64_t(1) << shift) - 1) >> shift;
+  return n < stride ? n : stride;
 }
 // Element offset of slot 0, dim 0 of `head` at position pos on page id.
 SWAMP_HD bool page_ok(int32_t id, int n_pages) { return uint32_t(id) < uint32_t(n_pages); }

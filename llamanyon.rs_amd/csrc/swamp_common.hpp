@@ -147,7 +147,7 @@ inline Scratch stream_scratch(hipStream_t s, size_t bytes) {
 
 // Internal launchers (defined in dequant.hip, gemv.hip, gemv_fused.hip,
 // gemv_tokens.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, producers.hip,
-// rope.hip, attn.hip).  They assume the arguments have been validated by api.cpp.
+// rope.hip, attn.hip, rows_i8.hip, beam.hip, pages.hip).  They assume the arguments have been validated by api.cpp.
 int swamp_launch_dequant(uint32_t dtype, const void *d_raw, float *d_dst,
                          size_t n, hipStream_t s);
 int swamp_launch_dequant_bf16(uint32_t dtype, const void *d_raw, void *d_dst, size_t n,
@@ -227,3 +227,21 @@ int swamp_launch_kv_append(const swamp::PagedCache &cache, const swamp::SeqBatch
                            hipStream_t s);
 size_t swamp_attn_scratch_bytes(const swamp::AttnCall &c);
 int swamp_launch_attn_paged(const swamp::AttnCall &c, swamp::Scratch &sc, hipStream_t s);
+int swamp_launch_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_stride, int8_t *d_q,
+                               int64_t q_stride, float *d_scale, int n_rows, int n_cols,
+                               hipStream_t s);
+size_t swamp_gemm_rows_i8_scratch_bytes(int m, int n_rows, int n_cols);
+int swamp_launch_gemm_rows_i8(const swamp::GemmI8Call &c, swamp::Scratch &sc, hipStream_t s);
+size_t swamp_beam_scratch_bytes(const swamp::BeamCall &c);
+int swamp_launch_beam_select(const swamp::BeamCall &c, swamp::Scratch &sc, hipStream_t s);
+int swamp_launch_pages_fork(const swamp::PagePool &pool, const swamp::PageTables &t,
+                            const int32_t *d_parent, hipStream_t s);
+int swamp_launch_pages_extend(const swamp::PagePool &pool, const swamp::PageTables &t,
+                              const int32_t *d_new, const swamp::PageMoves &moves, hipStream_t s);
+int swamp_launch_pages_trim(const swamp::PagePool &pool, const swamp::PageTables &t,
+                            const int32_t *d_keep, hipStream_t s);
+int swamp_launch_pages_compact(const swamp::PagePool &pool, const swamp::PageTables &t,
+                               const swamp::PageMoves &moves, hipStream_t s);
+// caches: n_caches of the geometry c
+int swamp_launch_kv_copy(const swamp::PagedCache &c, const swamp_kv_pages *caches, int n_caches,
+                         const swamp::PageMoves &moves, hipStream_t s);
