@@ -8,15 +8,17 @@
 //
 // Sums and totals are 64-bit: beams whose scores agree to 32 bits keep their order, and
 // equal ones the order of their tokens.  The exponential is 2^n 2^f, n = rint(x log2 e),
-// 2^f by its Taylor polynomial of degree 11 (|f| <= 1/2: off by 6e-15 of it): 18
-// operations of 64 bits an element, which the vector units issue at the rate of 32-bit
-// ones.
+// 2^f a polynomial of degree 9 through the Chebyshev nodes of |f| <= 1/2 (off by 2e-14 of
+// it): 16 operations of 64 bits an element, which the vector units issue at the rate of
+// 32-bit ones.
 //
-// Largest tokens without a sort: a wave's lanes each have a largest value, and the
-// n_out-th largest of those 64, found bit by bit with ballots, has n_out values at or
-// above it in the chunk.  What reaches the largest of the four waves' bounds, a few
-// times n_out tokens, is collected in LDS and ranked by counting.  Where too many do
-// (equal logits) the exact bound is found bit by bit over the whole chunk.
+// Largest tokens without a sort: a wave's lanes each have a largest value (of each four
+// of theirs, where n_out is large), and the n_out-th largest of those, found bit by bit
+// with ballots, has n_out values at or above it in the chunk.  What reaches the largest
+// of the four waves' bounds, a few times n_out tokens, is collected in LDS and ranked by
+// counting.  Where too many do (equal logits) the exact bound is found bit by bit over
+// the whole chunk.  The lists of a sequence are cut alike: n_out / r lists whose r-th
+// token reaches a bound have n_out tokens that do.
 #include "swamp_common.hpp"
 
 #include <type_traits>
@@ -31,6 +33,7 @@ constexpr int kChunk = kThreads * kEach;   // of a workgroup
 constexpr int kList = 1024;                // tokens that it ranks
 constexpr int kJoin = 2048;                // tokens that a sequence's workgroup ranks
 constexpr int kBeams = 64;
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
 
 struct Entry {
   float x;
@@ -44,7 +47,8 @@ struct Part {  // of a chunk
 struct Work {
   BeamCall c;
   int chunks;    // of a row
-  Entry *list;   // [row][chunk][n_out]
+  int pad;       // places of a list: n_out, a multiple of 4
+  Entry *list;   // [row][chunk][pad]
   Part *part;    // [row][chunk]
 };
 
@@ -58,26 +62,21 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kNone = 0x007FFFFFu;  // key of -infinity
 
-__device__ __forceinline__ double exp64(double x) {
-  x = x < -750.0 ? -750.0 : x;  // (0 from there on; NaN passes)
-  const double t = x * 1.4426950408889634074, n = __builtin_rint(t), f = t - n;
-  constexpr double c[12] = {1.0,
-                            6.931471805599453094e-1,
-                            2.402265069591007123e-1,
-                            5.550410866482157995e-2,
-                            9.618129107628477232e-3,
-                            1.333355814642844342e-3,
-                            1.540353039338160996e-4,
-                            1.525273380405984028e-5,
-                            1.321548679014430948e-6,
-                            1.017808600923969973e-7,
-                            7.054911620801123329e-9,
-                            4.445538271870811498e-10};
-  double p = c[11];
+// 2^t for t of any size; NaN passes, and t far below 0 gives 0.
+__device__ __forceinline__ double exp2_64(double t) {
+  const double n = __builtin_rint(t), f = t - n;
+  constexpr double c[10] = {1.000000000000013545e+00, 6.931471805599446201e-01,
+                            2.402265069563986055e-01, 5.550410866470367743e-02,
+                            9.618129194074795732e-03, 1.333355819593412062e-03,
+                            1.540343361871355534e-04, 1.525267453819431725e-05,
+                            1.325968083523608916e-06, 1.020575712504153700e-07};
+  double p = c[9];
 #pragma unroll
-  for (int i = 10; i >= 0; i--) p = __builtin_fma(p, f, c[i]);
+  for (int i = 8; i >= 0; i--) p = __builtin_fma(p, f, c[i]);
   return __builtin_amdgcn_ldexp(p, int(n));
 }
+constexpr double kLog2e64 = 1.4426950408889634074;
+constexpr float kLowest = -3.402823466e38f;
 
 // ---- a chunk --------------------------------------------------------------
 template <typename XT>
@@ -119,24 +118,45 @@ __device__ __forceinline__ double wave_sum64(double x) {
   for (int d = 32; d >= 1; d /= 2) x += __shfl_xor(x, d, 64);
   return x;
 }
-// A key that at least k of the wave's 64 reach, the largest such but for its low bits.
-__device__ __forceinline__ uint32_t reached_by(uint32_t key, int k) {
-  uint32_t t = 0;
+// Keys that at least k, and at least its share of k, of the wave's 64 N reach (of W
+// waves): the largest such but for their low bits.
+template <int W, int N, int kLow>
+__device__ __forceinline__ void reached_by(const uint32_t *keys, int k, uint32_t &all,
+                                           uint32_t &share) {
+  all = share = 0;
+  const int few = (k + W - 1) / W;
 #pragma unroll
-  for (int bit = 31; bit >= 10; bit--) {
-    const uint32_t up = t | 1u << bit;
-    if (__builtin_popcountll(__ballot(key >= up)) >= k) t = up;
+  for (int bit = 31; bit >= kLow; bit--) {
+    const uint32_t up = all | 1u << bit, up1 = share | 1u << bit;
+    int n = 0, n1 = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      n += __builtin_popcountll(__ballot(keys[i] >= up));
+      n1 += __builtin_popcountll(__ballot(keys[i] >= up1));
+    }
+    if (n >= k) all = up;
+    if (n1 >= few) share = up1;
   }
-  return t;
 }
-
+// What k of the workgroup's reach: the best of what k of a wave's do, or what every
+// wave's share does.
+template <int W>
+__device__ __forceinline__ uint32_t joint_bound(const uint32_t *all, const uint32_t *share) {
+  uint32_t a = all[0], q = share[0];
+#pragma unroll
+  for (int i = 1; i < W; i++) {
+    a = max(a, all[i]);
+    q = min(q, share[i]);
+  }
+  return max(a, q);
+}
 template <typename XT>
 __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
   typedef Chunk<XT> C;
-  __shared__ uint64_t list[kList];
+  __shared__ uint64_t list[kList];  // key, then place from the end
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
-  __shared__ uint32_t bounds[kWaves];
+  __shared__ uint32_t bounds[kWaves], shares[kWaves];
   __shared__ int listed, counts[kWaves];
   const int row = int(blockIdx.x / uint32_t(w.chunks)), chunk = int(blockIdx.x % uint32_t(w.chunks));
   if (w.c.done && w.c.done[row]) return;
@@ -145,35 +165,51 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
   float x[kEach];
   C::load(static_cast<const XT *>(w.c.logits) + row * w.c.stride + first, n, x);
   if (tid == 0) listed = 0;
-  float top = x[0];
+  constexpr int kGroups = kEach / 4;
+  float group[kGroups];
 #pragma unroll
-  for (int e = 1; e < kEach; e++) top = fmaxf(top, x[e]);
-  const float mine = fmaxf(top, -INFINITY);
-  top = wave_max(mine);
-  if ((tid & 63) == 0) tops[wave] = top;
-  const uint32_t bound = reached_by(key_of(mine), k);
-  if ((tid & 63) == 0) bounds[wave] = bound;
+  for (int i = 0; i < kGroups; i++)  // (-infinity for NaN)
+    group[i] = fmaxf(fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3])), -INFINITY);
+  float mine = group[0];
+#pragma unroll
+  for (int i = 1; i < kGroups; i++) mine = fmaxf(mine, group[i]);
+  float top = wave_max(mine);
+  // n_out of one wave's reach the one bound, a quarter of them of every wave's the other
+  uint32_t bound, share;
+  if (k <= 16) {
+    const uint32_t key = key_of(mine);
+    reached_by<kWaves, 1, 16>(&key, k, bound, share);
+  } else {
+    uint32_t tops4[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; i++) tops4[i] = key_of(group[i]);
+    reached_by<kWaves, kGroups, 13>(tops4, k, bound, share);
+  }
+  if ((tid & 63) == 0) {
+    tops[wave] = top;
+    bounds[wave] = bound;
+    shares[wave] = share;
+  }
   __syncthreads();
-  uint32_t least = kNone + 1;
 #pragma unroll
-  for (int i = 0; i < kWaves; i++) {
-    top = fmaxf(top, tops[i]);
-    least = max(least, bounds[i]);
-  }
-  // (the sum's exponentials come between the barriers of the list's)
+  for (int i = 0; i < kWaves; i++) top = fmaxf(top, tops[i]);
+  const float least = value_of(max(joint_bound<kWaves>(bounds, shares), kNone + 1));
+  if (__any(mine >= least)) {
 #pragma unroll
-  for (int e = 0; e < kEach; e++) {
-    const uint32_t key = key_of(fmaxf(x[e], -INFINITY));
-    if (__ballot(key >= least) == 0) continue;
-    if (key >= least) {
-      const int i = atomicAdd(&listed, 1);
-      if (i < kList) list[i] = uint64_t(key) << 32 | uint32_t(~C::at(e));
-    }
+    for (int e = 0; e < kEach; e++)
+      if (x[e] >= least) {
+        const int i = atomicAdd(&listed, 1);
+        if (i < kList) list[i] = uint64_t(key_of(x[e])) << 32 | uint32_t(~C::at(e));
+      }
   }
+  // (a chunk of nothing but -infinity: 0; an infinity: NaN, of -inf - -inf)
   const double base = top == -INFINITY ? 0.0 : double(top);
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < kEach; e++) sum += exp64(double(x[e]) - base);
+  for (int e = 0; e < kEach; e++) {
+    const float a = x[e] == -INFINITY ? kLowest : x[e];
+    sum += exp2_64((double(a) - base) * kLog2e64);
+  }
   sum = wave_sum64(sum);
   if ((tid & 63) == 0) sums[wave] = sum;
   __syncthreads();
@@ -211,14 +247,15 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
     c = listed;
   }
   const int64_t at = int64_t(row) * w.chunks + chunk;
-  Entry *out = w.list + at * k;
+  Entry *out = w.list + at * w.pad;
   for (int i = tid; i < c; i += kThreads) {
     const uint64_t me = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int o = 0; o < c; o++) rank += list[o] > me ? 1 : 0;
     if (rank < k) out[rank] = Entry{value_of(uint32_t(me >> 32)), first + int(~uint32_t(me))};
   }
-  for (int i = c + tid; i < k; i += kThreads) out[i] = Entry{0.f, -1};
+  for (int i = min(c, k) + tid; i < w.pad; i += kThreads) out[i] = Entry{0.f, -1};
   if (tid == 0) {
     sum = sums[0];
 #pragma unroll
@@ -236,116 +273,215 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
   return a.flat >= 0 && (b.flat < 0 || a.total > b.total || (a.total == b.total && a.flat < b.flat));
 }
 
+// A total as a whole number of the same order, for comparisons without branches.
+struct Ranked {
+  uint64_t key;
+  int flat, pad;
+};
+__device__ __forceinline__ Ranked ranked(const Best &b) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, b.total + 0.0);
+  return Ranked{u >> 63 ? ~u : u | uint64_t(1) << 63, b.flat, 0};
+}
+__device__ __forceinline__ double total_of(uint64_t key) {
+  return __builtin_bit_cast(double, key >> 63 ? key & ~(uint64_t(1) << 63) : ~key);
+}
+
 struct Row {  // of a beam
   double score, lse;
   int state;  // 0: it has no continuation, 1: tokens, 2: it has ended
 };
 
-// Place p of list l of sequence `seq`.
-__device__ __forceinline__ Best entry_of(const Work &w, const Row *rows, int seq, int l, int p) {
-  const int b = l / w.chunks;
-  const Row &r = rows[b];
+// x at place p of list l, of beam b.
+__device__ __forceinline__ Best best_of(const Work &w, const Row &r, int b, int l, int p, Entry x) {
   Best e{0.0, -1};
   if (r.state == 1) {
-    const Entry x = w.list[(int64_t(seq) * w.c.n_beam * w.chunks + l) * w.c.n_out + p];
     if (x.token >= 0) e = Best{r.score + (double(x.x) - r.lse), b * w.c.vocab + x.token};
   } else if (r.state == 2 && p == 0 && l == b * w.chunks) {
     e = Best{r.score, b * w.c.vocab + w.c.eos};
   }
   return e;
 }
+__device__ __forceinline__ const Entry *list_of(const Work &w, int seq, int l) {
+  return w.list + (int64_t(seq) * w.c.n_beam * w.chunks + l) * w.pad;
+}
 __device__ __forceinline__ uint32_t bound_key(const Best &e) {
   return e.flat < 0 ? 0u : key_of(float(e.total) + 0.f);
 }
+__device__ __forceinline__ Best wave_best(Best best) {
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) {
+    const Best o{__shfl_xor(best.total, d, 64), __shfl_xor(best.flat, d, 64)};
+    if (before(o, best)) best = o;
+  }
+  return best;
+}
 
-__global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
   __shared__ Row rows[kBeams];
-  __shared__ Best list[kJoin];
+  __shared__ __attribute__((aligned(16))) Ranked list[kJoin];
+  __shared__ uint32_t keys[kJoin];
+  __shared__ int16_t kept[kJoin];
   __shared__ Best picked[kBeams];
-  __shared__ Best waves[kWaves];
-  __shared__ uint32_t bounds[kWaves];
-  __shared__ int listed;
+  __shared__ Best waves[kJoinWaves];
+  __shared__ uint32_t bounds[kJoinWaves], shares[kJoinWaves];
+  __shared__ int listed, left;
   const int seq = int(blockIdx.x), tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int nb = w.c.n_beam, k = w.c.n_out, lists = nb * w.chunks;
-  if (tid == 0) listed = 0;
-  for (int b = wave; b < nb; b += kWaves) {
-    const int64_t row = int64_t(seq) * nb + b;
+  if (tid == 0) listed = left = 0;
+  // (on their way while the sums are joined) the first, 4th, 16th, 64th of a list
+  constexpr int kProbes = 4;
+  Entry probe[kProbes];
+  const Entry *mine_at = list_of(w, seq, min(tid, lists - 1));
+#pragma unroll
+  for (int i = 0; i < kProbes; i++) probe[i] = mine_at[min((1 << 2 * i) - 1, k - 1)];
+  // `team` lanes take a beam's chunks
+  int team = 1;
+  while (team < w.chunks && team < 64) team *= 2;
+  const int at = lane & (team - 1);
+  for (int b = tid / team; b < (nb + kJoinThreads / team - 1) / (kJoinThreads / team) * (kJoinThreads / team);
+       b += kJoinThreads / team) {
+    const int64_t row = int64_t(seq) * nb + min(b, nb - 1);
+    const Part *part = w.part + row * w.chunks;
     const bool ended = w.c.done && w.c.done[row];
-    float top = -INFINITY;
-    double sum = 0.0;
-    if (!ended) {
-      for (int i = lane; i < w.chunks; i += 64) top = fmaxf(top, w.part[row * w.chunks + i].top);
-      top = wave_max(top);
-      const double base = top == -INFINITY ? 0.0 : double(top);
-      for (int i = lane; i < w.chunks; i += 64) {
-        const Part p = w.part[row * w.chunks + i];
-        // (a chunk of nothing but -infinity has the sum 0; NaN and infinity pass)
-        sum += p.sum * exp64(double(p.top) - base);
-      }
-      sum = wave_sum64(sum);
-    }
-    if (lane == 0) {
-      Row r;
-      r.score = double(w.c.score[row]);
-      r.lse = ended ? 0.0 : double(top) + log(sum);
-      const bool fine = r.score - r.score == 0.0 && r.lse - r.lse == 0.0;  // both finite
-      r.state = !fine ? 0 : ended ? 2 : 1;
-      rows[b] = r;
+    const double score = double(w.c.score[row]);
+    Part mine = part[min(at, w.chunks - 1)];
+    if (ended || at >= w.chunks) mine = Part{0.0, -INFINITY, 0.f};
+    float top = mine.top;
+    if (!ended)
+      for (int i = at + 64; i < w.chunks; i += 64) top = fmaxf(top, part[i].top);
+    for (int d = team / 2; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const double base = top == -INFINITY ? 0.0 : double(top);
+    // (a chunk of nothing but -infinity has the sum 0; NaN passes)
+    auto term = [&](const Part &p) {
+      const float a = p.top == -INFINITY ? kLowest : p.top;
+      return p.sum * exp2_64((double(a) - base) * kLog2e64);
+    };
+    double sum = term(mine);
+    if (!ended)
+      for (int i = at + 64; i < w.chunks; i += 64) sum += term(part[i]);
+    for (int d = team / 2; d >= 1; d /= 2) sum += __shfl_xor(sum, d, 64);
+    const double lse = ended ? 0.0 : double(top) + log(sum);
+    if (at == 0 && b < nb) {
+      const bool fine = score - score == 0.0 && lse - lse == 0.0;  // both finite
+      rows[b] = Row{score, lse, !fine ? 0 : ended ? 2 : 1};
     }
   }
   __syncthreads();
-  // a bound that n_out totals reach, from the lists' heads
-  uint32_t head = 0;
-  for (int l = tid; l < lists; l += kThreads) head = max(head, bound_key(entry_of(w, rows, seq, l, 0)));
-  const uint32_t bound = reached_by(head, k);
-  if (lane == 0) bounds[wave] = bound;
-  __syncthreads();
-  uint32_t least = 1;
+  // a bound that n_out totals reach: of the lists' r-th tokens, for several r
+  uint32_t bound = 0, share = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; i++) least = max(least, bounds[i]);
-  for (int i = tid; i < lists * k; i += kThreads) {
-    const Best e = entry_of(w, rows, seq, i / k, i % k);
-    if (bound_key(e) >= least) {
-      const int at = atomicAdd(&listed, 1);
-      if (at < kJoin) list[at] = e;
+  for (int i = 0; i < kProbes; i++) {
+    const int r = 1 << 2 * i;
+    if (r > k) break;
+    uint32_t key = 0;
+    if (tid < lists) {
+      const int b = tid / w.chunks;
+      key = bound_key(best_of(w, rows[b], b, tid, r - 1, probe[i]));
+    }
+    for (int l = tid + kJoinThreads; l < lists; l += kJoinThreads) {
+      const int b = l / w.chunks;
+      key = max(key, bound_key(best_of(w, rows[b], b, l, r - 1, list_of(w, seq, l)[r - 1])));
+    }
+    uint32_t all, quarter;
+    reached_by<kJoinWaves, 1, 14>(&key, (k + r - 1) / r, all, quarter);
+    bound = max(bound, all);
+    share = max(share, quarter);
+  }
+  if (lane == 0) {
+    bounds[wave] = bound;
+    shares[wave] = share;
+  }
+  __syncthreads();
+  uint32_t least = max(joint_bound<kJoinWaves>(bounds, shares), 1u);
+  // Four places of a list at a time, `team` threads a list where there are few; a list
+  // falls, and is left at the first place below the bound.
+  team = 1;
+  while (team * lists * 2 <= kJoinThreads && team * 4 < k) team *= 2;
+  for (int l = tid / team; l < lists; l += kJoinThreads / team) {
+    const int b = l / w.chunks;
+    const Entry *from = list_of(w, seq, l);
+    for (int p = tid % team * 4; p < k; p += 4 * team) {
+      Entry x[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = from[p + i];
+      bool below = false;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const Best e = best_of(w, rows[b], b, l, p + i, x[i]);
+        below = bound_key(e) < least;
+        if (below) continue;
+        const int to = atomicAdd(&listed, 1);
+        if (to < kJoin) {
+          list[to] = ranked(e);
+          keys[to] = bound_key(e);
+        }
+      }
+      if (below) break;
     }
   }
   __syncthreads();
   const int c = listed;
   if (c <= kJoin) {
-    for (int i = tid; i < c; i += kThreads) {
-      const Best me = list[i];
-      int rank = 0;
-      for (int o = 0; o < c; o++) rank += before(list[o], me) ? 1 : 0;
-      if (rank < k) picked[rank] = me;
+    auto rank_all = [&](int n, auto at) {
+      for (int i = tid; i < n; i += kJoinThreads) {
+        const Ranked me = list[at(i)];
+        int rank = 0;
+#pragma unroll 8
+        for (int o = 0; o < n; o++) {
+          const Ranked x = list[at(o)];
+          rank += int(x.key > me.key) | (int(x.key == me.key) & int(x.flat < me.flat));
+        }
+        if (rank < k) picked[rank] = Best{total_of(me.key), me.flat};
+      }
+    };
+    if (c <= 96) {
+      rank_all(c, [](int i) { return i; });
+    } else {
+      // a bound again, of all that is listed (every wave looks for it): 445 of which 64
+      // are wanted take 10 us with it and 30 without, 9 of which 8 are 4 and 1
+      constexpr int kEachLane = 8;
+      least = 0;
+      if (c <= 64 * kEachLane) {
+        uint32_t mine[kEachLane], unused;
+#pragma unroll
+        for (int i = 0; i < kEachLane; i++) mine[i] = 64 * i + lane < c ? keys[64 * i + lane] : 0;
+        reached_by<1, kEachLane, 8>(mine, k, least, unused);
+      }
+      for (int i = tid; i < c; i += kJoinThreads)
+        if (keys[i] >= least) kept[atomicAdd(&left, 1)] = int16_t(i);
+      __syncthreads();
+      rank_all(left, [&](int i) { return int(kept[i]); });
     }
-    for (int i = c + tid; i < k; i += kThreads) picked[i] = Best{0.0, -1};
+    for (int i = c + tid; i < k; i += kJoinThreads) picked[i] = Best{0.0, -1};
   } else {
-    // one after the other: of the tokens behind the last one that was taken the first
-    Best last{INFINITY, -1};
-    for (int r = 0; r < k; r++) {
+    // One after the other: the first of the lists' heads, whose list goes on.  A thread
+    // keeps the first of its lists' heads; next[l] lies in the ranked list's place.
+    uint8_t *next = reinterpret_cast<uint8_t *>(list);
+    for (int l = tid; l < lists; l += kJoinThreads) next[l] = 0;
+    int from = 0;
+    auto first = [&]() {
       Best best{0.0, -1};
-      for (int i = tid; i < lists * k; i += kThreads) {
-        const Best e = entry_of(w, rows, seq, i / k, i % k);
-        if ((r == 0 || before(last, e)) && before(e, best)) best = e;
+      for (int l = tid; l < lists; l += kJoinThreads) {
+        const int b = l / w.chunks, p = next[l];
+        const Best e = p < k ? best_of(w, rows[b], b, l, p, list_of(w, seq, l)[p]) : Best{0.0, -1};
+        if (before(e, best)) best = e, from = l;
       }
-#pragma unroll
-      for (int d = 32; d >= 1; d /= 2) {
-        const Best o{__shfl_xor(best.total, d, 64), __shfl_xor(best.flat, d, 64)};
-        if (before(o, best)) best = o;
-      }
+      return best;
+    };
+    Best mine = first();
+    for (int r = 0; r < k; r++) {
+      const Best top = wave_best(mine);
       __syncthreads();
-      if (lane == 0) waves[wave] = best;
+      if (lane == 0) waves[wave] = top;
       __syncthreads();
-      best = waves[0];
+      Best best = waves[0];
 #pragma unroll
-      for (int i = 1; i < kWaves; i++)
+      for (int i = 1; i < kJoinWaves; i++)
         if (before(waves[i], best)) best = waves[i];
       if (tid == 0) picked[r] = best;
-      last = best;
-      if (best.flat < 0) {
-        for (int i = r + tid; i < k; i += kThreads) picked[i] = Best{0.0, -1};
-        break;
+      if (best.flat >= 0 && mine.flat == best.flat) {
+        next[from]++;
+        mine = first();
       }
     }
   }
@@ -354,22 +490,23 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Work w) {
     const Best e = picked[tid];
     const bool none = e.flat < 0;
     const int b = none ? 0 : e.flat / w.c.vocab, token = e.flat - b * w.c.vocab;
-    const int64_t at = int64_t(seq) * k + tid;
-    w.c.parent[at] = none ? -1 : seq * nb + b;
-    w.c.token[at] = none ? -1 : token;
-    w.c.out_score[at] = none ? -INFINITY : float(e.total);
+    const int64_t to = int64_t(seq) * k + tid;
+    w.c.parent[to] = none ? -1 : seq * nb + b;
+    w.c.token[to] = none ? -1 : token;
+    w.c.out_score[to] = none ? -INFINITY : float(e.total);
     if (w.c.out_done)
-      w.c.out_done[at] = !none && (rows[b].state == 2 || token == w.c.eos) ? 1 : 0;
+      w.c.out_done[to] = !none && (rows[b].state == 2 || token == w.c.eos) ? 1 : 0;
   }
 }
 
 int64_t chunks_of(const BeamCall &c) { return (c.vocab + kChunk - 1) / kChunk; }
+int pad_of(const BeamCall &c) { return (c.n_out + 3) / 4 * 4; }
 
 }  // namespace
 
 size_t swamp_beam_scratch_bytes(const BeamCall &c) {
   const size_t parts = size_t(c.n_seq) * size_t(c.n_beam) * size_t(chunks_of(c));
-  return swamp::scratch_round(parts * size_t(c.n_out) * sizeof(Entry)) +
+  return swamp::scratch_round(parts * size_t(pad_of(c)) * sizeof(Entry)) +
          swamp::scratch_round(parts * sizeof(Part));
 }
 
@@ -377,13 +514,14 @@ int swamp_launch_beam_select(const BeamCall &c, swamp::Scratch &sc, hipStream_t 
   Work w;
   w.c = c;
   w.chunks = int(chunks_of(c));
+  w.pad = pad_of(c);
   const int64_t parts = int64_t(c.n_seq) * c.n_beam * w.chunks;  // below 2^31
-  w.list = static_cast<Entry *>(sc.get(size_t(parts) * size_t(c.n_out) * sizeof(Entry)));
+  w.list = static_cast<Entry *>(sc.get(size_t(parts) * size_t(w.pad) * sizeof(Entry)));
   w.part = static_cast<Part *>(sc.get(size_t(parts) * sizeof(Part)));
   if (!w.list || !w.part) return SWAMP_EWORKSPACE;
   if (c.type == SWAMP_F32) chunk_kernel<float><<<unsigned(parts), kThreads, 0, s>>>(w);
   else if (c.type == SWAMP_F16) chunk_kernel<_Float16><<<unsigned(parts), kThreads, 0, s>>>(w);
   else chunk_kernel<__bf16><<<unsigned(parts), kThreads, 0, s>>>(w);
-  join_kernel<<<unsigned(c.n_seq), kThreads, 0, s>>>(w);
+  join_kernel<<<unsigned(c.n_seq), kJoinThreads, 0, s>>>(w);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
