@@ -9,9 +9,9 @@
 // Tiles.  Four waves a workgroup, WM x WN V_MFMA_I32_32X32X32_I8 blocks each.  A K step
 // is 64 codes: a stage holds the tile's rows of x, then of w, 64 bytes each, 16-byte
 // chunks XOR-swizzled by (row / 4) % 4, so that 16 consecutive lanes of a fragment read
-// meet no bank twice.  Five stages, filled by direct-to-LDS DMA three steps ahead; one
-// barrier a step, between its halves, whose counted wait leaves the last step and a half
-// of DMAs in flight.
+// meet no bank twice.  Stages are filled by direct-to-LDS DMA, two steps at a time, four to
+// twelve steps ahead; one barrier a step, between its halves, whose counted wait leaves
+// the DMAs of the steps behind the next one in flight.
 //
 // The last step of a sum is taken apart from the loop: its codes of x behind column K
 // are cleared, so that what lies in w there (a row's padding) counts for nothing.
@@ -30,31 +30,99 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 // ---- quantizer ------------------------------------------------------------
-// A workgroup a row.  HBM's: a row is read once (the second look is the cache's).
-template <typename XT>
-__global__ void __launch_bounds__(256) quantize_kernel(const XT *__restrict__ x, int64_t x_stride,
-                                                       int8_t *__restrict__ q, int64_t q_stride,
-                                                       float *__restrict__ scale, int n) {
-  __shared__ float tops[4];
-  const XT *row = x + int64_t(blockIdx.x) * x_stride;
-  int8_t *out = q + int64_t(blockIdx.x) * q_stride;
-  const int tid = int(threadIdx.x);
-  float top = 0.f;
-  for (int k = tid; k < n; k += 256) {
-    const float a = fabsf(float(row[k]));
-    top = !(a <= 3.402823466e38f) ? INFINITY : fmaxf(top, a);  // NaN counts as infinity
-  }
+// A workgroup a row.  HBM's: a row is read once where it fits its threads' registers (16
+// elements each, or 32), else the second look is the cache's.
+
+// The largest |x| of a workgroup's elements; NaN counts as infinity.
+__device__ __forceinline__ float raise(float top, float x) {
+  const float a = fabsf(x);
+  return !(a <= 3.402823466e38f) ? INFINITY : fmaxf(top, a);
+}
+__device__ __forceinline__ float workgroup_max(float top) {
+  __shared__ float tops[16];
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  const int waves = int(blockDim.x) >> 6;
+  if (waves == 1) return top;
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  top = tops[0];
+  for (int i = 1; i < waves; i++) top = fmaxf(top, tops[i]);
+  return top;
+}
+// The row's scale, written; 0 or less: its codes are 0.
+__device__ __forceinline__ float scale_of(float top, float *to) {
   const bool fine = top < INFINITY;
   float s = top / 127.f;
   if (s < 1.17549435e-38f) s = 0.f;
-  if (tid == 0) scale[blockIdx.x] = fine ? s : __builtin_nanf("");
-  for (int k = tid; k < n; k += 256)
-    out[k] = fine && s > 0.f ? int8_t(__builtin_rintf(float(row[k]) / s)) : int8_t(0);
+  if (threadIdx.x == 0) *to = fine ? s : __builtin_nanf("");
+  return fine ? s : -1.f;
+}
+__device__ __forceinline__ int code_of(float x, float s) {
+  return s > 0.f ? int(__builtin_rintf(x / s)) : 0;
+}
+
+// Rows of any length.
+template <typename XT>
+__global__ void __launch_bounds__(1024) quantize_any_kernel(const XT *__restrict__ x,
+                                                            int64_t x_stride,
+                                                            int8_t *__restrict__ q,
+                                                            int64_t q_stride,
+                                                            float *__restrict__ scale, int n) {
+  const XT *row = x + int64_t(blockIdx.x) * x_stride;
+  int8_t *out = q + int64_t(blockIdx.x) * q_stride;
+  float top = 0.f;
+  for (int k = int(threadIdx.x); k < n; k += int(blockDim.x)) top = raise(top, float(row[k]));
+  const float s = scale_of(workgroup_max(top), scale + blockIdx.x);
+  for (int k = int(threadIdx.x); k < n; k += int(blockDim.x))
+    out[k] = int8_t(code_of(float(row[k]), s));
+}
+
+// N elements of any place that their type allows.
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+  T v[N];
+};
+
+// Rows of up to kEach times the threads, 16 bytes a load.
+template <typename XT, int kEach>
+__global__ void __launch_bounds__(1024) quantize_kernel(const XT *__restrict__ x, int64_t x_stride,
+                                                        int8_t *__restrict__ q, int64_t q_stride,
+                                                        float *__restrict__ scale, int n) {
+  constexpr int V = 16 / int(sizeof(XT)), kLoads = kEach / V;
+  const XT *row = x + int64_t(blockIdx.x) * x_stride;
+  int8_t *out = q + int64_t(blockIdx.x) * q_stride;
+  Vec<XT, V> v[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; j++) {
+    const int at = (j * int(blockDim.x) + int(threadIdx.x)) * V;
+    if (at + V <= n) {
+      v[j] = *reinterpret_cast<const Vec<XT, V> *>(row + at);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k++) v[j].v[k] = at + k < n ? row[at + k] : XT(0);
+    }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < kLoads; j++)
+#pragma unroll
+    for (int k = 0; k < V; k++) top = raise(top, float(v[j].v[k]));
+  const float s = scale_of(workgroup_max(top), scale + blockIdx.x);
+#pragma unroll
+  for (int j = 0; j < kLoads; j++) {
+    const int at = (j * int(blockDim.x) + int(threadIdx.x)) * V;
+    Vec<int8_t, V> c;
+#pragma unroll
+    for (int k = 0; k < V; k++) c.v[k] = int8_t(code_of(float(v[j].v[k]), s));
+    if (at + V <= n) {
+      *reinterpret_cast<Vec<int8_t, V> *>(out + at) = c;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        if (at + k < n) out[at + k] = c.v[k];
+    }
+  }
 }
 
 // ---- products -------------------------------------------------------------
@@ -63,12 +131,15 @@ struct Shape {
   static constexpr int NW = NWM * NWN, kThreads = 64 * NW;
   static constexpr int TM = 32 * WM * NWM, TN = 32 * WN * NWN;  // tile: rows of x, of w
   static constexpr int kStage = (TM + TN) * 64;
-  static constexpr int kStages = 5;
+  // Pairs of steps on their way, as many as LDS holds with one step more, 6 at most.
+  static constexpr int kPairs = std::min(6, (160 * 1024 / kStage - 1) / 2);
+  static constexpr int kStages = 2 * kPairs + 1;
   static constexpr int kSmem = kStages * kStage;
   static constexpr int kDma = (TM + TN) / (16 * NW);  // 1 KB DMAs of a wave and step
   static constexpr int kDma0 = (kDma + 1) / 2;        // of them in a step's first half
   static_assert(TM % (16 * NW) == 0 && TN % (16 * NW) == 0, "a DMA fills 16 rows of one operand");
-  static_assert(kSmem <= 160 * 1024, "LDS");
+  static_assert(kPairs >= 2 && kSmem <= 160 * 1024, "LDS");
+  static_assert(2 * kPairs * kDma <= 63, "the memory counter");
 };
 
 // One 16-byte-per-lane DMA into LDS (lane L writes lds + 16 L).  Not a template: the
@@ -88,37 +159,45 @@ struct Work {
 };
 
 // sum times both scales into y, added to what is there or not.
-template <bool kAdd, typename Y>
-__device__ __forceinline__ void put(Y *y, int sum, float sx, double sw) {
+template <typename Y>
+__device__ __forceinline__ void put(Y *y, int sum, float sx, double sw, int add) {
   float v = float(double(sx) * sw * double(sum));
 #ifdef __HIP_DEVICE_COMPILE__
   asm volatile("" : "+v"(v));  // (or the compiler rounds to 16 bits from 64 at once)
 #endif
-  *y = Y(kAdd ? float(*y) + v : v);
+  *y = Y(add ? float(*y) + v : v);
 }
-// f with y's element type and whether to add.
-template <typename F>
-__device__ __forceinline__ void with_output(const GemmI8Call &c, F f) {
-  if (c.y_type == SWAMP_F32) {
-    if (c.accumulate) f(float{}, std::true_type{});
-    else f(float{}, std::false_type{});
-  } else if (c.y_type == SWAMP_F16) {
-    if (c.accumulate) f(_Float16{}, std::true_type{});
-    else f(_Float16{}, std::false_type{});
-  } else {
-    if (c.accumulate) f(__bf16{}, std::true_type{});
-    else f(__bf16{}, std::false_type{});
-  }
-}
-__device__ __forceinline__ void put_at(const GemmI8Call &c, int64_t i, int sum) {
-  const int m = int(i / c.n), n = int(i - int64_t(m) * c.n);
-  with_output(c, [&](auto yt, auto add) {
-    put<decltype(add)::value>(static_cast<decltype(yt) *>(c.y) + int64_t(m) * c.y_stride + n, sum,
-                              c.x_scale[m], double(c.w_scale[n]));
-  });
+__device__ __forceinline__ void put_at(const GemmI8Call &c, int m, int n, int sum) {
+  const int64_t at = int64_t(m) * c.y_stride + n;
+  const float sx = c.x_scale[m];
+  const double sw = double(c.w_scale[n]);
+  if (c.y_type == SWAMP_F32) put(static_cast<float *>(c.y) + at, sum, sx, sw, c.accumulate);
+  else if (c.y_type == SWAMP_F16) put(static_cast<_Float16 *>(c.y) + at, sum, sx, sw, c.accumulate);
+  else put(static_cast<__bf16 *>(c.y) + at, sum, sx, sw, c.accumulate);
 }
 
-template <int WM, int WN, int NWM, int NWN>
+// 32 rows of kCols sums, in LDS, to rows m0 on and columns n0 on of y, whose ends may lie
+// among them.
+template <int kCols, int kPitch, typename Y>
+__device__ __forceinline__ void store_strip(const GemmI8Call &c, const int32_t *strip,
+                                            const float *scales, int m0, int n0, int lane) {
+  constexpr int V = 16 / int(sizeof(Y)), kLanes = kCols / V, kRows = 64 / kLanes;
+  const int col = lane % kLanes * V, n = n0 + col;
+  if (n >= c.n) return;
+  float sw[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) sw[v] = c.w_scale[min(n + v, c.n - 1)];
+  for (int row = lane / kLanes; row < 32 && m0 + row < c.m; row += kRows) {
+    const float sx = scales[row];
+    Y *y = static_cast<Y *>(c.y) + int64_t(m0 + row) * c.y_stride + n;
+    const int32_t *sum = strip + row * kPitch + col;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      if (n + v < c.n) put(y + v, sum[v], sx, double(sw[v]), c.accumulate);
+  }
+}
+
+template <typename Y, int WM, int WN, int NWM, int NWN>
 __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
   using S = Shape<WM, WN, NWM, NWN>;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -140,22 +219,33 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
 
   const uint32_t xp = uint32_t(c.x_stride), wp = uint32_t(c.w_stride), k16 = uint32_t(K + 15) & ~15u;
   const uint32_t xm = uint32_t(min(S::TM, c.m - m0) - 1), wn_ = uint32_t(min(S::TN, c.n - n0) - 1);
-  const __amdgpu_buffer_rsrc_t xr = swamp::make_rsrc(c.x + m0 * c.x_stride, xm * xp + k16);
-  const __amdgpu_buffer_rsrc_t wr = swamp::make_rsrc(c.w + n0 * c.w_stride, wn_ * wp + k16);
+  const uint32_t x_bytes = xm * xp + k16, w_bytes = wn_ * wp + k16;
   // DMA i of wave w fills stage rows R = 16 (NW i + w) .. R + 15: lane L writes row
   // R + L / 4, physical chunk L % 4, which holds logical chunk (L % 4) ^ (L / 16 % 4).
   const uint32_t lrow4 = uint32_t(lane >> 2), chunk = uint32_t((lane & 3) ^ ((lane >> 4) & 3)) << 4;
   const uint32_t xv = lrow4 * xp + chunk, wv = lrow4 * wp + chunk;
 
-  auto dma_part = [&](uint8_t *st, int kt, auto i0c, auto i1c) {
+  // DMAs [i0, i1) of the steps kt and kt + 1: 64 bytes of a row and the 64 behind them
+  // directly after one another, so that the first level cache gets the line once.
+  auto dma_pair = [&](int kt, int stage, auto i0c, auto i1c) {
     constexpr int i0 = decltype(i0c)::value, i1 = decltype(i1c)::value;
+    uint8_t *st = smem + S::kStage * stage;
+    uint8_t *st1 = smem + S::kStage * (stage + 1 == S::kStages ? 0 : stage + 1);
+    // (past the end: nothing is fetched, and the count of DMAs stays)
+    const __amdgpu_buffer_rsrc_t xr =
+        swamp::make_rsrc(c.x + m0 * c.x_stride, kt < kt1 ? x_bytes : 0u);
+    const __amdgpu_buffer_rsrc_t wr =
+        swamp::make_rsrc(c.w + n0 * c.w_stride, kt < kt1 ? w_bytes : 0u);
 #pragma unroll
     for (int i = i0; i < i1; i++) {
       const int R = 16 * (S::NW * i + wave);
-      if (16 * S::NW * i < S::TM)
+      if (16 * S::NW * i < S::TM) {
         dma16(xr, st + R * 64, xv, uint32_t(R) * xp + uint32_t(kt) * 64u);
-      else
+        dma16(xr, st1 + R * 64, xv, uint32_t(R) * xp + uint32_t(kt) * 64u + 64u);
+      } else {
         dma16(wr, st + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(kt) * 64u);
+        dma16(wr, st1 + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(kt) * 64u + 64u);
+      }
     }
   };
   using I0 = std::integral_constant<int, 0>;
@@ -196,16 +286,16 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
   };
 
-  constexpr int NS = S::kStages;
-  // Step kt issues the DMA of step kt + 3, half in each half, into the stage of step
-  // kt - 2, which every wave finished reading before the previous barrier.  Past the
-  // end: the last step again.
+  // Steps go in pairs, 0 and 1, 2 and 3, ...: an odd step s issues the DMA of the pair
+  // behind the last one on its way, into the stages of steps s - 2 and s - 1, which every
+  // wave finished reading before the barrier of step s - 1.
+  constexpr int NS = S::kStages, kPairs = S::kPairs;
 #pragma unroll
-  for (int p = 0; p < 3; p++) {
-    dma_part(smem + S::kStage * p, min(kt0 + p, kt1 - 1), I0{}, IE{});
+  for (int p = 0; p < kPairs; p++) {
+    dma_pair(kt0 + 2 * p, 2 * p, I0{}, IE{});
     __builtin_amdgcn_sched_barrier(0);
   }
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * S::kDma) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kPairs - 1) * 2 * S::kDma) : "memory");
 
   i32x4 fa0[WM], fb0[WN], fa1[WM], fb1[WN];
   read_frags(smem, loff0, fa0, fb0);
@@ -226,29 +316,49 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
       }
     }
   };
-  using D0 = std::integral_constant<int, S::kDma0>;
-  using D1 = std::integral_constant<int, S::kDma - S::kDma0>;
+  using N0 = std::integral_constant<int, 0>;
+  using D0 = std::integral_constant<int, 2 * S::kDma0>;
+  using D1 = std::integral_constant<int, 2 * (S::kDma - S::kDma0)>;
 
   int cur = 0;
-  for (int kt = kt0; kt < kt1 - 1; kt++) {
+  auto step = [&](int kt, auto odd_c) {
+    constexpr bool odd = decltype(odd_c)::value;
     const int nxt = cur + 1 == NS ? 0 : cur + 1;
-    const int fill = cur + 3 < NS ? cur + 3 : cur + 3 - NS;
-    const int ktf = min(kt + 3, kt1 - 1);
+    const int fill = cur >= 2 ? cur - 2 : cur - 2 + NS, ktf = kt + 2 * kPairs - 1;
     read_frags(smem + S::kStage * cur, loff1, fa1, fb1);
     mfmas(fa0, fb0);
-    dma_part(smem + S::kStage * fill, ktf, I0{}, IH{});
-    order(D0{});
+    if constexpr (odd) {
+      dma_pair(ktf, fill, I0{}, IH{});
+      order(D0{});
+    } else {
+      order(N0{});
+    }
     __builtin_amdgcn_sched_barrier(0);
-    // step kt + 1 is there for every wave: only step kt + 2's DMA and the first half of
-    // step kt + 3's stay in flight
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::kDma + S::kDma0) : "memory");
+    // Step kt + 1 is there for every wave, and this one read.  (An even step's next came
+    // with it; else all but the pairs behind the next and what this step has issued.)
+    if constexpr (odd)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kPairs - 2) * 2 * S::kDma +
+                                                                       2 * S::kDma0)
+                   : "memory");
+    else
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     read_frags(smem + S::kStage * nxt, loff0, fa0, fb0);
     mfmas(fa1, fb1);
-    dma_part(smem + S::kStage * fill, ktf, IH{}, IE{});
-    order(D1{});
+    if constexpr (odd) {
+      dma_pair(ktf, fill, IH{}, IE{});
+      order(D1{});
+    } else {
+      order(N0{});
+    }
     __builtin_amdgcn_sched_barrier(0);
     cur = nxt;
+  };
+  int kt = kt0;
+  for (; kt + 1 < kt1 - 1; kt += 2) {
+    step(kt, std::false_type{});
+    step(kt + 1, std::true_type{});
   }
+  if (kt < kt1 - 1) step(kt, std::false_type{});
   // The last step, without what lies behind column K.
   read_frags(smem + S::kStage * cur, loff1, fa1, fb1);
   auto cut = [&](i32x4 (&f)[WM], int half) {
@@ -286,31 +396,181 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the workgroup
     return;
   }
-  // The scales of the tile's rows, in the stages' place once every wave is done with them.
+  // To y through LDS, 32 rows of a wave at a time, so that a store is 16 bytes a lane and
+  // whole runs of a row (from the blocks' own layout, one element a lane, a tile of 256 x
+  // 256 took 33 us).  Every wave is done with the stages.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   float *scales = reinterpret_cast<float *>(smem);
   for (int i = tid; i < S::TM; i += S::kThreads) scales[i] = c.x_scale[min(m0 + i, c.m - 1)];
   __syncthreads();
-  auto store = [&](auto yt, auto acc_c) {
-    typedef decltype(yt) Y;
-    constexpr bool kAdd = decltype(acc_c)::value;
+  // (rows 4 apart are written together: 128 bytes apart in the banks)
+  constexpr int kCols = 32 * WN, kPitch = kCols + 8;
+  static_assert(S::TM * 4 + S::NW * 32 * kPitch * 4 <= S::kSmem, "strips");
+  int32_t *strip = reinterpret_cast<int32_t *>(smem + S::TM * 4) + wave * 32 * kPitch;
+  auto fill = [&](auto ic) {
+    constexpr int i = decltype(ic)::value;
 #pragma unroll
-    for (int j = 0; j < WN; j++) {
-      const int n = nw + 32 * j;
-      const double sw_n = double(c.w_scale[min(n, c.n - 1)]);
+    for (int j = 0; j < WN; j++)
 #pragma unroll
-      for (int i = 0; i < WM; i++) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int row = wm * WM * 32 + 4 * fc + 32 * i + 8 * (e >> 2) + (e & 3), m = m0 + row;
-          if (m < c.m && n < c.n) put<kAdd>(static_cast<Y *>(c.y) + int64_t(m) * c.y_stride + n,
-                                            acc[i][j][e], scales[row], sw_n);
-        }
+      for (int e = 0; e < 16; e++) {
+        int32_t x = acc[i][j][e];
+#ifdef __HIP_DEVICE_COMPILE__
+        asm volatile("" : "+v"(x));  // (one by one: as pairs they moved whole blocks to memory)
+#endif
+        strip[(8 * (e >> 2) + 4 * fc + (e & 3)) * kPitch + 32 * j + fr] = x;
       }
+  };
+  const int mr = wm * WM * 32, nr = n0 + wn * kCols;  // the wave's first row in the tile, column
+  if (m0 + S::TM > c.m || n0 + S::TN > c.n || c.accumulate) {
+    auto part = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < WM) {
+        fill(ic);
+        store_strip<kCols, kPitch, Y>(c, strip, scales + mr + 32 * i, m0 + mr + 32 * i, nr, lane);
+      }
+    };
+    part(std::integral_constant<int, 0>{});
+    part(std::integral_constant<int, 1>{});
+    part(std::integral_constant<int, 2>{});
+    part(std::integral_constant<int, 3>{});
+    return;
+  }
+  // A whole tile: a strip's reads, the next one's writes (LDS keeps their order), and then
+  // the first's arithmetic; one wave a SIMD has nothing else to wait with.
+  constexpr int V = 16 / int(sizeof(Y)), kLanes = kCols / V, kRows = 64 / kLanes, T = 32 / kRows;
+  const int col = lane % kLanes * V, row0 = lane / kLanes;
+  double sw_n[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) sw_n[v] = double(c.w_scale[nr + col + v]);
+  Y *y = static_cast<Y *>(c.y) + int64_t(m0 + mr + row0) * c.y_stride + nr + col;
+  fill(std::integral_constant<int, 0>{});
+  auto whole = [&](auto ic) {
+    constexpr int i = decltype(ic)::value;
+    if constexpr (i < WM) {
+      i32x4 sum[T][V / 4];
+      float sx[T];
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+#pragma unroll
+        for (int v = 0; v < V / 4; v++)
+          sum[t][v] = *reinterpret_cast<const i32x4 *>(strip + (t * kRows + row0) * kPitch + col + 4 * v);
+        sx[t] = scales[mr + 32 * i + t * kRows + row0];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (i + 1 < WM) fill(std::integral_constant<int, i + 1>{});
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        Vec<Y, V> o;
+#pragma unroll
+        for (int v = 0; v < V; v++) put(&o.v[v], sum[t][v / 4][v % 4], sx[t], sw_n[v], 0);
+        *reinterpret_cast<Vec<Y, V> *>(y) = o;
+        y += kRows * c.y_stride;
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  with_output(c, store);
+  whole(std::integral_constant<int, 0>{});
+  whole(std::integral_constant<int, 1>{});
+  whole(std::integral_constant<int, 2>{});
+  whole(std::integral_constant<int, 3>{});
+}
+
+// ---- few rows of x --------------------------------------------------------
+// The weights' stream bounds it, so they go from memory to registers: a lane holds 16
+// codes of one row of w (R tiles of 16 rows), V_MFMA_I32_16X16X64_I8 multiplies 16 rows
+// by T times 16 of x.  A workgroup's waves take a share of the columns each, so that a
+// short matrix has all its bytes in flight at once, and their sums meet in LDS.  What of
+// x lies behind column K is cleared, rows behind the last are the descriptor's zeros.
+template <int R, int T>
+__global__ void __launch_bounds__(1024) few_kernel(GemmI8Call c) {
+  constexpr int U = 4 / (R * T > 2 ? 2 : 1);  // steps in flight, and as many to come
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  int32_t *parts = reinterpret_cast<int32_t *>(smem);
+  const int lane = int(threadIdx.x) & 63, r = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int waves = int(blockDim.x) >> 6, KT = (c.k + 63) / 64, n0 = int(blockIdx.x) * 16 * R;
+  const int share = (KT + waves - 1) / waves, s0 = min(wave * share, KT), s1 = min(s0 + share, KT);
+  const uint32_t xp = uint32_t(c.x_stride), wp = uint32_t(c.w_stride);
+  const uint32_t k16 = uint32_t(c.k + 15) & ~15u;
+  const __amdgpu_buffer_rsrc_t xr = swamp::make_rsrc(c.x, uint32_t(c.m - 1) * xp + k16);
+  const __amdgpu_buffer_rsrc_t wr = swamp::make_rsrc(
+      c.w + n0 * c.w_stride, uint32_t(min(16 * R, c.n - n0) - 1) * wp + k16);
+  uint32_t xv[T], wv[R];
+#pragma unroll
+  for (int j = 0; j < T; j++) xv[j] = uint32_t(16 * j + r) * xp + 16u * uint32_t(h);
+#pragma unroll
+  for (int i = 0; i < R; i++) wv[i] = uint32_t(16 * i + r) * wp + 16u * uint32_t(h);
+  i32x4 acc[R][T];
+#pragma unroll
+  for (int i = 0; i < R; i++)
+#pragma unroll
+    for (int j = 0; j < T; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+  struct Stage {
+    i32x4 w[U][R], x[U][T];
+  };
+  auto load = [&](Stage &st, int s) {
+    if (s >= s1) return;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t at = uint32_t(min(s + u, s1 - 1)) * 64u;
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        st.w[u][i] = __builtin_bit_cast(
+            i32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wv[i], at, 0));
+#pragma unroll
+      for (int j = 0; j < T; j++)
+        st.x[u][j] = __builtin_bit_cast(
+            i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xv[j], at, 0));
+    }
+  };
+  auto multiply = [&](Stage &st, int s) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s + u >= s1) break;
+      const int left = c.k - (s + u) * 64 - 16 * h;  // columns of this lane's 16
+      if ((s + u + 1) * 64 > c.k) {
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+          const int n = left - 4 * d;
+          const int32_t keep = n >= 4 ? ~0 : n <= 0 ? 0 : int32_t((1u << (8 * n)) - 1);
+#pragma unroll
+          for (int j = 0; j < T; j++) st.x[u][j][d] &= keep;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < T; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.x[u][j], st.w[u][i], acc[i][j], 0, 0,
+                                                            0);
+    }
+  };
+  if (s0 < s1) {
+    Stage a, b;
+    load(a, s0);
+    for (int s = s0; s < s1; s += 2 * U) {
+      load(b, s + U);
+      multiply(a, s);
+      load(a, s + 2 * U);
+      multiply(b, s + U);
+    }
+  }
+  // lane: column (row of w) r, rows (of x) 4 h .. 4 h + 3
+#pragma unroll
+  for (int i = 0; i < R; i++)
+#pragma unroll
+    for (int j = 0; j < T; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        parts[((wave * R + i) * T + j) * 256 + (4 * h + e) * 16 + r] = acc[i][j][e];
+  __syncthreads();
+  for (int o = int(threadIdx.x); o < R * T * 256; o += int(blockDim.x)) {
+    int sum = 0;
+    for (int w = 0; w < waves; w++) sum += parts[w * R * T * 256 + o];
+    const int i = o / (T * 256), j = o / 256 % T;
+    const int m = 16 * j + o % 256 / 16, n = n0 + 16 * i + o % 16;
+    if (m < c.m && n < c.n) put_at(c, m, n, sum);
+  }
 }
 
 // The pieces' sums (whole numbers: in any order the same) to y.
@@ -319,17 +579,19 @@ __global__ void __launch_bounds__(256) join_kernel(Work wk) {
   if (i >= mn) return;
   int sum = 0;
   for (int p = 0; p < wk.pieces; p++) sum += wk.part[p * mn + i];
-  put_at(wk.c, i, sum);
+  const int m = int(i / wk.c.n);
+  put_at(wk.c, m, int(i - int64_t(m) * wk.c.n), sum);
 }
 
 // A sum of nothing.
 __global__ void __launch_bounds__(256) nothing_kernel(GemmI8Call c) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i < int64_t(c.m) * c.n) put_at(c, i, 0);
+  const int m = int(i / c.n);
+  if (m < c.m) put_at(c, m, int(i - int64_t(m) * c.n), 0);
 }
 
 struct Plan {
-  int shape;  // 0: 64 x 256, 1: 128 x 128, 2: 256 x 256
+  int shape;  // -1: few rows, 0: 64 x 256, 1: 128 x 128, 2: 256 x 256, 3: 64 x 128
   int tiles_m, tiles_n, pieces, steps;
 };
 
@@ -341,29 +603,47 @@ Plan plan_of(int m, int n, int k) {
     p.tiles_n = (n + tn - 1) / tn;
     return int64_t(p.tiles_m) * p.tiles_n;
   };
+  if (m <= 32) {
+    p.shape = -1;
+    p.pieces = 1;
+    return p;
+  }
   p.shape = 2;
-  if (m <= 64) p.shape = 0;
+  if (m <= 64) p.shape = 3;
   else if (2 * tiles(256, 256) <= cus) p.shape = 1;
-  const int64_t t = p.shape == 0 ? tiles(64, 256) : p.shape == 1 ? tiles(128, 128) : tiles(256, 256);
+  const int64_t t = p.shape == 0 ? tiles(64, 256) : p.shape == 3 ? tiles(64, 128) : p.shape == 1 ? tiles(128, 128) : tiles(256, 256);
   p.pieces = int(std::max<int64_t>(1, std::min<int64_t>({cus / t, 8, KT / 8})));
-  p.steps = (KT + p.pieces - 1) / p.pieces;
+  p.steps = ((KT + p.pieces - 1) / p.pieces + 1) / 2 * 2;  // whole pairs
   p.pieces = (KT + p.steps - 1) / p.steps;
   return p;
 }
 
-template <int WM, int WN, int NWM, int NWN>
-int launch(const Work &wk, hipStream_t s) {
+template <int R, int T>
+int launch_few(const GemmI8Call &c, hipStream_t s) {
+  const int steps = (c.k + 63) / 64, waves = std::max(1, std::min(16, steps / 2));
+  few_kernel<R, T><<<unsigned((c.n + 16 * R - 1) / (16 * R)), 64 * waves, R * T * 1024 * waves, s>>>(c);
+  return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
+}
+
+template <typename Y, int WM, int WN, int NWM, int NWN>
+int launch_typed(const Work &wk, hipStream_t s) {
   using S = Shape<WM, WN, NWM, NWN>;
   static std::once_flag once;
   static hipError_t err = hipSuccess;
   std::call_once(once, [] {
-    err = hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_kernel<WM, WN, NWM, NWN>),
+    err = hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_kernel<Y, WM, WN, NWM, NWN>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   });
   if (err != hipSuccess) return SWAMP_ELAUNCH;
   const unsigned units = unsigned(wk.tiles_m) * unsigned(wk.tiles_n) * unsigned(wk.pieces);
-  gemm_kernel<WM, WN, NWM, NWN><<<units, S::kThreads, S::kSmem, s>>>(wk);
+  gemm_kernel<Y, WM, WN, NWM, NWN><<<units, S::kThreads, S::kSmem, s>>>(wk);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
+}
+template <int WM, int WN, int NWM, int NWN>
+int launch(const Work &wk, hipStream_t s) {
+  if (wk.c.y_type == SWAMP_F32) return launch_typed<float, WM, WN, NWM, NWN>(wk, s);
+  if (wk.c.y_type == SWAMP_F16) return launch_typed<_Float16, WM, WN, NWM, NWN>(wk, s);
+  return launch_typed<__bf16, WM, WN, NWM, NWN>(wk, s);
 }
 
 }  // namespace
@@ -373,8 +653,16 @@ int swamp_launch_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_strid
                                hipStream_t s) {
   auto go = [&](auto t) {
     typedef decltype(t) X;
-    quantize_kernel<X><<<unsigned(n_rows), 256, 0, s>>>(static_cast<const X *>(d_x), x_stride, d_q,
-                                                        q_stride, d_scale, n_cols);
+    const X *x = static_cast<const X *>(d_x);
+    const unsigned rows = unsigned(n_rows);
+    const int each = n_cols <= 1024 * 16 ? 16 : 32;
+    const int threads = std::max(1, (n_cols + 64 * each - 1) / (64 * each)) * 64;
+    if (n_cols <= 1024 * 16)
+      quantize_kernel<X, 16><<<rows, threads, 0, s>>>(x, x_stride, d_q, q_stride, d_scale, n_cols);
+    else if (n_cols <= 1024 * 32)
+      quantize_kernel<X, 32><<<rows, threads, 0, s>>>(x, x_stride, d_q, q_stride, d_scale, n_cols);
+    else
+      quantize_any_kernel<X><<<rows, 1024, 0, s>>>(x, x_stride, d_q, q_stride, d_scale, n_cols);
   };
   if (x_type == SWAMP_F32) go(float{});
   else if (x_type == SWAMP_F16) go(_Float16{});
@@ -385,7 +673,7 @@ int swamp_launch_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_strid
 size_t swamp_gemm_rows_i8_scratch_bytes(int m, int n_rows, int n_cols) {
   if (n_cols == 0) return 0;
   const Plan p = plan_of(m, n_rows, n_cols);
-  return p.pieces > 1 ? size_t(p.pieces) * size_t(m) * size_t(n_rows) * 4 : 0;
+  return p.pieces > 1 ? swamp::scratch_round(size_t(p.pieces) * size_t(m) * size_t(n_rows) * 4) : 0;
 }
 
 int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream_t s) {
@@ -395,6 +683,7 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
     return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
   }
   Plan p = plan_of(c.m, c.n, c.k);
+  if (p.shape < 0) return c.m <= 16 ? launch_few<1, 1>(c, s) : launch_few<2, 2>(c, s);
   Work wk{c, p.tiles_m, p.tiles_n, 8, p.pieces, p.steps, nullptr};
   if (p.pieces > 1) {
     wk.part = static_cast<int32_t *>(sc.get(size_t(p.pieces) * size_t(c.m) * size_t(c.n) * 4));
@@ -405,6 +694,7 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
   }
   const int rc = p.shape == 0   ? launch<2, 2, 1, 4>(wk, s)
                  : p.shape == 1 ? launch<2, 2, 2, 2>(wk, s)
+                 : p.shape == 3 ? launch<1, 2, 2, 2>(wk, s)
                                 : launch<4, 4, 2, 2>(wk, s);
   if (rc != SWAMP_OK || wk.pieces == 1) return rc;
   join_kernel<<<unsigned(blocks), 256, 0, s>>>(wk);
