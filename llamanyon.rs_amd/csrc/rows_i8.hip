@@ -216,6 +216,11 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
   const int m0 = (g0 + r % gs) * S::TM, n0 = r / gs * S::TN;
   const int K = c.k, KT = (K + 63) / 64;
   const int kt0 = piece * wk.steps, kt1 = min(KT, kt0 + wk.steps);
+  // Where every row of w is one workgroup's, each begins its whole pairs of steps at
+  // another place: side by side they would read the same columns of rows a power of two
+  // apart, which are a few memory channels'.
+  const int turn = wk.tiles_m == 1 && (kt1 - kt0) % 2 == 0 && K % 64 == 0
+                       ? 2 * (5 * (t + piece) % ((kt1 - kt0) / 2)) : 0;
 
   const uint32_t xp = uint32_t(c.x_stride), wp = uint32_t(c.w_stride), k16 = uint32_t(K + 15) & ~15u;
   const uint32_t xm = uint32_t(min(S::TM, c.m - m0) - 1), wn_ = uint32_t(min(S::TN, c.n - n0) - 1);
@@ -231,6 +236,7 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
     constexpr int i0 = decltype(i0c)::value, i1 = decltype(i1c)::value;
     uint8_t *st = smem + S::kStage * stage;
     uint8_t *st1 = smem + S::kStage * (stage + 1 == S::kStages ? 0 : stage + 1);
+    const int at = kt + turn < kt1 ? kt + turn : kt + turn - (kt1 - kt0);
     // (past the end: nothing is fetched, and the count of DMAs stays)
     const __amdgpu_buffer_rsrc_t xr =
         swamp::make_rsrc(c.x + m0 * c.x_stride, kt < kt1 ? x_bytes : 0u);
@@ -240,11 +246,11 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
     for (int i = i0; i < i1; i++) {
       const int R = 16 * (S::NW * i + wave);
       if (16 * S::NW * i < S::TM) {
-        dma16(xr, st + R * 64, xv, uint32_t(R) * xp + uint32_t(kt) * 64u);
-        dma16(xr, st1 + R * 64, xv, uint32_t(R) * xp + uint32_t(kt) * 64u + 64u);
+        dma16(xr, st + R * 64, xv, uint32_t(R) * xp + uint32_t(at) * 64u);
+        dma16(xr, st1 + R * 64, xv, uint32_t(R) * xp + uint32_t(at) * 64u + 64u);
       } else {
-        dma16(wr, st + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(kt) * 64u);
-        dma16(wr, st1 + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(kt) * 64u + 64u);
+        dma16(wr, st + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(at) * 64u);
+        dma16(wr, st1 + R * 64, wv, uint32_t(R - S::TM) * wp + uint32_t(at) * 64u + 64u);
       }
     }
   };
