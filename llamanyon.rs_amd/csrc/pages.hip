@@ -18,7 +18,6 @@ using swamp::PageTables;
 
 constexpr int kSeqs = swamp::kMaxPageSeqs;
 constexpr int kTile = 16;     // table columns that a workgroup turns at a time
-constexpr int kBlock = 1024;  // threads of the one workgroup that ranks pages
 
 // ---- fork -----------------------------------------------------------------
 // T'[s] = T[parent s], in place: a workgroup takes 16 columns of all rows into LDS.
@@ -92,23 +91,23 @@ __global__ void __launch_bounds__(256) fork_finish_kernel(PagePool pool, PageTab
 
 // ---- one workgroup's sums -------------------------------------------------
 // The sum of x over the threads before this one, and over all; `part` holds a value
-// for each wave and is free again after the next barrier of the caller.
-template <typename T>
-__device__ __forceinline__ T scan(T x, T *part, T &total) {
+// for each wave and is free again on return.
+template <int kBlock>
+__device__ __forceinline__ int64_t scan(int64_t x, int64_t *part, int64_t &total) {
   const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
-  T incl = x;
+  int64_t incl = x;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const T below = __shfl_up(incl, d, 64);
+    const int64_t below = __shfl_up(incl, d, 64);
     if (lane >= d) incl += below;
   }
   if (lane == 63) part[wave] = incl;
   __syncthreads();
-  T before = 0;
+  int64_t before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kBlock / 64; w++) {
-    const T p = part[w];
+    const int64_t p = part[w];
     if (w < wave) before += p;
     total += p;
   }
@@ -125,24 +124,31 @@ __device__ __forceinline__ uint32_t used_word(const PagePool &pool, int64_t w, b
   return fill ? x | ~there : x & there;
 }
 
-constexpr int kWords = 4;  // of a thread in a round: 131072 pages
+constexpr int kWords = 4;  // of a thread in a round, at most
 
 // ---- extend ---------------------------------------------------------------
 // One workgroup: what every sequence needs (two a thread), where its pages begin in
 // the row of all pages handed out, then one pass over the free pages in rising
 // order, each finding its owner by bisection.  Of the h sequences that would write
-// one shared page in turn, the j-th finds refs - j tables naming it.
+// one shared page in turn, the j-th finds refs - j tables naming it.  A chain of loads
+// and sums: 64 sequences of 31 pages XX us, of which the launch is 2.
+template <int kBlock>
 __global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTables t,
                                                         const int32_t *__restrict__ d_new,
-                                                        PageMoves moves) {
-  __shared__ __attribute__((aligned(16))) int tail[kSeqs];  // the shared page it would write, or -1
-  __shared__ int copy[kSeqs];     // its place in the list, or -1
-  __shared__ int first[kSeqs];    // its first new column
-  __shared__ int64_t off[kSeqs + 1];
+                                                        PageMoves moves, int per) {
+  constexpr int kMost = 2 * kBlock;  // sequences
+  __shared__ __attribute__((aligned(16))) int tail[kMost];  // the shared page it would write, or -1
+  __shared__ int copy[kMost];     // its place in the list, or -1
+  __shared__ int first[kMost];    // its first new column
+  __shared__ int64_t off[kMost];
   __shared__ int64_t part[kBlock / 64];
   __shared__ int listed;
   const int n = t.n_seq, tid = int(threadIdx.x);
   const int mask = (1 << pool.shift) - 1;
+  const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
+  uint32_t free[kWords];  // of the first round, on their way
+#pragma unroll
+  for (int i = 0; i < kWords; i++) free[i] = i < per ? ~used_word(pool, tid * per + i, true) : 0u;
   bool bad = false;
   int refs[2], grown[2], fresh[2];
   if (tid == 0) listed = 0;
@@ -173,52 +179,55 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTable
     }
   }
   __syncthreads();
-  int copies[2];
-  int64_t need = 0, total;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int s = 2 * tid + i;
-    copies[i] = 0;
-    if (tail[s] >= 0) {
-      int before = 0;
-      for (int o = 0; o < s; o++) before += tail[o] == tail[s] ? 1 : 0;
-      copies[i] = before < refs[i] - 1 ? 1 : 0;
+  const int mine[2] = {tail[2 * tid], tail[2 * tid + 1]};
+  int before[2] = {0, 0}, copies[2];
+  if (mine[0] >= 0 || mine[1] >= 0)
+#pragma unroll 4
+    for (int o = 0; o < 2 * tid; o += 2) {
+      const int a = tail[o], b = tail[o + 1];
+      before[0] += (a == mine[0] ? 1 : 0) + (b == mine[0] ? 1 : 0);
+      before[1] += (a == mine[1] ? 1 : 0) + (b == mine[1] ? 1 : 0);
     }
-    need += copies[i] + fresh[i];
-  }
-  const int64_t at = scan<int64_t>(need, part, total);
-  int64_t n_copies;
-  const int64_t place = scan<int64_t>(copies[0] + copies[1], part, n_copies);
+  before[1] += mine[0] == mine[1] ? 1 : 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) copies[i] = mine[i] >= 0 && before[i] < refs[i] - 1 ? 1 : 0;
+  // pages in the low 48 bits (2048 times less than 2^31 at most), copies above
+  constexpr int kCopy = 48;
+  int64_t total;
+  int64_t at = scan<kBlock>(int64_t(copies[0]) + fresh[0] + copies[1] + fresh[1] +
+                                (int64_t(copies[0] + copies[1]) << kCopy),
+                            part, total);
+  const int place = int(at >> kCopy);
+  at &= (int64_t(1) << kCopy) - 1;
+  total &= (int64_t(1) << kCopy) - 1;
   off[2 * tid] = at;
   off[2 * tid + 1] = at + copies[0] + fresh[0];
-  copy[2 * tid] = copies[0] ? int(place) : -1;
-  copy[2 * tid + 1] = copies[1] ? int(place) + copies[0] : -1;
-  if (tid == 0) off[kSeqs] = total;
+  copy[2 * tid] = copies[0] ? place : -1;
+  copy[2 * tid + 1] = copies[1] ? place + copies[0] : -1;
 #pragma unroll
   for (int i = 0; i < 2; i++)
-    if (copies[i]) atomicSub(&pool.refs[tail[2 * tid + i]], 1);
+    if (copies[i]) atomicSub(&pool.refs[mine[i]], 1);
   __syncthreads();
 
   int64_t base = 0;  // free pages before this round's
-  const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
-  for (int64_t w0 = 0; base < total && w0 < words; w0 += kBlock * kWords) {
-    uint32_t free[kWords];
-    int mine = 0;
+  for (int64_t w0 = 0; base < total && w0 < words; w0 += kBlock * per) {
+    if (w0 > 0)
 #pragma unroll
-    for (int i = 0; i < kWords; i++) {
-      free[i] = ~used_word(pool, w0 + tid * kWords + i, true);
-      mine += __builtin_popcount(free[i]);
-    }
+      for (int i = 0; i < kWords; i++)
+        free[i] = i < per ? ~used_word(pool, w0 + tid * per + i, true) : 0u;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; i++) count += __builtin_popcount(free[i]);
     int64_t found;
-    int64_t rank = base + scan<int64_t>(mine, part, found);
+    int64_t rank = base + scan<kBlock>(count, part, found);
 #pragma unroll
     for (int i = 0; i < kWords; i++) {
-      const int64_t w = w0 + tid * kWords + i;
+      const int64_t w = w0 + tid * per + i;
       uint32_t left = free[i];
       while (left != 0 && rank < total) {
         const int bit = __builtin_ctz(left), id = int(32 * w) + bit;
         left &= left - 1;
-        int lo = 0, hi = kSeqs;  // off[lo] <= rank < off[hi]
+        int lo = 0, hi = n;  // off[lo] <= rank < off[hi]
         while (hi - lo > 1) {
           const int mid = (lo + hi) / 2;
           if (off[mid] <= rank) lo = mid;
@@ -274,49 +283,73 @@ __global__ void __launch_bounds__(256) trim_kernel(PagePool pool, PageTables t,
 }
 
 // ---- compact --------------------------------------------------------------
-__global__ void __launch_bounds__(kBlock) compact_list_kernel(PagePool pool, PageMoves moves) {
-  __shared__ int64_t part[kBlock / 64];
+// One workgroup: the words of a round, with the holes below U and the pages at U and
+// above that lie before each, go to LDS; then a thread a page, whose rank is its place.
+constexpr int kListBlock = 1024, kListWords = 2;
+__global__ void __launch_bounds__(kListBlock) compact_list_kernel(PagePool pool, PageMoves moves) {
+  constexpr int kRound = kListBlock * kListWords;
+  __shared__ int64_t part[kListBlock / 64];
+  __shared__ uint32_t word[kRound], hole_at[kRound], up_at[kRound];
   const int tid = int(threadIdx.x);
   const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
   int64_t n_used = 0, sum;
-  for (int64_t w = tid; w < words; w += kBlock) n_used += __builtin_popcount(used_word(pool, w, false));
-  scan<int64_t>(n_used, part, sum);
+  for (int64_t w = tid; w < words; w += kListBlock)
+    n_used += __builtin_popcount(used_word(pool, w, false));
+  scan<kListBlock>(n_used, part, sum);
   n_used = sum;
   int64_t holes = 0, high = 0;  // before this round's words
-  for (int64_t w0 = 0; w0 < words; w0 += kBlock * kWords) {
-    uint32_t hole[kWords], up[kWords];
+  for (int64_t w0 = 0; w0 < words; w0 += kRound) {
+    uint32_t x[kListWords], low[kListWords];
     int64_t mine = 0;  // holes, and 2^32 times the pages above
 #pragma unroll
-    for (int i = 0; i < kWords; i++) {
-      const int64_t w = w0 + tid * kWords + i, below = n_used - 32 * w;
-      const uint32_t low = below >= 32 ? ~0u : below <= 0 ? 0u : (1u << below) - 1;
-      hole[i] = ~used_word(pool, w, true) & low;
-      up[i] = used_word(pool, w, false) & ~low;
-      mine += __builtin_popcount(hole[i]) + (int64_t(__builtin_popcount(up[i])) << 32);
+    for (int i = 0; i < kListWords; i++) {
+      const int64_t w = w0 + tid * kListWords + i, below = n_used - 32 * w;
+      low[i] = below >= 32 ? ~0u : below <= 0 ? 0u : (1u << below) - 1;
+      x[i] = used_word(pool, w, false);
+      mine += __builtin_popcount(~x[i] & low[i]) + (int64_t(__builtin_popcount(x[i] & ~low[i])) << 32);
     }
-    const int64_t before = scan<int64_t>(mine, part, sum);
-    int64_t h = holes + (before & 0xFFFFFFFF), u = high + (before >> 32);
+    const int64_t before = scan<kListBlock>(mine, part, sum);
+    uint32_t h = uint32_t(holes + (before & 0xFFFFFFFF)), u = uint32_t(high + (before >> 32));
 #pragma unroll
-    for (int i = 0; i < kWords; i++) {
-      const int first = int(32 * (w0 + tid * kWords + i));
-      for (uint32_t x = hole[i]; x != 0 && h < moves.cap; x &= x - 1)
-        moves.dst[h++] = first + __builtin_ctz(x);
-      for (uint32_t x = up[i]; x != 0 && u < moves.cap; x &= x - 1)
-        moves.src[u++] = first + __builtin_ctz(x);
+    for (int i = 0; i < kListWords; i++) {
+      word[tid * kListWords + i] = x[i];
+      hole_at[tid * kListWords + i] = h;
+      up_at[tid * kListWords + i] = u;
+      h += uint32_t(__builtin_popcount(~x[i] & low[i]));
+      u += uint32_t(__builtin_popcount(x[i] & ~low[i]));
     }
+    __syncthreads();
+    const int64_t last = min(int64_t(pool.n_pages), 32 * (w0 + kRound));
+    for (int64_t id = 32 * w0 + tid; id < last; id += kListBlock) {
+      const int at = int(id / 32 - w0);
+      const uint32_t bit = 1u << (id % 32), under = bit - 1, w = word[at];
+      const int64_t below = n_used - id / 32 * 32;
+      const uint32_t lower = below >= 32 ? ~0u : below <= 0 ? 0u : (1u << below) - 1;
+      if (id < n_used && !(w & bit)) {
+        const uint32_t r = hole_at[at] + uint32_t(__builtin_popcount(~w & lower & under));
+        if (r < uint32_t(moves.cap)) moves.dst[r] = int(id);
+      } else if (id >= n_used && (w & bit)) {
+        const uint32_t r = up_at[at] + uint32_t(__builtin_popcount(w & ~lower & under));
+        if (r < uint32_t(moves.cap)) moves.src[r] = int(id);
+      }
+    }
+    __syncthreads();
     holes += sum & 0xFFFFFFFF;
     high += sum >> 32;
   }
   if (tid == 0) *moves.count = int(min(high, int64_t(moves.cap)));
 }
 
-// Counts of the pages that move (block column 0), and a row's entries: where the
-// list, which rises, holds an entry as a source it becomes the place it moves to.
+// Counts of the pages that move, and a row's entries: where the list, which rises,
+// holds an entry as a source it becomes the place it moves to (found by bisection,
+// among every step-th source in LDS first).
+constexpr int kProbes = 2048;
 __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTables t,
                                                            PageMoves moves) {
+  __shared__ int probe[kProbes];
   const int n = *moves.count;
   if (n == 0) return;
-  const int from = moves.src[0], to = moves.src[n - 1];
+  const int step = (n + kProbes - 1) / kProbes, probes = (n + step - 1) / step;
   const int64_t threads = int64_t(gridDim.x) * gridDim.y * 256;
   const int64_t me = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   for (int64_t i = me; i < n; i += threads) {
@@ -329,16 +362,26 @@ __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTa
   const int s = int(blockIdx.x);
   if (s >= t.n_seq) return;
   const int64_t cols = held_cols(t.len[s], pool.shift, t.stride);
+  if (int64_t(blockIdx.y) * 256 >= cols) return;
+  for (int i = int(threadIdx.x); i < probes; i += 256) probe[i] = moves.src[int64_t(i) * step];
+  __syncthreads();
+  const int from = probe[0], to = moves.src[n - 1];
   for (int64_t c = int64_t(blockIdx.y) * 256 + threadIdx.x; c < cols; c += int64_t(gridDim.y) * 256) {
     const int id = t.pages[s * t.stride + c];
     if (id < from || id > to) continue;
-    int lo = 0, hi = n;  // src[lo] <= id < src[hi]
+    int lo = 0, hi = probes;  // probe[lo] <= id < probe[hi]
     while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (moves.src[mid] <= id) lo = mid;
+      const int mid = (lo + hi) / 2;
+      if (probe[mid] <= id) lo = mid;
       else hi = mid;
     }
-    if (moves.src[lo] == id) t.pages[s * t.stride + c] = moves.dst[lo];
+    int64_t a = int64_t(lo) * step, b = min(a + step, int64_t(n));
+    while (b - a > 1) {
+      const int64_t mid = (a + b) / 2;
+      if (moves.src[mid] <= id) a = mid;
+      else b = mid;
+    }
+    if ((step == 1 ? probe[lo] : moves.src[a]) == id) t.pages[s * t.stride + c] = moves.dst[a];
   }
 }
 
@@ -406,7 +449,13 @@ int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int
 
 int swamp_launch_pages_extend(const PagePool &pool, const PageTables &t, const int32_t *d_new,
                               const PageMoves &moves, hipStream_t s) {
-  extend_kernel<<<1, kBlock, 0, s>>>(pool, t, d_new, moves);
+  // (a small workgroup waits less at its barriers)
+  const int64_t words = (int64_t(pool.n_pages) + 31) / 32;
+  auto per = [&](int block) { return int(std::max<int64_t>(1, std::min<int64_t>(kWords, (words + block - 1) / block))); };
+  if (t.n_seq <= 512 && words <= 256 * kWords)
+    extend_kernel<256><<<1, 256, 0, s>>>(pool, t, d_new, moves, per(256));
+  else
+    extend_kernel<1024><<<1, 1024, 0, s>>>(pool, t, d_new, moves, per(1024));
   return launched();
 }
 
@@ -418,7 +467,7 @@ int swamp_launch_pages_trim(const PagePool &pool, const PageTables &t, const int
 
 int swamp_launch_pages_compact(const PagePool &pool, const PageTables &t, const PageMoves &moves,
                                hipStream_t s) {
-  compact_list_kernel<<<1, kBlock, 0, s>>>(pool, moves);
+  compact_list_kernel<<<1, kListBlock, 0, s>>>(pool, moves);
   const dim3 grid(unsigned(std::max(t.n_seq, 64)),
                   unsigned(std::max<int64_t>(1, std::min<int64_t>(t.stride / 256, 16))));
   compact_move_kernel<<<grid, 256, 0, s>>>(pool, t, moves);

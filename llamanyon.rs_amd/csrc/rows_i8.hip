@@ -596,32 +596,63 @@ __global__ void __launch_bounds__(256) nothing_kernel(GemmI8Call c) {
   if (m < c.m) put_at(c, m, int(i - int64_t(m) * c.n), 0);
 }
 
+// Which tiles, and in how many pieces the sums: of every choice its time by a model, with
+// both sides of 171 sizes (1 to 1024 rows of x, 640 to 28672 of w, 512 to 14336 columns)
+// measured in up to 40 ways.  A round of tiles costs a tile's filling and storing and its
+// steps, a last one that does not fill the CUs 0.7 of that and the rest by its share; pieces
+// cost their sums' writing and reading.  Of 144 sizes above 16 rows the choice is 1.4%
+// slower than the fastest on average, 23% at worst but for one (192 x 16384 x 512, 17.3 us
+// for 11.4).
+struct Tiles {
+  int tm, tn;
+  double step, fixed;  // us
+};
+constexpr Tiles kTiles[] = {
+    {64, 128, 0.205, 6.4}, {128, 128, 0.24, 9.5}, {256, 128, 0.5, 7.0}, {128, 256, 0.5, 7.0},
+    {256, 256, 0.84, 12.5}};
+
 struct Plan {
-  int shape;  // -1: few rows, 0: 64 x 256, 1: 128 x 128, 2: 256 x 256, 3: 64 x 128
+  int shape;  // of kTiles; -1: few_kernel, of `tiles_n` tiles of 16 rows a workgroup
   int tiles_m, tiles_n, pieces, steps;
 };
 
 Plan plan_of(int m, int n, int k) {
   const int cus = swamp::device_info().num_cus, KT = (k + 63) / 64;
-  Plan p;
-  auto tiles = [&](int tm, int tn) {
-    p.tiles_m = (m + tm - 1) / tm;
-    p.tiles_n = (n + tn - 1) / tn;
-    return int64_t(p.tiles_m) * p.tiles_n;
-  };
-  if (m <= 32) {
-    p.shape = -1;
-    p.pieces = 1;
-    return p;
+  Plan best{-1, 1, 1, 1, KT};
+  // Up to 16 rows: as few workgroups as one round takes (one row of 6144 x 4096: 7.3 us
+  // with two tiles of 16 a workgroup, 9.6 with one, 10.5 with four).  Up to 32, where the
+  // round holds them and the columns are few enough for every wave's x: 8.8 us at 17 rows,
+  // where 64 x 128 tiles take 11.3 (4096 x 14336: 20 and 17).
+  if (m <= 16) {
+    while (best.tiles_n < 4 && (n + 16 * best.tiles_n - 1) / (16 * best.tiles_n) > cus)
+      best.tiles_n *= 2;
+    return best;
   }
-  p.shape = 2;
-  if (m <= 64) p.shape = 3;
-  else if (2 * tiles(256, 256) <= cus) p.shape = 1;
-  const int64_t t = p.shape == 0 ? tiles(64, 256) : p.shape == 3 ? tiles(64, 128) : p.shape == 1 ? tiles(128, 128) : tiles(256, 256);
-  p.pieces = int(std::max<int64_t>(1, std::min<int64_t>({cus / t, 8, KT / 8})));
-  p.steps = ((KT + p.pieces - 1) / p.pieces + 1) / 2 * 2;  // whole pairs
-  p.pieces = (KT + p.steps - 1) / p.steps;
-  return p;
+  if (m <= 32 && (n + 31) / 32 <= cus && k <= 8192) return best;
+  double least = 0;
+  for (int i = 0; i < int(sizeof(kTiles) / sizeof(kTiles[0])); i++) {
+    const Tiles &t = kTiles[i];
+    Plan p;
+    p.shape = i;
+    p.tiles_m = (m + t.tm - 1) / t.tm;
+    p.tiles_n = (n + t.tn - 1) / t.tn;
+    const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+    for (int pieces = 1; pieces <= 8 && (pieces == 1 || (KT / pieces >= 4 && tiles * pieces <= 3 * cus));
+         pieces++) {
+      p.steps = ((KT + pieces - 1) / pieces + 1) / 2 * 2;  // whole pairs
+      p.pieces = (KT + p.steps - 1) / p.steps;
+      const int64_t units = tiles * p.pieces, rem = units % cus;
+      const double round = t.fixed + p.steps * t.step;
+      double us = double(units / cus) * round;
+      if (rem) us += round * (0.7 + 0.3 * double(rem) / cus);
+      if (p.pieces > 1) us += 1.0 + p.pieces * (double(m) * n * 8.0 / 2.9e6);
+      if (best.shape < 0 || us < least) {
+        least = us;
+        best = p;
+      }
+    }
+  }
+  return best;
 }
 
 template <int R, int T>
@@ -689,7 +720,11 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
     return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
   }
   Plan p = plan_of(c.m, c.n, c.k);
-  if (p.shape < 0) return c.m <= 16 ? launch_few<1, 1>(c, s) : launch_few<2, 2>(c, s);
+  if (p.shape < 0)
+    return c.m > 16         ? launch_few<2, 2>(c, s)
+           : p.tiles_n == 1 ? launch_few<1, 1>(c, s)
+           : p.tiles_n == 2 ? launch_few<2, 1>(c, s)
+                            : launch_few<4, 1>(c, s);
   Work wk{c, p.tiles_m, p.tiles_n, 8, p.pieces, p.steps, nullptr};
   if (p.pieces > 1) {
     wk.part = static_cast<int32_t *>(sc.get(size_t(p.pieces) * size_t(c.m) * size_t(c.n) * 4));
@@ -698,9 +733,10 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
       wk.steps = (c.k + 63) / 64;
     }
   }
-  const int rc = p.shape == 0   ? launch<2, 2, 1, 4>(wk, s)
+  const int rc = p.shape == 0   ? launch<1, 2, 2, 2>(wk, s)
                  : p.shape == 1 ? launch<2, 2, 2, 2>(wk, s)
-                 : p.shape == 3 ? launch<1, 2, 2, 2>(wk, s)
+                 : p.shape == 2 ? launch<4, 2, 2, 2>(wk, s)
+                 : p.shape == 3 ? launch<2, 4, 2, 2>(wk, s)
                                 : launch<4, 4, 2, 2>(wk, s);
   if (rc != SWAMP_OK || wk.pieces == 1) return rc;
   join_kernel<<<unsigned(blocks), 256, 0, s>>>(wk);
