@@ -25,12 +25,26 @@ constexpr int kTile = 16;     // table columns that a workgroup turns at a time
 // pages lie together and name them in the same column: a thread runs down a column
 // and adds a run of equal pages' gains at once, and where a prompt's beams only
 // change places the sum is 0 and nothing is written.
-__global__ void __launch_bounds__(256) fork_tables_kernel(PagePool pool, PageTables t,
-                                                          const int32_t *__restrict__ d_parent) {
+//
+// kOne: the one workgroup of a small call also does what else comes in a launch of its
+// own, when every count is final: which pages are in use, and the lengths.
+template <bool kOne>
+__global__ void __launch_bounds__(256) fork_kernel(PagePool pool, PageTables t,
+                                                   const int32_t *__restrict__ d_parent) {
   extern __shared__ int smem[];
-  const int n = t.n_seq, tid = int(threadIdx.x);
-  int *tile = smem, *gain = tile + n * kTile, *cols = gain + n, *parent = cols + n;
+  const int n = t.n_seq, tid = int(threadIdx.x), c = tid % kTile;
+  int *tile = smem, *gain = tile + n * kTile, *lens = gain + n, *parent = lens + n;
   __shared__ int most;
+  // the first tile's entries, on their way while lengths and parents come in (those past a
+  // sequence's pages, which the table has room for, are not looked at)
+  constexpr int kAhead = 8;
+  int ahead[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) {
+    const int s = j * (256 / kTile) + tid / kTile;
+    const int64_t col = int64_t(blockIdx.x) * kTile + c;
+    ahead[j] = s < n && col < t.stride ? t.pages[s * t.stride + col] : -1;
+  }
   if (tid == 0) most = 0;
   for (int s = tid; s < n; s += 256) gain[s] = -1;
   __syncthreads();
@@ -38,19 +52,24 @@ __global__ void __launch_bounds__(256) fork_tables_kernel(PagePool pool, PageTab
   for (int s = tid; s < n; s += 256) {
     const int p = d_parent[s];
     parent[s] = uint32_t(p) < uint32_t(n) ? p : -1;
-    cols[s] = int(held_cols(t.len[s], pool.shift, t.stride));
-    top = max(top, cols[s]);
+    lens[s] = t.len[s];
+    top = max(top, int(held_cols(lens[s], pool.shift, t.stride)));
     if (uint32_t(p) < uint32_t(n)) atomicAdd(&gain[p], 1);
   }
-  atomicMax(&most, top);
+  if (top > 0) atomicMax(&most, top);
   __syncthreads();
-  const int c = tid % kTile;
   const int rows = (n + 15) / 16, r0 = min(tid / kTile * rows, n), r1 = min(r0 + rows, n);
-  for (int64_t c0 = int64_t(blockIdx.x) * kTile; c0 < most; c0 += int64_t(gridDim.x) * kTile) {
-    for (int i = tid; i < n * kTile; i += 256) {
-      const int s = i / kTile;
-      tile[i] = c0 + c < cols[s] ? t.pages[s * t.stride + c0 + c] : -1;
+  const int64_t mine = int64_t(blockIdx.x) * kTile;
+  for (int64_t c0 = mine; c0 < most; c0 += int64_t(gridDim.x) * kTile) {
+    auto held = [&](int s) { return c0 + c < held_cols(lens[s], pool.shift, t.stride); };
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int s = j * (256 / kTile) + tid / kTile;
+      if (s < n)
+        tile[s * kTile + c] = !held(s) ? -1 : c0 == mine ? ahead[j] : t.pages[s * t.stride + c0 + c];
     }
+    for (int s = kAhead * (256 / kTile) + tid / kTile; s < n; s += 256 / kTile)
+      tile[s * kTile + c] = held(s) ? t.pages[s * t.stride + c0 + c] : -1;
     __syncthreads();
     int id = -1, sum = 0;
     for (int s = r0; s < r1; s++) {
@@ -63,12 +82,25 @@ __global__ void __launch_bounds__(256) fork_tables_kernel(PagePool pool, PageTab
       sum += gain[s];
     }
     if (sum != 0 && page_ok(id, pool.n_pages)) atomicAdd(&pool.refs[id], sum);
-    for (int i = tid; i < n * kTile; i += 256) {
-      const int s = i / kTile, p = parent[s];
-      if (p != s && p >= 0 && c0 + c < cols[p])
-        t.pages[s * t.stride + c0 + c] = tile[p * kTile + c];
+    for (int s = tid / kTile; s < n; s += 256 / kTile) {
+      const int p = parent[s];
+      if (p != s && p >= 0 && held(p)) t.pages[s * t.stride + c0 + c] = tile[p * kTile + c];
     }
     __syncthreads();
+  }
+  if constexpr (kOne) {
+    __threadfence();
+    __syncthreads();
+    for (int s = tid; s < n; s += 256) t.len[s] = parent[s] < 0 ? 0 : lens[parent[s]];
+    for (int64_t first = 0; first < pool.n_pages; first += 256) {
+      const int64_t p = first + tid;
+      // (counts as the adds left them, not as a cache may hold them)
+      const bool held = p < pool.n_pages && __hip_atomic_load(&pool.refs[p], __ATOMIC_RELAXED,
+                                                              __HIP_MEMORY_SCOPE_AGENT) > 0;
+      const uint64_t used = __ballot(held);
+      if (tid % 32 == 0 && p < pool.n_pages)
+        pool.used[p / 32] = uint32_t(tid % 64 ? used >> 32 : used);
+    }
   }
 }
 
@@ -124,12 +156,12 @@ __device__ __forceinline__ uint32_t used_word(const PagePool &pool, int64_t w, b
   return fill ? x | ~there : x & there;
 }
 
-constexpr int kWords = 4;  // of a thread in a round, at most
+constexpr int kWords = 2;  // of a thread in a round, at most
 
 // ---- extend ---------------------------------------------------------------
 // One workgroup: what every sequence needs (two a thread), where its pages begin in
 // the row of all pages handed out, then one pass over the free pages in rising
-// order, each finding its owner by bisection.  Of the h sequences that would write
+// order: a thread a page, which finds the page's word and its owner by bisection.  Of the h sequences that would write
 // one shared page in turn, the j-th finds refs - j tables naming it.  A chain of loads
 // and sums: 64 sequences of 31 pages XX us, of which the launch is 2.
 template <int kBlock>
@@ -141,6 +173,8 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTable
   __shared__ int copy[kMost];     // its place in the list, or -1
   __shared__ int first[kMost];    // its first new column
   __shared__ int64_t off[kMost];
+  __shared__ uint32_t word[kWords * kBlock];  // free pages of a round's words
+  __shared__ int word_at[kWords * kBlock];    // and how many lie before each
   __shared__ int64_t part[kBlock / 64];
   __shared__ int listed;
   const int n = t.n_seq, tid = int(threadIdx.x);
@@ -219,36 +253,67 @@ __global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTable
 #pragma unroll
     for (int i = 0; i < kWords; i++) count += __builtin_popcount(free[i]);
     int64_t found;
-    int64_t rank = base + scan<kBlock>(count, part, found);
+    const int64_t rank = base + scan<kBlock>(count, part, found);
+    int64_t before = rank;
 #pragma unroll
     for (int i = 0; i < kWords; i++) {
-      const int64_t w = w0 + tid * per + i;
-      uint32_t left = free[i];
-      while (left != 0 && rank < total) {
-        const int bit = __builtin_ctz(left), id = int(32 * w) + bit;
-        left &= left - 1;
-        int lo = 0, hi = n;  // off[lo] <= rank < off[hi]
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) / 2;
-          if (off[mid] <= rank) lo = mid;
-          else hi = mid;
+      if (i >= per) continue;
+      word[tid * per + i] = free[i];
+      word_at[tid * per + i] = int(before - base);
+      const int have = __builtin_popcount(free[i]);
+      if (before < total && have > 0) {
+        // the lowest of the word's free pages are taken, all of them but in the last word
+        uint32_t left = 0;
+        if (before + have > total) {
+          left = free[i];
+          for (int64_t r = before; r < total; r++) left &= left - 1;
         }
-        const int which = int(rank - off[lo]);
-        int32_t *row = t.pages + lo * t.stride;
-        const int c = copy[lo];
-        if (c >= 0 && which == 0) {
-          row[first[lo] - 1] = id;
-          moves.src[c] = tail[lo];
-          moves.dst[c] = id;
-          atomicAdd(&listed, 1);
-        } else {
-          row[first[lo] + which - (c >= 0 ? 1 : 0)] = id;
-        }
-        pool.refs[id] = 1;
-        rank++;
+        const int64_t w = w0 + tid * per + i;
+        pool.used[w] = used_word(pool, w, false) | (free[i] & ~left);
       }
-      if (left != free[i]) pool.used[w] = used_word(pool, w, false) | (free[i] & ~left);
+      before += have;
     }
+    __syncthreads();
+    // a thread a page
+    for (int64_t r = base + tid; r < min(base + found, total); r += kBlock) {
+      int at = 0, end = kBlock * per;  // word_at[at] <= r - base < word_at[end]
+      while (end - at > 1) {
+        const int mid = (at + end) / 2;
+        if (word_at[mid] <= int(r - base)) at = mid;
+        else end = mid;
+      }
+      uint32_t left = word[at];
+      int bit = 0, nth = int(r - base) - word_at[at];  // the nth bit that is set
+#pragma unroll
+      for (int half = 16; half >= 1; half /= 2) {
+        const int low = __builtin_popcount(left & ((1u << half) - 1));
+        if (nth >= low) {
+          nth -= low;
+          left >>= half;
+          bit += half;
+        }
+      }
+      const int id = int(32 * (w0 + at)) + bit;
+      int lo = 0, hi = n;  // off[lo] <= r < off[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (off[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      const int which = int(r - off[lo]);
+      int32_t *row = t.pages + lo * t.stride;
+      const int c = copy[lo];
+      if (c >= 0 && which == 0) {
+        row[first[lo] - 1] = id;
+        moves.src[c] = tail[lo];
+        moves.dst[c] = id;
+        atomicAdd(&listed, 1);
+      } else {
+        row[first[lo] + which - (c >= 0 ? 1 : 0)] = id;
+      }
+      pool.refs[id] = 1;
+    }
+    __syncthreads();
     base += found;
   }
   // what no page was left for
@@ -340,40 +405,70 @@ __global__ void __launch_bounds__(kListBlock) compact_list_kernel(PagePool pool,
   if (tid == 0) *moves.count = int(min(high, int64_t(moves.cap)));
 }
 
-// Counts of the pages that move, and a row's entries: where the list, which rises,
-// holds an entry as a source it becomes the place it moves to (found by bisection,
-// among every step-th source in LDS first).
+// Counts of the pages that move (the last layer of workgroups), and the rows' entries
+// (a workgroup a row and layer): where the list, which rises,
+// holds an entry as a source it becomes the place it moves to, found by bisection.  Lists
+// of up to 2048 lie in LDS whole; of longer ones every step-th source does.
 constexpr int kProbes = 2048;
 __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTables t,
                                                            PageMoves moves) {
-  __shared__ int probe[kProbes];
+  __shared__ int probe[kProbes], place[kProbes];
+  const int s = int(blockIdx.x), tid = int(threadIdx.x);
+  // (loads are on their way before the list's length is known; what lies behind it is not
+  // used)
+  if (blockIdx.y == gridDim.y - 1) {  // counts
+    int64_t i = int64_t(s) * 256 + tid;
+    int a = i < moves.cap ? moves.src[i] : -1, b = i < moves.cap ? moves.dst[i] : -1;
+    int refs = page_ok(a, pool.n_pages) ? pool.refs[a] : 0;
+    for (const int n = *moves.count; i < n;) {
+      pool.refs[b] = refs;
+      pool.refs[a] = 0;
+      atomicAnd(&pool.used[a / 32], ~(1u << (a % 32)));
+      atomicOr(&pool.used[b / 32], 1u << (b % 32));
+      i += int64_t(gridDim.x) * 256;
+      if (i >= n) break;
+      a = moves.src[i];
+      b = moves.dst[i];
+      refs = pool.refs[a];
+    }
+    return;
+  }
+  int src[kProbes / 256], dst[kProbes / 256], id = -1;
+#pragma unroll
+  for (int j = 0; j < kProbes / 256; j++) {
+    const int i = 256 * j + tid;
+    src[j] = i < moves.cap ? moves.src[i] : 0;
+    dst[j] = i < moves.cap ? moves.dst[i] : 0;
+  }
+  const int64_t first = int64_t(blockIdx.y) * 256 + tid;
+  if (s < t.n_seq && first < t.stride) id = t.pages[s * t.stride + first];
+  const int64_t cols = s < t.n_seq ? held_cols(t.len[s], pool.shift, t.stride) : 0;
   const int n = *moves.count;
   if (n == 0) return;
   const int step = (n + kProbes - 1) / kProbes, probes = (n + step - 1) / step;
-  const int64_t threads = int64_t(gridDim.x) * gridDim.y * 256;
-  const int64_t me = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
-  for (int64_t i = me; i < n; i += threads) {
-    const int a = moves.src[i], b = moves.dst[i];
-    pool.refs[b] = pool.refs[a];
-    pool.refs[a] = 0;
-    atomicAnd(&pool.used[a / 32], ~(1u << (a % 32)));
-    atomicOr(&pool.used[b / 32], 1u << (b % 32));
-  }
-  const int s = int(blockIdx.x);
-  if (s >= t.n_seq) return;
-  const int64_t cols = held_cols(t.len[s], pool.shift, t.stride);
   if (int64_t(blockIdx.y) * 256 >= cols) return;
-  for (int i = int(threadIdx.x); i < probes; i += 256) probe[i] = moves.src[int64_t(i) * step];
+  if (step == 1) {
+#pragma unroll
+    for (int j = 0; j < kProbes / 256; j++) {
+      probe[256 * j + tid] = src[j];
+      place[256 * j + tid] = dst[j];
+    }
+  } else {
+    for (int i = tid; i < probes; i += 256) probe[i] = moves.src[int64_t(i) * step];
+  }
   __syncthreads();
-  const int from = probe[0], to = moves.src[n - 1];
-  for (int64_t c = int64_t(blockIdx.y) * 256 + threadIdx.x; c < cols; c += int64_t(gridDim.y) * 256) {
-    const int id = t.pages[s * t.stride + c];
-    if (id < from || id > to) continue;
+  for (int64_t c = first; c < cols; c += int64_t(gridDim.y - 1) * 256) {
+    if (c != first) id = t.pages[s * t.stride + c];
+    if (id < probe[0]) continue;
     int lo = 0, hi = probes;  // probe[lo] <= id < probe[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (probe[mid] <= id) lo = mid;
       else hi = mid;
+    }
+    if (step == 1) {
+      if (probe[lo] == id) t.pages[s * t.stride + c] = place[lo];
+      continue;
     }
     int64_t a = int64_t(lo) * step, b = min(a + step, int64_t(n));
     while (b - a > 1) {
@@ -381,7 +476,7 @@ __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTa
       if (moves.src[mid] <= id) a = mid;
       else b = mid;
     }
-    if ((step == 1 ? probe[lo] : moves.src[a]) == id) t.pages[s * t.stride + c] = moves.dst[a];
+    if (moves.src[a] == id) t.pages[s * t.stride + c] = moves.dst[a];
   }
 }
 
@@ -436,12 +531,17 @@ int launched() { return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUN
 int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int32_t *d_parent,
                             hipStream_t s) {
   const size_t lds = size_t(t.n_seq) * (kTile + 3) * 4;
+  const int64_t tiles = std::max<int64_t>(1, (t.stride + kTile - 1) / kTile);
+  // (two tiles in turn take 9.4 us, in two launches 8)
+  if (tiles <= 1 && t.n_seq <= 256 && pool.n_pages <= 8192) {
+    fork_kernel<true><<<1, 256, lds, s>>>(pool, t, d_parent);
+    return launched();
+  }
   if (lds > 64 * 1024 &&
-      hipFuncSetAttribute(reinterpret_cast<const void *>(&fork_tables_kernel),
+      hipFuncSetAttribute(reinterpret_cast<const void *>(&fork_kernel<false>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)) != hipSuccess)
     return SWAMP_ELAUNCH;
-  const int64_t tiles = std::max<int64_t>(1, (t.stride + kTile - 1) / kTile);
-  fork_tables_kernel<<<unsigned(std::min<int64_t>(tiles, 1024)), 256, lds, s>>>(pool, t, d_parent);
+  fork_kernel<false><<<unsigned(std::min<int64_t>(tiles, 1024)), 256, lds, s>>>(pool, t, d_parent);
   const unsigned blocks = unsigned(std::max<int64_t>(1, (int64_t(pool.n_pages) + 255) / 256));
   fork_finish_kernel<<<blocks, 256, 0, s>>>(pool, t, d_parent);
   return launched();
@@ -469,7 +569,7 @@ int swamp_launch_pages_compact(const PagePool &pool, const PageTables &t, const 
                                hipStream_t s) {
   compact_list_kernel<<<1, kListBlock, 0, s>>>(pool, moves);
   const dim3 grid(unsigned(std::max(t.n_seq, 64)),
-                  unsigned(std::max<int64_t>(1, std::min<int64_t>(t.stride / 256, 16))));
+                  unsigned(1 + std::max<int64_t>(1, std::min<int64_t>(t.stride / 256, 16))));
   compact_move_kernel<<<grid, 256, 0, s>>>(pool, t, moves);
   return launched();
 }
