@@ -52,7 +52,7 @@ struct Work {
   Part *part;    // [row][chunk]
 };
 
-// Floats in the order of their keys (NaN: as -infinity, it takes its row with it).
+// Floats in the order of their keys (-0 below 0: 0 is added where that counts).
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -61,6 +61,15 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 constexpr uint32_t kNone = 0x007FFFFFu;  // key of -infinity
+
+// x, which the compiler no longer knows: what a rare path computes from it is not kept in
+// registers meanwhile.
+__device__ __forceinline__ float fresh(float x) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
 
 // 2^t for t of any size; NaN passes, and t far below 0 gives 0.
 __device__ __forceinline__ double exp2_64(double t) {
@@ -98,11 +107,11 @@ struct Chunk {
       if (first + kPer <= n) {
         const Vec<XT> v = *reinterpret_cast<const Vec<XT> *>(row + first);
 #pragma unroll
-        for (int i = 0; i < kPer; i++) x[j * kPer + i] = float(v.v[i]) + 0.f;  // -0 counts as 0
+        for (int i = 0; i < kPer; i++) x[j * kPer + i] = float(v.v[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; i++)
-          x[j * kPer + i] = first + i < n ? float(row[first + i]) + 0.f : -INFINITY;
+          x[j * kPer + i] = first + i < n ? float(row[first + i]) : -INFINITY;
       }
     }
   }
@@ -151,7 +160,7 @@ __device__ __forceinline__ uint32_t joint_bound(const uint32_t *all, const uint3
   return max(a, q);
 }
 template <typename XT>
-__global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
+__global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
   typedef Chunk<XT> C;
   __shared__ uint64_t list[kList];  // key, then place from the end
   __shared__ float tops[kWaves];
@@ -199,16 +208,29 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
     for (int e = 0; e < kEach; e++)
       if (x[e] >= least) {
         const int i = atomicAdd(&listed, 1);
-        if (i < kList) list[i] = uint64_t(key_of(x[e])) << 32 | uint32_t(~C::at(e));
+        if (i < kList) list[i] = uint64_t(key_of(x[e] + 0.f)) << 32 | uint32_t(~C::at(e));
       }
   }
-  // (a chunk of nothing but -infinity: 0; an infinity: NaN, of -inf - -inf)
+  // (a chunk of nothing but -infinity: 0; an infinity: NaN, of inf - inf)
   const double base = top == -INFINITY ? 0.0 : double(top);
   double sum = 0.0;
+  float low = x[0];
 #pragma unroll
-  for (int e = 0; e < kEach; e++) {
-    const float a = x[e] == -INFINITY ? kLowest : x[e];
-    sum += exp2_64((double(a) - base) * kLog2e64);
+  for (int e = 1; e < kEach; e++) low = fminf(low, x[e]);
+  if (__any(low == -INFINITY)) {  // masked tokens: no work where all of the wave's are
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+      if (__any(x[e] != -INFINITY)) {
+        __builtin_amdgcn_sched_barrier(0);
+        const float a = x[e] == -INFINITY ? kLowest : x[e];
+        sum += exp2_64((double(a) - base) * kLog2e64);
+      }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+      sum += exp2_64((double(x[e]) - base) * kLog2e64);
+    }
   }
   sum = wave_sum64(sum);
   if ((tid & 63) == 0) sums[wave] = sum;
@@ -222,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
       int reach = 0;
 #pragma unroll
       for (int e = 0; e < kEach; e++) {
-        const uint32_t key = key_of(fmaxf(x[e], -INFINITY));
+        const uint32_t key = key_of(fmaxf(fresh(x[e]), -INFINITY) + 0.f);
         const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e));
         reach += __builtin_popcountll(__ballot(key > kNone && place >= up));
       }
@@ -238,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Work w) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
-      const uint32_t key = key_of(fmaxf(x[e], -INFINITY));
+      const uint32_t key = key_of(fmaxf(fresh(x[e]), -INFINITY) + 0.f);
       const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e));
       if (key > kNone && place >= t)
         list[atomicAdd(&listed, 1)] = uint64_t(key) << 32 | uint32_t(~C::at(e));
