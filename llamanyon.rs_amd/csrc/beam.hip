@@ -12,13 +12,18 @@
 // it): 16 operations of 64 bits an element, which the vector units issue at the rate of
 // 32-bit ones.
 //
-// Largest tokens without a sort: a wave's lanes each have a largest value (of each four
-// of theirs, where n_out is large), and the n_out-th largest of those, found bit by bit
-// with ballots, has n_out values at or above it in the chunk.  What reaches the largest
-// of the four waves' bounds, a few times n_out tokens, is collected in LDS and ranked by
-// counting.  Where too many do (equal logits) the exact bound is found bit by bit over
-// the whole chunk.  The lists of a sequence are cut alike: n_out / r lists whose r-th
-// token reaches a bound have n_out tokens that do.
+// Largest tokens without a sort: a wave's lanes each have a largest value.  Where a quarter
+// of n_out of every wave's reach a bound (found bit by bit with ballots), or n_out of one
+// wave's do, so do n_out values of the chunk.  What reaches it, little more than n_out
+// tokens, is collected in LDS and ranked by counting.  Where too many do (equal logits) the
+// exact bound is found bit by bit over the whole chunk.  The lists of a sequence are cut
+// alike: n_out / r lists whose r-th token reaches a bound have n_out tokens that do.
+//
+// Measured, the two kernels: 4 beams of 128256 f32 logits, 8 best, 5.9 + 6.6 us; 16 x 4 of
+// them 14.0 + 6.7 (2.3 TB/s in the first); 4 x 32 of 32000 bf16, 64 best, 14.4 + 15.8; 50 x 5
+// of 50257 f16, nearly all masked, 14.8 + 7.6.  The first is bound by the ballots of its
+// bounds and the 64-bit polynomial, the second by its chain of steps in one workgroup (sums
+// 2.3 us, bound 2, collection 1, ranks 1).
 #include "swamp_common.hpp"
 
 #include <type_traits>
@@ -64,7 +69,8 @@ constexpr uint32_t kNone = 0x007FFFFFu;  // key of -infinity
 
 // x, which the compiler no longer knows: what a rare path computes from it is not kept in
 // registers meanwhile.
-__device__ __forceinline__ float fresh(float x) {
+template <typename T>
+__device__ __forceinline__ T fresh(T x) {
 #ifdef __HIP_DEVICE_COMPILE__
   asm volatile("" : "+v"(x));
 #endif
@@ -93,26 +99,25 @@ struct __attribute__((packed, aligned(sizeof(XT)))) Vec {
   XT v[16 / sizeof(XT)];
 };
 
-// The chunk's elements: load j of a thread holds kPer neighbours.
+// The chunk's elements: load j of a thread holds kPer neighbours; of a row's last chunk,
+// which is short, every thread has one of each 256, so that all waves have their share.
 template <typename XT>
 struct Chunk {
   static constexpr int kPer = 16 / int(sizeof(XT)), kLoads = kEach / kPer;
-  static __device__ __forceinline__ int at(int e) {
-    return (e / kPer) * kThreads * kPer + int(threadIdx.x) * kPer + e % kPer;
+  static __device__ __forceinline__ int at(int e, bool whole, int tid = int(threadIdx.x)) {
+    return whole ? (e / kPer) * kThreads * kPer + tid * kPer + e % kPer : e * kThreads + tid;
   }
-  static __device__ __forceinline__ void load(const XT *row, int n, float *x) {
+  static __device__ __forceinline__ void load(const XT *row, int n, bool whole, float *x) {
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < kLoads; j++) {
-      const int first = at(j * kPer);
-      if (first + kPer <= n) {
-        const Vec<XT> v = *reinterpret_cast<const Vec<XT> *>(row + first);
+      for (int j = 0; j < kLoads; j++) {
+        const Vec<XT> v = *reinterpret_cast<const Vec<XT> *>(row + at(j * kPer, true));
 #pragma unroll
         for (int i = 0; i < kPer; i++) x[j * kPer + i] = float(v.v[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; i++)
-          x[j * kPer + i] = first + i < n ? float(row[first + i]) : -INFINITY;
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEach; e++) x[e] = at(e, false) < n ? float(row[at(e, false)]) : -INFINITY;
     }
   }
 };
@@ -127,13 +132,12 @@ __device__ __forceinline__ double wave_sum64(double x) {
   for (int d = 32; d >= 1; d /= 2) x += __shfl_xor(x, d, 64);
   return x;
 }
-// Keys that at least k, and at least its share of k, of the wave's 64 N reach (of W
-// waves): the largest such but for their low bits.
-template <int W, int N, int kLow>
-__device__ __forceinline__ void reached_by(const uint32_t *keys, int k, uint32_t &all,
+// Keys that at least k, and at least `few` (k over the waves), of the wave's 64 N reach:
+// the largest such but for their low bits.
+template <int N, int kLow>
+__device__ __forceinline__ void reached_by(const uint32_t *keys, int k, int few, uint32_t &all,
                                            uint32_t &share) {
   all = share = 0;
-  const int few = (k + W - 1) / W;
 #pragma unroll
   for (int bit = 31; bit >= kLow; bit--) {
     const uint32_t up = all | 1u << bit, up1 = share | 1u << bit;
@@ -159,41 +163,32 @@ __device__ __forceinline__ uint32_t joint_bound(const uint32_t *all, const uint3
   }
   return max(a, q);
 }
+
 template <typename XT>
 __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
   typedef Chunk<XT> C;
   __shared__ uint64_t list[kList];  // key, then place from the end
+  __shared__ int16_t kept[kList];
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
   __shared__ uint32_t bounds[kWaves], shares[kWaves];
-  __shared__ int listed, counts[kWaves];
+  __shared__ int listed, left, counts[kWaves];
   const int row = int(blockIdx.x / uint32_t(w.chunks)), chunk = int(blockIdx.x % uint32_t(w.chunks));
   if (w.c.done && w.c.done[row]) return;
   const int tid = int(threadIdx.x), wave = tid >> 6, k = w.c.n_out;
   const int first = chunk * kChunk, n = min(w.c.vocab - first, kChunk);
+  const bool whole = n == kChunk;
   float x[kEach];
-  C::load(static_cast<const XT *>(w.c.logits) + row * w.c.stride + first, n, x);
-  if (tid == 0) listed = 0;
-  constexpr int kGroups = kEach / 4;
-  float group[kGroups];
+  C::load(static_cast<const XT *>(w.c.logits) + row * w.c.stride + first, n, whole, x);
+  if (tid == 0) listed = left = 0;
+  float mine = -INFINITY;  // (and for NaN)
 #pragma unroll
-  for (int i = 0; i < kGroups; i++)  // (-infinity for NaN)
-    group[i] = fmaxf(fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3])), -INFINITY);
-  float mine = group[0];
-#pragma unroll
-  for (int i = 1; i < kGroups; i++) mine = fmaxf(mine, group[i]);
+  for (int e = 0; e < kEach; e++) mine = fmaxf(mine, x[e]);
   float top = wave_max(mine);
-  // n_out of one wave's reach the one bound, a quarter of them of every wave's the other
+  // n_out of one wave's lanes reach the one bound, a quarter of them of every wave's the other
   uint32_t bound, share;
-  if (k <= 16) {
-    const uint32_t key = key_of(mine);
-    reached_by<kWaves, 1, 16>(&key, k, bound, share);
-  } else {
-    uint32_t tops4[kGroups];
-#pragma unroll
-    for (int i = 0; i < kGroups; i++) tops4[i] = key_of(group[i]);
-    reached_by<kWaves, kGroups, 13>(tops4, k, bound, share);
-  }
+  const uint32_t key = key_of(mine);
+  reached_by<1, 15>(&key, k, (k + kWaves - 1) / kWaves, bound, share);
   if ((tid & 63) == 0) {
     tops[wave] = top;
     bounds[wave] = bound;
@@ -208,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
     for (int e = 0; e < kEach; e++)
       if (x[e] >= least) {
         const int i = atomicAdd(&listed, 1);
-        if (i < kList) list[i] = uint64_t(key_of(x[e] + 0.f)) << 32 | uint32_t(~C::at(e));
+        if (i < kList)
+          list[i] = uint64_t(key_of(x[e] + 0.f)) << 32 | uint32_t(~C::at(e, whole, fresh(tid)));
       }
   }
   // (a chunk of nothing but -infinity: 0; an infinity: NaN, of inf - inf)
@@ -245,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
 #pragma unroll
       for (int e = 0; e < kEach; e++) {
         const uint32_t key = key_of(fmaxf(fresh(x[e]), -INFINITY) + 0.f);
-        const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e));
+        const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e, whole, fresh(tid)));
         reach += __builtin_popcountll(__ballot(key > kNone && place >= up));
       }
       __syncthreads();
@@ -261,21 +257,48 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
       const uint32_t key = key_of(fmaxf(fresh(x[e]), -INFINITY) + 0.f);
-      const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e));
+      const uint64_t place = uint64_t(key) << 12 | uint32_t(kChunk - 1 - C::at(e, whole, fresh(tid)));
       if (key > kNone && place >= t)
-        list[atomicAdd(&listed, 1)] = uint64_t(key) << 32 | uint32_t(~C::at(e));
+        list[atomicAdd(&listed, 1)] = uint64_t(key) << 32 | uint32_t(~C::at(e, whole, fresh(tid)));
     }
     __syncthreads();
     c = listed;
   }
   const int64_t at = int64_t(row) * w.chunks + chunk;
   Entry *out = w.list + at * w.pad;
-  for (int i = tid; i < c; i += kThreads) {
-    const uint64_t me = list[i];
-    int rank = 0;
+  auto rank_all = [&](int n, auto at) {
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t me = list[at(i)];
+      int rank = 0;
 #pragma unroll 8
-    for (int o = 0; o < c; o++) rank += list[o] > me ? 1 : 0;
-    if (rank < k) out[rank] = Entry{value_of(uint32_t(me >> 32)), first + int(~uint32_t(me))};
+      for (int o = 0; o < n; o++) rank += list[at(o)] > me ? 1 : 0;
+      if (rank < k) out[rank] = Entry{value_of(uint32_t(me >> 32)), first + int(~uint32_t(me))};
+    }
+  };
+  if (c <= 256) {
+    rank_all(c, [](int i) { return i; });
+  } else {
+    // a bound again, of all that is listed.  Up to 256 every thread ranks at most one: 4 x 32
+    // beams of 32000 bf16 logits, 64 best, take 29 us in both kernels, 33 if the bound is
+    // renewed from 97 on, and 4 of 128256, 8 best, 13 and, if it always is, 16.
+    constexpr int kEachLane = kList / kThreads;
+    uint32_t some[kEachLane], all, part;
+#pragma unroll
+    for (int i = 0; i < kEachLane; i++) {
+      const int from = (64 * i + (tid & 63)) * kWaves + wave;
+      some[i] = from < c ? uint32_t(list[from] >> 32) : 0;
+    }
+    reached_by<kEachLane, 8>(some, k, (k + kWaves - 1) / kWaves, all, part);
+    if ((tid & 63) == 0) {
+      bounds[wave] = all;
+      shares[wave] = part;
+    }
+    __syncthreads();
+    const uint32_t enough = joint_bound<kWaves>(bounds, shares);
+    for (int i = tid; i < c; i += kThreads)
+      if (uint32_t(list[i] >> 32) >= enough) kept[atomicAdd(&left, 1)] = int16_t(i);
+    __syncthreads();
+    rank_all(left, [&](int i) { return int(kept[i]); });
   }
   for (int i = min(c, k) + tid; i < w.pad; i += kThreads) out[i] = Entry{0.f, -1};
   if (tid == 0) {
@@ -353,7 +376,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
   // (on their way while the sums are joined) the first, 4th, 16th, 64th of a list
   constexpr int kProbes = 4;
   Entry probe[kProbes];
-  const Entry *mine_at = list_of(w, seq, min(tid, lists - 1));
+  // `full` waves have 64 lists or more and take them in turn, so that none has but one
+  // beam's; another wave may have a few
+  const int full = min(max(lists / 64, 1), kJoinWaves);
+  const int mine = wave < full ? lane * full + wave : tid;
+  const Entry *mine_at = list_of(w, seq, min(mine, lists - 1));
 #pragma unroll
   for (int i = 0; i < kProbes; i++) probe[i] = mine_at[min((1 << 2 * i) - 1, k - 1)];
   // `team` lanes take a beam's chunks
@@ -366,9 +393,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     const Part *part = w.part + row * w.chunks;
     const bool ended = w.c.done && w.c.done[row];
     const double score = double(w.c.score[row]);
-    Part mine = part[min(at, w.chunks - 1)];
-    if (ended || at >= w.chunks) mine = Part{0.0, -INFINITY, 0.f};
-    float top = mine.top;
+    Part own = part[min(at, w.chunks - 1)];
+    if (ended || at >= w.chunks) own = Part{0.0, -INFINITY, 0.f};
+    float top = own.top;
     if (!ended)
       for (int i = at + 64; i < w.chunks; i += 64) top = fmaxf(top, part[i].top);
     for (int d = team / 2; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
@@ -378,7 +405,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
       const float a = p.top == -INFINITY ? kLowest : p.top;
       return p.sum * exp2_64((double(a) - base) * kLog2e64);
     };
-    double sum = term(mine);
+    double sum = term(own);
     if (!ended)
       for (int i = at + 64; i < w.chunks; i += 64) sum += term(part[i]);
     for (int d = team / 2; d >= 1; d /= 2) sum += __shfl_xor(sum, d, 64);
@@ -396,19 +423,21 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     const int r = 1 << 2 * i;
     if (r > k) break;
     uint32_t key = 0;
-    if (tid < lists) {
-      const int b = tid / w.chunks;
-      key = bound_key(best_of(w, rows[b], b, tid, r - 1, probe[i]));
+    if (mine < lists) {
+      const int b = mine / w.chunks;
+      key = bound_key(best_of(w, rows[b], b, mine, r - 1, probe[i]));
     }
-    for (int l = tid + kJoinThreads; l < lists; l += kJoinThreads) {
+    for (int l = mine + kJoinThreads; l < lists; l += kJoinThreads) {
       const int b = l / w.chunks;
       key = max(key, bound_key(best_of(w, rows[b], b, l, r - 1, list_of(w, seq, l)[r - 1])));
     }
     uint32_t all, quarter;
-    reached_by<kJoinWaves, 1, 14>(&key, (k + r - 1) / r, all, quarter);
+    const int need = (k + r - 1) / r;
+    reached_by<1, 14>(&key, need, (need + full - 1) / full, all, quarter);
     bound = max(bound, all);
     share = max(share, quarter);
   }
+  if (wave >= full) share = ~0u;
   if (lane == 0) {
     bounds[wave] = bound;
     shares[wave] = share;
@@ -456,19 +485,26 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
         if (rank < k) picked[rank] = Best{total_of(me.key), me.flat};
       }
     };
-    if (c <= 96) {
+    if (c <= 256) {
       rank_all(c, [](int i) { return i; });
     } else {
-      // a bound again, of all that is listed (every wave looks for it): 445 of which 64
-      // are wanted take 10 us with it and 30 without, 9 of which 8 are 4 and 1
-      constexpr int kEachLane = 8;
-      least = 0;
-      if (c <= 64 * kEachLane) {
-        uint32_t mine[kEachLane], unused;
+      // a bound again, of all that is listed: 3 x 28 beams of 99882 bf16 logits, 56 best, take
+      // 33.5 us in both kernels without it and 36 with it from 97 on; 7 x 63 beams of 20764,
+      // 64 best, 41 with it and 42 without.
+      constexpr int kEachLane = kJoin / kJoinThreads;
+      uint32_t some[kEachLane], all, part;
 #pragma unroll
-        for (int i = 0; i < kEachLane; i++) mine[i] = 64 * i + lane < c ? keys[64 * i + lane] : 0;
-        reached_by<1, kEachLane, 8>(mine, k, least, unused);
+      for (int i = 0; i < kEachLane; i++) {
+        const int at = (64 * i + lane) * kJoinWaves + wave;
+        some[i] = at < c ? keys[at] : 0;
       }
+      reached_by<kEachLane, 8>(some, k, (k + kJoinWaves - 1) / kJoinWaves, all, part);
+      if (lane == 0) {
+        bounds[wave] = all;
+        shares[wave] = part;
+      }
+      __syncthreads();
+      least = joint_bound<kJoinWaves>(bounds, shares);
       for (int i = tid; i < c; i += kJoinThreads)
         if (keys[i] >= least) kept[atomicAdd(&left, 1)] = int16_t(i);
       __syncthreads();
@@ -490,9 +526,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
       }
       return best;
     };
-    Best mine = first();
+    Best head = first();
     for (int r = 0; r < k; r++) {
-      const Best top = wave_best(mine);
+      const Best top = wave_best(head);
       __syncthreads();
       if (lane == 0) waves[wave] = top;
       __syncthreads();
@@ -501,9 +537,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
       for (int i = 1; i < kJoinWaves; i++)
         if (before(waves[i], best)) best = waves[i];
       if (tid == 0) picked[r] = best;
-      if (best.flat >= 0 && mine.flat == best.flat) {
+      if (best.flat >= 0 && head.flat == best.flat) {
         next[from]++;
-        mine = first();
+        head = first();
       }
     }
   }
