@@ -161,9 +161,9 @@ constexpr int kWords = 2;  // of a thread in a round, at most
 // ---- extend ---------------------------------------------------------------
 // One workgroup: what every sequence needs (two a thread), where its pages begin in
 // the row of all pages handed out, then one pass over the free pages in rising
-// order: a thread a page, which finds the page's word and its owner by bisection.  Of the h sequences that would write
-// one shared page in turn, the j-th finds refs - j tables naming it.  A chain of loads
-// and sums: 64 sequences of 31 pages XX us, of which the launch is 2.
+// order: a thread a page, which finds the page's word and its owner by bisection.  Of the h
+// sequences that would write one shared page in turn, the j-th finds refs - j tables naming
+// it.  A chain of loads and sums: 64 sequences of 31 pages take 7.3 us.
 template <int kBlock>
 __global__ void __launch_bounds__(kBlock) extend_kernel(PagePool pool, PageTables t,
                                                         const int32_t *__restrict__ d_new,
@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(kListBlock) compact_list_kernel(PagePool pool,
 }
 
 // Counts of the pages that move (the last layer of workgroups), and the rows' entries
-// (a workgroup a row and layer): where the list, which rises,
-// holds an entry as a source it becomes the place it moves to, found by bisection.  Lists
-// of up to 2048 lie in LDS whole; of longer ones every step-th source does.
+// (a workgroup a row and layer): where the list, which rises, holds an entry as a source it
+// becomes the place it moves to, found by bisection.  Lists of up to 2048 lie in LDS whole;
+// of longer ones every step-th source does.
 constexpr int kProbes = 2048;
 __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTables t,
                                                            PageMoves moves) {
@@ -532,8 +532,10 @@ int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int
                             hipStream_t s) {
   const size_t lds = size_t(t.n_seq) * (kTile + 3) * 4;
   const int64_t tiles = std::max<int64_t>(1, (t.stride + kTile - 1) / kTile);
-  // (two tiles in turn take 9.4 us, in two launches 8)
-  if (tiles <= 1 && t.n_seq <= 256 && pool.n_pages <= 8192) {
+  // Two launches take 5.5 to 8 us (64 sequences 8).  One takes 3.4, 0.6 a thousand pages and,
+  // a tile, 0.5 and 0.04 a sequence: 4 sequences of 30 pages among 512 take 4.8 us in one and
+  // 6.4 in two, 64 of 30 among 2048 10.2 and 8.4, 4 of 8 among 8192 9.3 and 6.0.
+  if (pool.n_pages / 1024 + tiles * (16 + t.n_seq) / 32 <= 4 && t.n_seq <= 256) {
     fork_kernel<true><<<1, 256, lds, s>>>(pool, t, d_parent);
     return launched();
   }
