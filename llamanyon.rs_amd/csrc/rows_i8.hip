@@ -487,9 +487,18 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
 // by T times 16 of x.  A workgroup's waves take a share of the columns each, so that a
 // short matrix has all its bytes in flight at once, and their sums meet in LDS.  What of
 // x lies behind column K is cleared, rows behind the last are the descriptor's zeros.
+// One row of 6144 x 4096: 7.6 us, 5.0 of them its bytes; 32 rows 10.4 (5.1); 64 rows of 4096 x
+// 4096 11.9 (3.6): there every workgroup's own reading of x, 16 codes a lane and product.
+//
+// Waves and steps in flight are what the registers hold: 16 of 128 each, or 8 of 256.
 template <int R, int T>
-__global__ void __launch_bounds__(1024) few_kernel(GemmI8Call c) {
-  constexpr int U = 4 / (R * T > 2 ? 2 : 1);  // steps in flight, and as many to come
+struct Few {
+  static constexpr int kWaves = R * T >= 8 ? 8 : 16;
+  static constexpr int U = R * T <= 2 || (R == 4 && T == 2) ? 4 : 2;  // and as many to come
+};
+template <int R, int T>
+__global__ void __launch_bounds__((64 * Few<R, T>::kWaves)) few_kernel(GemmI8Call c) {
+  constexpr int U = Few<R, T>::U;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   int32_t *parts = reinterpret_cast<int32_t *>(smem);
   const int lane = int(threadIdx.x) & 63, r = lane & 15, h = lane >> 4;
@@ -516,18 +525,19 @@ __global__ void __launch_bounds__(1024) few_kernel(GemmI8Call c) {
   };
   auto load = [&](Stage &st, int s) {
     if (s >= s1) return;
+    // (a row's steps one after another: two are a cache line)
+    auto from = [&](const __amdgpu_buffer_rsrc_t &rsrc, uint32_t at, int u) {
+      return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                           rsrc, at, uint32_t(min(s + u, s1 - 1)) * 64u, 0));
+    };
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t at = uint32_t(min(s + u, s1 - 1)) * 64u;
+    for (int i = 0; i < R; i++)
 #pragma unroll
-      for (int i = 0; i < R; i++)
-        st.w[u][i] = __builtin_bit_cast(
-            i32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wv[i], at, 0));
+      for (int u = 0; u < U; u++) st.w[u][i] = from(wr, wv[i], u);
 #pragma unroll
-      for (int j = 0; j < T; j++)
-        st.x[u][j] = __builtin_bit_cast(
-            i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xv[j], at, 0));
-    }
+    for (int j = 0; j < T; j++)
+#pragma unroll
+      for (int u = 0; u < U; u++) st.x[u][j] = from(xr, xv[j], u);
   };
   auto multiply = [&](Stage &st, int s) {
 #pragma unroll
@@ -600,9 +610,9 @@ __global__ void __launch_bounds__(256) nothing_kernel(GemmI8Call c) {
 // both sides of 171 sizes (1 to 1024 rows of x, 640 to 28672 of w, 512 to 14336 columns)
 // measured in up to 40 ways.  A round of tiles costs a tile's filling and storing and its
 // steps, a last one that does not fill the CUs 0.7 of that and the rest by its share; pieces
-// cost their sums' writing and reading.  Of 144 sizes above 16 rows the choice is 1.4%
-// slower than the fastest on average, 23% at worst but for one (192 x 16384 x 512, 17.3 us
-// for 11.4).
+// cost their sums' writing and reading.  Of 144 sizes above 16 rows the choice among tiles
+// is 1.4% slower than the fastest on average, 23% at worst but for one (192 x 16384 x 512,
+// 17.3 us for 11.4).
 struct Tiles {
   int tm, tn;
   double step, fixed;  // us
@@ -619,16 +629,25 @@ struct Plan {
 Plan plan_of(int m, int n, int k) {
   const int cus = swamp::device_info().num_cus, KT = (k + 63) / 64;
   Plan best{-1, 1, 1, 1, KT};
-  // Up to 16 rows: as few workgroups as one round takes (one row of 6144 x 4096: 7.3 us
-  // with two tiles of 16 a workgroup, 9.6 with one, 10.5 with four).  Up to 32, where the
-  // round holds them and the columns are few enough for every wave's x: 8.8 us at 17 rows,
-  // where 64 x 128 tiles take 11.3 (4096 x 14336: 20 and 17).
-  if (m <= 16) {
-    while (best.tiles_n < 4 && (n + 16 * best.tiles_n - 1) / (16 * best.tiles_n) > cus)
-      best.tiles_n *= 2;
+  // Up to 64 rows, where one round of few_kernel's workgroups takes all of w: the smallest of
+  // them that do (one row of 6144 x 4096: 7.6 us with two tiles of 16 a workgroup, 9.5 with
+  // one, 10.6 with four).  The limits are where tiles overtake it, us here and there:
+  //   m      n x k          here  tiles        n x k          here  tiles
+  //   16     16384 x 4096   16.4  18.4         28672 x 4096   29.5  27.1
+  //   16     28672 x 1024    8.6  10.5         28672 x 2048   15.2  15.3
+  //   32     8192 x 6144    14.5  18.1         8192 x 8192    21.0  19.3
+  //   32     16384 x 2048   10.0  14.1         16384 x 5120   22.3  22.0
+  //   64     4096 x 4096    11.9  15.0         4096 x 8192    21.2  17.0
+  //   64     8192 x 4096    15.5  16.8         8192 x 6144    21.3  20.1
+  const int wide = (n + 15) / 16 <= cus ? 1
+                   : (n + 31) / 32 <= cus ? 2
+                   : (n + 63) / 64 <= cus || k <= 2048 ? 4 : 0;
+  if (wide && (m <= 16 || (n + 63) / 64 <= cus) &&
+      (m <= 16 || (m <= 32 && k <= (wide <= 2 ? 8192 : 4096)) ||
+       (m <= 64 && wide <= 2 && k <= 4096))) {
+    best.tiles_n = wide;
     return best;
   }
-  if (m <= 32 && (n + 31) / 32 <= cus && k <= 8192) return best;
   double least = 0;
   for (int i = 0; i < int(sizeof(kTiles) / sizeof(kTiles[0])); i++) {
     const Tiles &t = kTiles[i];
@@ -657,7 +676,10 @@ Plan plan_of(int m, int n, int k) {
 
 template <int R, int T>
 int launch_few(const GemmI8Call &c, hipStream_t s) {
-  const int steps = (c.k + 63) / 64, waves = std::max(1, std::min(16, steps / 2));
+  // (as many waves as take the same whole turns)
+  using F = Few<R, T>;
+  const int steps = (c.k + 63) / 64, each = (steps + F::U * F::kWaves - 1) / (F::U * F::kWaves) * F::U;
+  const int waves = (steps + each - 1) / each;
   few_kernel<R, T><<<unsigned((c.n + 16 * R - 1) / (16 * R)), 64 * waves, R * T * 1024 * waves, s>>>(c);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
 }
@@ -720,11 +742,18 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
     return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
   }
   Plan p = plan_of(c.m, c.n, c.k);
-  if (p.shape < 0)
-    return c.m > 16         ? launch_few<2, 2>(c, s)
-           : p.tiles_n == 1 ? launch_few<1, 1>(c, s)
-           : p.tiles_n == 2 ? launch_few<2, 1>(c, s)
-                            : launch_few<4, 1>(c, s);
+  if (p.shape < 0) {
+    auto few = [&](auto r) {
+      constexpr int R = decltype(r)::value;
+      if (c.m <= 16) return launch_few<R, 1>(c, s);
+      if (c.m <= 32) return launch_few<R, 2>(c, s);
+      if constexpr (R <= 2) return launch_few<R, 4>(c, s);
+      return int(SWAMP_EINVAL);  // (no plan)
+    };
+    return p.tiles_n == 1   ? few(std::integral_constant<int, 1>{})
+           : p.tiles_n == 2 ? few(std::integral_constant<int, 2>{})
+                            : few(std::integral_constant<int, 4>{});
+  }
   Work wk{c, p.tiles_m, p.tiles_n, 8, p.pieces, p.steps, nullptr};
   if (p.pieces > 1) {
     wk.part = static_cast<int32_t *>(sc.get(size_t(p.pieces) * size_t(c.m) * size_t(c.n) * 4));

@@ -177,6 +177,18 @@ def test_every_column_count(pkg, dev, m):
         assert torch.equal(y.cpu(), product(x[:, :k], w[:, :k], sx, sw, F32))
 
 
+@pytest.mark.parametrize("n", [4090, 4100, 8200, 16400])
+@pytest.mark.parametrize("m", [1, 16, 30, 33, 61])
+def test_few_rows(pkg, dev, m, n):
+    """Every way to share out the rows of w among workgroups, columns that end anywhere."""
+    for k in (1, 63, 64, 100, 257, 450, 1000, 4100):
+        say("few rows", m, n, k)
+        ops = operands(m, n, k, gap=16 * (k % 3))
+        y = run(pkg, ops, m, n, k, F32)
+        x, w, sx, sw, _ = ops
+        assert torch.equal(y.cpu(), product(x[:, :k], w[:, :k], sx, sw, F32))
+
+
 @pytest.mark.parametrize("m", [1, 20, 130])
 def test_largest_sum(pkg, dev, m):
     """131071 columns of -128: 2^31 - 2^14, the int32 that is left."""
