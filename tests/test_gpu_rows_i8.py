@@ -91,6 +91,47 @@ def test_quantize_strided(pkg, dev, xt, k, x_gap, q_gap, shift):
         assert torch.all(got == 77)
 
 
+@pytest.mark.parametrize("xt", [F32, F16, BF16])
+def test_quantize_lengths(pkg, dev, xt):
+    """Rows about every length where a thread takes more elements."""
+    for k in (511, 512, 513, 8192, 8193, 16389, 32768, 32769, 65536, 65537, 131071, 140003):
+        say("quantize length", xt, k)
+        x = torch.randn((3, k), generator=torch.Generator().manual_seed(k)).to(TORCH[xt])
+        x[1, -1] = 9.0
+        x[2, 0] = -11.0
+        dx = x.cuda()
+        q = torch.full((3, k), 77, dtype=torch.int8, device=dev)
+        scale = torch.empty(3, device=dev)
+        pkg.quantize_rows(dx.data_ptr(), xt, q.data_ptr(), scale.data_ptr(), 3, k, stream=stream())
+        torch.cuda.synchronize()
+        want, s = codes_of(x.float())
+        assert torch.equal(scale.cpu(), s)
+        assert torch.equal(q.cpu(), want)
+
+
+def test_quantize_half_way(pkg, dev):
+    """Quotients at half way between two codes and up to 4 steps of fp32 beside it, for
+    scales of any mantissa and size."""
+    say("quantize half way")
+    g = torch.Generator().manual_seed(5)
+    n, k = 400, 2048
+    s = torch.exp2(torch.rand(n, generator=g) * 200 - 100)
+    top = s * 127
+    scale = top / 127
+    x = (torch.randint(-127, 127, (n, k), generator=g) + 0.5) * scale[:, None]
+    bits = x.view(torch.int32) + torch.randint(-4, 5, (n, k), generator=g, dtype=torch.int32)
+    x = bits.view(torch.float32)
+    x[:, 0] = top
+    dx = x.cuda()
+    q = torch.full((n, k), 77, dtype=torch.int8, device=dev)
+    got = torch.empty(n, device=dev)
+    pkg.quantize_rows(dx.data_ptr(), F32, q.data_ptr(), got.data_ptr(), n, k, stream=stream())
+    torch.cuda.synchronize()
+    want, s = codes_of(x)
+    assert torch.equal(got.cpu(), s)
+    assert torch.equal(q.cpu(), want)
+
+
 def test_quantize_limits(pkg, dev):
     """Infinities and NaN take their row, tiny rows are zeros, the largest keep theirs."""
     say("quantize limits")
