@@ -474,8 +474,8 @@ SWAMP_API int swamp_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_st
  * x_stride and w_stride bytes apart (0: dense), multiples of 16 below 2^23, d_x and
  * d_w 16-byte aligned: of every row n_cols bytes are used; those between the rows, and
  * behind the last one up to the next multiple of 16, may be read.  y_stride in elements
- * (0: dense), d_y aligned to its element; m n_rows < 2^38.  n_cols == 0: a sum of
- * nothing.
+ * (0: dense), d_y aligned to its element; m and n_rows up to 2^30, m n_rows < 2^38.
+ * n_cols == 0: a sum of nothing.
  * Few rows split the sum over workgroups, whose parts meet in the stream's scratch
  * (swamp_gemm_rows_i8_workspace reports it); without it the sum is not split.  The
  * bits are the same either way. */
@@ -509,6 +509,7 @@ typedef struct swamp_beam_spec {
  * parent and token -1, score -infinity and done 0.
  * With n_out == n_beam, d_out_score may be d_score and d_out_done may be d_done;
  * otherwise outputs and inputs must not overlap.  d_logits aligned to its element.
+ * SWAMP_ESHAPE for 2^24 chunks of 4096 logits or more, over all rows.
  * Takes scratch for the rows' parts (swamp_beam_select_workspace); SWAMP_EWORKSPACE
  * without it. */
 SWAMP_API int swamp_beam_select(const swamp_beam_spec *spec, const void *d_logits, uint32_t type,

@@ -2,7 +2,8 @@
 //
 // Validation and dispatch only; kernels live in dequant.hip, gemv.hip,
 // gemv_fused.hip, gemv_batched.hip, gemm.hip, gemm_i8.hip, rope.hip, attn.hip, rows_i8.hip,
-// beam.hip and pages.hip, and the rules that choose between them by size in dispatch.hpp.  The error behaviour mirrors the
+// beam.hip and pages.hip, and the rules that choose between them by size in dispatch.hpp.
+// The error behaviour mirrors the
 // reference: shape asserts of fused_gemv_q4k (fused_gemv_q4k.rs:66-70) and
 // the bail! of forward_linear (linear.rs:23-25) become negative return
 // codes, checked before anything is launched; the two legacy host-pointer
@@ -200,11 +201,15 @@ int check_stride(int64_t &stride, int n_rows, int n) { return check_rows(stride,
 
 constexpr int kMaxBeams = 64, kMaxVocab = 1 << 20, kMaxCodeCols = 131071;
 constexpr int64_t kMaxCodeStride = int64_t(1) << 23, kMaxProducts = int64_t(1) << 38;
+constexpr int kMaxCodeRows = 1 << 30;
+// chunks of logits, a workgroup each: a launch holds less than 2^32 threads
+constexpr int64_t kMaxBeamChunks = int64_t(1) << 24;
 
 int check_beams(const swamp_beam_spec *b, BeamCall &c) {
   if (!b || b->n_seq < 0 || b->eos < -1) return SWAMP_EINVAL;
   if (b->n_beam < 1 || b->n_beam > kMaxBeams || b->n_out < 1 || b->n_out > kMaxBeams ||
-      b->vocab < 1 || b->vocab > kMaxVocab || b->eos >= b->vocab || b->n_seq > kMaxSeqs)
+      b->vocab < 1 || b->vocab > kMaxVocab || b->eos >= b->vocab || b->n_seq > kMaxSeqs ||
+      int64_t(b->n_seq) * b->n_beam * ((b->vocab + 4095) / 4096) >= kMaxBeamChunks)
     return SWAMP_ESHAPE;
   c.n_seq = b->n_seq;
   c.n_beam = b->n_beam;
@@ -795,7 +800,7 @@ int swamp_gemm_rows_i8(const int8_t *d_x, int64_t x_stride, const float *d_x_sca
                        int accumulate, void *stream) {
   if (!is_float(y_type)) return SWAMP_EDTYPE;
   if (m < 0 || n_rows < 0 || n_cols < 0) return SWAMP_EINVAL;
-  if (n_cols > kMaxCodeCols) return SWAMP_ESHAPE;
+  if (n_cols > kMaxCodeCols || m > kMaxCodeRows || n_rows > kMaxCodeRows) return SWAMP_ESHAPE;
   if (int rc = check_stride(x_stride, m, n_cols)) return rc;
   if (int rc = check_stride(w_stride, n_rows, n_cols)) return rc;
   if (int rc = check_stride(y_stride, m, n_rows)) return rc;
@@ -818,7 +823,7 @@ int swamp_gemm_rows_i8(const int8_t *d_x, int64_t x_stride, const float *d_x_sca
 
 size_t swamp_gemm_rows_i8_workspace(int m, int n_rows, int n_cols) {
   if (m <= 0 || n_rows <= 0 || n_cols <= 0 || n_cols > kMaxCodeCols ||
-      int64_t(m) * n_rows >= kMaxProducts)
+      m > kMaxCodeRows || n_rows > kMaxCodeRows || int64_t(m) * n_rows >= kMaxProducts)
     return 0;
   if (ensure_device(nullptr) != SWAMP_OK) return 0;
   return swamp_gemm_rows_i8_scratch_bytes(m, n_rows, n_cols);

@@ -35,15 +35,19 @@ __global__ void __launch_bounds__(256) fork_kernel(PagePool pool, PageTables t,
   const int n = t.n_seq, tid = int(threadIdx.x), c = tid % kTile;
   int *tile = smem, *gain = tile + n * kTile, *lens = gain + n, *parent = lens + n;
   __shared__ int most;
-  // the first tile's entries, on their way while lengths and parents come in (those past a
-  // sequence's pages, which the table has room for, are not looked at)
+  // the first tile's entries, on their way while lengths and parents come in
   constexpr int kAhead = 8;
   int ahead[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; j++) {
     const int s = j * (256 / kTile) + tid / kTile;
+    ahead[j] = s < n ? t.len[s] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) {
+    const int s = j * (256 / kTile) + tid / kTile;
     const int64_t col = int64_t(blockIdx.x) * kTile + c;
-    ahead[j] = s < n && col < t.stride ? t.pages[s * t.stride + col] : -1;
+    ahead[j] = col < held_cols(ahead[j], pool.shift, t.stride) ? t.pages[s * t.stride + col] : -1;
   }
   if (tid == 0) most = 0;
   for (int s = tid; s < n; s += 256) gain[s] = -1;
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(256) fork_kernel(PagePool pool, PageTables t,
     for (int j = 0; j < kAhead; j++) {
       const int s = j * (256 / kTile) + tid / kTile;
       if (s < n)
-        tile[s * kTile + c] = !held(s) ? -1 : c0 == mine ? ahead[j] : t.pages[s * t.stride + c0 + c];
+        tile[s * kTile + c] = c0 == mine ? ahead[j] : held(s) ? t.pages[s * t.stride + c0 + c] : -1;
     }
     for (int s = kAhead * (256 / kTile) + tid / kTile; s < n; s += 256 / kTile)
       tile[s * kTile + c] = held(s) ? t.pages[s * t.stride + c0 + c] : -1;
@@ -441,8 +445,8 @@ __global__ void __launch_bounds__(256) compact_move_kernel(PagePool pool, PageTa
     dst[j] = i < moves.cap ? moves.dst[i] : 0;
   }
   const int64_t first = int64_t(blockIdx.y) * 256 + tid;
-  if (s < t.n_seq && first < t.stride) id = t.pages[s * t.stride + first];
   const int64_t cols = s < t.n_seq ? held_cols(t.len[s], pool.shift, t.stride) : 0;
+  if (first < cols) id = t.pages[s * t.stride + first];
   const int n = *moves.count;
   if (n == 0) return;
   const int step = (n + kProbes - 1) / kProbes, probes = (n + step - 1) / step;

@@ -93,10 +93,10 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec {
 // Those at place `at` of a row of n; zeros behind it.
 template <typename XT, int V>
 __device__ __forceinline__ Vec<XT, V> take(const XT *row, int at, int n) {
-  if (at + V <= n) return *reinterpret_cast<const Vec<XT, V> *>(row + at);
+  if (at <= n - V) return *reinterpret_cast<const Vec<XT, V> *>(row + at);
   Vec<XT, V> x;
 #pragma unroll
-  for (int k = 0; k < V; k++) x.v[k] = at + k < n ? row[at + k] : XT(0);
+  for (int k = 0; k < V; k++) x.v[k] = k < n - at ? row[at + k] : XT(0);
   return x;
 }
 template <typename XT, int V>
@@ -104,12 +104,12 @@ __device__ __forceinline__ void give(int8_t *out, int at, int n, const Vec<XT, V
                                      float r) {
   Vec<int8_t, V> c;
   codes_of<V>(x.v, s, r, c.v);
-  if (at + V <= n) {
+  if (at <= n - V) {
     *reinterpret_cast<Vec<int8_t, V> *>(out + at) = c;
   } else {
 #pragma unroll
     for (int k = 0; k < V; k++)
-      if (at + k < n) out[at + k] = c.v[k];
+      if (k < n - at) out[at + k] = c.v[k];
   }
 }
 
@@ -633,9 +633,11 @@ __global__ void __launch_bounds__(256) join_kernel(Work wk) {
 
 // A sum of nothing.
 __global__ void __launch_bounds__(256) nothing_kernel(GemmI8Call c) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int m = int(i / c.n);
-  if (m < c.m) put_at(c, m, int(i - int64_t(m) * c.n), 0);
+  const int64_t mn = int64_t(c.m) * c.n;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < mn; i += int64_t(gridDim.x) * 256) {
+    const int m = int(i / c.n);
+    put_at(c, m, int(i - int64_t(m) * c.n), 0);
+  }
 }
 
 // Which tiles, and in how many pieces the sums: of every choice its time by a model, with
@@ -742,25 +744,29 @@ int launch(const Work &wk, hipStream_t s) {
 int swamp_launch_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_stride, int8_t *d_q,
                                int64_t q_stride, float *d_scale, int n_rows, int n_cols,
                                hipStream_t s) {
+  // (a launch holds less than 2^32 threads)
+  constexpr int kRows = 1 << 21;
   auto go = [&](auto t) {
     typedef decltype(t) X;
-    const X *x = static_cast<const X *>(d_x);
-    auto rows = [&](auto each_c) {
-      constexpr int each = decltype(each_c)::value;
-      const int threads = std::max(1, (n_cols + 64 * each - 1) / (64 * each)) * 64;
-      quantize_kernel<X, each><<<unsigned(n_rows), threads, 0, s>>>(x, x_stride, d_q, q_stride,
-                                                                    d_scale, n_cols);
-    };
-    // (rows in few waves wait less for each other: 4096 x 14336 bf16 40 us with 32 elements a
-    // thread and 48 with 16, 4096 x 4096 17.4 and 15.6, 16384 x 512 9.5 with 8 and 11.3 with 16,
-    // 512 x 40000 f32 21 with 64 and 46 in two looks)
-    if (n_cols <= 512) rows(std::integral_constant<int, 8>{});
-    else if (n_cols <= 1024 * 8) rows(std::integral_constant<int, 16>{});
-    else if (n_cols <= 1024 * 32) rows(std::integral_constant<int, 32>{});
-    else if (n_cols <= 1024 * 64) rows(std::integral_constant<int, 64>{});
-    else
-      quantize_any_kernel<X><<<unsigned(n_rows), 1024, 0, s>>>(x, x_stride, d_q, q_stride, d_scale,
-                                                               n_cols);
+    for (int64_t r0 = 0; r0 < n_rows; r0 += kRows) {
+      const X *x = static_cast<const X *>(d_x) + r0 * x_stride;
+      int8_t *q = d_q + r0 * q_stride;
+      float *scale = d_scale + r0;
+      const unsigned n = unsigned(std::min<int64_t>(n_rows - r0, kRows));
+      auto rows = [&](auto each_c) {
+        constexpr int each = decltype(each_c)::value;
+        const int threads = std::max(1, (n_cols + 64 * each - 1) / (64 * each)) * 64;
+        quantize_kernel<X, each><<<n, threads, 0, s>>>(x, x_stride, q, q_stride, scale, n_cols);
+      };
+      // (rows in few waves wait less for each other: 4096 x 14336 bf16 40 us with 32 elements
+      // a thread and 48 with 16, 4096 x 4096 17.4 and 15.6, 16384 x 512 9.5 with 8 and 11.3
+      // with 16, 512 x 40000 f32 21 with 64 and 46 in two looks)
+      if (n_cols <= 512) rows(std::integral_constant<int, 8>{});
+      else if (n_cols <= 1024 * 8) rows(std::integral_constant<int, 16>{});
+      else if (n_cols <= 1024 * 32) rows(std::integral_constant<int, 32>{});
+      else if (n_cols <= 1024 * 64) rows(std::integral_constant<int, 64>{});
+      else quantize_any_kernel<X><<<n, 1024, 0, s>>>(x, x_stride, q, q_stride, scale, n_cols);
+    }
   };
   if (x_type == SWAMP_F32) go(float{});
   else if (x_type == SWAMP_F16) go(_Float16{});
@@ -777,7 +783,7 @@ size_t swamp_gemm_rows_i8_scratch_bytes(int m, int n_rows, int n_cols) {
 int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream_t s) {
   const int64_t blocks = (int64_t(c.m) * c.n + 255) / 256;
   if (c.k == 0) {
-    nothing_kernel<<<unsigned(blocks), 256, 0, s>>>(c);
+    nothing_kernel<<<unsigned(std::min<int64_t>(blocks, 1 << 16)), 256, 0, s>>>(c);
     return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
   }
   Plan p = plan_of(c.m, c.n, c.k);

@@ -38,10 +38,12 @@ def test_gemm_rows_i8(pkg, L):
     # sums past int32; rows that do not begin at multiples of 16; strides of 8 MB; rows that overlap
     for bad in ({"k": 131072, "xs": 131072, "ws": 131072}, {"k": 60}, {"k": 60, "xs": 64},
                 {"xs": 72}, {"ws": 72}, {"xs": 1 << 23}, {"ws": 1 << 23}, {"xs": 48}, {"ys": 7},
-                {"m": 1 << 20, "n": 1 << 18}):
+                {"m": 1 << 20, "n": 1 << 18}, {"m": (1 << 30) + 1, "n": 1},
+                {"m": 1, "n": (1 << 30) + 1}, {"m": 1, "n": (1 << 31) - 1, "k": 1, "xs": 16, "ws": 16}):
         assert call(**bad) == pkg.ESHAPE, bad
     assert call(m=0, x=None, y=None) == pkg.OK and call(n=0, w=None, y=None) == pkg.OK
-    for none in ((0, 8, 64), (8, -1, 64), (8, 8, 0), (8, 8, 131072), (1 << 20, 1 << 18, 64)):
+    for none in ((0, 8, 64), (8, -1, 64), (8, 8, 0), (8, 8, 131072), (1 << 20, 1 << 18, 64),
+                 (1, (1 << 30) + 1, 16), ((1 << 30) + 1, 1, 16)):
         assert L.swamp_gemm_rows_i8_workspace(*none) == 0
 
 
@@ -59,7 +61,8 @@ def test_beam_select(pkg, L):
                 {"token": FAKE + 2}, {"out": FAKE + 2}):
         assert call(**bad) == pkg.EINVAL, bad
     for bad in ({"b": 0}, {"b": 65}, {"k": 0}, {"k": 65}, {"v": 0}, {"v": (1 << 20) + 1},
-                {"eos": 100}, {"n": 65536}, {"st": 99}):
+                {"eos": 100}, {"n": 65536}, {"st": 99}, {"n": 1024, "b": 64, "v": 1 << 20},
+                {"n": 65535, "b": 64, "v": 4096 * 4 + 1}):
         assert call(**bad) == pkg.ESHAPE, bad
     assert call(n=0, logits=None, score=None) == pkg.OK
     assert L.swamp_beam_select_workspace(pkg.BeamSpec(0, 4, 100, 8)) == 0
