@@ -25,6 +25,7 @@
 // bounds and the 64-bit polynomial, the second by its chain of steps in one workgroup (sums
 // 2.3 us, bound 2, collection 1, ranks 1).
 #include "swamp_common.hpp"
+#include "wave.hpp"
 
 #include <type_traits>
 
@@ -122,16 +123,6 @@ struct Chunk {
   }
 };
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) x = fmaxf(x, __shfl_xor(x, d, 64));
-  return x;
-}
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) x += __shfl_xor(x, d, 64);
-  return x;
-}
 // Keys that at least k, and at least `few` (k over the waves), of the wave's 64 N reach:
 // the largest such but for their low bits.
 template <int N, int kLow>
@@ -184,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
   float mine = -INFINITY;  // (and for NaN)
 #pragma unroll
   for (int e = 0; e < kEach; e++) mine = fmaxf(mine, x[e]);
-  float top = wave_max(mine);
+  float top = swamp::group_max(mine, 64);
   // n_out of one wave's lanes reach the one bound, a quarter of them of every wave's the other
   uint32_t bound, share;
   const uint32_t key = key_of(mine);
@@ -228,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
       sum += exp2_64((double(x[e]) - base) * kLog2e64);
     }
   }
-  sum = wave_sum64(sum);
+  sum = swamp::group_sum(sum, 64);
   if ((tid & 63) == 0) sums[wave] = sum;
   __syncthreads();
   int c = listed;
@@ -398,7 +389,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     float top = own.top;
     if (!ended)
       for (int i = at + 64; i < w.chunks; i += 64) top = fmaxf(top, part[i].top);
-    for (int d = team / 2; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    top = swamp::group_max(top, team);
     const double base = top == -INFINITY ? 0.0 : double(top);
     // (a chunk of nothing but -infinity has the sum 0; NaN passes)
     auto term = [&](const Part &p) {
@@ -408,7 +399,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     double sum = term(own);
     if (!ended)
       for (int i = at + 64; i < w.chunks; i += 64) sum += term(part[i]);
-    for (int d = team / 2; d >= 1; d /= 2) sum += __shfl_xor(sum, d, 64);
+    sum = swamp::group_sum(sum, team);
     const double lse = ended ? 0.0 : double(top) + log(sum);
     if (at == 0 && b < nb) {
       const bool fine = score - score == 0.0 && lse - lse == 0.0;  // both finite

@@ -17,6 +17,7 @@
 // are cleared, so that what lies in w there (a row's padding) counts for nothing.
 #include "swamp_common.hpp"
 #include "swamp_items.hpp"
+#include "wave.hpp"
 
 #include <algorithm>
 #include <mutex>
@@ -46,8 +47,7 @@ __device__ __forceinline__ uint32_t raise(uint32_t top, float x) {
 }
 __device__ __forceinline__ uint32_t workgroup_max(uint32_t top) {
   __shared__ uint32_t tops[16];
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) top = max(top, uint32_t(__shfl_xor(int(top), d, 64)));
+  top = swamp::group_max(top, 64);
   const int waves = int(blockDim.x) >> 6;
   if (waves == 1) return top;
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
