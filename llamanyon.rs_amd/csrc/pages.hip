@@ -5,6 +5,7 @@
 // A page's count is the number of page tables that name it, so a call's results are
 // sums and lowest places, which no order of atomics changes.
 #include "swamp_common.hpp"
+#include "wave.hpp"
 
 #include <algorithm>
 
@@ -131,12 +132,7 @@ __global__ void __launch_bounds__(256) fork_finish_kernel(PagePool pool, PageTab
 template <int kBlock>
 __device__ __forceinline__ int64_t scan(int64_t x, int64_t *part, int64_t &total) {
   const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
-  int64_t incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t below = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += below;
-  }
+  const int64_t incl = swamp::sum_to_here(x);
   if (lane == 63) part[wave] = incl;
   __syncthreads();
   int64_t before = 0;

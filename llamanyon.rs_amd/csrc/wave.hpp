@@ -76,4 +76,25 @@ __device__ __forceinline__ double group_sum(double x, int n) {
   return x;
 }
 
+// The sum of x over this lane and those before it.
+#ifdef __HIP_DEVICE_COMPILE__
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int64_t shifted(int64_t x) {  // 0 where nothing comes in
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(x), kCtrl, kRows, 0xF, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(x >> 32), kCtrl, kRows, 0xF, false));
+  return int64_t(uint64_t(hi) << 32 | lo);
+}
+#endif
+__device__ __forceinline__ int64_t sum_to_here(int64_t x) {
+#ifdef __HIP_DEVICE_COMPILE__
+  x += shifted<0x111, 0xF>(x);  // 1, 2, 4, 8 lanes up within 16
+  x += shifted<0x112, 0xF>(x);
+  x += shifted<0x114, 0xF>(x);
+  x += shifted<0x118, 0xF>(x);
+  x += shifted<0x142, 0xA>(x);  // lane 15 of 16 to the next 16, the second and the fourth
+  x += shifted<0x143, 0xC>(x);  // lane 31 to the upper 32
+#endif
+  return x;
+}
+
 }  // namespace swamp
