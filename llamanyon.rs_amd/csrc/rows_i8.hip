@@ -6,8 +6,10 @@
 // the vector unit, where scales a block of 32 cost a conversion and an FMA for every 32
 // terms (gemm_i8.hip).
 //
-// Tiles.  Four waves a workgroup, WM x WN V_MFMA_I32_32X32X32_I8 blocks each.  A K step
-// is 64 codes: a stage holds the tile's rows of x, then of w, 64 bytes each, 16-byte
+// Tiles.  Eight waves a workgroup (64 x 128: four), WM x WN V_MFMA_I32_32X32X32_I8 blocks
+// each: two waves a SIMD fill each other's waits at the barriers and in the epilogue (four
+// waves of twice the blocks: 640 x 14336 x 4096 68 us, 58 so; 3000 x 5000 x 5000 107, 95).  A
+// K step is 64 codes: a stage holds the tile's rows of x, then of w, 64 bytes each, 16-byte
 // chunks XOR-swizzled by (row / 4) % 4, so that 16 consecutive lanes of a fragment read
 // meet no bank twice.  Stages are filled by direct-to-LDS DMA, two steps at a time, four to
 // twelve steps ahead; one barrier a step, between its halves, whose counted wait leaves
@@ -16,7 +18,7 @@
 // The last step of a sum is taken apart from the loop: its codes of x behind column K
 // are cleared, so that what lies in w there (a row's padding) counts for nothing.
 //
-// Measured: 4096 rows of x by 28672 x 4096 in tiles of 256 x 256 429 to 462 us (2.1 to 2.2
+// Measured: 4096 rows of x by 28672 x 4096 in tiles of 256 x 256 430 to 475 us (2.0 to 2.2
 // POP/s, bf16 out), bound by the matrix pipes, busy 60% of the time at the clock that the
 // card holds, and by each tile's start and end (about 12 of its 66 us); 64 rows by the same
 // weights in tiles of 64 x 128 26.7 us, 4.7 TB/s, bound by HBM.
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
     return;
   }
   // A whole tile: a strip's reads, the next one's writes (LDS keeps their order), and then
-  // the first's arithmetic; one wave a SIMD has nothing else to wait with.
+  // the first's arithmetic.
   constexpr int V = 16 / int(sizeof(Y)), kLanes = kCols / V, kRows = 64 / kLanes, T = 32 / kRows;
   const int col = lane % kLanes * V, row0 = lane / kLanes;
   double sw_n[V];
@@ -813,10 +815,10 @@ int swamp_launch_gemm_rows_i8(const GemmI8Call &c, swamp::Scratch &sc, hipStream
     }
   }
   const int rc = p.shape == 0   ? launch<1, 2, 2, 2>(wk, s)
-                 : p.shape == 1 ? launch<2, 2, 2, 2>(wk, s)
-                 : p.shape == 2 ? launch<4, 2, 2, 2>(wk, s)
-                 : p.shape == 3 ? launch<2, 4, 2, 2>(wk, s)
-                                : launch<4, 4, 2, 2>(wk, s);
+                 : p.shape == 1 ? launch<2, 1, 2, 4>(wk, s)
+                 : p.shape == 2 ? launch<2, 2, 4, 2>(wk, s)
+                 : p.shape == 3 ? launch<2, 2, 2, 4>(wk, s)
+                                : launch<4, 2, 2, 4>(wk, s);
   if (rc != SWAMP_OK || wk.pieces == 1) return rc;
   join_kernel<<<unsigned(blocks), 256, 0, s>>>(wk);
   return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH;
