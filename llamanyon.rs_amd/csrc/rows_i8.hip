@@ -647,20 +647,20 @@ __global__ void __launch_bounds__(256) nothing_kernel(GemmI8Call c) {
   }
 }
 
-// Which tiles, and in how many pieces the sums: of every choice its time by a model, with
-// both sides of 171 sizes (1 to 1024 rows of x, 640 to 28672 of w, 512 to 14336 columns)
-// measured in up to 40 ways.  A round of tiles costs a tile's filling and storing and its
-// steps, a last one that does not fill the CUs 0.7 of that and the rest by its share; pieces
-// cost their sums' writing and reading.  Of 144 sizes above 16 rows the choice among tiles
-// is 1.4% slower than the fastest on average, 23% at worst but for one (192 x 16384 x 512,
-// 17.3 us for 11.4).
+// Which tiles, and in how many pieces the sums: of every choice its time by a model, whose
+// numbers are fitted to 148 sizes (48 to 2048 rows of x, 640 to 28672 of w, 512 to 14336
+// columns), each measured in up to 25 ways.  A round of tiles costs a tile's filling and
+// storing and its steps, a last one that does not fill the CUs 0.73 of that and the rest by
+// its share; pieces cost their sums' writing and reading.  The choice is 1.6% slower than the
+// fastest on average, 33% at worst (192 x 16384 x 512, 13 us for 10), then 26% (160 rows of
+// the same, 65 x 1024 x 1024), 24% (640 x 4096 x 14336, 75 us for 61) and 17%.
 struct Tiles {
   int tm, tn;
   double step, fixed;  // us
 };
 constexpr Tiles kTiles[] = {
-    {64, 128, 0.205, 6.4}, {128, 128, 0.24, 9.5}, {256, 128, 0.5, 7.0}, {128, 256, 0.5, 7.0},
-    {256, 256, 0.84, 12.5}};
+    {64, 128, 0.205, 5.9},  {128, 128, 0.24, 9.0}, {256, 128, 0.468, 7.0},
+    {128, 256, 0.516, 6.4}, {256, 256, 0.86, 13.6}};
 
 struct Plan {
   int shape;  // of kTiles; -1: few_kernel, of `tiles_n` tiles of 16 rows a workgroup
@@ -704,8 +704,8 @@ Plan plan_of(int m, int n, int k) {
       const int64_t units = tiles * p.pieces, rem = units % cus;
       const double round = t.fixed + p.steps * t.step;
       double us = double(units / cus) * round;
-      if (rem) us += round * (0.7 + 0.3 * double(rem) / cus);
-      if (p.pieces > 1) us += 1.0 + p.pieces * (double(m) * n * 8.0 / 2.9e6);
+      if (rem) us += round * (0.73 + 0.27 * double(rem) / cus);
+      if (p.pieces > 1) us += 0.9 + p.pieces * (double(m) * n * 8.0 / 3.6e6);
       if (best.shape < 0 || us < least) {
         least = us;
         best = p;
