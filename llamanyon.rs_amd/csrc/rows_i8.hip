@@ -19,7 +19,7 @@
 // are cleared, so that what lies in w there (a row's padding) counts for nothing.
 //
 // Measured: 4096 rows of x by 28672 x 4096 in tiles of 256 x 256 430 to 475 us (2.0 to 2.2
-// POP/s, bf16 out), bound by the matrix pipes, busy 60% of the time at the clock that the
+// POP/s, bf16 out), bound by the matrix pipes, busy 65% of the time at the clock that the
 // card holds, and by each tile's start and end (about 12 of its 66 us); 64 rows by the same
 // weights in tiles of 64 x 128 26.7 us, 4.7 TB/s, bound by HBM.
 #include "swamp_common.hpp"
