@@ -495,8 +495,9 @@ typedef struct swamp_beam_spec {
 /* The best continuations of every sequence over its beams and the vocabulary.
  * Token v of beam b scores d_score[b] + x_v - log sum_u exp x_u, x the beam's row of
  * d_logits (type F32, F16 or BF16, rows stride elements apart, 0: dense), in 64 bits.
- * The n_out largest of a sequence are written in falling order, equal ones by beam,
- * then token:
+ * The n_out largest of a sequence are written in falling order, equal ones (in all 64
+ * bits) by beam, then the larger logit, then the lower token, so that the best n are the
+ * head of the best n + 1:
  *   d_parent[n_seq][n_out]    the row (sequence * n_beam + beam) that is continued
  *   d_token[n_seq][n_out]     by this token
  *   d_out_score[n_seq][n_out] the score, rounded to fp32

@@ -6,11 +6,11 @@
 // n_out largest logits in falling order.  The second, a workgroup a sequence, joins the
 // sums and ranks the lists' tokens by their totals.
 //
-// Sums and totals are 64-bit: beams whose scores agree to 32 bits keep their order, and
-// equal ones the order of their tokens.  The exponential is 2^n 2^f, n = rint(x log2 e),
-// 2^f a polynomial of degree 9 through the Chebyshev nodes of |f| <= 1/2 (off by 2e-14 of
-// it): 16 operations of 64 bits an element, which the vector units issue at the rate of
-// 32-bit ones.
+// Sums and totals are 64-bit: beams whose scores agree to 32 bits keep their order.  Equal
+// totals go by beam, then the larger logit, then the lower token.  The exponential is
+// 2^n 2^f, n = rint(x log2 e), 2^f a polynomial of degree 9 through the Chebyshev nodes of
+// |f| <= 1/2 (off by 2e-14 of it): 16 operations of 64 bits an element, which the vector
+// units issue at the rate of 32-bit ones.
 //
 // Largest tokens without a sort: a wave's lanes each have a largest value.  Where a quarter
 // of n_out of every wave's reach a bound (found bit by bit with ballots), or n_out of one
@@ -301,22 +301,35 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
 }
 
 // ---- a sequence -----------------------------------------------------------
+// The order of continuations: the larger total, then the lower place: the beam, above the
+// logit's key turned round, above the token.  Totals of one beam fall with its logits or stay
+// equal (a logit of 1e18 leaves no other two apart in 64 bits), so the chunks' lists, cut by
+// logits, are in this order too, and the best n are the head of the best n + 1.
 struct Best {
   double total;
-  int flat;  // beam * vocab + token; -1: none
+  uint64_t place;
 };
+constexpr int kTokenBits = 20, kBeamShift = 52;  // vocabularies of up to 2^20
+constexpr uint64_t kNobody = ~uint64_t(0);  // place of no continuation
+__device__ __forceinline__ uint64_t place_of(int beam, float x, int token) {
+  return uint64_t(beam) << kBeamShift | uint64_t(~key_of(x)) << kTokenBits | uint32_t(token);
+}
+__device__ __forceinline__ int beam_at(uint64_t place) { return int(place >> kBeamShift); }
+__device__ __forceinline__ int token_at(uint64_t place) {
+  return int(uint32_t(place) & ((1u << kTokenBits) - 1));
+}
 __device__ __forceinline__ bool before(const Best &a, const Best &b) {
-  return a.flat >= 0 && (b.flat < 0 || a.total > b.total || (a.total == b.total && a.flat < b.flat));
+  return a.place != kNobody &&
+         (b.place == kNobody || a.total > b.total || (a.total == b.total && a.place < b.place));
 }
 
 // A total as a whole number of the same order, for comparisons without branches.
 struct Ranked {
-  uint64_t key;
-  int flat, pad;
+  uint64_t key, place;
 };
 __device__ __forceinline__ Ranked ranked(const Best &b) {
   const uint64_t u = __builtin_bit_cast(uint64_t, b.total + 0.0);
-  return Ranked{u >> 63 ? ~u : u | uint64_t(1) << 63, b.flat, 0};
+  return Ranked{u >> 63 ? ~u : u | uint64_t(1) << 63, b.place};
 }
 __device__ __forceinline__ double total_of(uint64_t key) {
   return __builtin_bit_cast(double, key >> 63 ? key & ~(uint64_t(1) << 63) : ~key);
@@ -329,11 +342,11 @@ struct Row {  // of a beam
 
 // x at place p of list l, of beam b.
 __device__ __forceinline__ Best best_of(const Work &w, const Row &r, int b, int l, int p, Entry x) {
-  Best e{0.0, -1};
+  Best e{0.0, kNobody};
   if (r.state == 1) {
-    if (x.token >= 0) e = Best{r.score + (double(x.x) - r.lse), b * w.c.vocab + x.token};
+    if (x.token >= 0) e = Best{r.score + (double(x.x) - r.lse), place_of(b, x.x, x.token)};
   } else if (r.state == 2 && p == 0 && l == b * w.chunks) {
-    e = Best{r.score, b * w.c.vocab + w.c.eos};
+    e = Best{r.score, place_of(b, 0.f, w.c.eos)};
   }
   return e;
 }
@@ -341,12 +354,13 @@ __device__ __forceinline__ const Entry *list_of(const Work &w, int seq, int l) {
   return w.list + (int64_t(seq) * w.c.n_beam * w.chunks + l) * w.pad;
 }
 __device__ __forceinline__ uint32_t bound_key(const Best &e) {
-  return e.flat < 0 ? 0u : key_of(float(e.total) + 0.f);
+  return e.place == kNobody ? 0u : key_of(float(e.total) + 0.f);
 }
 __device__ __forceinline__ Best wave_best(Best best) {
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) {
-    const Best o{__shfl_xor(best.total, d, 64), __shfl_xor(best.flat, d, 64)};
+    const Best o{__shfl_xor(best.total, d, 64),
+                 uint64_t(__shfl_xor(static_cast<unsigned long long>(best.place), d, 64))};
     if (before(o, best)) best = o;
   }
   return best;
@@ -471,9 +485,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
 #pragma unroll 8
         for (int o = 0; o < n; o++) {
           const Ranked x = list[at(o)];
-          rank += int(x.key > me.key) | (int(x.key == me.key) & int(x.flat < me.flat));
+          rank += int(x.key > me.key) | (int(x.key == me.key) & int(x.place < me.place));
         }
-        if (rank < k) picked[rank] = Best{total_of(me.key), me.flat};
+        if (rank < k) picked[rank] = Best{total_of(me.key), me.place};
       }
     };
     if (c <= 256) {
@@ -501,7 +515,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
       __syncthreads();
       rank_all(left, [&](int i) { return int(kept[i]); });
     }
-    for (int i = c + tid; i < k; i += kJoinThreads) picked[i] = Best{0.0, -1};
+    for (int i = c + tid; i < k; i += kJoinThreads) picked[i] = Best{0.0, kNobody};
   } else {
     // One after the other: the first of the lists' heads, whose list goes on.  A thread
     // keeps the first of its lists' heads; next[l] lies in the ranked list's place.
@@ -509,10 +523,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     for (int l = tid; l < lists; l += kJoinThreads) next[l] = 0;
     int from = 0;
     auto first = [&]() {
-      Best best{0.0, -1};
+      Best best{0.0, kNobody};
       for (int l = tid; l < lists; l += kJoinThreads) {
         const int b = l / w.chunks, p = next[l];
-        const Best e = p < k ? best_of(w, rows[b], b, l, p, list_of(w, seq, l)[p]) : Best{0.0, -1};
+        const Best e = p < k ? best_of(w, rows[b], b, l, p, list_of(w, seq, l)[p]) : Best{0.0, kNobody};
         if (before(e, best)) best = e, from = l;
       }
       return best;
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
       for (int i = 1; i < kJoinWaves; i++)
         if (before(waves[i], best)) best = waves[i];
       if (tid == 0) picked[r] = best;
-      if (best.flat >= 0 && head.flat == best.flat) {
+      if (best.place != kNobody && head.place == best.place) {
         next[from]++;
         head = first();
       }
@@ -537,8 +551,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
   __syncthreads();
   if (tid < k) {
     const Best e = picked[tid];
-    const bool none = e.flat < 0;
-    const int b = none ? 0 : e.flat / w.c.vocab, token = e.flat - b * w.c.vocab;
+    const bool none = e.place == kNobody;
+    const int b = none ? 0 : beam_at(e.place), token = token_at(e.place);
     const int64_t to = int64_t(seq) * k + tid;
     w.c.parent[to] = none ? -1 : seq * nb + b;
     w.c.token[to] = none ? -1 : token;

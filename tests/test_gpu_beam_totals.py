@@ -1,0 +1,108 @@
+"""swamp_beam_select where totals agree in all of their 64 bits: by beam, then the larger
+logit, then the lower token, whatever the number of best, of chunks and of tokens that reach
+the bound.
+
+Parents and tokens have to be equal: the rows are made so that totals are far apart or the
+same by the formula, not by the last bit of a sum.  Scores: one rounding to fp32, 2^-24 of the
+score, and 1e-13 for the 64-bit sums."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_beam import BF16, F32, check, select
+
+pytestmark = pytest.mark.gpu
+INF = math.inf
+
+
+@pytest.fixture(scope="module")
+def dev(pkg):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    torch.cuda.init()
+    pkg.init()
+    return torch.device("cuda")
+
+
+def say(*a):
+    print("[gpu case]", *a, flush=True)
+
+
+def plain(logits, score, n, b, k):
+    """(parent, token, 64-bit score, done) of each sequence's k best, nothing ended, no eos."""
+    out = []
+    for s in range(n):
+        found = []
+        for r in range(s * b, (s + 1) * b):
+            x = logits[r].double()
+            top = x.max()
+            if not math.isfinite(top) or not math.isfinite(score[r]):
+                continue
+            total = score[r].double() + ((x - top) - torch.exp(x - top).sum().log())
+            token = torch.nonzero(x > -INF)[:, 0]
+            token = token[torch.sort(x[token], descending=True, stable=True).indices[:k]]
+            found += [(-t, r - s * b, -l, v) for t, l, v in
+                      zip(total[token].tolist(), x[token].tolist(), token.tolist())]
+        found.sort()
+        rows = [(s * b + beam, v, -t, 0) for t, beam, _, v in found[:k]]
+        out += rows + [(-1, -1, -INF, 0)] * (k - len(rows))
+    return out
+
+
+@pytest.mark.parametrize("v,far", [(100, 9), (4096, 4000), (9000, 5000), (70000, 69999)])
+def test_logits_below_the_last_bit(pkg, dev, v, far):
+    """Two logits that no total of 64 bits tells apart, in one chunk and in two: the larger
+    one first, alone as well as before the other."""
+    say("below the last bit", v, far)
+    logits = torch.full((1, v), -5.0)
+    logits[0, 5], logits[0, far] = 0.0, 1e-20
+    score = torch.tensor([-1.0])
+    for k, first in ((1, [far]), (2, [far, 5]), (3, [far, 5, 0]), (64, [far, 5] + list(range(5)))):
+        got = select(pkg, logits, F32, score, None, 1, 1, k, -1)
+        want = plain(logits, score, 1, 1, k)
+        assert [w[1] for w in want[:len(first)]] == first
+        check(got, want)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n,b,v", [(1, 1, 60), (2, 3, 4097), (1, 4, 20000), (1, 64, 300), (1, 20, 9000)])
+def test_one_logit_forced(pkg, dev, t, n, b, v):
+    """A logit of 1e18 leaves every other of its row at one total: they follow by logit."""
+    say("one logit forced", t, n, b, v)
+    g = torch.Generator().manual_seed(v + b)
+    logits = torch.randn((n * b, v), generator=g) * 3
+    logits[torch.arange(n * b), torch.randint(0, v, (n * b,), generator=g)] = 1e18
+    logits = logits.to({F32: torch.float32, BF16: torch.bfloat16}[t])
+    score = -torch.rand(n * b, generator=g)
+    last = None
+    for k in (64, 33, 3, 2, 1):
+        want = plain(logits, score, n, b, k)
+        got = select(pkg, logits, t, score, None, n, b, k, -1)
+        check(got, want)
+        tokens = torch.tensor(got[1]).view(n, k)
+        assert last is None or torch.equal(tokens, last[:, :k])
+        last = tokens
+
+
+@pytest.mark.parametrize("b,v", [(64, 300), (40, 9000), (3, 90000)])
+def test_more_equal_totals_than_are_listed(pkg, dev, b, v):
+    """All totals of all beams equal, 64 tokens a list: more than a workgroup ranks at once
+    (64 x 64, 40 x 3 x 64) and less.  Logits that differ below the last bit keep their order
+    within a beam, and beams theirs."""
+    say("more than are listed", b, v)
+    logits = torch.zeros((b, v))
+    g = torch.Generator().manual_seed(b)
+    for r in range(b):
+        logits[r, torch.randperm(v, generator=g)[:5]] = torch.arange(1, 6) * 1e-20
+    score = torch.zeros(b)
+    for k in (1, 4, 64):
+        check(select(pkg, logits, F32, score, None, 1, b, k, -1), plain(logits, score, 1, b, k))
+    # a beam of three tokens comes first; the others' scores agree to 32 bits, not to 64
+    logits[1] = -INF
+    logits[1, 7:10] = torch.tensor([0.0, 2e-20, 1e-20])
+    score = torch.randperm(b, generator=g) * 1e-9
+    score[1] = 5.0
+    want = plain(logits, score, 1, b, 64)
+    assert [w[:2] for w in want[:3]] == [(1, 8), (1, 9), (1, 7)]
+    check(select(pkg, logits, F32, score, None, 1, b, 64, -1), want)
