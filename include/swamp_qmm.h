@@ -494,7 +494,9 @@ typedef struct swamp_beam_spec {
 
 /* The best continuations of every sequence over its beams and the vocabulary.
  * Token v of beam b scores d_score[b] + x_v - log sum_u exp x_u, x the beam's row of
- * d_logits (type F32, F16 or BF16, rows stride elements apart, 0: dense), in 64 bits.
+ * d_logits (type F32, F16 or BF16, rows stride elements apart, 0: dense), in 64 bits, the
+ * row's largest logit m taken out first: d_score[b] + ((x_v - m) - log sum_u exp(x_u - m)),
+ * so that in a row of one value, the type's lowest among them, a token scores -log(vocab).
  * The n_out largest of a sequence are written in falling order, equal ones (in all 64
  * bits) by beam, then the larger logit, then the lower token, so that the best n are the
  * head of the best n + 1:

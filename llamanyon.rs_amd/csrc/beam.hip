@@ -1,5 +1,6 @@
 // beam.hip -- swamp_beam_select: the best continuations of every sequence over its
-// beams and the vocabulary.  total(b, v) = score_b + x_bv - log sum_u exp x_bu.
+// beams and the vocabulary.  total(b, v) = score_b + x_bv - log sum_u exp x_bu, taken as
+// score_b + ((x_bv - m_b) - log sum_u exp(x_bu - m_b)), m_b the row's largest logit.
 //
 // Two launches.  The first cuts every row of logits into chunks of 4096, one a
 // workgroup, held in registers: the chunk's maximum m, its sum of exp(x - m), and its
@@ -335,8 +336,11 @@ __device__ __forceinline__ double total_of(uint64_t key) {
   return __builtin_bit_cast(double, key >> 63 ? key & ~(uint64_t(1) << 63) : ~key);
 }
 
+// The largest logit and the log of the sum of exp(x - top) stay apart: in one number a top
+// of 1e15, or one of the type's lowest value (a row whose mask leaves nothing), takes log_sum
+// with it even in 64 bits.
 struct Row {  // of a beam
-  double score, lse;
+  double score, top, log_sum;
   int state;  // 0: it has no continuation, 1: tokens, 2: it has ended
 };
 
@@ -344,7 +348,8 @@ struct Row {  // of a beam
 __device__ __forceinline__ Best best_of(const Work &w, const Row &r, int b, int l, int p, Entry x) {
   Best e{0.0, kNobody};
   if (r.state == 1) {
-    if (x.token >= 0) e = Best{r.score + (double(x.x) - r.lse), place_of(b, x.x, x.token)};
+    if (x.token >= 0)
+      e = Best{r.score + ((double(x.x) - r.top) - r.log_sum), place_of(b, x.x, x.token)};
   } else if (r.state == 2 && p == 0 && l == b * w.chunks) {
     e = Best{r.score, place_of(b, 0.f, w.c.eos)};
   }
@@ -414,10 +419,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Work w) {
     if (!ended)
       for (int i = at + 64; i < w.chunks; i += 64) sum += term(part[i]);
     sum = swamp::group_sum(sum, team);
-    const double lse = ended ? 0.0 : double(top) + log(sum);
+    // (finite only where the row's top is: a row of -infinity has the sum 0, and one that holds
+    // NaN or infinity a NaN)
+    const double log_sum = ended ? 0.0 : log(sum);
     if (at == 0 && b < nb) {
-      const bool fine = score - score == 0.0 && lse - lse == 0.0;  // both finite
-      rows[b] = Row{score, lse, !fine ? 0 : ended ? 2 : 1};
+      const bool fine = score - score == 0.0 && log_sum - log_sum == 0.0;  // both finite
+      rows[b] = Row{score, double(top), log_sum, !fine ? 0 : ended ? 2 : 1};
     }
   }
   __syncthreads();

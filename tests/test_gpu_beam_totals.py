@@ -1,16 +1,18 @@
-"""swamp_beam_select where totals agree in all of their 64 bits: by beam, then the larger
-logit, then the lower token, whatever the number of best, of chunks and of tokens that reach
-the bound.
+"""swamp_beam_select's totals where 64 bits are few: totals that agree in all of them (by
+beam, then the larger logit, then the lower token, whatever the number of best, of chunks and
+of tokens that reach the bound), and rows whose largest logit is far from 0.
 
 Parents and tokens have to be equal: the rows are made so that totals are far apart or the
 same by the formula, not by the last bit of a sum.  Scores: one rounding to fp32, 2^-24 of the
-score, and 1e-13 for the 64-bit sums."""
+score, and 1e-13 for the 64-bit sums (score, x - top and the log of the sum, each of them in
+64 bits and small where the total is).
+"""
 import math
 
 import pytest
 import torch
 
-from test_gpu_beam import BF16, F32, check, select
+from test_gpu_beam import BF16, F16, F32, TORCH, check, select
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
@@ -73,7 +75,7 @@ def test_one_logit_forced(pkg, dev, t, n, b, v):
     g = torch.Generator().manual_seed(v + b)
     logits = torch.randn((n * b, v), generator=g) * 3
     logits[torch.arange(n * b), torch.randint(0, v, (n * b,), generator=g)] = 1e18
-    logits = logits.to({F32: torch.float32, BF16: torch.bfloat16}[t])
+    logits = logits.to(TORCH[t])
     score = -torch.rand(n * b, generator=g)
     last = None
     for k in (64, 33, 3, 2, 1):
@@ -106,3 +108,36 @@ def test_more_equal_totals_than_are_listed(pkg, dev, b, v):
     want = plain(logits, score, 1, b, 64)
     assert [w[:2] for w in want[:3]] == [(1, 8), (1, 9), (1, 7)]
     check(select(pkg, logits, F32, score, None, 1, b, 64, -1), want)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("v", [1, 60, 6000, 50257])
+def test_row_far_from_zero(pkg, dev, t, v):
+    """Rows at the type's lowest value, at -1e15 and at 1e15 throughout (60000 in fp16): every
+    token scores its beam's score less log(vocabulary), which 64 bits would lose beside the
+    row's largest logit, and stands behind those of a beam of the same score that has a choice."""
+    say("far from zero", t, v)
+    kind = TORCH[t]
+    for value in (torch.finfo(kind).min, -1e15, 1e15):
+        value = max(min(value, 60000.0), torch.finfo(kind).min) if t == F16 else value
+        logits = torch.full((4, v), value, dtype=kind)
+        logits[1] = 0.0
+        logits[1, v // 2] = 20.0
+        score = torch.tensor([-1.0, -1.0, -2.0, -1.5])
+        for k in (1, 5, 64):
+            want = plain(logits, score, 2, 2, k)
+            if v > 1:
+                assert want[0][:2] == (1, v // 2) and abs(want[k][2] + 1.5 + math.log(v)) < 1e-9
+            check(select(pkg, logits, t, score, None, 2, 2, k, -1), want)
+
+
+@pytest.mark.parametrize("v", [300, 9000])
+def test_row_far_from_zero_with_others(pkg, dev, v):
+    """Differences of a few units at 1e7 and at -3e9 (one step of fp32: 1 and 256)."""
+    say("far from zero, with others", v)
+    g = torch.Generator().manual_seed(v)
+    logits = torch.randint(0, 12, (4, v), generator=g).float() + 1e7
+    logits[2:] = torch.randint(0, 2, (2, v), generator=g) * 256.0 - 3e9
+    score = -torch.rand(4, generator=g)
+    for k in (3, 64):
+        check(select(pkg, logits, F32, score, None, 1, 4, k, -1), plain(logits, score, 1, 4, k))
