@@ -210,8 +210,9 @@ __global__ void __launch_bounds__(kThreads, 8) chunk_kernel(Work w) {
     for (int e = 0; e < kEach; e++)
       if (__any(x[e] != -INFINITY)) {
         __builtin_amdgcn_sched_barrier(0);
-        const float a = x[e] == -INFINITY ? kLowest : x[e];
-        sum += exp2_64((double(a) - base) * kLog2e64);
+        // (0 itself: beside a top of the lowest value any finite stand-in would count)
+        const double term = exp2_64((double(x[e]) - base) * kLog2e64);
+        sum += x[e] == -INFINITY ? 0.0 : term;
       }
   } else {
 #pragma unroll

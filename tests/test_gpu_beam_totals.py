@@ -141,3 +141,23 @@ def test_row_far_from_zero_with_others(pkg, dev, v):
     score = -torch.rand(4, generator=g)
     for k in (3, 64):
         check(select(pkg, logits, F32, score, None, 1, 4, k, -1), plain(logits, score, 1, 4, k))
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("v,every", [(60, 2), (64, 63), (9000, 2), (9000, 3), (9000, 1000), (50257, 7)])
+def test_lowest_beside_masked(pkg, dev, t, v, every):
+    """A row of the type's lowest value and -infinity: the masked tokens count for nothing in
+    its sum, in their wave, their chunk and the row."""
+    say("lowest beside masked", t, v, every)
+    low = torch.finfo(TORCH[t]).min
+    logits = torch.full((4, v), -INF, dtype=TORCH[t])
+    logits[0, ::every] = low
+    logits[1, every - 1::every] = low
+    logits[2, v - 1] = low
+    logits[3, : v // 2] = low
+    score = torch.tensor([-1.0, -2.0, -9.0, -3.0])
+    for k in (1, 8, 64):
+        want = plain(logits, score, 1, 4, k)
+        left = (logits[0] == low).sum().item()
+        assert abs(want[0][2] + 1.0 + math.log(left)) < 1e-9 or left > 600
+        check(select(pkg, logits, t, score, None, 1, 4, k, -1), want)
