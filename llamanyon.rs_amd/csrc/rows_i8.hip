@@ -215,6 +215,14 @@ __device__ __forceinline__ void put_at(const GemmI8Call &c, int m, int n, int su
   else put(static_cast<__bf16 *>(c.y) + at, sum, sx, sw, c.accumulate);
 }
 
+// Between LDS that a wave's lanes write and its other lanes read: LDS keeps a wave's order by
+// itself, and this makes the compiler keep it.  No instruction of its own.
+__device__ __forceinline__ void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // 32 rows of kCols sums, in LDS, to rows m0 on and columns n0 on of y, whose ends may lie
 // among them.
 template <int kCols, int kPitch, typename Y>
@@ -470,7 +478,9 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
     auto part = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
       if constexpr (i < WM) {
+        lanes_meet();
         fill(ic);
+        lanes_meet();
         store_strip<kCols, kPitch, Y>(c, strip, scales + mr + 32 * i, m0 + mr + 32 * i, nr, lane);
       }
     };
@@ -489,6 +499,7 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
   for (int v = 0; v < V; v++) sw_n[v] = double(c.w_scale[nr + col + v]);
   Y *y = static_cast<Y *>(c.y) + int64_t(m0 + mr + row0) * c.y_stride + nr + col;
   fill(std::integral_constant<int, 0>{});
+  lanes_meet();
   auto whole = [&](auto ic) {
     constexpr int i = decltype(ic)::value;
     if constexpr (i < WM) {
@@ -502,7 +513,11 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
         sx[t] = scales[mr + 32 * i + t * kRows + row0];
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (i + 1 < WM) fill(std::integral_constant<int, i + 1>{});
+      if constexpr (i + 1 < WM) {
+        lanes_meet();
+        fill(std::integral_constant<int, i + 1>{});
+        lanes_meet();
+      }
 #pragma unroll
       for (int t = 0; t < T; t++) {
         Vec<Y, V> o;
