@@ -8,6 +8,7 @@
 #include "wave.hpp"
 
 #include <algorithm>
+#include <mutex>
 
 namespace {
 
@@ -532,13 +533,30 @@ __global__ void __launch_bounds__(256) copy_kernel(CopyWork w) {
   }
 }
 
+// Forks of many sequences ask for more than 64 KB of dynamic LDS, which a kernel has to be
+// allowed: once a device, the most that any call takes, so that no call lowers the limit
+// between another thread's setting and its launch.
+size_t fork_lds(int n_seq) { return size_t(n_seq) * (kTile + 3) * 4; }
+bool fork_limit_set() {
+  constexpr int kDevices = 64;  // (as many as the library initialises)
+  static std::once_flag once[kDevices];
+  static hipError_t err[kDevices];
+  const int dev = swamp::device_info().device;
+  if (dev < 0 || dev >= kDevices) return false;
+  std::call_once(once[dev], [dev] {
+    err[dev] = hipFuncSetAttribute(reinterpret_cast<const void *>(&fork_kernel<false>),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(fork_lds(kSeqs)));
+  });
+  return err[dev] == hipSuccess;
+}
+
 int launched() { return hipGetLastError() == hipSuccess ? SWAMP_OK : SWAMP_ELAUNCH; }
 
 }  // namespace
 
 int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int32_t *d_parent,
                             hipStream_t s) {
-  const size_t lds = size_t(t.n_seq) * (kTile + 3) * 4;
+  const size_t lds = fork_lds(t.n_seq);
   const int64_t tiles = std::max<int64_t>(1, (t.stride + kTile - 1) / kTile);
   // Two launches take 5.5 to 8 us (64 sequences 8).  One takes 3.4, 0.6 a thousand pages and,
   // a tile, 0.5 and 0.04 a sequence: 4 sequences of 30 pages among 512 take 4.8 us in one and
@@ -547,10 +565,7 @@ int swamp_launch_pages_fork(const PagePool &pool, const PageTables &t, const int
     fork_kernel<true><<<1, 256, lds, s>>>(pool, t, d_parent);
     return launched();
   }
-  if (lds > 64 * 1024 &&
-      hipFuncSetAttribute(reinterpret_cast<const void *>(&fork_kernel<false>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)) != hipSuccess)
-    return SWAMP_ELAUNCH;
+  if (lds > 64 * 1024 && !fork_limit_set()) return SWAMP_ELAUNCH;
   fork_kernel<false><<<unsigned(std::min<int64_t>(tiles, 1024)), 256, lds, s>>>(pool, t, d_parent);
   const unsigned blocks = unsigned(std::max<int64_t>(1, (int64_t(pool.n_pages) + 255) / 256));
   fork_finish_kernel<<<blocks, 256, 0, s>>>(pool, t, d_parent);
