@@ -33,6 +33,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a HIP device (MI355X / gfx950)")
 
 
+# These two expect a token of a row of 6000 equal logits, fp32's or bf16's lowest value, to score
+# d_score (x - logsumexp x, where 64 bits lose the logarithm beside 3.4e38).  By the definition it
+# scores d_score - log 6000, as fp16's row in the same test does; test_gpu_beam_totals.py holds
+# that.  They run and fail at the end, so that a run that stops at its first failure is whole.
+_HOLD_A_WRONG_VALUE = ("test_gpu_beam.py::test_masks_and_limits[0]",
+                       "test_gpu_beam.py::test_masks_and_limits[30]")
+
+
+def pytest_collection_modifyitems(items):
+    items.sort(key=lambda item: item.nodeid.endswith(_HOLD_A_WRONG_VALUE))
+
+
 @pytest.fixture(scope="session")
 def pkg():
     return load_pkg()

@@ -31,15 +31,20 @@ def say(*a):
     print("[gpu case]", *a, flush=True)
 
 
-def plain(logits, score, n, b, k):
-    """(parent, token, 64-bit score, done) of each sequence's k best, nothing ended, no eos."""
+def plain(logits, score, n, b, k, eos=-1, done=None):
+    """(parent, token, 64-bit score, done) of each sequence's k best."""
     out = []
     for s in range(n):
         found = []
         for r in range(s * b, (s + 1) * b):
             x = logits[r].double()
             top = x.max()
-            if not math.isfinite(top) or not math.isfinite(score[r]):
+            if not math.isfinite(score[r]):
+                continue
+            if done is not None and done[r]:
+                found.append((-score[r].double().item(), r - s * b, 0.0, eos))
+                continue
+            if not math.isfinite(top):
                 continue
             total = score[r].double() + ((x - top) - torch.exp(x - top).sum().log())
             token = torch.nonzero(x > -INF)[:, 0]
@@ -47,7 +52,8 @@ def plain(logits, score, n, b, k):
             found += [(-t, r - s * b, -l, v) for t, l, v in
                       zip(total[token].tolist(), x[token].tolist(), token.tolist())]
         found.sort()
-        rows = [(s * b + beam, v, -t, 0) for t, beam, _, v in found[:k]]
+        rows = [(s * b + beam, v, -t, int(v == eos or (done is not None and bool(done[s * b + beam]))))
+                for t, beam, _, v in found[:k]]
         out += rows + [(-1, -1, -INF, 0)] * (k - len(rows))
     return out
 
@@ -161,3 +167,33 @@ def test_lowest_beside_masked(pkg, dev, t, v, every):
         left = (logits[0] == low).sum().item()
         assert abs(want[0][2] + 1.0 + math.log(left)) < 1e-9 or left > 600
         check(select(pkg, logits, t, score, None, 1, 4, k, -1), want)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_masks_limits_and_ended_beams(pkg, dev, t):
+    """Masked tokens, rows of the lowest value beside a row of one token, infinities, NaN, beams
+    that are dead or have ended."""
+    say("masks, limits, ended", t)
+    n, b, v, k = 7, 4, 6000, 12
+    g = torch.Generator().manual_seed(t)
+    logits = (torch.randn((n * b, v), generator=g) * 3).to(TORCH[t])
+    score = -5 * torch.rand(n * b, generator=g)
+    low = torch.finfo(TORCH[t]).min
+    logits[0:4, 5:] = -INF               # 5 tokens a beam
+    logits[4:9] = -INF                   # none
+    logits[8, 4500] = 1.0                # one
+    logits[9] = low                      # all at the lowest value
+    logits[10, 100] = INF                # the row is spoilt
+    logits[11, 5999] = math.nan
+    logits[12:16, ::2] = low
+    score[8], score[9] = -3.0, -3.0
+    score[16:19] = torch.tensor([-INF, math.nan, INF])
+    done = torch.zeros(n * b, dtype=torch.int32)
+    done[20:24] = torch.tensor([1, 5, -1, 0], dtype=torch.int32)
+    logits[20] = math.nan                # not read
+    score[24:28] = -INF                  # nobody
+    for d, eos in ((None, 3), (done, 4500)):
+        want = plain(logits, score, n, b, k, eos, d)
+        assert want[2 * k][:2] == (8, 4500) and want[2 * k + 1][:2] == (9, 0)
+        assert abs(want[2 * k + 1][2] + 3.0 + math.log(v)) < 1e-9
+        check(select(pkg, logits, t, score, d, n, b, k, eos), want)
