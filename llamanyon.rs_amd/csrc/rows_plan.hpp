@@ -16,10 +16,14 @@ namespace swamp_rows {
 struct Tiles {
   int tm, tn;
   double step, fixed;  // us
+  int threads;
 };
 constexpr Tiles kTiles[] = {
-    {64, 128, 0.205, 5.9},  {128, 128, 0.24, 9.0}, {256, 128, 0.468, 7.0},
-    {128, 256, 0.516, 6.4}, {256, 256, 0.86, 13.6}};
+    {64, 128, 0.205, 5.9, 256},  {128, 128, 0.24, 9.0, 512}, {256, 128, 0.468, 7.0, 512},
+    {128, 256, 0.516, 6.4, 512}, {256, 256, 0.86, 13.6, 512}};
+// A launch holds less threads than this.  256 x 256 tiles stay below it for every call of less
+// than 2^38 products.
+constexpr int64_t kMostThreads = int64_t(1) << 32;
 
 struct Plan {
   int shape;  // of kTiles; -1: few_kernel, of `tiles_n` tiles of 16 rows a workgroup
@@ -56,6 +60,7 @@ inline Plan plan_of(int m, int n, int k, int cus) {
     p.tiles_m = (m + t.tm - 1) / t.tm;
     p.tiles_n = (n + t.tn - 1) / t.tn;
     const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+    if (tiles * t.threads >= kMostThreads) continue;
     for (int pieces = 1; pieces <= 8 && (pieces == 1 || (KT / pieces >= 4 && tiles * pieces <= 3 * cus));
          pieces++) {
       p.steps = ((KT + pieces - 1) / pieces + 1) / 2 * 2;  // whole pairs

@@ -57,10 +57,14 @@ def test_tiles_of_the_tested_sizes(plan):
 
 
 def test_plans_are_sound(plan):
-    """Tiles cover the result, pieces the sum, none of them empty."""
+    """Tiles cover the result, pieces the sum, none of them empty, and a launch holds less than
+    2^32 threads."""
     rng = random.Random(3)
     sizes = [(1 << 30, 1, 131071), (1, 1 << 30, 64), (64, 1 << 30, 16), (100, 1 << 30, 16),
              (1 << 30, 255, 16), (1 << 19, (1 << 19) - 1, 64), (17, 1 << 28, 512)]
+    for few in (1, 17, 65, 127, 129, 255, 257, 513, 1025, 4097):
+        many = min(1 << 30, ((1 << 38) - 1) // few)
+        sizes += [(few, many, 16), (many, few, 16), (few, many, 131071), (many, few, 131071)]
     for _ in range(4000):
         m, n = (int(2 ** rng.uniform(0, 20)) for _ in range(2))
         sizes.append((m, n, int(2 ** rng.uniform(0, 17)) % 131072 or 1))
@@ -77,5 +81,7 @@ def test_plans_are_sound(plan):
             assert tiles_m == -(-m // tm) and tiles_n == -(-n // tn), (m, n, k)
             assert 1 <= pieces <= 8 and (pieces - 1) * steps < total <= pieces * steps, (m, n, k)
             assert steps % 2 == 0 or pieces == 1, (m, n, k)
+            threads = 256 if (tm, tn) == (64, 128) else 512
+            assert tiles_m * tiles_n * pieces * threads < 1 << 32, (m, n, k)
             # partial sums: none but where tiles are few
             assert pieces == 1 or tiles_m * tiles_n * pieces <= 3 * cus, (m, n, k)
