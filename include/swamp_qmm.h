@@ -512,7 +512,9 @@ typedef struct swamp_beam_spec {
  * parent and token -1, score -infinity and done 0.
  * With n_out == n_beam, d_out_score may be d_score and d_out_done may be d_done;
  * otherwise outputs and inputs must not overlap.  d_logits aligned to its element.
- * SWAMP_ESHAPE for 2^24 chunks of 4096 logits or more, over all rows.
+ * SWAMP_EINVAL for d_done without an eos (-1), which an ended beam's continuation needs;
+ * SWAMP_ESHAPE for more than 65535 sequences, an eos that is no token, and 2^24 chunks of
+ * 4096 logits or more, over all rows.
  * Takes scratch for the rows' parts (swamp_beam_select_workspace); SWAMP_EWORKSPACE
  * without it. */
 SWAMP_API int swamp_beam_select(const swamp_beam_spec *spec, const void *d_logits, uint32_t type,
