@@ -20,9 +20,9 @@
 // exact bound is found bit by bit over the whole chunk.  The lists of a sequence are cut
 // alike: n_out / r lists whose r-th token reaches a bound have n_out tokens that do.
 //
-// Measured, the two kernels: 4 beams of 128256 f32 logits, 8 best, 5.8 + 6.4 us; 16 x 4 of
-// them 13.4 + 7.0 (2.4 TB/s in the first); 4 x 32 of 32000 bf16, 64 best, 13.6 + 15.5; 50 x 5
-// of 50257 f16, nearly all masked, 14.1 + 7.3.  The first is bound by the ballots of its
+// Measured, the two kernels: 4 beams of 128256 f32 logits, 8 best, 5.6 + 6.3 us; 16 x 4 of
+// them 13.4 + 6.5 (2.4 TB/s in the first); 4 x 32 of 32000 bf16, 64 best, 13.9 + 14.5; 50 x 5
+// of 50257 f16, nearly all masked, 14.0 + 7.0.  The first is bound by the ballots of its
 // bounds and the 64-bit polynomial (vector units busy half of the time), the second by its
 // chain of steps in one workgroup (sums 2 us, bound 2, collection 1, ranks 1).
 #include "swamp_common.hpp"

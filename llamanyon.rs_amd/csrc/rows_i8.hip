@@ -46,9 +46,9 @@ typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 // A code is rint(x / s), the quotient rounded to fp32.  x times 1 / s lies within 127.1 2^-23
 // of x / s, and that within 127 2^-24 of the rounded quotient, 2.3e-5 in all: where it is
 // further than 2^-15 from half way between two codes it names the code, and only elsewhere
-// (1024 elements of a wave meet one in 6 of 100) is there a division.  4096 x 4096 bf16 take
-// 16 us (3.1 TB/s), f32 16 (5.2 TB/s; 17.6 with a division for each), 4096 x 14336 bf16 47
-// (3.7 TB/s; 63).
+// (1024 elements of a wave meet one in 6 of 100) is there a division.  From HBM, into codes
+// that go there: 4096 x 4096 bf16 15.9 us (3.2 TB/s; 19.0 with a division for each), f32 17.0
+// (4.9 TB/s; 19.4), 4096 x 14336 bf16 41.0 (4.3 TB/s; 50.2).
 
 // The largest |x| of a workgroup's elements, as bits: infinity and NaN come last.
 __device__ __forceinline__ uint32_t raise(uint32_t top, float x) {
@@ -476,6 +476,8 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
       }
   };
   const int mr = wm * WM * 32, nr = n0 + wn * kCols;  // the wave's first row in the tile, column
+  // Ragged tiles, and all tiles of a call that adds to y, element by element: 4096 x 28672 x
+  // 4096 bf16 420 us, added 650; 4096 x 4096 x 14336 190 and 230.
   if (m0 + S::TM > c.m || n0 + S::TN > c.n || c.accumulate) {
     auto part = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
@@ -543,8 +545,8 @@ __global__ void __launch_bounds__(64 * NWM * NWN, 1) gemm_kernel(Work wk) {
 // by T times 16 of x.  A workgroup's waves take a share of the columns each, so that a
 // short matrix has all its bytes in flight at once, and their sums meet in LDS.  What of
 // x lies behind column K is cleared, rows behind the last are the descriptor's zeros.
-// One row of 6144 x 4096: 7.6 us, 5.0 of them its bytes; 32 rows 10.4 (5.1); 64 rows of 4096 x
-// 4096 11.9 (3.6): there every workgroup's own reading of x, 16 codes a lane and product.
+// One row of 6144 x 4096: 7.6 us, 4.5 of them its bytes at 5.6 TB/s; 32 rows 10.4 (4.6); 64 rows
+// of 4096 x 4096 11.9 (3.2): there every workgroup's own reading of x, 16 codes a lane and product.
 //
 // Waves and steps in flight are what the registers hold: 16 of 128 each, or 8 of 256.
 template <int R, int T>
@@ -714,9 +716,9 @@ int swamp_launch_quantize_rows(const void *d_x, uint32_t x_type, int64_t x_strid
         const int threads = std::max(1, (n_cols + 64 * each - 1) / (64 * each)) * 64;
         quantize_kernel<X, each><<<n, threads, 0, s>>>(x, x_stride, q, q_stride, scale, n_cols);
       };
-      // (rows in few waves wait less for each other: 4096 x 14336 bf16 40 us with 32 elements
-      // a thread and 48 with 16, 4096 x 4096 17.4 and 15.6, 16384 x 512 9.5 with 8 and 11.3
-      // with 16, 512 x 40000 f32 21 with 64 and 46 in two looks)
+      // (rows in few waves wait less for each other; from HBM: 4096 x 14336 bf16 41 us with 32
+      // elements a thread and 45 with 16, 4096 x 4096 18.6 and 15.3, 16384 x 512 9.1 with 8 and
+      // 10.8 with 16, 512 x 40000 f32 24 with 64 and 32 in two looks)
       if (n_cols <= 512) rows(std::integral_constant<int, 8>{});
       else if (n_cols <= 1024 * 8) rows(std::integral_constant<int, 16>{});
       else if (n_cols <= 1024 * 32) rows(std::integral_constant<int, 32>{});
